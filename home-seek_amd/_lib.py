@@ -74,6 +74,15 @@ _SIGNATURES = {
     "hsmoe_moe_prefill_workspace_size": (_size, [_i64, _i64, _i64, _i64, _int]),
     "hsmoe_moe_prefill": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int, _c_void_p, _i64, _int,
                                  _c_void_p, _f32, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "hsmoe_moe_sort_workspace_size": (_size, [_i64, _int, _i64]),
+    "hsmoe_moe_sort": (_int, [_c_void_p, _i64, _int, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size,
+                              _c_void_p]),
+    "hsmoe_moe_gather": (_int, [_c_void_p, _i64, _i64, _i64, _int, _c_void_p, _i64, _c_void_p, _int, _c_void_p,
+                                _c_void_p]),
+    "hsmoe_moe_combine": (_int, [_c_void_p, _int, _i64, _i64, _i64, _c_void_p, _c_void_p, _int, _c_void_p, _int,
+                                 _c_void_p, _c_void_p]),
+    "hsmoe_moe_combine_grad": (_int, [_c_void_p, _int, _c_void_p, _int, _i64, _i64, _c_void_p, _i64, _c_void_p,
+                                      _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p]),
     "hsmoe_lm_head_workspace_size": (_size, [_i64, _i64]),
     "hsmoe_lm_head_accept": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p, _c_void_p, _size, _c_void_p]),

@@ -8,7 +8,9 @@ zero, so stream-ordered calls can share them.
 from __future__ import annotations
 
 import array
+import contextlib
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -20,7 +22,7 @@ __all__ = [
     "moe_decode", "moe_layer_decode", "moe_layer_decode_routed", "NormTail", "moe_layer_status", "moe_layer_status_words",
     "clear_moe_layer_status", "check_moe_layer_status", "lm_head_accept", "expert_table", "shared_entry",
     "dequant_blocked", "xor_checksum", "MAX_DECODE_TOKENS", "MAX_LAYER_EXPERTS", "embed_add_rms_norm", "mtp_input",
-    "decode_step_record",
+    "decode_step_record", "ExpertOrder", "moe_sort", "moe_gather", "moe_combine", "moe_combine_grad",
 ]
 
 MAX_DECODE_TOKENS = 8
@@ -271,6 +273,139 @@ def moe_prefill(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, t
                                      ws.numel(), stream_ptr(dev))
         check(rc, "hsmoe_moe_prefill")
     return out_bf16, out_f32
+
+
+_ROW_KINDS = {torch.bfloat16: _lib.OUT_BF16, torch.float32: _lib.OUT_F32}
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """Makes dev the current device around a launch (its stream belongs to it)."""
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _row_kind(dtype: torch.dtype, what: str) -> int:
+    kind = _ROW_KINDS.get(dtype)
+    if kind is None:
+        raise TypeError(f"{what} must be bf16 or fp32, got {dtype}")
+    return kind
+
+
+class ExpertOrder(NamedTuple):
+    """(token, slot) pairs in the order of their experts (moe_sort), int32 device tensors.
+    Pair q = t * top_k + j is token t's slot j."""
+    offsets: torch.Tensor  # [E + 1]: expert e has rows offsets[e] .. offsets[e + 1] - 1
+    pairs: torch.Tensor    # [M * top_k]: the pair of each row, -1 from row offsets[E] on
+    rows: torch.Tensor     # [M, top_k]: the row of each pair, -1 for a dropped one
+
+    @property
+    def n_experts(self) -> int:
+        return self.offsets.numel() - 1
+
+    def check(self) -> tuple[int, int]:
+        """(tokens, top_k) of a well-formed order."""
+        off, pairs, rows = self
+        for t in self:
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise TypeError("an expert order holds contiguous int32 tensors")
+        if rows.dim() != 2 or pairs.numel() != rows.numel() or off.dim() != 1 or off.numel() < 2:
+            raise ValueError("an expert order is offsets [E + 1], pairs [M * top_k], rows [M, top_k]")
+        return rows.shape
+
+
+def moe_sort(topk_idx: torch.Tensor, n_experts: int) -> ExpertOrder:
+    """The (token, slot) pairs of topk_idx [M, k] sorted by expert, stably; ids < 0
+    or >= n_experts are dropped (hsmoe_moe_sort)."""
+    dev = require_cuda(topk_idx)
+    if topk_idx.dim() != 2:
+        raise ValueError("topk_idx must be [M, top_k]")
+    if topk_idx.is_floating_point() or topk_idx.dtype == torch.bool:
+        raise TypeError(f"topk_idx must hold integers, got {topk_idx.dtype}")
+    topk_idx = topk_idx.to(torch.int64).contiguous()
+    m, k = topk_idx.shape
+    offsets = torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev)
+    pairs = torch.empty(m * k, dtype=torch.int32, device=dev)
+    rows = torch.empty(m, k, dtype=torch.int32, device=dev)
+    # a workspace of the call's own: calls of two captured graphs may run at once
+    nbytes = lib().hsmoe_moe_sort_workspace_size(m, k, n_experts)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev):
+        check(lib().hsmoe_moe_sort(ptr(topk_idx), m, k, n_experts, ptr(offsets), ptr(pairs), ptr(rows), ptr(ws), nbytes,
+                                   stream_ptr(dev)), "hsmoe_moe_sort")
+    return ExpertOrder(offsets, pairs, rows)
+
+
+def moe_gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
+    """[M * k, D] rows of x [M, D] (bf16 or fp32) in the order's sequence; the rows
+    behind the last sorted one are zeros (hsmoe_moe_gather).  Its gradient is
+    moe_combine(d_rows, order)."""
+    dev = require_cuda(x, *order)
+    m, k = order.check()
+    kind = _row_kind(x.dtype, "rows")
+    if x.dim() != 2 or x.shape[0] != m:
+        raise ValueError(f"x {tuple(x.shape)} does not have the order's {m} tokens")
+    d = x.shape[1]
+    if x.stride(1) != 1 or x.stride(0) < d:
+        x = x.contiguous()
+    out = torch.empty(m * k, d, dtype=x.dtype, device=dev)
+    with _on(dev):
+        check(lib().hsmoe_moe_gather(ptr(x), max(x.stride(0), d), m, d, kind, ptr(order.offsets), order.n_experts,
+                                     ptr(order.rows), k, ptr(out), stream_ptr(dev)), "hsmoe_moe_gather")
+    return out
+
+
+def moe_combine(rows: torch.Tensor, order: ExpertOrder, topk_w: torch.Tensor | None = None,
+                residual: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """[M, D]: every token's rows summed with its weights topk_w [M, k] (1 when
+    None) in fp32, in slot order, plus residual [M, D] (hsmoe_moe_combine); bf16 or
+    fp32 as out_dtype, the residual or the rows say."""
+    dev = require_cuda(rows, topk_w, residual, *order)
+    m, k = order.check()
+    kind = _row_kind(rows.dtype, "rows")
+    if out_dtype is None:
+        out_dtype = rows.dtype if residual is None else residual.dtype
+    out_kind = _row_kind(out_dtype, "the output")
+    if rows.dim() != 2 or rows.shape[0] != m * k:
+        raise ValueError(f"rows {tuple(rows.shape)} do not match the order's {m} x {k} pairs")
+    d = rows.shape[1]
+    rows = rows.contiguous()
+    if topk_w is not None:
+        if topk_w.shape != order.rows.shape:
+            raise ValueError(f"weights {tuple(topk_w.shape)} do not match the order's [{m}, {k}]")
+        topk_w = topk_w.to(torch.float32).contiguous()
+    if residual is not None:
+        if residual.shape != (m, d) or residual.dtype != out_dtype:
+            raise ValueError(f"the residual must be [{m}, {d}] of the output's dtype")
+        residual = residual.contiguous()
+    out = torch.empty(m, d, dtype=out_dtype, device=dev)
+    with _on(dev):
+        check(lib().hsmoe_moe_combine(ptr(rows), kind, m * k, m, d, ptr(order.rows), ptr(topk_w), k, ptr(residual),
+                                      out_kind, ptr(out), stream_ptr(dev)), "hsmoe_moe_combine")
+    return out
+
+
+def moe_combine_grad(d_out: torch.Tensor, rows: torch.Tensor, order: ExpertOrder, topk_w: torch.Tensor | None = None,
+                     need_rows: bool = True, need_w: bool = True):
+    """The gradient of moe_combine for d_out [M, D]: (d_rows like rows, those behind
+    the last sorted one zeros; d_w fp32 [M, k], 0 where a pair is dropped), None
+    where not needed (hsmoe_moe_combine_grad).  The residual's is d_out."""
+    dev = require_cuda(d_out, rows, topk_w, *order)
+    m, k = order.check()
+    kind, out_kind = _row_kind(rows.dtype, "rows"), _row_kind(d_out.dtype, "d_out")
+    if rows.dim() != 2 or rows.shape[0] != m * k or d_out.shape != (m, rows.shape[1]):
+        raise ValueError(f"rows {tuple(rows.shape)} and d_out {tuple(d_out.shape)} do not match the order's {m} x {k} pairs")
+    d_out, rows = d_out.contiguous(), rows.contiguous()
+    if topk_w is not None:
+        if topk_w.shape != order.rows.shape:
+            raise ValueError(f"weights {tuple(topk_w.shape)} do not match the order's [{m}, {k}]")
+        topk_w = topk_w.to(torch.float32).contiguous()
+    d_rows = torch.empty_like(rows) if need_rows else None
+    d_w = torch.empty(m, k, dtype=torch.float32, device=dev) if need_w else None
+    with _on(dev):
+        check(lib().hsmoe_moe_combine_grad(ptr(d_out), out_kind, ptr(rows), kind, m, rows.shape[1], ptr(order.offsets),
+                                           order.n_experts, ptr(order.rows), ptr(topk_w), k, ptr(d_rows), ptr(d_w),
+                                           stream_ptr(dev)), "hsmoe_moe_combine_grad")
+    return d_rows, d_w
 
 
 def moe_decode_stage(stage: int, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,

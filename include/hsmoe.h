@@ -304,6 +304,55 @@ int hsmoe_moe_prefill(const void* x_dev, int64_t m, int64_t d, int64_t i, const 
                       void* out_bf16_dev, void* workspace_dev, size_t workspace_bytes, hsmoe_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * The expert layer in its parts: (token, slot) pairs sorted by expert, token
+ * rows in that order, and back.  For programs that run the experts' products
+ * themselves (hsmoe_linear with groups, other GPUs' experts, training).  The
+ * reference sorts by masking the whole batch per expert (fused_moe.py:458-551);
+ * hsmoe_moe_prefill holds its own sort inside.
+ *
+ * hsmoe_moe_sort: pair q = t * top_k + j is slot j of token t; ids < 0 or
+ * >= n_experts are dropped.  Row r is the r-th valid pair in the order of
+ * (id, q): a stable sort, two equal ids of one token are two rows.
+ *   offsets     int32 [n_experts + 1]: expert e has rows offsets[e] .. offsets[e + 1] - 1
+ *   pair_of_row int32 [m * top_k]: the pair of each row, -1 for rows from offsets[n_experts] on
+ *   row_of_pair int32 [m, top_k]: the row of each pair, -1 for a dropped one
+ * n_experts <= 1024, top_k <= 16, m < 2^24 (0 included), here and below.  The
+ * workspace (any contents, 0 bytes for few pairs) must hold
+ * hsmoe_moe_sort_workspace_size bytes. */
+size_t hsmoe_moe_sort_workspace_size(int64_t m, int top_k, int64_t n_experts);
+int hsmoe_moe_sort(const int64_t* topk_idx_dev, int64_t m, int top_k, int64_t n_experts, int32_t* offsets_dev,
+                   int32_t* pair_of_row_dev, int32_t* row_of_pair_dev, void* workspace_dev, size_t workspace_bytes,
+                   hsmoe_stream_t stream);
+
+/* rows_out[row_of_pair[t, j]] = x[t] for every pair that has a row; rows from
+ * offsets[n_experts] on are zeros.  x: [m, d] rows x_row_stride elements apart;
+ * rows_out: [m * top_k, d] contiguous, not overlapping x; row_kind
+ * HSMOE_OUT_BF16 or HSMOE_OUT_F32.  Any d up to 2^23 (16-byte aligned rows move in 16-byte
+ * vectors).  Its gradient is hsmoe_moe_combine without weights. */
+int hsmoe_moe_gather(const void* x_dev, int64_t x_row_stride, int64_t m, int64_t d, int row_kind,
+                     const int32_t* offsets_dev, int64_t n_experts, const int32_t* row_of_pair_dev, int top_k,
+                     void* rows_out_dev, hsmoe_stream_t stream);
+
+/* out[t] = sum_j topk_w[t, j] * rows[row_of_pair[t, j]] (+ residual[t]) over the
+ * pairs that have a row, in slot order, summed in fp32 and rounded once; a token
+ * without rows gets zeros (+ residual).  topk_w fp32 [m, top_k] or NULL (weights
+ * 1); rows [n_rows, d], residual and out [m, d] (residual of out's kind, or NULL;
+ * out may be residual).  Row numbers outside [0, n_rows) count as dropped. */
+int hsmoe_moe_combine(const void* rows_dev, int row_kind, int64_t n_rows, int64_t m, int64_t d,
+                      const int32_t* row_of_pair_dev, const float* topk_w_dev, int top_k, const void* residual_dev,
+                      int out_kind, void* out_dev, hsmoe_stream_t stream);
+
+/* The gradient of hsmoe_moe_combine for d_out [m, d] of out_kind:
+ *   d_rows[row_of_pair[t, j]] = topk_w[t, j] * d_out[t]   (rows' kind; rows behind the last: zeros)
+ *   d_w[t, j] = <d_out[t], rows[row_of_pair[t, j]]>       (fp32; 0 for a dropped pair)
+ * d_rows ([m * top_k, d]) or d_w may be NULL (rows may be NULL without d_w);
+ * the residual's gradient is d_out itself.  Deterministic. */
+int hsmoe_moe_combine_grad(const void* d_out_dev, int out_kind, const void* rows_dev, int row_kind, int64_t m,
+                           int64_t d, const int32_t* offsets_dev, int64_t n_experts,
+                           const int32_t* row_of_pair_dev, const float* topk_w_dev, int top_k, void* d_rows_dev,
+                           float* d_w_dev, hsmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * lm_head logits + greedy argmax + longest-prefix draft acceptance.
  * Replaces the logits / acceptance loop of _mtp_verify_batched
  * (reference src/home_seek/inference_engine/engine.py:2480-2497) and the greedy
