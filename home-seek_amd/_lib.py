@@ -19,6 +19,9 @@ DATA_FP4 = 0
 DATA_E4M3 = 1
 OUT_F32 = 0
 OUT_BF16 = 1
+ACT_NONE = 0
+ACT_SILU = 1
+ACT_SWIGLU = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -83,6 +86,16 @@ _SIGNATURES = {
                                  _c_void_p, _c_void_p]),
     "hsmoe_moe_combine_grad": (_int, [_c_void_p, _int, _c_void_p, _int, _i64, _i64, _c_void_p, _i64, _c_void_p,
                                       _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p]),
+    "hsmoe_linear": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64,
+                            _c_void_p, _c_void_p, _c_void_p, _i64, _int, _f32, _int, _c_void_p, _c_void_p,
+                            _c_void_p]),
+    "hsmoe_linear_act_grad_workspace_size": (_size, [_i64, _i64, _i64, _int]),
+    "hsmoe_linear_act_grad": (_int, [_c_void_p, _i64, _c_void_p, _i64, _i64, _int, _f32, _c_void_p, _i64, _c_void_p,
+                                     _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "hsmoe_linear_grad_input": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64,
+                                       _c_void_p, _i64, _c_void_p, _c_void_p]),
+    "hsmoe_linear_grad_weight": (_int, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _int,
+                                        _c_void_p, _c_void_p, _c_void_p]),
     "hsmoe_lm_head_workspace_size": (_size, [_i64, _i64]),
     "hsmoe_lm_head_accept": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p, _c_void_p, _size, _c_void_p]),

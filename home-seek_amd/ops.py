@@ -23,6 +23,7 @@ __all__ = [
     "clear_moe_layer_status", "check_moe_layer_status", "lm_head_accept", "expert_table", "shared_entry",
     "dequant_blocked", "xor_checksum", "MAX_DECODE_TOKENS", "MAX_LAYER_EXPERTS", "embed_add_rms_norm", "mtp_input",
     "decode_step_record", "ExpertOrder", "moe_sort", "moe_gather", "moe_combine", "moe_combine_grad",
+    "linear", "linear_grad", "LinearGrad",
 ]
 
 MAX_DECODE_TOKENS = 8
@@ -406,6 +407,184 @@ def moe_combine_grad(d_out: torch.Tensor, rows: torch.Tensor, order: ExpertOrder
                                            order.n_experts, ptr(order.rows), ptr(topk_w), k, ptr(d_rows), ptr(d_w),
                                            stream_ptr(dev)), "hsmoe_moe_combine_grad")
     return d_rows, d_w
+
+
+_ACTS = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "swiglu": _lib.ACT_SWIGLU}
+
+
+def _act(act: str | None, limit: float | None, w_up: torch.Tensor | None) -> tuple[int, float]:
+    if act not in _ACTS:
+        raise ValueError(f"activation must be None, 'silu' or 'swiglu', got {act!r}")
+    if (act == "swiglu") != (w_up is not None):
+        raise ValueError("an up weight (w_up) goes with act='swiglu', and only with it")
+    if limit is not None and act != "swiglu":
+        raise ValueError("a limit goes with act='swiglu'")
+    limit = float("inf") if limit is None else float(limit)
+    if not limit > 0:
+        raise ValueError("the limit must be positive")
+    return _ACTS[act], limit
+
+
+def _bf16_matrix(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{what} must be bf16, got {t.dtype}")
+    return t
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy where its rows are not 16-byte aligned ones of consecutive elements."""
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for s in t.stride()[:-1]):
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    if t.dim() > 1 and t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]:
+        return t.contiguous()
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return max(t.stride(-2), t.shape[-1]) if t.shape[-2] > 1 else t.shape[-1]
+
+
+def _weights(w: torch.Tensor, w_up: torch.Tensor | None, order: ExpertOrder | None):
+    """(w, w_up, row stride, group stride) of weights [N, K] or, with an order, [E, N, K]."""
+    dims = 2 if order is None else 3
+    for t in (w, w_up):
+        if t is not None and (t.dim() != dims or t.shape != w.shape):
+            raise ValueError(f"weights must be {'[N, K]' if order is None else '[E, N, K]'} tensors of one shape, got "
+                             f"{tuple(t.shape)}")
+    if order is not None and w.shape[0] != order.n_experts:
+        raise ValueError(f"{w.shape[0]} weight matrices for an order of {order.n_experts} experts")
+    w = _rows16(_bf16_matrix(w, "weights"))
+    if w_up is not None:
+        w_up = _rows16(_bf16_matrix(w_up, "weights"))
+        if w_up.stride() != w.stride():
+            w, w_up = w.contiguous(), w_up.contiguous()
+    return w, w_up, _row_stride(w), (w.stride(0) if order is not None else 0)
+
+
+def _linear_rows(x: torch.Tensor, what: str, cols: int, order: ExpertOrder | None) -> torch.Tensor:
+    """x as rows [M, cols] that the kernels can read."""
+    _bf16_matrix(x, what)
+    if x.dim() < 1 or x.shape[-1] != cols:
+        raise ValueError(f"{what} {tuple(x.shape)} does not have rows of {cols}")
+    if order is not None and (x.dim() != 2 or x.shape[0] != order.pairs.numel()):
+        raise ValueError(f"{what} {tuple(x.shape)} does not have the order's {order.pairs.numel()} rows")
+    return _rows16(x if x.dim() == 2 else x.reshape(-1, cols))
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+           act: str | None = None, w_up: torch.Tensor | None = None, bias_up: torch.Tensor | None = None,
+           limit: float | None = None, order: ExpertOrder | None = None, out_dtype: torch.dtype = torch.bfloat16,
+           want_pre: bool = False):
+    """act(x w^T + bias) + residual for bf16 tensors (hsmoe_linear): x [..., K],
+    w [N, K], bias [N], residual [..., N] -> [..., N] bf16 or fp32.
+
+    act: None, "silu", or "swiglu" = silu(min(g, limit)) * clamp(u, -limit, limit)
+    with g from w, bias and u from w_up, bias_up.  With `order` (moe_sort) x and
+    the result are its sorted rows [M * k, .], w is [E, N, K] and bias [E, N], and
+    a row goes through its expert's; the rows behind the last sorted one are zeros.
+    want_pre: -> (result, pre), pre the bf16 sums (with bias) before the
+    activation, [..., N] or [..., 2 N] (gate, up), for linear_grad.
+    N and K must be multiples of 8."""
+    dev = require_cuda(x, w, w_up, bias, bias_up, residual, *(order or ()))
+    code, limit = _act(act, limit, w_up)
+    if order is not None:
+        order.check()
+    w, w_up, ldw, group = _weights(w, w_up, order)
+    n, k = w.shape[-2:]
+    lead = x.shape[:-1]
+    x = _linear_rows(x, "x", k, order)
+    m = x.shape[0]
+    if bias_up is not None and act != "swiglu":
+        raise ValueError("an up bias goes with act='swiglu'")
+    biases = []
+    for b in (bias, bias_up):
+        if b is not None:
+            if b.shape != w.shape[:-1]:
+                raise ValueError(f"bias {tuple(b.shape)} does not match weights {tuple(w.shape)}")
+            b = _bf16_matrix(b, "bias").contiguous()
+            b = b if b.data_ptr() % 16 == 0 else b.clone()
+        biases.append(b)
+    ld_res = n
+    if residual is not None:
+        if residual.shape != lead + (n,):
+            raise ValueError(f"residual {tuple(residual.shape)} does not match the result's {tuple(lead) + (n,)}")
+        residual = _linear_rows(residual, "residual", n, None)
+        ld_res = _row_stride(residual)
+    kind = _row_kind(out_dtype, "the output")
+    out = torch.empty(lead + (n,), dtype=out_dtype, device=dev)
+    pre = torch.empty(lead + (2 * n if act == "swiglu" else n,), dtype=torch.bfloat16, device=dev) if want_pre else None
+    with _on(dev):
+        check(lib().hsmoe_linear(ptr(x), _row_stride(x), m, k, ptr(w), ptr(w_up), ldw, group, n,
+                                 None if order is None else ptr(order.offsets),
+                                 1 if order is None else order.n_experts, ptr(biases[0]), ptr(biases[1]), ptr(residual),
+                                 ld_res, code, limit, kind, ptr(out), ptr(pre), stream_ptr(dev)), "hsmoe_linear")
+    return (out, pre) if want_pre else out
+
+
+class LinearGrad(NamedTuple):
+    """The gradient of linear; None where not needed."""
+    x: torch.Tensor | None
+    w: torch.Tensor | None
+    bias: torch.Tensor | None
+    w_up: torch.Tensor | None
+    bias_up: torch.Tensor | None
+
+
+def linear_grad(d_out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str | None = None,
+                pre: torch.Tensor | None = None, w_up: torch.Tensor | None = None, limit: float | None = None,
+                order: ExpertOrder | None = None, need_x: bool = True, need_w: bool = True, need_bias: bool = False,
+                w_dtype: torch.dtype = torch.bfloat16) -> LinearGrad:
+    """The gradient of linear(x, w, ...) for d_out [..., N] (bf16): x in bf16, the
+    weights in w_dtype (bf16 or fp32), the biases in fp32; the residual's is d_out.
+    pre: what linear(want_pre=True) returned (not needed without an activation).
+    With `order`, an expert without rows has gradient zero, and so have the rows
+    behind the last sorted one (hsmoe_linear_act_grad, _grad_input, _grad_weight)."""
+    dev = require_cuda(d_out, x, w, w_up, pre, *(order or ()))
+    code, limit = _act(act, limit, w_up)
+    if order is not None:
+        order.check()
+    w, w_up, ldw, group = _weights(w, w_up, order)
+    n, k = w.shape[-2:]
+    lead = x.shape[:-1]
+    if d_out.shape != lead + (n,):
+        raise ValueError(f"d_out {tuple(d_out.shape)} does not match the result's {tuple(lead) + (n,)}")
+    x = _linear_rows(x, "x", k, order)
+    d_out = _linear_rows(d_out, "d_out", n, order)
+    m = x.shape[0]
+    mats = 2 if act == "swiglu" else 1
+    kind = _row_kind(w_dtype, "the weights' gradient")
+    off = None if order is None else ptr(order.offsets)
+    groups = 1 if order is None else order.n_experts
+    if act is not None:
+        if pre is None:
+            raise ValueError("the gradient of an activation needs pre (linear(..., want_pre=True))")
+        if pre.shape != lead + (mats * n,):
+            raise ValueError(f"pre {tuple(pre.shape)} must be {tuple(lead) + (mats * n,)}")
+        pre = _linear_rows(pre, "pre", mats * n, None).contiguous()
+    need_dz = act is not None and (need_x or need_w)
+    dz = torch.empty(m, mats * n, dtype=torch.bfloat16, device=dev) if need_dz else d_out
+    db = [None, None]
+    dx = None
+    dw = [None, None]
+    with _on(dev):
+        if need_bias or need_dz:
+            nbytes = lib().hsmoe_linear_act_grad_workspace_size(m, n, groups, code) if need_bias else 0
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
+            if need_bias:
+                db[:mats] = [torch.empty(w.shape[:-1], dtype=torch.float32, device=dev) for _ in range(mats)]
+            check(lib().hsmoe_linear_act_grad(ptr(d_out), _row_stride(d_out), ptr(pre) if act else None, m, n, code, limit,
+                                              off, groups, ptr(dz) if need_dz else None, ptr(db[0]), ptr(db[1]), ptr(ws),
+                                              nbytes, stream_ptr(dev)), "hsmoe_linear_act_grad")
+        if need_x:
+            dx = torch.empty(lead + (k,), dtype=torch.bfloat16, device=dev)
+            check(lib().hsmoe_linear_grad_input(ptr(dz), _row_stride(dz), m, n, ptr(w), ptr(w_up), ldw, group, k, off,
+                                                groups, ptr(dx), stream_ptr(dev)), "hsmoe_linear_grad_input")
+        if need_w:
+            dw[:mats] = [torch.empty(w.shape, dtype=w_dtype, device=dev) for _ in range(mats)]
+            check(lib().hsmoe_linear_grad_weight(ptr(dz), _row_stride(dz), ptr(x), _row_stride(x), m, n, k, off, groups,
+                                                 kind, ptr(dw[0]), ptr(dw[1]), stream_ptr(dev)),
+                  "hsmoe_linear_grad_weight")
+    return LinearGrad(dx, dw[0], db[0], dw[1], db[1])
 
 
 def moe_decode_stage(stage: int, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,

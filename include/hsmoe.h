@@ -353,6 +353,57 @@ int hsmoe_moe_combine_grad(const void* d_out_dev, int out_kind, const void* rows
                            float* d_w_dev, hsmoe_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Matrix product with bias, activation and residual in its epilogue, dense or
+ * with one matrix per group of rows (the experts, over rows sorted by
+ * hsmoe_moe_sort), for bf16 weights.  The reference has torch's linear here
+ * (fused_moe.py:573-598 for the shared expert, one expert at a time in
+ * _forward_legacy fused_moe.py:458-551) and no gradients.
+ *   z[r]   = x[r] w[g]^T + bias[g]                  g: the group of row r
+ *   zu[r]  = x[r] w_up[g]^T + bias_up[g]            (HSMOE_ACT_SWIGLU only)
+ *   y      = z | z sigmoid(z) | min(z, L) sigmoid(min(z, L)) clamp(zu, -L, L)
+ *   out[r] = y + residual[r]
+ * fp32 sums, one rounding.  pre, if given, receives z (and zu beside it, [m, 2 n])
+ * in bf16: what hsmoe_linear_act_grad wants.
+ * x [m, k], w and w_up [n_groups, n, k], bias and bias_up [n_groups, n],
+ * residual [m, n]: bf16, rows row strides apart, matrices w_group_stride apart
+ * (both for w_up too); out [m, n] bf16 or fp32 (out_kind), contiguous.  NULL: no
+ * bias, residual, pre.  offsets int32 [n_groups + 1]: group g is rows offsets[g]
+ * .. offsets[g + 1] - 1; rows from offsets[n_groups] on are zeros (no bias, no
+ * residual); NULL: n_groups = 1, all rows.  limit > 0 (INFINITY: none), read for
+ * swiglu only.  n and k multiples of 8, rows 16-byte aligned, row strides at most
+ * 2^22 - 1, n_groups <= 1024, m < 2^31. */
+#define HSMOE_ACT_NONE 0
+#define HSMOE_ACT_SILU 1
+#define HSMOE_ACT_SWIGLU 2
+int hsmoe_linear(const void* x_dev, int64_t x_row_stride, int64_t m, int64_t k, const void* w_dev,
+                 const void* w_up_dev, int64_t w_row_stride, int64_t w_group_stride, int64_t n,
+                 const int32_t* offsets_dev, int64_t n_groups, const void* bias_dev, const void* bias_up_dev,
+                 const void* residual_dev, int64_t res_row_stride, int act, float limit, int out_kind, void* out_dev,
+                 void* pre_dev, hsmoe_stream_t stream);
+
+/* The gradient of hsmoe_linear in three parts (the residual's is d_out).
+ *   act_grad:    dz = d_out y'(pre) in bf16 ([m, n], or [m, 2 n] for swiglu) and
+ *                d_bias[g] = sum of dz over the rows of g, fp32, from the unrounded
+ *                values.  y' is 0 for what the limit cuts off.  dz, d_bias,
+ *                d_bias_up may be NULL; pre is not read for HSMOE_ACT_NONE
+ *                (there dz is d_out).  Rows of no group are not written.
+ *   grad_input:  dx = dz w (+ dz_up w_up), bf16 [m, k]; rows of no group zeros
+ *   grad_weight: dw[g] = dz^T x over the rows of g, [n_groups, n, k] bf16 or fp32
+ *                (out_kind); a group without rows gets zeros; dw_up with swiglu
+ * Deterministic (no atomics).  Shapes as in hsmoe_linear; m may be 0. */
+size_t hsmoe_linear_act_grad_workspace_size(int64_t m, int64_t n, int64_t n_groups, int act);
+int hsmoe_linear_act_grad(const void* d_out_dev, int64_t d_row_stride, const void* pre_dev, int64_t m, int64_t n,
+                          int act, float limit, const int32_t* offsets_dev, int64_t n_groups, void* dz_dev,
+                          float* d_bias_dev, float* d_bias_up_dev, void* workspace_dev, size_t workspace_bytes,
+                          hsmoe_stream_t stream);
+int hsmoe_linear_grad_input(const void* dz_dev, int64_t dz_row_stride, int64_t m, int64_t n, const void* w_dev,
+                            const void* w_up_dev, int64_t w_row_stride, int64_t w_group_stride, int64_t k,
+                            const int32_t* offsets_dev, int64_t n_groups, void* dx_dev, hsmoe_stream_t stream);
+int hsmoe_linear_grad_weight(const void* dz_dev, int64_t dz_row_stride, const void* x_dev, int64_t x_row_stride,
+                             int64_t m, int64_t n, int64_t k, const int32_t* offsets_dev, int64_t n_groups,
+                             int out_kind, void* dw_dev, void* dw_up_dev, hsmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * lm_head logits + greedy argmax + longest-prefix draft acceptance.
  * Replaces the logits / acceptance loop of _mtp_verify_batched
  * (reference src/home_seek/inference_engine/engine.py:2480-2497) and the greedy
