@@ -30,10 +30,15 @@ HIP_FLAGS = [
     f"-I{CSRC}",
 ]
 
+# Flags of one source.  hsmoe_linear: matrix sums in ordinary registers; left to
+# itself the compiler keeps them in the accumulation file and, in kernels of one
+# wave per SIMD, moves 64 of them back and forth in every pass of the loop.
+SOURCE_FLAGS = {"hsmoe_linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def _compile(src: Path) -> Path:
     obj = OBJ_DIR / (src.stem + ".o")
-    cmd = [HIPCC, *HIP_FLAGS, "-c", str(src), "-o", str(obj)]
+    cmd = [HIPCC, *HIP_FLAGS, *SOURCE_FLAGS.get(src.stem, []), "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed for {src.name}:\n{res.stderr}")

@@ -88,14 +88,16 @@ _SIGNATURES = {
                                       _c_void_p, _int, _c_void_p, _c_void_p, _c_void_p]),
     "hsmoe_linear": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64,
                             _c_void_p, _c_void_p, _c_void_p, _i64, _int, _f32, _int, _c_void_p, _c_void_p,
-                            _c_void_p]),
+                            _c_void_p, _size, _c_void_p]),
+    "hsmoe_linear_workspace_size": (_size, [_i64, _i64, _i64, _i64, _int]),
+    "hsmoe_linear_grad_workspace_size": (_size, [_i64, _i64, _i64, _i64, _int]),
     "hsmoe_linear_act_grad_workspace_size": (_size, [_i64, _i64, _i64, _int]),
     "hsmoe_linear_act_grad": (_int, [_c_void_p, _i64, _c_void_p, _i64, _i64, _int, _f32, _c_void_p, _i64, _c_void_p,
                                      _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_linear_grad_input": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64,
-                                       _c_void_p, _i64, _c_void_p, _c_void_p]),
+                                       _c_void_p, _i64, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_linear_grad_weight": (_int, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _int,
-                                        _c_void_p, _c_void_p, _c_void_p]),
+                                        _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_lm_head_workspace_size": (_size, [_i64, _i64]),
     "hsmoe_lm_head_accept": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p, _c_void_p, _size, _c_void_p]),

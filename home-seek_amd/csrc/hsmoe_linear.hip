@@ -33,44 +33,93 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 }
 
 // ---------------------------------------------------------------- tiles
+// 16 bytes per lane from global memory to LDS, lane l's to dst + 16 l.  Written
+// out because the compiler waits for every such load it knows of before each
+// ds_read_b64_tr_b16, whatever it reads; the waits are reduce_*'s.  No register
+// is written: the load takes its address when it is issued.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void lds_load16(i32x4 r, uint32_t off, const char* dst) {
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)dst;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(at), "v"(off), "s"(r)
+               : "memory", "m0");
+}
+// A resource over `bytes` bytes from base on (both the same in every lane), as make_buf's.
+__device__ __forceinline__ i32x4 lds_buf(const char* base, uint32_t bytes) {
+  const uint64_t b = (uint64_t)base;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)b), __builtin_amdgcn_readfirstlane((int)(b >> 32) & 0xffff),
+               __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000};
+}
+
 // One stage of one operand: kBK reduction steps of kRows rows, bf16.
-//   contiguous  [kRows][64]: 128 bytes per row, its 16-byte chunk c at place c ^ (row & 7)
-//   transposed  [64][kRows]: chunk c of step r at place c ^ 2 f(r), f = (r & 3) + 4 * (r >> 3 & 1)
-// so that the lanes which read together (8 rows of a chunk, or 4 + 4 steps of a
-// 32-byte piece) touch different banks.  The loads write LDS in lane order, so
-// the lane that fills a place loads that place's chunk.
-template <int kRows, int kWaves, bool kTrans>
+//   contiguous  [kRows][kBK]: a row's 16-byte chunk c at place c ^ turn(row)
+//   transposed  [kBK][kRows]: chunk c of step r at place c ^ turn(r)
+// so that the lanes which read together touch different banks.  The loads write
+// LDS in lane order, so the lane that fills a place loads that place's chunk.
+//
+// The matrix instruction hands a lane four results: rows 4 (lane / 16) ..+3 of
+// its first operand, the tile's columns.  kCols: block j of that operand takes
+// its 16 columns such that the lane's four of blocks 2 P and 2 P + 1 are eight
+// in a row (column 32 P + 8 (i / 4) + 4 (j & 1) + i % 4 is row i of block j), so
+// that results leave in 16-byte stores of 64 bytes per output row.
+template <int kRows, int kWaves, bool kTrans, bool kCols, bool kGated>
 struct Operand {
   static constexpr int kBytes = kRows * kBK * 2;
   static constexpr int kLoads = kBytes / 1024 / kWaves;  // 1 KiB instructions per wave and stage
   static_assert(kBytes % (1024 * kWaves) == 0, "every wave loads whole instructions");
+  static_assert(!kTrans || kRows >= 128, "a transposed step has the 16 chunks that turn() permutes");
 
-  // Byte offset of the lane's chunk in load i (wave's), relative to the stage's
-  // first row and step; beyond kFar past `left` reduction steps (an OR, since
-  // the compiler makes divergent branches around the load of a select).
-  static __device__ __forceinline__ uint32_t offset(int i, int wave, int lane, uint32_t ld, int left) {
-    const int q = wave * kLoads + i;
-    if (!kTrans) {
-      const int chunk = (lane & 7) ^ (lane >> 3);
-      return ((uint32_t)(8 * q + (lane >> 3)) * ld + chunk * 16) | past(chunk * 8, left);
-    }
-    constexpr int kPer = kRows / 8;  // chunks per step
-    const int r = q * (64 / kPer) + lane / kPer;
-    const int chunk = (lane % kPer) ^ (2 * ((r & 3) | ((r >> 1) & 4)));
-    return ((uint32_t)r * ld + chunk * 16) | past(r, left);
+  static constexpr bool kTransposed = kTrans;
+
+  // Contiguous: lanes read 16 rows 0-15, or with kCols 0-3, 8-11, 16-19, 24-27
+  // (+ 4).  Transposed: 4 steps r .. r + 3 of one 32-byte piece, or with kCols of
+  // four pieces of 8 bytes 16 apart, in four groups 8 steps apart.
+  static __device__ __forceinline__ int turn(int row) {
+    if (kTrans) return kCols ? (row & 3) << 2 : (row & 3) << 1 | (row & 8);
+    return kCols ? (row & 3) | (row >> 1 & 4) : row & 7;
   }
 
-  // The MFMA operand of 16 rows from row0 on (a multiple of 16), reduction
-  // steps 32 kk + 8 (lane / 16) ..+7.
-  static __device__ __forceinline__ bf16x8 frag(const char* stage, int row0, int kk, int lane) {
+  // Load i of a wave fills 1 KiB of LDS: the lane's row (step, if transposed) and
+  // chunk of it there, and the row that it comes from.
+  static __device__ __forceinline__ int place(int i, int wave, int lane) {
+    const int q = wave * kLoads + i;
+    return kTrans ? q * (512 / kRows) + lane / (kRows / 8) : 8 * q + (lane >> 3);
+  }
+  static __device__ __forceinline__ int chunk(int i, int wave, int lane) {
+    return (kTrans ? lane % (kRows / 8) : lane & 7) ^ turn(place(i, wave, lane));
+  }
+  // kGated: LDS rows are blocks of 16 rows of two matrices in turn.
+  static __device__ __forceinline__ int line(int i, int wave, int lane) {
+    const int r = place(i, wave, lane);
+    return kGated ? (r >> 5) * 16 + (r & 15) : r;
+  }
+  static __device__ __forceinline__ bool second(int i, int wave) { return kGated && ((wave * kLoads + i) >> 1 & 1); }
+
+  // The MFMA operand of block j of a wave whose rows begin at row0 (a multiple
+  // of 32): reduction steps 32 kk + 8 (lane / 16) ..+7 of 16 rows.  kGated:
+  // blocks j and j + 1 are the same columns of both matrices.
+  static __device__ __forceinline__ bf16x8 frag(const char* stage, int row0, int j, int kk, int lane) {
+    const int i = lane & 15;
     if (!kTrans) {
-      const int place = (4 * kk + (lane >> 4)) ^ (lane & 7);
-      return *reinterpret_cast<const bf16x8*>(stage + (row0 + (lane & 15)) * 128 + place * 16);
+      int row = row0 + 16 * j + i;
+      if (kCols && kGated)
+        row = row0 + 64 * (j >> 2) + 16 * (j & 1) + 4 * (j >> 1 & 1) + 32 * (i >> 3) + 8 * (i >> 2 & 1) + (i & 3);
+      else if (kCols)
+        row = row0 + 32 * (j >> 1) + 4 * (j & 1) + 8 * (i >> 2) + (i & 3);
+      const int place = (4 * kk + (lane >> 4)) ^ (kCols ? (i & 7) : turn(i));
+      return *reinterpret_cast<const bf16x8*>(stage + row * (kBK * 2) + place * 16);
     }
-    const int i = lane & 15, f = (i >> 2) | ((lane >> 2) & 4);
-    const char* p = stage + (32 * kk + 8 * (lane >> 4) + (i >> 2)) * (kRows * 2) + (((row0 >> 4) ^ f) << 5) +
-                    (i & 3) * 8;
+    // the 16 lanes of a group address four values each of steps r .. r + 3 and
+    // get four values down one column each
+    const int r = 32 * kk + 8 * (lane >> 4) + (i >> 2);
+    int at;
+    if (kCols)
+      at = (((row0 >> 3) + 4 * (j >> 1) + (i & 3)) ^ turn(r)) * 16 + 8 * (j & 1);
+    else
+      at = ((((row0 >> 3) + 2 * j + (i >> 1 & 1)) ^ turn(r)) * 16) + 8 * (i & 1);
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const char* p = stage + r * (kRows * 2) + at;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * kRows * 2));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -79,49 +128,208 @@ struct Operand {
   }
 };
 
-__device__ __forceinline__ void lds_load16(BufRsrc r, uint32_t off, char* dst) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, (int)off, 0, 0, 0);
-}
+// What a tile reads of one operand, stage by stage: kRows rows of `count`
+// reduction steps, `ld` bytes apart (rows, or steps if transposed).  Reads
+// beyond the rows or the steps that there are give zeros: past the resource's
+// end, or (steps of contiguous rows) by an offset beyond kFar, ORed in since the
+// compiler makes divergent branches around the load of a select.  Stages beyond
+// the last read nothing.
+template <typename Op>
+struct Source {
+  static_assert(Op::kLoads % 2 == 0, "two loads of a wave in turn have the lane's chunk at its two places");
+  const char* base[2];  // the second matrix: kGated
+  uint32_t ld, width;   // width: bytes of a step (transposed), of the whole operand (contiguous)
+  uint32_t at[Op::kLoads];
+  int edge[2];  // contiguous: the first step of the lane's chunk, in even and odd loads
 
-// A resource over what an operand has from `base` on, `bytes` of it.
-__device__ __forceinline__ BufRsrc range(const char* base, int64_t bytes) {
-  return make_buf((uint64_t)base, (uint32_t)imin64(bytes < 0 ? 0 : bytes, kMaxRange));
-}
-
-template <int kBR, int kBC, int kWR, int kWC, bool kTR, bool kTC>
-struct Tile {
-  static constexpr int kWaves = kWR * kWC;
-  static constexpr int kThreads = kWaves * 64;
-  static constexpr int kFR = kBR / kWR / 16, kFC = kBC / kWC / 16;  // 16 x 16 blocks per wave
-  using R = Operand<kBR, kWaves, kTR>;
-  using C = Operand<kBC, kWaves, kTC>;
-  static constexpr int kStage = R::kBytes + C::kBytes;
-
-  // One stage's products.
-  static __device__ __forceinline__ void multiply(const char* stage, int wr, int wc, int lane, f32x4 (&acc)[kFR][kFC]) {
-    const char* cs = stage + R::kBytes;
+  // contiguous: `rows` rows of `bytes` each; transposed: steps of `bytes` each
+  __device__ __forceinline__ void open(const char* p, const char* second, int64_t ld_, int rows, int64_t bytes, int wave,
+                                       int lane) {
+    base[0] = p;
+    base[1] = second;
+    ld = (uint32_t)ld_;
+    width = Op::kTransposed ? (uint32_t)bytes : (uint32_t)(rows - 1) * ld + (uint32_t)bytes;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 c[kFC], r[kFR];
+    for (int i = 0; i < Op::kLoads; ++i)
+      at[i] = (uint32_t)Op::line(i, wave, lane) * ld + (uint32_t)Op::chunk(i, wave, lane) * 16;
+    edge[0] = Op::chunk(0, wave, lane) * 8;
+    edge[1] = Op::chunk(1, wave, lane) * 8;
+  }
+  // Loads kFrom .. kTo - 1 of the stage of steps first ..+63, `left` of them there
+  // (first: times 2 bytes, or ld if transposed, from base).
+  template <int kFrom, int kTo>
+  __device__ __forceinline__ void load(int64_t first, int left, char* stage, int wave) const {
+    if (Op::kTransposed) {
+      const int n = left < kBK ? left : kBK;
+      const i32x4 r = lds_buf(base[0] + first * ld, n > 0 ? (uint32_t)(n - 1) * ld + width : 0u);
 #pragma unroll
-      for (int j = 0; j < kFC; ++j) c[j] = C::frag(cs, wc * kFC * 16 + 16 * j, kk, lane);
+      for (int i = kFrom; i < kTo; ++i) lds_load16(r, at[i], stage + (wave * Op::kLoads + i) * 1024);
+    } else {
+      const uint32_t k = (uint32_t)first * 2, far[2] = {past(edge[0], left), past(edge[1], left)};
 #pragma unroll
-      for (int i = 0; i < kFR; ++i) r[i] = R::frag(stage, wr * kFR * 16 + 16 * i, kk, lane);
-#pragma unroll
-      for (int i = 0; i < kFR; ++i)
-#pragma unroll
-        for (int j = 0; j < kFC; ++j) acc[i][j] = mfma16x16x32(c[j], r[i], acc[i][j]);
+      for (int i = kFrom; i < kTo; ++i) {
+        const i32x4 r = lds_buf(Op::second(i, wave) ? base[1] : base[0], width);
+        lds_load16(r, (at[i] + k) | far[i & 1], stage + (wave * Op::kLoads + i) * 1024);
+      }
     }
   }
 };
 
-// Every wave waits for its own loads (and its LDS reads, whose products may come
-// later), then all meet: the stage that was loaded is whole, and nobody reads
-// the other one any more.
-__device__ __forceinline__ void stage_ready() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
+// Which of a stage's loads: all, the first half, the second half.
+template <int kValue>
+struct Part {
+  static constexpr int value = kValue;
+};
+constexpr Part<-1> kAll;
+constexpr Part<0> kFirst;
+constexpr Part<1> kSecond;
+
+template <int kBR, int kBC, int kWR, int kWC, int kStages_, bool kTR, bool kTC, bool kGated = false>
+struct Tile {
+  static constexpr int kStages = kStages_ == 0 ? 2 : kStages_;
+  static constexpr bool kTurns = kStages_ == 0;
+  static constexpr int kWaves = kWR * kWC;
+  static constexpr int kThreads = kWaves * 64;
+  static constexpr int kFR = kBR / kWR / 16, kFC = kBC / kWC / 16;  // 16 x 16 blocks per wave
+  static_assert(kFC % (kGated ? 4 : 2) == 0, "eight columns in a row per lane");
+  static constexpr bool kRowsTrans = kTR, kColsTrans = kTC;
+  using R = Operand<kBR, kWaves, kTR, false, false>;
+  using C = Operand<kBC, kWaves, kTC, true, kGated>;
+  static constexpr int kStage = R::kBytes + C::kBytes;
+  static constexpr int kLoads = R::kLoads + C::kLoads;  // per wave and stage
+
+  // A stage's loads: all of them (part -1), or either half.
+  template <int kPart>
+  static __device__ __forceinline__ void load(const Source<R>& rs, int64_t r_first, const Source<C>& cs, int64_t c_first,
+                                              int left, char* stage, int wave) {
+    rs.template load<kPart == 1 ? R::kLoads / 2 : 0, kPart == 0 ? R::kLoads / 2 : R::kLoads>(r_first, left, stage, wave);
+    cs.template load<kPart == 1 ? C::kLoads / 2 : 0, kPart == 0 ? C::kLoads / 2 : C::kLoads>(c_first, left,
+                                                                                              stage + R::kBytes, wave);
+  }
+
+  static __device__ __forceinline__ void read(const char* stage, int wr, int wc, int kk, int lane, bf16x8 (&c)[kFC],
+                                              bf16x8 (&r)[kFR]) {
+#pragma unroll
+    for (int j = 0; j < kFC; ++j) c[j] = C::frag(stage + R::kBytes, wc * kFC * 16, j, kk, lane);
+#pragma unroll
+    for (int i = 0; i < kFR; ++i) r[i] = R::frag(stage, wr * kFR * 16, i, kk, lane);
+  }
+  static __device__ __forceinline__ void product(const bf16x8 (&c)[kFC], const bf16x8 (&r)[kFR],
+                                                 f32x4 (&acc)[kFR][kFC]) {
+#pragma unroll
+    for (int i = 0; i < kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < kFC; ++j) acc[i][j] = mfma16x16x32(c[j], r[i], acc[i][j]);
+  }
+  // One stage's products.
+  static __device__ __forceinline__ void multiply(const char* stage, int wr, int wc, int lane, f32x4 (&acc)[kFR][kFC]) {
+#pragma unroll
+    for (int kk = 0; kk < kBK / 32; ++kk) {
+      bf16x8 c[kFC], r[kFR];
+      read(stage, wr, wc, kk, lane, c, r);
+      product(c, r, acc);
+    }
+  }
+};
+
+// The reduction with one wave per SIMD, three stages or more: operands of the next 32
+// reduction steps are read, and half a stage's loads are issued, between the
+// products of the current ones.  A stage's first half is read before the stage
+// before it is done, so the wait and the barrier for it come in mid-stage; the
+// place of the stage that is loaded was read to its end before the last barrier.
+template <typename T, typename Load>
+__device__ __forceinline__ void reduce_ahead(const char* lds, int steps, int wr, int wc, int lane, const Load& load,
+                                             f32x4 (&acc)[T::kFR][T::kFC]) {
+  constexpr int S = T::kStages, kHalf = T::kLoads / 2;
+  static_assert(S >= 3 && T::kLoads % 2 == 0, "a stage is waited for while two others are in use");
+  constexpr int kReads = T::kFC * (T::kColsTrans ? 2 : 1) + T::kFR * (T::kRowsTrans ? 2 : 1);
+  constexpr int kGroups = kHalf, kMfma = T::kFR * T::kFC / kGroups;
+  bf16x8 c[2][T::kFC], r[2][T::kFR];
+  auto wait = [&](bool all) {
+    __builtin_amdgcn_sched_barrier(0);
+    if (all)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 3) * T::kLoads + kHalf) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  };
+  auto mix = [&]() {  // the order of what stands between two barriers
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);                                   // a load
+      __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kGroups - 1) / kGroups, 0);  // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x008, kMfma, 0);                               // products
+    }
+  };
+  if (steps == 0) return;
+  for (int s = 0; s < S - 1; ++s) load(s, s, kAll);
+  wait(true);
+  T::read(lds, wr, wc, 0, lane, c[0], r[0]);
+  int at = 0, next = S - 1;
+  for (int s = 0; s < steps; ++s) {
+    const int after = at + 1 == S ? 0 : at + 1;
+    load(s + S - 1, next, kFirst);
+    T::read(lds + at * T::kStage, wr, wc, 1, lane, c[1], r[1]);
+    T::product(c[0], r[0], acc);
+    mix();
+    wait(false);
+    load(s + S - 1, next, kSecond);
+    T::read(lds + after * T::kStage, wr, wc, 0, lane, c[0], r[0]);
+    T::product(c[1], r[1], acc);
+    mix();
+    at = after;
+    next = next + 1 == S ? 0 : next + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup's end
+}
+
+// The reduction by eight waves of which two share a SIMD (w and w + 4), in turns:
+// one half's waves read a stage's operands and issue the next stage's loads
+// while the other half's multiply, with a barrier between the turns.  The second
+// half is one turn behind.  Turns of one stage, first half / second half:
+//   read 0, load / multiply 1 of the stage before;  multiply 0 / read 0, load;
+//   read 1 / multiply 0;  multiply 1 / read 1
+// so both have read a stage when the first half starts on the next but one,
+// which goes into its place, and a stage's loads have two turns at least
+// between their issue and the wait for them at the end of the last turn.
+template <typename T, typename Load>
+__device__ __forceinline__ void reduce_turns(const char* lds, int steps, int wave, int wr, int wc, int lane,
+                                             const Load& load, f32x4 (&acc)[T::kFR][T::kFC]) {
+  static_assert(T::kWaves == 8 && T::kStages == 2, "two waves per SIMD, two stages");
+  const bool second = wave >= 4;
+  bf16x8 c[T::kFC], r[T::kFR];
+  auto read = [&](int s, int kk) { T::read(lds + (s & 1) * T::kStage, wr, wc, kk, lane, c, r); };
+  auto multiply = [&]() {
+    __builtin_amdgcn_s_setprio(1);
+    T::product(c, r, acc);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto turn = [&](bool loads) {  // ends a turn; loads: the wave's own loads are in LDS
+    if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  };
+  if (steps > 0) load(0, 0, kAll);
+  turn(true);
+  if (second) turn(false);
+  for (int s = 0; s < steps; ++s) {
+    read(s, 0);
+    if (s + 1 < steps) load(s + 1, (s + 1) & 1, kAll);
+    turn(false);
+    multiply();
+    turn(false);
+    read(s, 1);
+    turn(second);
+    multiply();
+    turn(!second);
+  }
+  if (!second) turn(false);
 }
 
 // ---------------------------------------------------------------- groups
@@ -205,6 +413,25 @@ __device__ __forceinline__ bool place_tile(int b, int row_tiles, int col_tiles, 
   return true;
 }
 
+template <typename T, typename Load>
+__device__ __forceinline__ void reduce(const char* lds, int steps, int wave, int wr, int wc, int lane, const Load& load,
+                                       f32x4 (&acc)[T::kFR][T::kFC]) {
+  if constexpr (T::kTurns)
+    reduce_turns<T>(lds, steps, wave, wr, wc, lane, load, acc);
+  else
+    reduce_ahead<T>(lds, steps, wr, wc, lane, load, acc);
+}
+
+// The reduction in `splits` parts: where few tiles would leave CUs idle, that
+// many workgroups share a tile and a join adds their fp32 sums in order.
+struct Steps {
+  int first, count;
+};
+__device__ __forceinline__ Steps part_of(int steps, int splits, int part) {
+  const int per = (steps + splits - 1) / splits, first = part * per;
+  return {first, steps - first < per ? (steps > first ? steps - first : 0) : per};
+}
+
 // ---------------------------------------------------------------- forward
 struct LinearParams {
   const char* x;         // [n_rows] rows of k, ldx bytes apart
@@ -217,151 +444,346 @@ struct LinearParams {
   int64_t n_rows, n, k, ldx, ldw, w_group, ld_res;
   int n_groups, act, out_f32;
   float limit;
+  float* part;  // fp32 [splits][n_rows][n * mats]: the reduction in parts, or NULL
+  int splits;
 };
 
-// From exp(-|z|), which does not overflow: below -88 the result is small, not 0
-// (0 times an infinite up value would be NaN).
+// From t = exp(-z) by the hardware's exp2 and reciprocal (1 ulp each).  A finite
+// exponent stops at 125, so that the result is small there and not 0 (0 times an
+// infinite up value would be NaN); that of -inf is 0.  kFine: the product with log2(e) as a head
+// and what its rounding left, which keeps t good to 3 ulp; without it the error
+// of t is |z| 2^-24, nothing beside the half step of a bf16 result.
+template <bool kFine>
 __device__ __forceinline__ float sigmoid(float z) {
-  const float t = expf(-__builtin_fabsf(z));
-  return (z < 0.0f ? t : 1.0f) / (1.0f + t);
+  const float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629911e-8f;
+  const float h = -z * kLog2e;
+  float t = __builtin_amdgcn_exp2f(h < __builtin_inff() ? __builtin_fminf(h, 125.0f) : h);
+  if (kFine) {
+    const float rest = __builtin_fmaf(-z, kLog2eLow, __builtin_fmaf(-z, kLog2e, -h));  // NaN for infinities: 0.5 then
+    t = __builtin_fmaf(t, __builtin_fminf(rest, 0.5f) * 0.6931471805599453f, t);
+  }
+  return __builtin_amdgcn_rcpf(1.0f + t);
 }
 
 // min / max that hand a NaN on, as torch's clamp does
 __device__ __forceinline__ float clamp_top(float v, float l) { return v > l ? l : v; }
 __device__ __forceinline__ float clamp_both(float v, float l) { return v > l ? l : v < -l ? -l : v; }
 
-__device__ __forceinline__ f32x4 unpack4(uint2 u) {
-  return f32x4{bf16_bits_to_f32(u.x & 0xffffu), __uint_as_float(u.x & 0xffff0000u), bf16_bits_to_f32(u.y & 0xffffu),
-               __uint_as_float(u.y & 0xffff0000u)};
+// Eight values of a row: sums, or what eight bf16 stand for.
+struct Row8 {
+  float v[8];
+};
+__device__ __forceinline__ Row8 row8(f32x4 a, f32x4 b) { return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}}; }
+__device__ __forceinline__ Row8 unpack8(uint4 u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  Row8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : bf16_bits_to_f32(w[i >> 1] & 0xffffu);
+  return r;
 }
-__device__ __forceinline__ uint2 pack4(f32x4 v) {
-  return make_uint2(f32_to_bf16_bits(v[0]) | f32_to_bf16_bits(v[1]) << 16,
-                    f32_to_bf16_bits(v[2]) | f32_to_bf16_bits(v[3]) << 16);
+__device__ __forceinline__ uint4 pack8(const Row8& r) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16_bits(r.v[2 * i]) | f32_to_bf16_bits(r.v[2 * i + 1]) << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 load16(const void* p) { return ldg<uint4>(p); }
+__device__ __forceinline__ void store8(char* base, int64_t at, const Row8& r, bool f32) {
+  if (f32) {
+    float4* o = reinterpret_cast<float4*>(base + at * 4);
+    o[0] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
+    o[1] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(base + at * 2) = pack8(r);
+  }
 }
 
-// Four outputs of row m from column n on: z (and z_up) are the sums.
-__device__ __forceinline__ void finish4(const LinearParams& p, int group, int64_t m, int64_t n, f32x4 z, f32x4 zu) {
-  if (p.bias[0]) z += unpack4(*reinterpret_cast<const uint2*>(p.bias[0] + (group * p.n + n) * 2));
-  if (p.act == HSMOE_ACT_SWIGLU && p.bias[1])
-    zu += unpack4(*reinterpret_cast<const uint2*>(p.bias[1] + (group * p.n + n) * 2));
-  if (p.pre) {
-    const int64_t ldp = p.act == HSMOE_ACT_SWIGLU ? 2 * p.n : p.n;
-    *reinterpret_cast<uint2*>(p.pre + m * ldp + n) = pack4(z);
-    if (p.act == HSMOE_ACT_SWIGLU) *reinterpret_cast<uint2*>(p.pre + m * ldp + p.n + n) = pack4(zu);
-  }
-  f32x4 y = z;
-  if (p.act == HSMOE_ACT_SILU) {
+template <bool kFine>
+__device__ __forceinline__ Row8 activate(const LinearParams& p, const Row8& z, const Row8& zu) {
+  Row8 y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = z[i] * sigmoid(z[i]);
-  } else if (p.act == HSMOE_ACT_SWIGLU) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float g = clamp_top(z[i], p.limit);
-      y[i] = g * sigmoid(g) * clamp_both(zu[i], p.limit);
+  for (int i = 0; i < 8; ++i) {
+    if (p.act == HSMOE_ACT_SILU) {
+      y.v[i] = z.v[i] * sigmoid<kFine>(z.v[i]);
+    } else {
+      const float g = clamp_top(z.v[i], p.limit);
+      y.v[i] = g * sigmoid<kFine>(g) * clamp_both(zu.v[i], p.limit);
     }
   }
-  if (p.residual) y += unpack4(*reinterpret_cast<const uint2*>(p.residual + m * p.ld_res + n * 2));
+  return y;
+}
+
+// Eight outputs of row m from column n on: z (and zu) are the sums with bias.
+__device__ __forceinline__ void finish8(const LinearParams& p, int64_t m, int64_t n, const Row8& z, const Row8& zu,
+                                        uint4 residual) {
+  if (p.pre) {
+    const int64_t ldp = p.act == HSMOE_ACT_SWIGLU ? 2 * p.n : p.n;
+    *reinterpret_cast<uint4*>(p.pre + m * ldp + n) = pack8(z);
+    if (p.act == HSMOE_ACT_SWIGLU) *reinterpret_cast<uint4*>(p.pre + m * ldp + p.n + n) = pack8(zu);
+  }
+  Row8 y = z;
+  if (p.act != HSMOE_ACT_NONE) y = p.out_f32 ? activate<true>(p, z, zu) : activate<false>(p, z, zu);
+  if (p.residual) {
+    const Row8 r = unpack8(residual);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.v[i] += r.v[i];
+  }
+  store8(p.out, m * p.n + n, y, p.out_f32);
+}
+
+// One output; a row of no group gets zeros.
+__device__ __forceinline__ void finish1(const LinearParams& p, int group, int64_t m, int64_t n, float z, float zu) {
+  const bool none = group >= p.n_groups;
+  auto bf = [](const void* q, int64_t at) { return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(q)[at]); };
+  if (!none && p.bias[0]) z += bf(p.bias[0], group * p.n + n);
+  if (!none && p.bias[1]) zu += bf(p.bias[1], group * p.n + n);
+  if (p.pre) {
+    const int64_t at = m * (p.act == HSMOE_ACT_SWIGLU ? 2 * p.n : p.n) + n;
+    p.pre[at] = (uint16_t)f32_to_bf16_bits(z);
+    if (p.act == HSMOE_ACT_SWIGLU) p.pre[at + p.n] = (uint16_t)f32_to_bf16_bits(zu);
+  }
+  float y = z;
+  if (p.act == HSMOE_ACT_SILU) {
+    y = z * sigmoid<true>(z);
+  } else if (p.act == HSMOE_ACT_SWIGLU) {
+    const float g = clamp_top(z, p.limit);
+    y = g * sigmoid<true>(g) * clamp_both(zu, p.limit);
+  }
+  if (!none && p.residual) y += bf(p.residual + m * p.ld_res, n);
   if (p.out_f32)
-    *reinterpret_cast<f32x4*>(p.out + (m * p.n + n) * 4) = y;
+    reinterpret_cast<float*>(p.out)[m * p.n + n] = y;
   else
-    *reinterpret_cast<uint2*>(p.out + (m * p.n + n) * 2) = pack4(y);
+    reinterpret_cast<uint16_t*>(p.out)[m * p.n + n] = (uint16_t)f32_to_bf16_bits(y);
 }
 
 // Rows of no group: zeros.
-__device__ __forceinline__ void clear4(const LinearParams& p, int64_t m, int64_t n) {
-  if (p.out_f32)
-    *reinterpret_cast<f32x4*>(p.out + (m * p.n + n) * 4) = f32x4{};
-  else
-    *reinterpret_cast<uint2*>(p.out + (m * p.n + n) * 2) = make_uint2(0u, 0u);
+__device__ __forceinline__ void clear8(const LinearParams& p, int64_t m, int64_t n) {
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  store8(p.out, m * p.n + n, Row8{}, p.out_f32);
   if (p.pre) {
     const int64_t ldp = p.act == HSMOE_ACT_SWIGLU ? 2 * p.n : p.n;
-    *reinterpret_cast<uint2*>(p.pre + m * ldp + n) = make_uint2(0u, 0u);
-    if (p.act == HSMOE_ACT_SWIGLU) *reinterpret_cast<uint2*>(p.pre + m * ldp + p.n + n) = make_uint2(0u, 0u);
+    *reinterpret_cast<uint4*>(p.pre + m * ldp + n) = zero;
+    if (p.act == HSMOE_ACT_SWIGLU) *reinterpret_cast<uint4*>(p.pre + m * ldp + p.n + n) = zero;
   }
 }
 
 // kGated: the column tile is made of blocks of 16 gate columns and the same 16
 // up columns in turn, so that a lane holds a gate sum and its up sum.
-template <int kBR, int kBC, int kWR, int kWC, bool kGated>
-__global__ void __launch_bounds__(kWR* kWC * 64) linear_kernel(LinearParams p) {
-  using T = Tile<kBR, kBC, kWR, kWC, false, false>;
-  __shared__ __align__(1024) char lds[2][T::kStage];
+template <int kBR, int kBC, int kWR, int kWC, int kStages, bool kGated>
+__global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) linear_kernel(LinearParams p) {
+  using T = Tile<kBR, kBC, kWR, kWC, kStages, false, false, kGated>;
+  __shared__ __align__(1024) char lds[T::kStages * T::kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kCols = kGated ? kBC / 2 : kBC;  // output columns per tile
   const TileScan scan = scan_tiles<kBR>(p.offsets, p.n_groups, p.n_rows, lane);
   int rt, ct;
-  if (!place_tile(blockIdx.x, scan.total, (int)((p.n + kCols - 1) / kCols), rt, ct)) return;
+  const int col_tiles = (int)((p.n + kCols - 1) / kCols);
+  if (!place_tile(blockIdx.x, scan.total, col_tiles * p.splits, rt, ct)) return;
   const Span sp = find_tile<kBR>(scan, rt, p.offsets, p.n_groups, p.n_rows);
-  const int64_t n0 = (int64_t)ct * kCols;
+  const int split = ct / col_tiles;
+  const int64_t n0 = (int64_t)(ct % col_tiles) * kCols;
   const int rows = (int)imin64(kBR, sp.end - sp.row);
   const int cols = (int)imin64(kCols, p.n - n0);
-  if (sp.group >= p.n_groups) {
-    for (int i = threadIdx.x; i < rows * (cols / 4); i += T::kThreads)
-      clear4(p, sp.row + i / (cols / 4), n0 + i % (cols / 4) * 4);
+  if (sp.group >= p.n_groups) {  // (the join clears them)
+    for (int i = p.part ? rows * cols : threadIdx.x; i < rows * (cols / 8); i += T::kThreads)
+      clear8(p, sp.row + i / (cols / 8), n0 + i % (cols / 8) * 8);
     return;
   }
-  const char* xb = p.x + sp.row * p.ldx;
-  const char* wb[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) wb[s] = p.w[kGated ? s : 0] + sp.group * p.w_group + n0 * p.ldw;
-  const int64_t x_bytes = (rows - 1) * p.ldx + p.k * 2, w_bytes = (cols - 1) * p.ldw + p.k * 2;
-  const int steps = (int)((p.k + kBK - 1) / kBK);
-
-  auto load = [&](int s) {
-    char* stage = lds[s & 1];
-    const int64_t at = (int64_t)s * kBK * 2;
-    const int left = (int)imin64(kBK, p.k - (int64_t)s * kBK);
-    const BufRsrc xr = range(xb + at, x_bytes - at);
-#pragma unroll
-    for (int i = 0; i < T::R::kLoads; ++i)
-      lds_load16(xr, T::R::offset(i, wave, lane, (uint32_t)p.ldx, left), stage + (wave * T::R::kLoads + i) * 1024);
-    if (!kGated) {
-      const BufRsrc wr = range(wb[0] + at, w_bytes - at);
-#pragma unroll
-      for (int i = 0; i < T::C::kLoads; ++i)
-        lds_load16(wr, T::C::offset(i, wave, lane, (uint32_t)p.ldw, left),
-                   stage + T::R::kBytes + (wave * T::C::kLoads + i) * 1024);
-    } else {
-      // load q fills LDS rows 8 q ..+7: rows 16 (q / 4) + 8 (q & 1) ..+7 of matrix (q >> 1) & 1
-      const BufRsrc wr[2] = {range(wb[0] + at, w_bytes - at), range(wb[1] + at, w_bytes - at)};
-      const int chunk = (lane & 7) ^ (lane >> 3);
-#pragma unroll
-      for (int i = 0; i < T::C::kLoads; ++i) {
-        const int q = wave * T::C::kLoads + i;
-        const uint32_t row = 16 * (q >> 2) + 8 * (q & 1) + (lane >> 3);
-        const uint32_t off = (row * (uint32_t)p.ldw + chunk * 16) | past(chunk * 8, left);
-        char* dst = stage + T::R::kBytes + q * 1024;
-        if ((q >> 1) & 1) lds_load16(wr[1], off, dst);
-        else lds_load16(wr[0], off, dst);
-      }
-    }
+  const Steps steps = part_of((int)((p.k + kBK - 1) / kBK), p.splits, split);
+  const int64_t wo = sp.group * p.w_group + n0 * p.ldw;
+  Source<typename T::R> xs;
+  xs.open(p.x + sp.row * p.ldx, nullptr, p.ldx, rows, p.k * 2, wave, lane);
+  Source<typename T::C> ws;
+  ws.open(p.w[0] + wo, p.w[1] + wo, p.ldw, cols, p.k * 2, wave, lane);
+  auto load = [&](int s, int slot, auto part) {
+    const int first = (steps.first + s) * kBK;
+    T::template load<decltype(part)::value>(xs, first, ws, first, s < steps.count ? (int)p.k - first : 0,
+                                            lds + slot * T::kStage, wave);
   };
-
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
-  load(0);
-  for (int s = 0; s < steps; ++s) {
-    stage_ready();
-    if (s + 1 < steps) load(s + 1);
-    T::multiply(lds[s & 1], wr, wc, lane, acc);
+  reduce<T>(lds, steps.count, wave, wr, wc, lane, load, acc);
+  if (p.part) {
+    const int64_t width = kGated ? 2 * p.n : p.n;
+    char* base = (char*)(p.part + split * p.n_rows * width);
+#pragma unroll
+    for (int i = 0; i < T::kFR; ++i) {
+      const int r = (wr * T::kFR + i) * 16 + (lane & 15);
+      if (r >= rows) continue;
+#pragma unroll
+      for (int j = 0; j < T::kFC; j += kGated ? 4 : 2) {
+        const int c = (wc * T::kFC + j) * (kGated ? 8 : 16) + 8 * (lane >> 4);
+        if (c >= cols) continue;
+        const int64_t at = (sp.row + r) * width + n0 + c;
+        store8(base, at, kGated ? row8(acc[i][j], acc[i][j + 2]) : row8(acc[i][j], acc[i][j + 1]), true);
+        if (kGated) store8(base, at + p.n, row8(acc[i][j + 1], acc[i][j + 3]), true);
+      }
+    }
+    return;
   }
+  // a lane has kE times eight columns of kFR rows; the next row's residual is on
+  // its way while a row is finished
+  constexpr int kStep = kGated ? 4 : 2, kE = T::kFC / kStep;
+  const int r0 = wr * T::kFR * 16 + (lane & 15), cw = wc * kE * 32 + 8 * (lane >> 4);
+  Row8 bias[2][kE];
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+#pragma unroll
+    for (int s = 0; s < (kGated ? 2 : 1); ++s) {
+      const int64_t at = sp.group * p.n + n0 + cw + 32 * e;
+      bias[s][e] = p.bias[s] && cw + 32 * e < cols ? unpack8(load16(p.bias[s] + at * 2)) : Row8{};
+    }
+  uint4 res[2][kE] = {};
+  auto load_res = [&](int i) {
+    if (p.residual && r0 + 16 * i < rows) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        if (cw + 32 * e < cols)
+          res[i & 1][e] = load16(p.residual + (sp.row + r0 + 16 * i) * p.ld_res + (n0 + cw + 32 * e) * 2);
+    }
+  };
+  load_res(0);
 #pragma unroll
   for (int i = 0; i < T::kFR; ++i) {
-    const int r = (wr * T::kFR + i) * 16 + (lane & 15);
-    if (r >= rows) continue;
-    const int64_t m = sp.row + r;
-    if (kGated) {
+    if (i + 1 < T::kFR) load_res(i + 1);
+    if (r0 + 16 * i >= rows) continue;
 #pragma unroll
-      for (int j = 0; j < T::kFC; j += 2) {
-        const int c = (wc * T::kFC + j) * 8 + 4 * (lane >> 4);
-        if (c < cols) finish4(p, sp.group, m, n0 + c, acc[i][j], acc[i][j + 1]);
-      }
-    } else {
+    for (int e = 0; e < kE; ++e) {
+      if (cw + 32 * e >= cols) continue;
+      Row8 z = kGated ? row8(acc[i][4 * e], acc[i][4 * e + 2]) : row8(acc[i][2 * e], acc[i][2 * e + 1]), zu{};
+      if (kGated) zu = row8(acc[i][4 * e + 1], acc[i][4 * e + 3]);
 #pragma unroll
-      for (int j = 0; j < T::kFC; ++j) {
-        const int c = (wc * T::kFC + j) * 16 + 4 * (lane >> 4);
-        if (c < cols) finish4(p, sp.group, m, n0 + c, acc[i][j], f32x4{});
+      for (int v = 0; v < 8; ++v) {
+        z.v[v] += bias[0][e].v[v];
+        if (kGated) zu.v[v] += bias[1][e].v[v];
       }
+      finish8(p, sp.row + r0 + 16 * i, n0 + cw + 32 * e, z, zu, res[i & 1][e]);
+    }
+  }
+}
+
+__device__ __forceinline__ Row8 load8(const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+// The sum of `splits` values of eight, `stride` apart, in order.
+__device__ __forceinline__ Row8 sum_parts(const float* p, int64_t stride, int splits) {
+  Row8 z = load8(p);
+  for (int s = 1; s < splits; ++s) {
+    const Row8 q = load8(p + s * stride);
+#pragma unroll
+    for (int v = 0; v < 8; ++v) z.v[v] += q.v[v];
+  }
+  return z;
+}
+__device__ __forceinline__ int64_t end_of_groups(const int* offsets, int n_groups, int64_t n_rows) {
+  return offsets ? cut(offsets[n_groups], n_rows) : n_rows;
+}
+
+// The parts of a split reduction added, and the epilogue: eight columns per thread.
+__global__ void __launch_bounds__(256) linear_join_kernel(LinearParams p) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, per = p.n / 8, m = at / per, n = at % per * 8;
+  if (m >= p.n_rows) return;
+  if (m >= end_of_groups(p.offsets, p.n_groups, p.n_rows)) return clear8(p, m, n);
+  const bool gated = p.act == HSMOE_ACT_SWIGLU;
+  const int64_t width = gated ? 2 * p.n : p.n;
+  const float* part = p.part + m * width + n;
+  Row8 z = sum_parts(part, p.n_rows * width, p.splits), zu{};
+  if (gated) zu = sum_parts(part + p.n, p.n_rows * width, p.splits);
+  if (p.bias[0] || p.bias[1]) {
+    int lo = 0;  // the row's group: the last one that begins at or before it
+    for (int hi = p.n_groups; p.offsets && hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (p.offsets[mid] <= m) lo = mid;
+      else hi = mid;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (!p.bias[s]) continue;
+      const Row8 b = unpack8(load16(p.bias[s] + (lo * p.n + n) * 2));
+#pragma unroll
+      for (int v = 0; v < 8; ++v) (s ? zu : z).v[v] += b.v[v];
+    }
+  }
+  finish8(p, m, n, z, zu, p.residual ? load16(p.residual + m * p.ld_res + n * 2) : make_uint4(0u, 0u, 0u, 0u));
+}
+
+// ---------------------------------------------------------------- few rows
+// Up to 16 rows (of a group) against all of w: what counts is w's stream.  A
+// tile is 16 rows of w (kGated: 8 of each matrix), and a workgroup's eight waves
+// share its reduction, a wave's part in batches of kBatch units of 128 steps, 16
+// bytes per lane and load, a batch's loads in flight before its first product.
+// w goes to the matrix cores straight from registers as their first operand; its
+// lanes read 64 bytes of 16 rows per load, a unit's four loads 256 in a row.
+// Two workgroups per CU go through the tiles in turn (one launch of a workgroup
+// per tile costs a quarter more where experts bring thousands of them).
+constexpr int kNarrowRows = 16, kNarrowWaves = 8, kUnit = 128, kBatch = 2;
+
+// bf16 x 8 from p, zeros where !there
+__device__ __forceinline__ bf16x8 load_frag(const char* p, bool there) {
+  const uint4 u = there ? load16(p) : make_uint4(0u, 0u, 0u, 0u);
+  return __builtin_bit_cast(bf16x8, u);
+}
+
+template <bool kGated>
+__global__ void __launch_bounds__(kNarrowWaves * 64) __attribute__((amdgpu_waves_per_eu(4)))
+linear_narrow_kernel(LinearParams p) {
+  constexpr int kCols = kGated ? 8 : 16;
+  __shared__ float s_part[2][kNarrowWaves][kNarrowRows][17];  // [tile's parity][wave][row][row of w], padded
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const TileScan scan = scan_tiles<kNarrowRows>(p.offsets, p.n_groups, p.n_rows, lane);
+  const int col_tiles = (int)((p.n + kCols - 1) / kCols);
+  const int64_t total = (int64_t)scan.total * col_tiles;
+  int turn = 0;
+  for (int64_t tile = blockIdx.x; tile < total; tile += gridDim.x, turn ^= 1) {
+    const int rt = (int)(tile / col_tiles), ct = (int)(tile % col_tiles);
+    const Span sp = find_tile<kNarrowRows>(scan, rt, p.offsets, p.n_groups, p.n_rows);
+    const int rows = (int)imin64(kNarrowRows, sp.end - sp.row);
+    const int64_t n0 = (int64_t)ct * kCols;
+    const int cols = (int)imin64(kCols, p.n - n0);
+    if (sp.group < p.n_groups) {
+      const int i = lane & 15, g = lane >> 4, mat = kGated && i >= 8 ? 1 : 0;
+      const int wrow = kGated ? i & 7 : i;
+      // rows of w beyond the last one read the last one again; their sums go nowhere
+      const char* wp = p.w[mat] + sp.group * p.w_group + (n0 + (wrow < cols ? wrow : cols - 1)) * p.ldw + 16 * g;
+      const char* xp = p.x + (sp.row + i) * p.ldx + 16 * g;
+      const int units = (int)((p.k + kUnit - 1) / kUnit), per = (units + kNarrowWaves - 1) / kNarrowWaves;
+      const int u1 = units < (wave + 1) * per ? units : (wave + 1) * per;
+      f32x4 acc = {};
+      for (int u = wave * per; u < u1; u += kBatch) {
+        bf16x8 w[kBatch][4], x[kBatch][4];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          const int first = (u + b) * kUnit + 8 * g, left = u + b < u1 ? (int)p.k : 0;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const bool there = first + 32 * t < left;
+            const int64_t at = (int64_t)(u + b) * (kUnit * 2) + 64 * t;
+            w[b][t] = load_frag(wp + at, there);
+            x[b][t] = load_frag(xp + at, there && i < rows);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc = mfma16x16x32(w[b][t], x[b][t], acc);
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) s_part[turn][wave][i][4 * g + v] = acc[v];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * kCols; e += kNarrowWaves * 64) {
+      const int r = e / kCols, c = e % kCols;
+      if (c >= cols) continue;
+      float z = 0.0f, zu = 0.0f;
+      if (sp.group < p.n_groups) {
+#pragma unroll
+        for (int w = 0; w < kNarrowWaves; ++w) {
+          z += s_part[turn][w][r][c];
+          if (kGated) zu += s_part[turn][w][r][c + 8];
+        }
+      }
+      finish1(p, sp.group, sp.row + r, n0 + c, z, zu);
     }
   }
 }
@@ -376,121 +798,112 @@ struct LinearGradParams {
   const int* offsets;
   int64_t n_rows, n, k, ldz, ldx, ldw, w_group;
   int n_groups, mats, dw_f32;
+  float* part;  // fp32 [splits][n_rows][k], or [splits][n_groups][mats][n][k]: the reduction in parts, or NULL
+  int splits;
 };
+
+// The sums of a tile to rows row0 .. and columns col0 .. of a matrix of `width`.
+template <typename T>
+__device__ __forceinline__ void store_tile(char* out, int64_t width, int64_t row0, int64_t col0, int rows, int cols,
+                                           bool f32, int wr, int wc, int lane, const f32x4 (&acc)[T::kFR][T::kFC]) {
+  const int r0 = wr * T::kFR * 16 + (lane & 15), cw = wc * T::kFC * 16 + 8 * (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < T::kFR; ++i) {
+    if (r0 + 16 * i >= rows) continue;
+#pragma unroll
+    for (int e = 0; e < T::kFC / 2; ++e)
+      if (cw + 32 * e < cols)
+        store8(out, (row0 + r0 + 16 * i) * width + col0 + cw + 32 * e, row8(acc[i][2 * e], acc[i][2 * e + 1]), f32);
+  }
+}
 
 // dx = dz w (+ dz_up w_up): the reduction runs over the n columns of dz and the
 // rows of w, then over those of up.
-template <int kBR, int kBC, int kWR, int kWC>
-__global__ void __launch_bounds__(kWR* kWC * 64) linear_grad_input_kernel(LinearGradParams p) {
-  using T = Tile<kBR, kBC, kWR, kWC, false, true>;
-  __shared__ __align__(1024) char lds[2][T::kStage];
+template <int kBR, int kBC, int kWR, int kWC, int kStages>
+__global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) linear_grad_input_kernel(LinearGradParams p) {
+  using T = Tile<kBR, kBC, kWR, kWC, kStages, false, true>;
+  __shared__ __align__(1024) char lds[T::kStages * T::kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const TileScan scan = scan_tiles<kBR>(p.offsets, p.n_groups, p.n_rows, lane);
   int rt, ct;
-  if (!place_tile(blockIdx.x, scan.total, (int)((p.k + kBC - 1) / kBC), rt, ct)) return;
+  const int col_tiles = (int)((p.k + kBC - 1) / kBC);
+  if (!place_tile(blockIdx.x, scan.total, col_tiles * p.splits, rt, ct)) return;
   const Span sp = find_tile<kBR>(scan, rt, p.offsets, p.n_groups, p.n_rows);
-  const int64_t c0 = (int64_t)ct * kBC;
+  const int split = ct / col_tiles;
+  const int64_t c0 = (int64_t)(ct % col_tiles) * kBC;
   const int rows = (int)imin64(kBR, sp.end - sp.row), cols = (int)imin64(kBC, p.k - c0);
-  if (sp.group >= p.n_groups) {
-    for (int i = threadIdx.x; i < rows * (cols / 4); i += T::kThreads)
-      *reinterpret_cast<uint2*>(p.dx + ((sp.row + i / (cols / 4)) * p.k + c0 + i % (cols / 4) * 4) * 2) =
-          make_uint2(0u, 0u);
+  if (sp.group >= p.n_groups) {  // (the join clears them)
+    for (int i = p.part ? rows * cols : threadIdx.x; i < rows * (cols / 8); i += T::kThreads)
+      store8(p.dx, (sp.row + i / (cols / 8)) * p.k + c0 + i % (cols / 8) * 8, Row8{}, false);
     return;
   }
-  const int per = (int)((p.n + kBK - 1) / kBK), steps = per * p.mats;
-  auto load = [&](int s) {
-    char* stage = lds[s & 1];
-    const int mat = s >= per ? 1 : 0;
-    const int64_t r0 = (int64_t)(s - mat * per) * kBK;
-    const int left = (int)imin64(kBK, p.n - r0);
-    const int64_t at = (mat * p.n + r0) * 2;
-    const BufRsrc zr = range(p.dz + sp.row * p.ldz + at, (rows - 1) * p.ldz + left * 2);
-#pragma unroll
-    for (int i = 0; i < T::R::kLoads; ++i)
-      lds_load16(zr, T::R::offset(i, wave, lane, (uint32_t)p.ldz, left), stage + (wave * T::R::kLoads + i) * 1024);
-    const BufRsrc wr = range(p.w[mat] + sp.group * p.w_group + r0 * p.ldw + c0 * 2, (left - 1) * p.ldw + cols * 2);
-#pragma unroll
-    for (int i = 0; i < T::C::kLoads; ++i)
-      lds_load16(wr, T::C::offset(i, wave, lane, (uint32_t)p.ldw, left),
-                 stage + T::R::kBytes + (wave * T::C::kLoads + i) * 1024);
+  const int per = (int)((p.n + kBK - 1) / kBK);
+  const Steps steps = part_of(per * p.mats, p.splits, split);
+  Source<typename T::R> zs;
+  zs.open(p.dz + sp.row * p.ldz, nullptr, p.ldz, rows, p.n * p.mats * 2, wave, lane);
+  Source<typename T::C> ws;
+  const int64_t wo = sp.group * p.w_group + c0 * 2;
+  ws.open(p.w[0] + wo, nullptr, p.ldw, 0, cols * 2, wave, lane);
+  auto load = [&](int s, int slot, auto part) {
+    const int step = steps.first + s, mat = step >= per ? 1 : 0, first = (step - mat * per) * kBK;
+    ws.base[0] = (mat ? p.w[1] : p.w[0]) + wo;
+    T::template load<decltype(part)::value>(zs, mat * p.n + first, ws, first, s < steps.count ? (int)p.n - first : 0,
+                                            lds + slot * T::kStage, wave);
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
-  load(0);
-  for (int s = 0; s < steps; ++s) {
-    stage_ready();
-    if (s + 1 < steps) load(s + 1);
-    T::multiply(lds[s & 1], wr, wc, lane, acc);
-  }
-#pragma unroll
-  for (int i = 0; i < T::kFR; ++i) {
-    const int r = (wr * T::kFR + i) * 16 + (lane & 15);
-    if (r >= rows) continue;
-#pragma unroll
-    for (int j = 0; j < T::kFC; ++j) {
-      const int c = (wc * T::kFC + j) * 16 + 4 * (lane >> 4);
-      if (c < cols) *reinterpret_cast<uint2*>(p.dx + ((sp.row + r) * p.k + c0 + c) * 2) = pack4(acc[i][j]);
-    }
-  }
+  reduce<T>(lds, steps.count, wave, wr, wc, lane, load, acc);
+  char* out = p.part ? (char*)(p.part + split * p.n_rows * p.k) : p.dx;
+  store_tile<T>(out, p.k, sp.row, c0, rows, cols, p.part != nullptr, wr, wc, lane, acc);
 }
 
 // dw[g] = dz^T x over the rows of group g: a tile of n x k per workgroup, all
 // groups and both matrices in one launch; a group without rows gets zeros.
-template <int kBR, int kBC, int kWR, int kWC>
-__global__ void __launch_bounds__(kWR* kWC * 64) linear_grad_weight_kernel(LinearGradParams p) {
-  using T = Tile<kBR, kBC, kWR, kWC, true, true>;
-  __shared__ __align__(1024) char lds[2][T::kStage];
+template <int kBR, int kBC, int kWR, int kWC, int kStages>
+__global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) linear_grad_weight_kernel(LinearGradParams p) {
+  using T = Tile<kBR, kBC, kWR, kWC, kStages, true, true>;
+  __shared__ __align__(1024) char lds[T::kStages * T::kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row_tiles = (int)((p.n + kBR - 1) / kBR), col_tiles = (int)((p.k + kBC - 1) / kBC);
   int rt, ct;
-  if (!place_tile(blockIdx.x, p.n_groups * p.mats * row_tiles, col_tiles, rt, ct)) return;
-  const int gm = rt / row_tiles, group = gm / p.mats, mat = gm % p.mats;
-  const int64_t n0 = (int64_t)(rt % row_tiles) * kBR, c0 = (int64_t)ct * kBC;
+  if (!place_tile(blockIdx.x, p.n_groups * p.mats * row_tiles, col_tiles * p.splits, rt, ct)) return;
+  const int gm = rt / row_tiles, group = gm / p.mats, mat = gm % p.mats, split = ct / col_tiles;
+  const int64_t n0 = (int64_t)(rt % row_tiles) * kBR, c0 = (int64_t)(ct % col_tiles) * kBC;
   const int64_t first = p.offsets ? cut(p.offsets[group], p.n_rows) : 0;
   const int64_t end = p.offsets ? cut(p.offsets[group + 1], p.n_rows) : p.n_rows;
   const int64_t count = end > first ? end - first : 0;
   const int nrow = (int)imin64(kBR, p.n - n0), ncol = (int)imin64(kBC, p.k - c0);
-  const char* zb = p.dz + first * p.ldz + (mat * p.n + n0) * 2;
-  const char* xb = p.x + first * p.ldx + c0 * 2;
-  const int steps = (int)((count + kBK - 1) / kBK);
-  auto load = [&](int s) {
-    char* stage = lds[s & 1];
-    const int64_t r0 = (int64_t)s * kBK;
-    const int left = (int)imin64(kBK, count - r0);
-    const BufRsrc zr = range(zb + r0 * p.ldz, (left - 1) * p.ldz + nrow * 2);
-#pragma unroll
-    for (int i = 0; i < T::R::kLoads; ++i)
-      lds_load16(zr, T::R::offset(i, wave, lane, (uint32_t)p.ldz, left), stage + (wave * T::R::kLoads + i) * 1024);
-    const BufRsrc xr = range(xb + r0 * p.ldx, (left - 1) * p.ldx + ncol * 2);
-#pragma unroll
-    for (int i = 0; i < T::C::kLoads; ++i)
-      lds_load16(xr, T::C::offset(i, wave, lane, (uint32_t)p.ldx, left),
-                 stage + T::R::kBytes + (wave * T::C::kLoads + i) * 1024);
+  const Steps steps = part_of((int)((count + kBK - 1) / kBK), p.splits, split);
+  Source<typename T::R> zs;
+  zs.open(p.dz + first * p.ldz + (mat * p.n + n0) * 2, nullptr, p.ldz, 0, nrow * 2, wave, lane);
+  Source<typename T::C> xs;
+  xs.open(p.x + first * p.ldx + c0 * 2, nullptr, p.ldx, 0, ncol * 2, wave, lane);
+  auto load = [&](int s, int slot, auto part) {
+    const int first_step = (steps.first + s) * kBK;
+    T::template load<decltype(part)::value>(zs, first_step, xs, first_step, s < steps.count ? (int)count - first_step : 0,
+                                            lds + slot * T::kStage, wave);
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
-  if (steps > 0) load(0);
-  for (int s = 0; s < steps; ++s) {
-    stage_ready();
-    if (s + 1 < steps) load(s + 1);
-    T::multiply(lds[s & 1], wr, wc, lane, acc);
-  }
-  const int es = p.dw_f32 ? 4 : 2;
-  char* ob = p.dw[mat] + (int64_t)group * p.n * p.k * es;
-#pragma unroll
-  for (int i = 0; i < T::kFR; ++i) {
-    const int r = (wr * T::kFR + i) * 16 + (lane & 15);
-    if (r >= nrow) continue;
-#pragma unroll
-    for (int j = 0; j < T::kFC; ++j) {
-      const int c = (wc * T::kFC + j) * 16 + 4 * (lane >> 4);
-      if (c >= ncol) continue;
-      char* o = ob + ((n0 + r) * p.k + c0 + c) * es;
-      if (p.dw_f32)
-        *reinterpret_cast<f32x4*>(o) = acc[i][j];
-      else
-        *reinterpret_cast<uint2*>(o) = pack4(acc[i][j]);
-    }
+  reduce<T>(lds, steps.count, wave, wr, wc, lane, load, acc);
+  const bool f32 = p.part || p.dw_f32;
+  char* out = p.part ? (char*)(p.part + ((int64_t)split * p.n_groups * p.mats + gm) * p.n * p.k)
+                     : p.dw[mat] + (int64_t)group * p.n * p.k * (f32 ? 4 : 2);
+  store_tile<T>(out, p.k, n0, c0, nrow, ncol, f32, wr, wc, lane, acc);
+}
+
+// The parts of a split reduction added: kWeight: dw (and dw_up), else dx.
+template <bool kWeight>
+__global__ void __launch_bounds__(256) linear_grad_join_kernel(LinearGradParams p) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  const int64_t total = (kWeight ? (int64_t)p.n_groups * p.mats * p.n : p.n_rows) * p.k;
+  if (at >= total) return;
+  if (kWeight) {
+    const int64_t size = p.n * p.k, gm = at / size;
+    store8(p.dw[gm % p.mats], gm / p.mats * size + at % size, sum_parts(p.part + at, total, p.splits), p.dw_f32);
+  } else {
+    const bool none = at / p.k >= end_of_groups(p.offsets, p.n_groups, p.n_rows);
+    store8(p.dx, at, none ? Row8{} : sum_parts(p.part + at, total, p.splits), false);
   }
 }
 
@@ -543,11 +956,11 @@ __global__ void __launch_bounds__(kActThreads) act_grad_kernel(ActGradParams p) 
         o[0] = d;
         if (kMats == 2) {
           const float z = half(pw[0][i >> 1]), zu = half(pw[kMats - 1][i >> 1]);
-          const float g = clamp_top(z, p.limit), s = sigmoid(g);
+          const float g = clamp_top(z, p.limit), s = sigmoid<true>(g);
           o[0] = z > p.limit ? 0.0f : d * clamp_both(zu, p.limit) * (s + g * s * (1.0f - s));
           o[kMats - 1] = zu > p.limit || zu < -p.limit ? 0.0f : d * (g * s);
         } else if (p.act == HSMOE_ACT_SILU) {
-          const float z = half(pw[0][i >> 1]), s = sigmoid(z);
+          const float z = half(pw[0][i >> 1]), s = sigmoid<true>(z);
           o[0] = d * (s + z * s * (1.0f - s));
         }
 #pragma unroll
@@ -610,7 +1023,8 @@ int check_counts(const char* what, int64_t m, int64_t n, int64_t k, int64_t n_gr
   if (n_groups > kMaxGroups) return fail(HSMOE_ERR_SHAPE, "%s: at most %d groups", what, kMaxGroups);
   if (!offsets && n_groups != 1) return fail(HSMOE_ERR_ARG, "%s: groups need their offsets", what);
   if (n % 8 != 0 || k % 8 != 0) return fail(HSMOE_ERR_SHAPE, "%s: n and k must be multiples of 8", what);
-  if (m > INT32_MAX) return fail(HSMOE_ERR_SHAPE, "%s: m must be below 2^31", what);
+  // (steps are counted in 32 bits, up to four stages beyond the last one)
+  if (m > INT32_MAX - 1024) return fail(HSMOE_ERR_SHAPE, "%s: m must be below 2^31 - 1024", what);
   if (offsets && !aligned(offsets, 4)) return fail(HSMOE_ERR_SHAPE, "%s: misaligned offsets", what);
   return HSMOE_OK;
 }
@@ -634,39 +1048,125 @@ unsigned tile_grid(int64_t row_tiles, int64_t cols, int bc) {
   return total > (1 << 22) - 8 ? 0 : (unsigned)((total + 7) / 8 * 8);
 }
 
-// Whether tiles of 256 x 256 still give every CU one (rows and cols of the
-// output, in `groups` of equal size).
-bool big_tiles(int64_t rows, int64_t cols, int64_t groups) {
-  const int64_t per = (rows + groups - 1) / groups;
-  return per > 128 && groups * ((per + 255) / 256) * ((cols + 255) / 256) >= device_cus();
+// How a product is done: the tile, and the parts of its reduction.
+struct Plan {
+  int tile;  // kNarrow or an index into kTiles
+  int splits;
+  size_t bytes;  // of the parts
+};
+constexpr int kNarrow = -1;
+
+// The tiles, with what a workgroup takes for 64 reduction steps and for the rest
+// (first loads, epilogue), in us, as measured with every CU at work:
+//   256 x 256, turns of eight waves    1.30 + 14
+//   128 x 128, four waves, 4 stages    0.62 + 7
+//   64 x 128, four waves, 4 stages     0.44 + 5
+// The tile and the number of parts with the least time by these figures are
+// taken; parts cost the fp32 sums' way to memory and back and a launch.
+struct TileCost {
+  int rows, cols;
+  double step, rest;
+};
+constexpr TileCost kTiles[] = {{256, 256, 1.30, 14.0}, {128, 128, 0.62, 7.0}, {64, 128, 0.44, 5.0}};
+
+// rows: of the output, in `groups` groups of which at most `active` have any;
+// cols: tiles' columns (twice the output's for swiglu); sums: fp32 values of one part.
+Plan plan_tiles(double rows, double active, double groups, int64_t cols, int64_t steps, double sums, int n_tiles) {
+  const double cus = device_cus();
+  Plan best{0, 1, 0};
+  double least = 1e30;
+  for (int t = 0; t < n_tiles; ++t) {
+    const TileCost& c = kTiles[t];
+    double row_tiles = groups == 1 ? __builtin_ceil(rows / c.rows) : rows / c.rows + 0.5 * active;
+    if (row_tiles < active) row_tiles = active;
+    const double tiles = row_tiles * (double)((cols + c.cols - 1) / c.cols);
+    for (int s = 1; s <= 16; s *= 2) {
+      const int64_t per = (steps + s - 1) / s;
+      if (s > 1 && (per < 4 || (steps + per - 1) / per != s)) continue;
+      double us = __builtin_ceil(tiles * s / cus) * (per * c.step + c.rest);
+      if (s > 1) us += 4.0 + s * sums * 8.0 / 5e6;
+      if (us < least) {
+        least = us;
+        best = {t, s, s > 1 ? (size_t)(s * sums * 4.0) : 0};
+      }
+    }
+  }
+  return best;
 }
 
-template <int kBR, int kBC, int kWR, int kWC>
+// Up to 16 rows per group on average: the kernel that streams w.
+Plan plan_linear(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
+  const int64_t active = n_groups < m ? n_groups : m, mats = act == HSMOE_ACT_SWIGLU ? 2 : 1;
+  if (m <= 16 * active) return {kNarrow, 1, 0};
+  return plan_tiles((double)m, (double)active, (double)n_groups, n * mats, (k + kBK - 1) / kBK, (double)m * n * mats, 3);
+}
+Plan plan_grad_input(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
+  const int64_t active = n_groups < m ? n_groups : m;
+  return plan_tiles((double)m, (double)active, (double)n_groups, k, (n + kBK - 1) / kBK * mats, (double)m * k, 3);
+}
+// (both operands transposed: no tile of 64 rows)
+Plan plan_grad_weight(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
+  const double groups = (double)n_groups * mats, sums = groups * n * k;
+  const int64_t rows = (m + n_groups - 1) / n_groups;
+  Plan p = plan_tiles((double)n, 1, 1, k * n_groups * mats, (rows + kBK - 1) / kBK, sums, 2);
+  return p;
+}
+
+int check_workspace(const char* what, const Plan& plan, const void* ws, size_t bytes) {
+  if (!plan.bytes) return HSMOE_OK;
+  if (!ws || bytes < plan.bytes) return fail(HSMOE_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, plan.bytes);
+  if (!aligned(ws, 16)) return fail(HSMOE_ERR_SHAPE, "%s: the workspace must be 16-byte aligned", what);
+  return HSMOE_OK;
+}
+
+unsigned join_grid(int64_t values) { return (unsigned)((values / 8 + 255) / 256); }
+
+template <int kBR, int kBC, int kWR, int kWC, int kStages>
 int launch_linear(const LinearParams& p, hipStream_t st) {
   const bool gated = p.act == HSMOE_ACT_SWIGLU;
-  const unsigned grid = tile_grid(max_row_tiles(p.n_rows, kBR, p.offsets, p.n_groups), p.n, gated ? kBC / 2 : kBC);
+  const int64_t row_tiles = max_row_tiles(p.n_rows, kBR, p.offsets, p.n_groups) * p.splits;
+  const unsigned grid = tile_grid(row_tiles, p.n, gated ? kBC / 2 : kBC);
   if (!grid) return fail(HSMOE_ERR_SHAPE, "hsmoe_linear: too many tiles");
   const dim3 block(kWR * kWC * 64);
   if (gated)
-    hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, true>), dim3(grid), block, 0, st, p);
+    hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, kStages, true>), dim3(grid), block, 0, st, p);
   else
-    hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, false>), dim3(grid), block, 0, st, p);
+    hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, kStages, false>), dim3(grid), block, 0, st, p);
+  if (p.part) hipLaunchKernelGGL(linear_join_kernel, dim3(join_grid(p.n_rows * p.n)), dim3(256), 0, st, p);
   return check_launch("hsmoe_linear");
 }
 
-template <int kBR, int kBC, int kWR, int kWC>
+int launch_narrow(const LinearParams& p, hipStream_t st) {
+  const bool gated = p.act == HSMOE_ACT_SWIGLU;
+  const int64_t tiles = max_row_tiles(p.n_rows, kNarrowRows, p.offsets, p.n_groups), cols = gated ? 8 : 16;
+  int64_t grid = tiles * ((p.n + cols - 1) / cols), most = 2 * device_cus();  // what the chip holds at once
+  if (grid > most) grid = most;
+  const dim3 block(kNarrowWaves * 64);
+  if (gated)
+    hipLaunchKernelGGL(linear_narrow_kernel<true>, dim3((unsigned)grid), block, 0, st, p);
+  else
+    hipLaunchKernelGGL(linear_narrow_kernel<false>, dim3((unsigned)grid), block, 0, st, p);
+  return check_launch("hsmoe_linear");
+}
+
+template <int kBR, int kBC, int kWR, int kWC, int kStages>
 int launch_grad_input(const LinearGradParams& p, hipStream_t st) {
-  const unsigned grid = tile_grid(max_row_tiles(p.n_rows, kBR, p.offsets, p.n_groups), p.k, kBC);
+  const unsigned grid = tile_grid(max_row_tiles(p.n_rows, kBR, p.offsets, p.n_groups) * p.splits, p.k, kBC);
   if (!grid) return fail(HSMOE_ERR_SHAPE, "hsmoe_linear_grad_input: too many tiles");
-  hipLaunchKernelGGL((linear_grad_input_kernel<kBR, kBC, kWR, kWC>), dim3(grid), dim3(kWR * kWC * 64), 0, st, p);
+  hipLaunchKernelGGL((linear_grad_input_kernel<kBR, kBC, kWR, kWC, kStages>), dim3(grid), dim3(kWR * kWC * 64), 0, st, p);
+  if (p.part)
+    hipLaunchKernelGGL(linear_grad_join_kernel<false>, dim3(join_grid(p.n_rows * p.k)), dim3(256), 0, st, p);
   return check_launch("hsmoe_linear_grad_input");
 }
 
-template <int kBR, int kBC, int kWR, int kWC>
+template <int kBR, int kBC, int kWR, int kWC, int kStages>
 int launch_grad_weight(const LinearGradParams& p, hipStream_t st) {
-  const unsigned grid = tile_grid((p.n + kBR - 1) / kBR * p.n_groups * p.mats, p.k, kBC);
+  const int64_t groups = (int64_t)p.n_groups * p.mats;
+  const unsigned grid = tile_grid((p.n + kBR - 1) / kBR * groups * p.splits, p.k, kBC);
   if (!grid) return fail(HSMOE_ERR_SHAPE, "hsmoe_linear_grad_weight: too many tiles");
-  hipLaunchKernelGGL((linear_grad_weight_kernel<kBR, kBC, kWR, kWC>), dim3(grid), dim3(kWR * kWC * 64), 0, st, p);
+  hipLaunchKernelGGL((linear_grad_weight_kernel<kBR, kBC, kWR, kWC, kStages>), dim3(grid), dim3(kWR * kWC * 64), 0, st, p);
+  if (p.part)
+    hipLaunchKernelGGL(linear_grad_join_kernel<true>, dim3(join_grid(groups * p.n * p.k)), dim3(256), 0, st, p);
   return check_launch("hsmoe_linear_grad_weight");
 }
 
@@ -684,11 +1184,15 @@ int act_shares(int64_t m, int64_t n, int64_t n_groups) {
 
 using namespace hsmoe;
 
+extern "C" size_t hsmoe_linear_workspace_size(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
+  return m < 1 || n < 1 || k < 1 || n_groups < 1 ? 0 : plan_linear(m, n, k, n_groups, act).bytes;
+}
+
 extern "C" int hsmoe_linear(const void* x, int64_t x_row_stride, int64_t m, int64_t k, const void* w, const void* w_up,
                             int64_t w_row_stride, int64_t w_group_stride, int64_t n, const int32_t* offsets,
                             int64_t n_groups, const void* bias, const void* bias_up, const void* residual,
                             int64_t res_row_stride, int act, float limit, int out_kind, void* out, void* pre,
-                            hsmoe_stream_t stream) {
+                            void* workspace, size_t workspace_bytes, hsmoe_stream_t stream) {
   if (int rc = check_counts("hsmoe_linear", m, n, k, n_groups, offsets)) return rc;
   if (act != HSMOE_ACT_NONE && act != HSMOE_ACT_SILU && act != HSMOE_ACT_SWIGLU)
     return fail(HSMOE_ERR_ARG, "hsmoe_linear: bad activation %d", act);
@@ -723,8 +1227,14 @@ extern "C" int hsmoe_linear(const void* x, int64_t x_row_stride, int64_t m, int6
   p.n_rows = m, p.n = n, p.k = k;
   p.ldx = x_row_stride * 2, p.ldw = w_row_stride * 2, p.w_group = w_group_stride * 2, p.ld_res = res_row_stride * 2;
   p.n_groups = (int)n_groups, p.act = act, p.out_f32 = out_kind == HSMOE_OUT_F32, p.limit = limit;
-  if (big_tiles(m, gated ? 2 * n : n, n_groups)) return launch_linear<256, 256, 2, 4>(p, (hipStream_t)stream);
-  return launch_linear<128, 128, 2, 2>(p, (hipStream_t)stream);
+  const Plan plan = plan_linear(m, n, k, n_groups, act);
+  if (int rc = check_workspace("hsmoe_linear", plan, workspace, workspace_bytes)) return rc;
+  p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (plan.tile == kNarrow) return launch_narrow(p, st);
+  if (plan.tile == 0) return launch_linear<256, 256, 2, 4, 0>(p, st);
+  if (plan.tile == 1) return launch_linear<128, 128, 2, 2, 4>(p, st);
+  return launch_linear<64, 128, 2, 2, 4>(p, st);
 }
 
 extern "C" size_t hsmoe_linear_act_grad_workspace_size(int64_t m, int64_t n, int64_t n_groups, int act) {
@@ -778,9 +1288,17 @@ extern "C" int hsmoe_linear_act_grad(const void* d_out, int64_t d_row_stride, co
   return check_launch("hsmoe_linear_act_grad");
 }
 
+extern "C" size_t hsmoe_linear_grad_workspace_size(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
+  if (m < 1 || n < 1 || k < 1 || n_groups < 1) return 0;
+  const int mats = act == HSMOE_ACT_SWIGLU ? 2 : 1;
+  const size_t a = plan_grad_input(m, n, k, n_groups, mats).bytes, b = plan_grad_weight(m, n, k, n_groups, mats).bytes;
+  return a > b ? a : b;
+}
+
 extern "C" int hsmoe_linear_grad_input(const void* dz, int64_t dz_row_stride, int64_t m, int64_t n, const void* w,
                                        const void* w_up, int64_t w_row_stride, int64_t w_group_stride, int64_t k,
-                                       const int32_t* offsets, int64_t n_groups, void* dx, hsmoe_stream_t stream) {
+                                       const int32_t* offsets, int64_t n_groups, void* dx, void* workspace,
+                                       size_t workspace_bytes, hsmoe_stream_t stream) {
   if (int rc = check_counts("hsmoe_linear_grad_input", m, n, k, n_groups, offsets)) return rc;
   if (m == 0) return HSMOE_OK;
   const int mats = w_up ? 2 : 1;
@@ -799,13 +1317,19 @@ extern "C" int hsmoe_linear_grad_input(const void* dz, int64_t dz_row_stride, in
   p.n_rows = m, p.n = n, p.k = k;
   p.ldz = dz_row_stride * 2, p.ldw = w_row_stride * 2, p.w_group = w_group_stride * 2;
   p.n_groups = (int)n_groups, p.mats = mats;
-  if (big_tiles(m, k, n_groups)) return launch_grad_input<256, 256, 2, 4>(p, (hipStream_t)stream);
-  return launch_grad_input<128, 128, 2, 2>(p, (hipStream_t)stream);
+  const Plan plan = plan_grad_input(m, n, k, n_groups, mats);
+  if (int rc = check_workspace("hsmoe_linear_grad_input", plan, workspace, workspace_bytes)) return rc;
+  p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (plan.tile == 0) return launch_grad_input<256, 256, 2, 4, 0>(p, st);
+  if (plan.tile == 1) return launch_grad_input<128, 128, 2, 2, 4>(p, st);
+  return launch_grad_input<64, 128, 2, 2, 4>(p, st);
 }
 
 extern "C" int hsmoe_linear_grad_weight(const void* dz, int64_t dz_row_stride, const void* x, int64_t x_row_stride,
                                         int64_t m, int64_t n, int64_t k, const int32_t* offsets, int64_t n_groups,
-                                        int out_kind, void* dw, void* dw_up, hsmoe_stream_t stream) {
+                                        int out_kind, void* dw, void* dw_up, void* workspace, size_t workspace_bytes,
+                                        hsmoe_stream_t stream) {
   if (int rc = check_counts("hsmoe_linear_grad_weight", m, n, k, n_groups, offsets)) return rc;
   if (out_kind != HSMOE_OUT_F32 && out_kind != HSMOE_OUT_BF16)
     return fail(HSMOE_ERR_ARG, "hsmoe_linear_grad_weight: bad output kind %d", out_kind);
@@ -824,6 +1348,10 @@ extern "C" int hsmoe_linear_grad_weight(const void* dz, int64_t dz_row_stride, c
   p.n_rows = m, p.n = n, p.k = k;
   p.ldz = dz_row_stride * 2, p.ldx = x_row_stride * 2;
   p.n_groups = (int)n_groups, p.mats = mats, p.dw_f32 = out_kind == HSMOE_OUT_F32;
-  if (big_tiles(n * n_groups * mats, k, n_groups * mats)) return launch_grad_weight<256, 256, 2, 4>(p, (hipStream_t)stream);
-  return launch_grad_weight<128, 128, 2, 2>(p, (hipStream_t)stream);
+  const Plan plan = plan_grad_weight(m > 0 ? m : 1, n, k, n_groups, mats);
+  if (int rc = check_workspace("hsmoe_linear_grad_weight", plan, workspace, workspace_bytes)) return rc;
+  p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  if (plan.tile == 0) return launch_grad_weight<256, 256, 2, 4, 0>(p, st);
+  return launch_grad_weight<128, 128, 2, 2, 4>(p, st);
 }

@@ -514,10 +514,13 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
     out = torch.empty(lead + (n,), dtype=out_dtype, device=dev)
     pre = torch.empty(lead + (2 * n if act == "swiglu" else n,), dtype=torch.bfloat16, device=dev) if want_pre else None
     with _on(dev):
+        nbytes = lib().hsmoe_linear_workspace_size(m, n, k, 1 if order is None else order.n_experts, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
         check(lib().hsmoe_linear(ptr(x), _row_stride(x), m, k, ptr(w), ptr(w_up), ldw, group, n,
                                  None if order is None else ptr(order.offsets),
                                  1 if order is None else order.n_experts, ptr(biases[0]), ptr(biases[1]), ptr(residual),
-                                 ld_res, code, limit, kind, ptr(out), ptr(pre), stream_ptr(dev)), "hsmoe_linear")
+                                 ld_res, code, limit, kind, ptr(out), ptr(pre), ptr(ws), nbytes, stream_ptr(dev)),
+              "hsmoe_linear")
     return (out, pre) if want_pre else out
 
 
@@ -575,14 +578,17 @@ def linear_grad(d_out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str 
             check(lib().hsmoe_linear_act_grad(ptr(d_out), _row_stride(d_out), ptr(pre) if act else None, m, n, code, limit,
                                               off, groups, ptr(dz) if need_dz else None, ptr(db[0]), ptr(db[1]), ptr(ws),
                                               nbytes, stream_ptr(dev)), "hsmoe_linear_act_grad")
+        nbytes = lib().hsmoe_linear_grad_workspace_size(m, n, k, groups, code) if need_x or need_w else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # one product after the other
         if need_x:
             dx = torch.empty(lead + (k,), dtype=torch.bfloat16, device=dev)
             check(lib().hsmoe_linear_grad_input(ptr(dz), _row_stride(dz), m, n, ptr(w), ptr(w_up), ldw, group, k, off,
-                                                groups, ptr(dx), stream_ptr(dev)), "hsmoe_linear_grad_input")
+                                                groups, ptr(dx), ptr(ws), nbytes, stream_ptr(dev)),
+                  "hsmoe_linear_grad_input")
         if need_w:
             dw[:mats] = [torch.empty(w.shape, dtype=w_dtype, device=dev) for _ in range(mats)]
             check(lib().hsmoe_linear_grad_weight(ptr(dz), _row_stride(dz), ptr(x), _row_stride(x), m, n, k, off, groups,
-                                                 kind, ptr(dw[0]), ptr(dw[1]), stream_ptr(dev)),
+                                                 kind, ptr(dw[0]), ptr(dw[1]), ptr(ws), nbytes, stream_ptr(dev)),
                   "hsmoe_linear_grad_weight")
     return LinearGrad(dx, dw[0], db[0], dw[1], db[1])
 

@@ -370,16 +370,19 @@ int hsmoe_moe_combine_grad(const void* d_out_dev, int out_kind, const void* rows
  * bias, residual, pre.  offsets int32 [n_groups + 1]: group g is rows offsets[g]
  * .. offsets[g + 1] - 1; rows from offsets[n_groups] on are zeros (no bias, no
  * residual); NULL: n_groups = 1, all rows.  limit > 0 (INFINITY: none), read for
- * swiglu only.  n and k multiples of 8, rows 16-byte aligned, row strides at most
- * 2^22 - 1, n_groups <= 1024, m < 2^31. */
+ * swiglu only.  n and k multiples of 8, rows 16-byte aligned, row strides below
+ * 2^22, n_groups <= 1024, m < 2^31 - 1024.  Few rows: the reduction may be shared
+ * by several workgroups per tile, whose sums go through the workspace (any
+ * contents; hsmoe_linear_workspace_size bytes, 0 for most shapes). */
 #define HSMOE_ACT_NONE 0
 #define HSMOE_ACT_SILU 1
 #define HSMOE_ACT_SWIGLU 2
+size_t hsmoe_linear_workspace_size(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act);
 int hsmoe_linear(const void* x_dev, int64_t x_row_stride, int64_t m, int64_t k, const void* w_dev,
                  const void* w_up_dev, int64_t w_row_stride, int64_t w_group_stride, int64_t n,
                  const int32_t* offsets_dev, int64_t n_groups, const void* bias_dev, const void* bias_up_dev,
                  const void* residual_dev, int64_t res_row_stride, int act, float limit, int out_kind, void* out_dev,
-                 void* pre_dev, hsmoe_stream_t stream);
+                 void* pre_dev, void* workspace_dev, size_t workspace_bytes, hsmoe_stream_t stream);
 
 /* The gradient of hsmoe_linear in three parts (the residual's is d_out).
  *   act_grad:    dz = d_out y'(pre) in bf16 ([m, n], or [m, 2 n] for swiglu) and
@@ -390,18 +393,22 @@ int hsmoe_linear(const void* x_dev, int64_t x_row_stride, int64_t m, int64_t k, 
  *   grad_input:  dx = dz w (+ dz_up w_up), bf16 [m, k]; rows of no group zeros
  *   grad_weight: dw[g] = dz^T x over the rows of g, [n_groups, n, k] bf16 or fp32
  *                (out_kind); a group without rows gets zeros; dw_up with swiglu
- * Deterministic (no atomics).  Shapes as in hsmoe_linear; m may be 0. */
+ * Deterministic (no atomics).  Shapes as in hsmoe_linear; m may be 0.  The two
+ * products take a workspace of hsmoe_linear_grad_workspace_size bytes. */
 size_t hsmoe_linear_act_grad_workspace_size(int64_t m, int64_t n, int64_t n_groups, int act);
 int hsmoe_linear_act_grad(const void* d_out_dev, int64_t d_row_stride, const void* pre_dev, int64_t m, int64_t n,
                           int act, float limit, const int32_t* offsets_dev, int64_t n_groups, void* dz_dev,
                           float* d_bias_dev, float* d_bias_up_dev, void* workspace_dev, size_t workspace_bytes,
                           hsmoe_stream_t stream);
+size_t hsmoe_linear_grad_workspace_size(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act);
 int hsmoe_linear_grad_input(const void* dz_dev, int64_t dz_row_stride, int64_t m, int64_t n, const void* w_dev,
                             const void* w_up_dev, int64_t w_row_stride, int64_t w_group_stride, int64_t k,
-                            const int32_t* offsets_dev, int64_t n_groups, void* dx_dev, hsmoe_stream_t stream);
+                            const int32_t* offsets_dev, int64_t n_groups, void* dx_dev, void* workspace_dev,
+                            size_t workspace_bytes, hsmoe_stream_t stream);
 int hsmoe_linear_grad_weight(const void* dz_dev, int64_t dz_row_stride, const void* x_dev, int64_t x_row_stride,
                              int64_t m, int64_t n, int64_t k, const int32_t* offsets_dev, int64_t n_groups,
-                             int out_kind, void* dw_dev, void* dw_up_dev, hsmoe_stream_t stream);
+                             int out_kind, void* dw_dev, void* dw_up_dev, void* workspace_dev, size_t workspace_bytes,
+                             hsmoe_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * lm_head logits + greedy argmax + longest-prefix draft acceptance.
