@@ -18,6 +18,7 @@ constexpr uint32_t kFar = 0x7ffffff0u;      // an offset that no resource reache
 constexpr int64_t kMaxRange = 0x7fffffe0;   // bytes that one resource covers at most
 constexpr int kMaxGroups = 1024;
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -296,15 +297,18 @@ __device__ __forceinline__ void reduce_ahead(const char* lds, int steps, int wr,
 // which goes into its place, and a stage's loads have two turns at least
 // between their issue and the wait for them at the end of the last turn.
 template <typename T, typename Load>
-__device__ __forceinline__ void reduce_turns(const char* lds, int steps, int wave, int wr, int wc, int lane,
+__device__ __forceinline__ void reduce_turns(const char* lds, int steps, int rows, int wave, int wr, int wc, int lane,
                                              const Load& load, f32x4 (&acc)[T::kFR][T::kFC]) {
   static_assert(T::kWaves == 8 && T::kStages == 2, "two waves per SIMD, two stages");
   const bool second = wave >= 4;
   bf16x8 c[T::kFC], r[T::kFR];
   auto read = [&](int s, int kk) { T::read(lds + (s & 1) * T::kStage, wr, wc, kk, lane, c, r); };
+  // (a wave without rows in the tile only keeps the turns; skipping half of its
+  // blocks too costs the registers of a second copy of the products)
+  const bool live = rows > wr * T::kFR * 16;
   auto multiply = [&]() {
     __builtin_amdgcn_s_setprio(1);
-    T::product(c, r, acc);
+    if (live) T::product(c, r, acc);
     __builtin_amdgcn_s_setprio(0);
   };
   auto turn = [&](bool loads) {  // ends a turn; loads: the wave's own loads are in LDS
@@ -397,15 +401,20 @@ __device__ __forceinline__ Span find_tile(const TileScan& s, int tile, const int
   return {n_groups, n_rows, n_rows};
 }
 
-// The workgroup's place among total tiles.  Workgroup b runs on XCD b % 8: each
-// XCD takes a contiguous eighth, in which four row tiles go through the column
-// tiles together, so that its L2 serves a row tile to several column tiles and
-// a column tile to four row tiles.  False: nothing left for it.
+// The workgroup's place among row_tiles x col_tiles.  Tiles are numbered so that
+// four row tiles go through the column tiles together; workgroup b runs on XCD
+// b % 8, and the XCDs take the numbers in chunks of up to 32, one tile for each
+// of an XCD's CUs: its L2 serves a row tile to eight column tiles and a column
+// tile to four row tiles, and experts of unequal size are spread over all XCDs
+// (an eighth of all tiles in a row for each XCD: 1.4 times the time with 64
+// experts whose rows fall as 1 / sqrt(rank)).  False: nothing left for it.
+constexpr int kChunk = 32;
 __device__ __forceinline__ bool place_tile(int b, int row_tiles, int col_tiles, int& rt, int& ct) {
-  const int total = row_tiles * col_tiles;
-  const int q = total >> 3, rem = total & 7, x = b & 7, at = b >> 3;
-  if (at >= q + (x < rem ? 1 : 0)) return false;
-  const int t = x * q + (x < rem ? x : rem) + at;
+  const int total = row_tiles * col_tiles, size = total >= 8 * kChunk ? kChunk : (total + 7) / 8;
+  const int x = b & 7, at = b >> 3;
+  if (size <= 0) return false;
+  const int t = (at / size * 8 + x) * size + at % size;
+  if (t >= total) return false;
   const int band = 4 * col_tiles, b0 = t / band, in = t % band;
   const int height = row_tiles - 4 * b0 < 4 ? row_tiles - 4 * b0 : 4;
   rt = 4 * b0 + in % height;
@@ -414,10 +423,10 @@ __device__ __forceinline__ bool place_tile(int b, int row_tiles, int col_tiles, 
 }
 
 template <typename T, typename Load>
-__device__ __forceinline__ void reduce(const char* lds, int steps, int wave, int wr, int wc, int lane, const Load& load,
-                                       f32x4 (&acc)[T::kFR][T::kFC]) {
+__device__ __forceinline__ void reduce(const char* lds, int steps, int rows, int wave, int wr, int wc, int lane,
+                                       const Load& load, f32x4 (&acc)[T::kFR][T::kFC]) {
   if constexpr (T::kTurns)
-    reduce_turns<T>(lds, steps, wave, wr, wc, lane, load, acc);
+    reduce_turns<T>(lds, steps, rows, wave, wr, wc, lane, load, acc);
   else
     reduce_ahead<T>(lds, steps, wr, wc, lane, load, acc);
 }
@@ -513,14 +522,8 @@ __device__ __forceinline__ Row8 activate(const LinearParams& p, const Row8& z, c
   return y;
 }
 
-// Eight outputs of row m from column n on: z (and zu) are the sums with bias.
-__device__ __forceinline__ void finish8(const LinearParams& p, int64_t m, int64_t n, const Row8& z, const Row8& zu,
-                                        uint4 residual) {
-  if (p.pre) {
-    const int64_t ldp = p.act == HSMOE_ACT_SWIGLU ? 2 * p.n : p.n;
-    *reinterpret_cast<uint4*>(p.pre + m * ldp + n) = pack8(z);
-    if (p.act == HSMOE_ACT_SWIGLU) *reinterpret_cast<uint4*>(p.pre + m * ldp + p.n + n) = pack8(zu);
-  }
+// Eight outputs of a row: z (and zu) are the sums with bias.
+__device__ __forceinline__ Row8 outputs8(const LinearParams& p, const Row8& z, const Row8& zu, uint4 residual) {
   Row8 y = z;
   if (p.act != HSMOE_ACT_NONE) y = p.out_f32 ? activate<true>(p, z, zu) : activate<false>(p, z, zu);
   if (p.residual) {
@@ -528,7 +531,48 @@ __device__ __forceinline__ void finish8(const LinearParams& p, int64_t m, int64_
 #pragma unroll
     for (int i = 0; i < 8; ++i) y.v[i] += r.v[i];
   }
-  store8(p.out, m * p.n + n, y, p.out_f32);
+  return y;
+}
+
+// Row m's from column n on.
+__device__ __forceinline__ void finish8(const LinearParams& p, int64_t m, int64_t n, const Row8& z, const Row8& zu,
+                                        uint4 residual) {
+  if (p.pre) {
+    const int64_t ldp = p.act == HSMOE_ACT_SWIGLU ? 2 * p.n : p.n;
+    *reinterpret_cast<uint4*>(p.pre + m * ldp + n) = pack8(z);
+    if (p.act == HSMOE_ACT_SWIGLU) *reinterpret_cast<uint4*>(p.pre + m * ldp + p.n + n) = pack8(zu);
+  }
+  store8(p.out, m * p.n + n, outputs8(p, z, zu, residual), p.out_f32);
+}
+
+// Two rows of eight bf16 per lane, columns 8 g ..+7 and 32 + 8 g ..+7 of row r of
+// a block of 16 x 64 (r = lane % 16, g = lane / 16), to memory in whole 128-byte
+// lines: lanes r and r ^ 8 exchange one of theirs, and each store takes eight
+// rows.  `out` is the block's first value; rows and cols are what there is of it.
+template <bool kStream>
+__device__ __forceinline__ void store_lines(char* out, int64_t width, int rows, int cols, uint4 a, uint4 b, int lane) {
+  const int r = lane & 15, g = lane >> 4;
+  const bool low = r < 8;
+  const uint32_t va[4] = {a.x, a.y, a.z, a.w}, vb[4] = {b.x, b.y, b.z, b.w};
+  u32x4 first, second;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // row_ror:8, lane ^ 8
+    const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(low ? vb[i] : va[i]), 0x128, 0xf, 0xf, true);
+    first[i] = low ? va[i] : got;
+    second[i] = low ? got : vb[i];
+  }
+  const int col = 8 * g + (low ? 0 : 32), row = r & 7;
+  if (col >= cols) return;
+  u32x4* o = reinterpret_cast<u32x4*>(out + (row * width + col) * 2);
+  u32x4* o8 = reinterpret_cast<u32x4*>(out + ((row + 8) * width + col) * 2);
+  if (kStream) {
+    if (row < rows) __builtin_nontemporal_store(first, o);
+    if (row + 8 < rows) __builtin_nontemporal_store(second, o8);
+  } else {
+    if (row < rows) *o = first;
+    if (row + 8 < rows) *o8 = second;
+  }
 }
 
 // One output; a row of no group gets zeros.
@@ -602,7 +646,7 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
-  reduce<T>(lds, steps.count, wave, wr, wc, lane, load, acc);
+  reduce<T>(lds, steps.count, rows, wave, wr, wc, lane, load, acc);
   if (p.part) {
     const int64_t width = kGated ? 2 * p.n : p.n;
     char* base = (char*)(p.part + split * p.n_rows * width);
@@ -646,18 +690,35 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
 #pragma unroll
   for (int i = 0; i < T::kFR; ++i) {
     if (i + 1 < T::kFR) load_res(i + 1);
+    Row8 z[kE], zu[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      z[e] = kGated ? row8(acc[i][4 * e], acc[i][4 * e + 2]) : row8(acc[i][2 * e], acc[i][2 * e + 1]);
+      zu[e] = kGated ? row8(acc[i][4 * e + 1], acc[i][4 * e + 3]) : Row8{};
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        z[e].v[v] += bias[0][e].v[v];
+        if (kGated) zu[e].v[v] += bias[1][e].v[v];
+      }
+    }
+    if constexpr (!kGated) {
+      static_assert(kE == 2, "a wave has 64 columns");
+      const int64_t at = (sp.row + wr * T::kFR * 16 + 16 * i) * p.n + n0 + wc * 64;
+      const int left = rows - (wr * T::kFR + i) * 16, width = cols - wc * 64;
+      if (p.pre) store_lines<false>((char*)(p.pre + at), p.n, left, width, pack8(z[0]), pack8(z[1]), lane);
+      if (!p.out_f32) {
+        const uint4 a = pack8(outputs8(p, z[0], z[0], res[i & 1][0])), b = pack8(outputs8(p, z[1], z[1], res[i & 1][1]));
+        store_lines<false>(p.out + at * 2, p.n, left, width, a, b, lane);
+        continue;
+      }
+    }
     if (r0 + 16 * i >= rows) continue;
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       if (cw + 32 * e >= cols) continue;
-      Row8 z = kGated ? row8(acc[i][4 * e], acc[i][4 * e + 2]) : row8(acc[i][2 * e], acc[i][2 * e + 1]), zu{};
-      if (kGated) zu = row8(acc[i][4 * e + 1], acc[i][4 * e + 3]);
-#pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        z.v[v] += bias[0][e].v[v];
-        if (kGated) zu.v[v] += bias[1][e].v[v];
-      }
-      finish8(p, sp.row + r0 + 16 * i, n0 + cw + 32 * e, z, zu, res[i & 1][e]);
+      const int64_t m = sp.row + r0 + 16 * i, n = n0 + cw + 32 * e;
+      if (kGated) finish8(p, m, n, z[e], zu[e], res[i & 1][e]);
+      else store8(p.out, m * p.n + n, outputs8(p, z[e], z[e], res[i & 1][e]), true);
     }
   }
 }
@@ -803,17 +864,25 @@ struct LinearGradParams {
 };
 
 // The sums of a tile to rows row0 .. and columns col0 .. of a matrix of `width`.
-template <typename T>
+// kStream: past the caches (weights' gradients: far more than they hold, and
+// what the tiles read would be driven out of them).
+template <typename T, bool kStream>
 __device__ __forceinline__ void store_tile(char* out, int64_t width, int64_t row0, int64_t col0, int rows, int cols,
                                            bool f32, int wr, int wc, int lane, const f32x4 (&acc)[T::kFR][T::kFC]) {
-  const int r0 = wr * T::kFR * 16 + (lane & 15), cw = wc * T::kFC * 16 + 8 * (lane >> 4);
+  static_assert(T::kFC == 4, "a wave has 64 columns");
+  const int rb = wr * T::kFR * 16, cb = wc * 64;
 #pragma unroll
   for (int i = 0; i < T::kFR; ++i) {
-    if (r0 + 16 * i >= rows) continue;
-#pragma unroll
-    for (int e = 0; e < T::kFC / 2; ++e)
-      if (cw + 32 * e < cols)
-        store8(out, (row0 + r0 + 16 * i) * width + col0 + cw + 32 * e, row8(acc[i][2 * e], acc[i][2 * e + 1]), f32);
+    const Row8 a = row8(acc[i][0], acc[i][1]), b = row8(acc[i][2], acc[i][3]);
+    if (f32) {
+      const int r = rb + 16 * i + (lane & 15), c = cb + 8 * (lane >> 4);
+      const int64_t at = (row0 + r) * width + col0 + c;
+      if (r < rows && c < cols) store8(out, at, a, true);
+      if (r < rows && c + 32 < cols) store8(out, at + 32, b, true);
+    } else {
+      store_lines<kStream>(out + ((row0 + rb + 16 * i) * width + col0 + cb) * 2, width, rows - rb - 16 * i, cols - cb,
+                           pack8(a), pack8(b), lane);
+    }
   }
 }
 
@@ -852,9 +921,9 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
-  reduce<T>(lds, steps.count, wave, wr, wc, lane, load, acc);
+  reduce<T>(lds, steps.count, rows, wave, wr, wc, lane, load, acc);
   char* out = p.part ? (char*)(p.part + split * p.n_rows * p.k) : p.dx;
-  store_tile<T>(out, p.k, sp.row, c0, rows, cols, p.part != nullptr, wr, wc, lane, acc);
+  store_tile<T, false>(out, p.k, sp.row, c0, rows, cols, p.part != nullptr, wr, wc, lane, acc);
 }
 
 // dw[g] = dz^T x over the rows of group g: a tile of n x k per workgroup, all
@@ -885,11 +954,11 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
-  reduce<T>(lds, steps.count, wave, wr, wc, lane, load, acc);
+  reduce<T>(lds, steps.count, nrow, wave, wr, wc, lane, load, acc);
   const bool f32 = p.part || p.dw_f32;
   char* out = p.part ? (char*)(p.part + ((int64_t)split * p.n_groups * p.mats + gm) * p.n * p.k)
                      : p.dw[mat] + (int64_t)group * p.n * p.k * (f32 ? 4 : 2);
-  store_tile<T>(out, p.k, n0, c0, nrow, ncol, f32, wr, wc, lane, acc);
+  store_tile<T, true>(out, p.k, n0, c0, nrow, ncol, f32, wr, wc, lane, acc);
 }
 
 // The parts of a split reduction added: kWeight: dw (and dw_up), else dx.
@@ -1041,11 +1110,11 @@ int check_matrix(const char* what, const char* name, const void* p, int64_t cols
   return HSMOE_OK;
 }
 
-// Workgroups for tiles of bc columns, in whole rounds over the eight XCDs; 0 if
-// that is more than a launch can hold.
+// Workgroups for row_tiles x tiles of bc columns, as place_tile deals them out; 0
+// if that is more than a launch can hold.
 unsigned tile_grid(int64_t row_tiles, int64_t cols, int bc) {
-  const int64_t total = row_tiles * ((cols + bc - 1) / bc);
-  return total > (1 << 22) - 8 ? 0 : (unsigned)((total + 7) / 8 * 8);
+  const int64_t total = row_tiles * ((cols + bc - 1) / bc), unit = total > 8 * (kChunk - 1) ? 8 * kChunk : 8;
+  return total > (1 << 22) - unit ? 0 : (unsigned)((total + unit - 1) / unit * unit);
 }
 
 // How a product is done: the tile, and the parts of its reduction.
