@@ -233,6 +233,25 @@ struct Tile {
   }
 };
 
+// The reduction with two stages: one is on its way while the other is
+// multiplied, and the second workgroup of the CU fills what that leaves idle.
+// Every wave waits for its own loads of a stage (and for its LDS reads, whose
+// products may come later), then all meet: the stage is whole, and nobody reads
+// the one that is loaded next.
+template <typename T, typename Load>
+__device__ __forceinline__ void reduce_stages(const char* lds, int steps, int wr, int wc, int lane, const Load& load,
+                                              f32x4 (&acc)[T::kFR][T::kFC]) {
+  static_assert(T::kStages == 2, "a stage in use, a stage on its way");
+  if (steps > 0) load(0, 0, kAll);
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (s + 1 < steps) load(s + 1, (s + 1) & 1, kAll);
+    T::multiply(lds + (s & 1) * T::kStage, wr, wc, lane, acc);
+  }
+}
+
 // The reduction with one wave per SIMD, three stages or more: operands of the next 32
 // reduction steps are read, and half a stage's loads are issued, between the
 // products of the current ones.  A stage's first half is read before the stage
@@ -427,6 +446,8 @@ __device__ __forceinline__ void reduce(const char* lds, int steps, int rows, int
                                        const Load& load, f32x4 (&acc)[T::kFR][T::kFC]) {
   if constexpr (T::kTurns)
     reduce_turns<T>(lds, steps, rows, wave, wr, wc, lane, load, acc);
+  else if constexpr (T::kStages == 2)
+    reduce_stages<T>(lds, steps, wr, wc, lane, load, acc);
   else
     reduce_ahead<T>(lds, steps, wr, wc, lane, load, acc);
 }
@@ -634,13 +655,21 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
     return;
   }
   const Steps steps = part_of((int)((p.k + kBK - 1) / kBK), p.splits, split);
+  // Rows are often a power of two apart, and workgroups in step then read the
+  // same few memory channels.  With experts, each XCD begins at an eighth of the
+  // reduction of its own (64 matrices of 2048 x 4096 for 32 rows each: 262 -> 224
+  // us); the XCDs of a dense product read the same w, once in step (500 rows, two
+  // such matrices: 24 against 27 us turned), and the kernels with more stages, for
+  // few tiles, do without.
+  const int turned = T::kStages == 2 && p.offsets ? (blockIdx.x & 7) * steps.count >> 3 : 0;
   const int64_t wo = sp.group * p.w_group + n0 * p.ldw;
   Source<typename T::R> xs;
   xs.open(p.x + sp.row * p.ldx, nullptr, p.ldx, rows, p.k * 2, wave, lane);
   Source<typename T::C> ws;
   ws.open(p.w[0] + wo, p.w[1] + wo, p.ldw, cols, p.k * 2, wave, lane);
   auto load = [&](int s, int slot, auto part) {
-    const int first = (steps.first + s) * kBK;
+    const int at = s + turned < steps.count ? s + turned : s + turned - steps.count;
+    const int first = (steps.first + at) * kBK;
     T::template load<decltype(part)::value>(xs, first, ws, first, s < steps.count ? (int)p.k - first : 0,
                                             lds + slot * T::kStage, wave);
   };
@@ -1125,34 +1154,44 @@ struct Plan {
 };
 constexpr int kNarrow = -1;
 
-// The tiles, with what a workgroup takes for 64 reduction steps and for the rest
-// (first loads, epilogue), in us, as measured with every CU at work:
-//   256 x 256, turns of eight waves    1.30 + 14
-//   128 x 128, four waves, 4 stages    0.62 + 7
-//   64 x 128, four waves, 4 stages     0.44 + 5
-// The tile and the number of parts with the least time by these figures are
-// taken; parts cost the fp32 sums' way to memory and back and a launch.
+// The tiles, with what a round of workgroups (one or two per CU) takes for 64
+// reduction steps and for the rest (first loads, epilogue), in us with every CU
+// at work, and the rate at which they stream matrices that are read once:
+//   256 x 256, turns of eight waves        1.30 + 14, 4.7 TB/s
+//   128 x 128, 4 stages                    0.62 + 7,  5.4 TB/s
+//   64 x 128, 4 stages                     0.44 + 5,  5.3 TB/s
+//   128 x 128, 2 stages, two per CU        1.15 + 10, 5.8 TB/s
+// (swiglu's two matrices, in tiles of half the columns: 0.87 of that.)  The
+// kernel for few rows streams w at 5.3 TB/s less 3% per row.  What takes the
+// least time by these figures is taken; a split reduction costs the fp32 sums'
+// way to memory and back and a launch.
 struct TileCost {
-  int rows, cols;
-  double step, rest;
+  int rows, cols, per_cu;
+  double step, rest, rate;  // us, us, bytes per us
 };
-constexpr TileCost kTiles[] = {{256, 256, 1.30, 14.0}, {128, 128, 0.62, 7.0}, {64, 128, 0.44, 5.0}};
+constexpr TileCost kTiles[] = {{256, 256, 1, 1.30, 14.0, 4.7e6},
+                               {128, 128, 1, 0.62, 7.0, 5.4e6},
+                               {64, 128, 1, 0.44, 5.0, 5.3e6},
+                               {128, 128, 2, 1.15, 10.0, 5.8e6}};
 
-// rows: of the output, in `groups` groups of which at most `active` have any;
-// cols: tiles' columns (twice the output's for swiglu); sums: fp32 values of one part.
-Plan plan_tiles(double rows, double active, double groups, int64_t cols, int64_t steps, double sums, int n_tiles) {
+// rows: of the output, in groups of which at most `active` have any (one: dense);
+// cols: tiles' columns (twice the output's for swiglu); bytes: of the groups'
+// matrices; sums: fp32 values of one part.
+Plan plan_tiles(double rows, double active, int64_t cols, int64_t steps, double bytes, double sums, int tiles_from,
+                int tiles_to, double& least) {
   const double cus = device_cus();
-  Plan best{0, 1, 0};
-  double least = 1e30;
-  for (int t = 0; t < n_tiles; ++t) {
+  Plan best{tiles_from, 1, 0};
+  least = 1e30;
+  for (int t = tiles_from; t < tiles_to; ++t) {
     const TileCost& c = kTiles[t];
-    double row_tiles = groups == 1 ? __builtin_ceil(rows / c.rows) : rows / c.rows + 0.5 * active;
+    double row_tiles = active <= 1 ? __builtin_ceil(rows / c.rows) : rows / c.rows + 0.5 * active;
     if (row_tiles < active) row_tiles = active;
     const double tiles = row_tiles * (double)((cols + c.cols - 1) / c.cols);
     for (int s = 1; s <= 16; s *= 2) {
       const int64_t per = (steps + s - 1) / s;
       if (s > 1 && (per < 4 || (steps + per - 1) / per != s)) continue;
-      double us = __builtin_ceil(tiles * s / cus) * (per * c.step + c.rest);
+      double us = __builtin_ceil(tiles * s / (cus * c.per_cu)) * (per * c.step + c.rest);
+      if (us < bytes / c.rate) us = bytes / c.rate;
       if (s > 1) us += 4.0 + s * sums * 8.0 / 5e6;
       if (us < least) {
         least = us;
@@ -1163,22 +1202,27 @@ Plan plan_tiles(double rows, double active, double groups, int64_t cols, int64_t
   return best;
 }
 
-// Up to 16 rows per group on average: the kernel that streams w.
 Plan plan_linear(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
   const int64_t active = n_groups < m ? n_groups : m, mats = act == HSMOE_ACT_SWIGLU ? 2 : 1;
-  if (m <= 16 * active) return {kNarrow, 1, 0};
-  return plan_tiles((double)m, (double)active, (double)n_groups, n * mats, (k + kBK - 1) / kBK, (double)m * n * mats, 3);
+  const double rows = (double)m / (double)active, bytes = 2.0 * active * n * mats * k;
+  double tiled;
+  const Plan plan = plan_tiles((double)m, (double)active, n * mats, (k + kBK - 1) / kBK,
+                               mats == 2 ? bytes / 0.87 : bytes, (double)m * n * mats, 0, 4, tiled);
+  const double narrow = 2.0 + bytes / 5.3e6 * (1.0 + 0.03 * rows);
+  return rows <= kNarrowRows && narrow < tiled ? Plan{kNarrow, 1, 0} : plan;
 }
 Plan plan_grad_input(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
   const int64_t active = n_groups < m ? n_groups : m;
-  return plan_tiles((double)m, (double)active, (double)n_groups, k, (n + kBK - 1) / kBK * mats, (double)m * k, 3);
+  double us;
+  return plan_tiles((double)m, (double)active, k, (n + kBK - 1) / kBK * mats, 2.0 * active * n * mats * k, (double)m * k,
+                    0, 4, us);
 }
 // (both operands transposed: no tile of 64 rows)
 Plan plan_grad_weight(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
-  const double groups = (double)n_groups * mats, sums = groups * n * k;
   const int64_t rows = (m + n_groups - 1) / n_groups;
-  Plan p = plan_tiles((double)n, 1, 1, k * n_groups * mats, (rows + kBK - 1) / kBK, sums, 2);
-  return p;
+  double us;
+  return plan_tiles((double)n, 1, k * n_groups * mats, (rows + kBK - 1) / kBK, 0, (double)n_groups * mats * n * k, 0, 2,
+                    us);
 }
 
 int check_workspace(const char* what, const Plan& plan, const void* ws, size_t bytes) {
@@ -1303,7 +1347,8 @@ extern "C" int hsmoe_linear(const void* x, int64_t x_row_stride, int64_t m, int6
   if (plan.tile == kNarrow) return launch_narrow(p, st);
   if (plan.tile == 0) return launch_linear<256, 256, 2, 4, 0>(p, st);
   if (plan.tile == 1) return launch_linear<128, 128, 2, 2, 4>(p, st);
-  return launch_linear<64, 128, 2, 2, 4>(p, st);
+  if (plan.tile == 2) return launch_linear<64, 128, 2, 2, 4>(p, st);
+  return launch_linear<128, 128, 2, 2, 2>(p, st);
 }
 
 extern "C" size_t hsmoe_linear_act_grad_workspace_size(int64_t m, int64_t n, int64_t n_groups, int act) {
@@ -1392,7 +1437,8 @@ extern "C" int hsmoe_linear_grad_input(const void* dz, int64_t dz_row_stride, in
   hipStream_t st = (hipStream_t)stream;
   if (plan.tile == 0) return launch_grad_input<256, 256, 2, 4, 0>(p, st);
   if (plan.tile == 1) return launch_grad_input<128, 128, 2, 2, 4>(p, st);
-  return launch_grad_input<64, 128, 2, 2, 4>(p, st);
+  if (plan.tile == 2) return launch_grad_input<64, 128, 2, 2, 4>(p, st);
+  return launch_grad_input<128, 128, 2, 2, 2>(p, st);
 }
 
 extern "C" int hsmoe_linear_grad_weight(const void* dz, int64_t dz_row_stride, const void* x, int64_t x_row_stride,
