@@ -154,7 +154,9 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle, without a torch.cuda.Stream object (1.9 us of a call)."""
+    index = None if device is None else device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -12,6 +12,7 @@ safetensors' memory-mapped safe_open.  Keys are the reference's:
   layers.{L}.ffn.gate.{weight,scale,bias,tid2eid}, layers.{L}.ffn_norm.weight
                                                           engine.py:470-510
   mtp.0.ffn.gate.{weight,bias}, mtp.0.{enorm,hnorm,norm,ffn_norm}.weight
+  mtp.0.{e_proj,h_proj}.{weight,scale} (load_engine(mtp_projections=True) only)
                                                           engine.py:1864-1872
   embed.weight, head.weight, norm.weight                  engine.py:426-443
 Routed experts keep their bytes: int8 packed e2m1 and E8M0 scales (one byte
@@ -245,10 +246,13 @@ def select_lm_head(index: CheckpointIndex, config, embed, device):
     return embed
 
 
-def load_engine(weight_dir: str, config=None, device="cuda", with_mtp: bool = True, log=None):
+def load_engine(weight_dir: str, config=None, device="cuda", with_mtp: bool = True, log=None,
+                mtp_projections: bool = False):
     """A HomeSeekMoEEngine over a checkpoint: the expert store, the FFN layer
     weights, embed / lm_head (select_lm_head) / final
-    norm, and the MTP block's FFN weights and norms when present."""
+    norm, and the MTP block's FFN weights and norms when present.
+    mtp_projections: also mtp.0.e_proj and mtp.0.h_proj (both must be there); the
+    drafts then go through them."""
     from .engine import HomeSeekMoEEngine
     from .model_config import MoEConfig
     index = CheckpointIndex(weight_dir)
@@ -268,6 +272,12 @@ def load_engine(weight_dir: str, config=None, device="cuda", with_mtp: bool = Tr
         for n in ("enorm", "hnorm", "norm"):
             w = _bf16_weight(index, f"mtp.0.{n}.weight", device)
             if w is not None:
+                mtp[f"{n}.weight"] = w
+        if mtp_projections:
+            for n in ("e_proj", "h_proj"):
+                w = _bf16_weight(index, f"mtp.0.{n}.weight", device, f"mtp.0.{n}.scale")
+                if w is None:
+                    raise KeyError(f"the checkpoint has no mtp.0.{n}.weight")
                 mtp[f"{n}.weight"] = w
     index.close()
     return HomeSeekMoEEngine(config, store, lws, lm_head=head, norm_weight=norm,

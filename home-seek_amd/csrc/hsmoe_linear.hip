@@ -1024,7 +1024,8 @@ struct ActGradParams {
 
 constexpr int kActThreads = 256;
 
-template <int kMats>
+// kSums: the column sums are wanted (and with them dz before its rounding).
+template <int kMats, bool kSums>
 __global__ void __launch_bounds__(kActThreads) act_grad_kernel(ActGradParams p) {
   __shared__ float s_sum[kMats][8][256];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, group = blockIdx.y, share = blockIdx.z;
@@ -1034,49 +1035,50 @@ __global__ void __launch_bounds__(kActThreads) act_grad_kernel(ActGradParams p) 
   const int64_t count = end > first ? end - first : 0;
   const int64_t a = first + count * share / p.shares, b = first + count * (share + 1) / p.shares;
   float sum[kMats][8] = {};
-  if (col < p.n) {
-    for (int64_t r = a + ty; r < b; r += 8) {
-      const uint4 du = *reinterpret_cast<const uint4*>(p.d_out + r * p.ld_out + col);
-      const uint32_t dw[4] = {du.x, du.y, du.z, du.w};
-      uint32_t pw[kMats][4], ow[kMats][4];
+  // two rows' loads on their way before the first is used
+  constexpr int kAhead = 2;
+  for (int64_t r0 = a + ty; r0 < b && col < p.n; r0 += 8 * kAhead) {
+    uint4 d_out[kAhead], pre[kAhead][kMats] = {};
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) {
+      const int64_t r = r0 + 8 * h;
+      if (r >= b) continue;
+      d_out[h] = load16(p.d_out + r * p.ld_out + col);
       if (p.pre) {
 #pragma unroll
-        for (int t = 0; t < kMats; ++t) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p.pre + r * p.n * kMats + t * p.n + col);
-          pw[t][0] = u.x, pw[t][1] = u.y, pw[t][2] = u.z, pw[t][3] = u.w;
-        }
+        for (int t = 0; t < kMats; ++t) pre[h][t] = load16(p.pre + r * p.n * kMats + t * p.n + col);
       }
+    }
+#pragma unroll
+    for (int h = 0; h < kAhead; ++h) {
+      const int64_t r = r0 + 8 * h;
+      if (r >= b) continue;
+      const Row8 d = unpack8(d_out[h]), z = unpack8(pre[h][0]), zu = unpack8(pre[h][kMats - 1]);
+      Row8 o[kMats];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        auto half = [&](uint32_t w) { return i & 1 ? __uint_as_float(w & 0xffff0000u) : bf16_bits_to_f32(w & 0xffffu); };
-        const float d = half(dw[i >> 1]);
-        float o[kMats];
-        o[0] = d;
         if (kMats == 2) {
-          const float z = half(pw[0][i >> 1]), zu = half(pw[kMats - 1][i >> 1]);
-          const float g = clamp_top(z, p.limit), s = sigmoid<true>(g);
-          o[0] = z > p.limit ? 0.0f : d * clamp_both(zu, p.limit) * (s + g * s * (1.0f - s));
-          o[kMats - 1] = zu > p.limit || zu < -p.limit ? 0.0f : d * (g * s);
+          const float g = clamp_top(z.v[i], p.limit), s = sigmoid<kSums>(g), gs = g * s;
+          o[0].v[i] = z.v[i] > p.limit ? 0.0f : d.v[i] * clamp_both(zu.v[i], p.limit) * (s + gs * (1.0f - s));
+          o[kMats - 1].v[i] = zu.v[i] > p.limit || zu.v[i] < -p.limit ? 0.0f : d.v[i] * gs;
         } else if (p.act == HSMOE_ACT_SILU) {
-          const float z = half(pw[0][i >> 1]), s = sigmoid<true>(z);
-          o[0] = d * (s + z * s * (1.0f - s));
-        }
-#pragma unroll
-        for (int t = 0; t < kMats; ++t) {
-          sum[t][i] += o[t];
-          const uint32_t h = f32_to_bf16_bits(o[t]);
-          ow[t][i >> 1] = i & 1 ? ow[t][i >> 1] | h << 16 : h;
+          const float s = sigmoid<kSums>(z.v[i]);
+          o[0].v[i] = d.v[i] * (s + z.v[i] * s * (1.0f - s));
+        } else {
+          o[0].v[i] = d.v[i];
         }
       }
-      if (p.dz) {
 #pragma unroll
-        for (int t = 0; t < kMats; ++t)
-          *reinterpret_cast<uint4*>(p.dz + r * p.n * kMats + t * p.n + col) =
-              make_uint4(ow[t][0], ow[t][1], ow[t][2], ow[t][3]);
+      for (int t = 0; t < kMats; ++t) {
+        if (kSums) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[t][i] += o[t].v[i];
+        }
+        if (p.dz) *reinterpret_cast<uint4*>(p.dz + r * p.n * kMats + t * p.n + col) = pack8(o[t]);
       }
     }
   }
-  if (!p.part && !p.d_bias[0] && !p.d_bias[1]) return;
+  if (!kSums) return;
 #pragma unroll
   for (int t = 0; t < kMats; ++t)
 #pragma unroll
@@ -1393,10 +1395,15 @@ extern "C" int hsmoe_linear_act_grad(const void* d_out, int64_t d_row_stride, co
   p.n_groups = (int)n_groups, p.act = act, p.mats = gated ? 2 : 1, p.shares = shares, p.limit = limit;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)((n + 255) / 256), (unsigned)n_groups, (unsigned)shares);
-  if (gated)
-    hipLaunchKernelGGL(act_grad_kernel<2>, grid, dim3(kActThreads), 0, st, p);
+  const dim3 block(kActThreads);
+  if (gated && sums)
+    hipLaunchKernelGGL((act_grad_kernel<2, true>), grid, block, 0, st, p);
+  else if (gated)
+    hipLaunchKernelGGL((act_grad_kernel<2, false>), grid, block, 0, st, p);
+  else if (sums)
+    hipLaunchKernelGGL((act_grad_kernel<1, true>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL(act_grad_kernel<1>, grid, dim3(kActThreads), 0, st, p);
+    hipLaunchKernelGGL((act_grad_kernel<1, false>), grid, block, 0, st, p);
   if (need)
     hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)((n * p.mats * n_groups + 255) / 256)), dim3(256), 0, st, p);
   return check_launch("hsmoe_linear_act_grad");

@@ -27,21 +27,54 @@ __device__ __forceinline__ int pair_expert(const int64_t* idx, int64_t q, int n_
   return e >= 0 && e < n_experts ? (int)e : n_experts;
 }
 
-// Histogram of a chunk's experts (integer counts: the order of the LDS atomics
-// does not show).
+// Counts pairs [from, to) into rows 0-7 of cnt (those before `split`) or 8-15
+// (integers: the order of the LDS atomics does not show), sixteen ids per thread
+// on their way at a time.  Lane l counts in its row l % 8: a popular expert would
+// have the lanes of a wave add to one word in turn.
+constexpr int kCopies = kSortWaves / 2;
+__device__ __forceinline__ void count_pairs(const int64_t* idx, int64_t from, int64_t split, int64_t to, int n_experts,
+                                            int (&cnt)[kSortWaves][kSortMaxExperts]) {
+  const int copy = threadIdx.x & (kCopies - 1);
+  constexpr int kAhead = 16;
+  for (int64_t q = from + threadIdx.x; q < to; q += kAhead * kSortThreads) {
+    int e[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      e[i] = q + i * kSortThreads < to ? pair_expert(idx, q + i * kSortThreads, n_experts) : n_experts;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (e[i] < n_experts) atomicAdd(&cnt[copy + (q + i * kSortThreads < split ? 0 : kCopies)][e[i]], 1);
+  }
+}
+
+__device__ __forceinline__ void clear_counts(int n_experts, int (&cnt)[kSortWaves][kSortMaxExperts]) {
+  for (int c = threadIdx.x & 63; c < n_experts; c += 64) cnt[threadIdx.x >> 6][c] = 0;
+}
+// Thread e: the pairs of expert e before and from `split` on (0 for other threads).
+__device__ __forceinline__ void sum_counts(int n_experts, const int (&cnt)[kSortWaves][kSortMaxExperts], int& before,
+                                           int& after) {
+  before = after = 0;
+  if ((int)threadIdx.x >= n_experts) return;
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    before += cnt[i][threadIdx.x];
+    after += cnt[kCopies + i][threadIdx.x];
+  }
+}
+
+// Histogram of a chunk's experts.
 __global__ void __launch_bounds__(kSortThreads)
     sort_hist_kernel(const int64_t* __restrict__ idx, int64_t pairs, int n_experts, int64_t chunk,
                      int* __restrict__ hist) {
-  __shared__ int cnt[kSortMaxExperts];
-  if ((int)threadIdx.x < n_experts) cnt[threadIdx.x] = 0;
+  __shared__ int cnt[kSortWaves][kSortMaxExperts];
+  const int64_t q0 = blockIdx.x * chunk;
+  clear_counts(n_experts, cnt);
   __syncthreads();
-  const int64_t q0 = blockIdx.x * chunk, q1 = min(pairs, q0 + chunk);
-  for (int64_t q = q0 + threadIdx.x; q < q1; q += kSortThreads) {
-    const int e = pair_expert(idx, q, n_experts);
-    if (e < n_experts) atomicAdd(&cnt[e], 1);
-  }
+  count_pairs(idx, q0, q0, min(pairs, q0 + chunk), n_experts, cnt);
   __syncthreads();
-  if ((int)threadIdx.x < n_experts) hist[(int64_t)blockIdx.x * n_experts + threadIdx.x] = cnt[threadIdx.x];
+  int before, after;
+  sum_counts(n_experts, cnt, before, after);
+  if ((int)threadIdx.x < n_experts) hist[(int64_t)blockIdx.x * n_experts + threadIdx.x] = after;
 }
 
 // Inclusive sum over the workgroup's threads of one value each.
@@ -66,7 +99,8 @@ __device__ __forceinline__ int block_scan(int v, int* s_wave) {
 // lanes with its expert, found with one ballot per bit of the id; the waves'
 // counts are then summed in wave order, so pairs of one expert keep their
 // order and the result is the stable sort.
-// hist == NULL: one workgroup does all, and counts for itself first.
+// hist == NULL: every workgroup counts all pairs for itself, which costs what a
+// launch that counts and its gap do at 24576 pairs (13 us) and less below.
 __global__ void __launch_bounds__(kSortThreads)
     sort_place_kernel(const int64_t* __restrict__ idx, int64_t pairs, int n_experts, int64_t chunk,
                       const int* __restrict__ hist, int* __restrict__ offsets, int* __restrict__ pair_of,
@@ -75,10 +109,13 @@ __global__ void __launch_bounds__(kSortThreads)
   __shared__ int s_wave[kSortWaves];
   __shared__ int s_total;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t q0 = blockIdx.x * chunk, q1 = min(pairs, q0 + chunk);
   int total = 0, before = 0;  // pairs of expert tid: all, and those of earlier chunks
+  int e = q0 + tid < q1 ? pair_expert(idx, q0 + tid, n_experts) : n_experts;  // of the first 1024 pairs
   if (hist) {
     if (tid < n_experts) {
       const int* h = hist + tid;
+#pragma unroll 8
       for (int b = 0; b < (int)gridDim.x; ++b) {
         const int c = h[(int64_t)b * n_experts];
         before += b < (int)blockIdx.x ? c : 0;
@@ -86,14 +123,12 @@ __global__ void __launch_bounds__(kSortThreads)
       }
     }
   } else {
-    if (tid < n_experts) cnt[0][tid] = 0;
+    clear_counts(n_experts, cnt);
     __syncthreads();
-    for (int64_t q = tid; q < pairs; q += kSortThreads) {
-      const int e = pair_expert(idx, q, n_experts);
-      if (e < n_experts) atomicAdd(&cnt[0][e], 1);
-    }
+    count_pairs(idx, 0, q0, pairs, n_experts, cnt);
     __syncthreads();
-    if (tid < n_experts) total = cnt[0][tid];
+    sum_counts(n_experts, cnt, before, total);
+    total += before;
   }
   const int upto = block_scan(total, s_wave);
   int next = upto - total + before;
@@ -103,14 +138,12 @@ __global__ void __launch_bounds__(kSortThreads)
     if (tid == 0) offsets[0] = 0;
   }
   __syncthreads();
-  const int64_t q0 = blockIdx.x * chunk, q1 = min(pairs, q0 + chunk);
   for (int64_t q = max(q0, (int64_t)s_total) + tid; q < q1; q += kSortThreads) pair_of[q] = -1;  // rows behind the last
   const int bits = 32 - __clz(n_experts);
   for (int64_t base = q0; base < q1; base += kSortThreads) {
     const int64_t q = base + tid;
-    const int e = q < q1 ? pair_expert(idx, q, n_experts) : n_experts;
-    for (int c = tid; c < kSortWaves * n_experts; c += kSortThreads) cnt[c / n_experts][c % n_experts] = 0;
-    __syncthreads();
+    if (base > q0) e = q < q1 ? pair_expert(idx, q, n_experts) : n_experts;
+    clear_counts(n_experts, cnt);  // each wave its own row
     uint64_t same = ~0ull;
     for (int b = 0; b < bits; ++b) {
       const uint64_t set = __ballot((e >> b) & 1);
@@ -120,11 +153,13 @@ __global__ void __launch_bounds__(kSortThreads)
     if (e < n_experts && rank == 0) cnt[wave][e] = __popcll(same);
     __syncthreads();
     if (tid < n_experts) {
+      int c[kSortWaves];
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) c[w] = cnt[w][tid];
 #pragma unroll
       for (int w = 0; w < kSortWaves; ++w) {
-        const int c = cnt[w][tid];
         cnt[w][tid] = next;
-        next += c;
+        next += c[w];
       }
     }
     __syncthreads();
@@ -136,7 +171,7 @@ __global__ void __launch_bounds__(kSortThreads)
       }
       row_of[q] = row;
     }
-    __syncthreads();
+    if (base + kSortThreads < q1) __syncthreads();  // (which would wait for the stores)
   }
 }
 
@@ -354,8 +389,8 @@ void launch_combine_grad(const void* d_out, const void* rows, int64_t n_rows, in
 
 using namespace hsmoe;
 
-// Up to this many pairs one workgroup sorts alone.
-static constexpr int64_t kSortAlone = 2048;
+// Up to this many pairs every workgroup counts them all, and there is one launch.
+static constexpr int64_t kSortAlone = 32768;
 
 extern "C" size_t hsmoe_moe_sort_workspace_size(int64_t m, int top_k, int64_t n_experts) {
   if (m < 1 || top_k < 1 || n_experts < 1 || m >= (1 << 24) || top_k > 16) return 0;
@@ -381,10 +416,8 @@ extern "C" int hsmoe_moe_sort(const int64_t* topk_idx, int64_t m, int top_k, int
   if (need && (!workspace || workspace_bytes < need))
     return fail(HSMOE_ERR_WORKSPACE, "hsmoe_moe_sort: workspace of %zu bytes needed", need);
   hipStream_t st = (hipStream_t)stream;
-  int64_t chunk = pairs > 0 ? pairs : 1, blocks = 1;
+  const int64_t chunk = pairs > 0 ? sort_chunk(pairs) : 1, blocks = pairs > 0 ? (pairs + chunk - 1) / chunk : 1;
   if (need) {
-    chunk = sort_chunk(pairs);
-    blocks = (pairs + chunk - 1) / chunk;
     hipLaunchKernelGGL(sort_hist_kernel, dim3((unsigned)blocks), dim3(kSortThreads), 0, st, topk_idx, pairs,
                        (int)n_experts, chunk, (int*)workspace);
   }

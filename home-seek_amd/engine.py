@@ -25,9 +25,10 @@ Divergences from the reference, all deliberate:
   * the MTP draft module keeps the reference's data flow (hnorm of the main
     model's last hidden state + enorm of the token embedding, one MoE block
     with the MTP experts, the MTP norm, lm_head, greedy argmax; second draft
-    from the first) without its attention and without the e_proj / h_proj
-    projections, which are outside the MoE path; its experts are one more
-    layer of the HBM store (the checkpoint's mtp.0.ffn.experts.*).
+    from the first) without its attention, and without the e_proj / h_proj
+    projections unless mtp_weights holds them (then the sum is
+    h_proj(hnorm(h)) + e_proj(enorm(e)), two ops.linear calls); its experts are
+    one more layer of the HBM store (the checkpoint's mtp.0.ffn.experts.*).
 """
 from __future__ import annotations
 
@@ -49,7 +50,10 @@ class HomeSeekMoEEngine:
                  embed: torch.Tensor | None = None, mtp_weights: dict | None = None):
         self.config = config
         # mtp_weights: {"hnorm.weight", "enorm.weight", "norm.weight", "layer": layer
-        # weights of the MTP block (as for _forward_layer), "layer_idx": its store layer}
+        # weights of the MTP block (as for _forward_layer), "layer_idx": its store layer},
+        # and optionally both "e_proj.weight" and "h_proj.weight" (bf16 [D, D])
+        if mtp_weights is not None and ("e_proj.weight" in mtp_weights) != ("h_proj.weight" in mtp_weights):
+            raise ValueError("the MTP block has both projections (e_proj.weight, h_proj.weight) or none")
         self._mtp_weights = mtp_weights
         self.store = store
         self.device = store.device
@@ -330,8 +334,15 @@ class HomeSeekMoEEngine:
         h_prev = last_hidden.reshape(1, 1, D)
         tok = last_token_id.reshape(1, 1)
         lw = mw["layer"]
+        projected = "e_proj.weight" in mw
         for j in range(num_draft):
-            if lw.get("ffn_norm.weight") is not None and self._embed_fusable(tok):
+            if projected:
+                e = rms_norm(self._embed(tok).reshape(1, D), mw["enorm.weight"], eps)
+                g = rms_norm(h_prev.reshape(1, D), mw["hnorm.weight"], eps)
+                h_in = ops.linear(g, mw["h_proj.weight"], residual=ops.linear(e, mw["e_proj.weight"]))
+                h_prev, hf = self._forward_layer_norm(h_in.reshape(1, 1, D), lw, mw["layer_idx"], tok,
+                                                      mw["norm.weight"])
+            elif lw.get("ffn_norm.weight") is not None and self._embed_fusable(tok):
                 # embedding, enorm, hnorm, their sum, the residual add and ffn_norm in one launch
                 h1, hn = ops.mtp_input(tok, self.embed, h_prev, mw["enorm.weight"], mw["hnorm.weight"],
                                        lw["ffn_norm.weight"], lw.get("attn.residual"), eps)

@@ -461,6 +461,13 @@ def _weights(w: torch.Tensor, w_up: torch.Tensor | None, order: ExpertOrder | No
     return w, w_up, _row_stride(w), (w.stride(0) if order is not None else 0)
 
 
+def _bias(b: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    if b.shape != w.shape[:-1]:
+        raise ValueError(f"bias {tuple(b.shape)} does not match weights {tuple(w.shape)}")
+    b = _bf16_matrix(b, "bias").contiguous()
+    return b if b.data_ptr() % 16 == 0 else b.clone()
+
+
 def _linear_rows(x: torch.Tensor, what: str, cols: int, order: ExpertOrder | None) -> torch.Tensor:
     """x as rows [M, cols] that the kernels can read."""
     _bf16_matrix(x, what)
@@ -496,14 +503,10 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
     m = x.shape[0]
     if bias_up is not None and act != "swiglu":
         raise ValueError("an up bias goes with act='swiglu'")
-    biases = []
-    for b in (bias, bias_up):
-        if b is not None:
-            if b.shape != w.shape[:-1]:
-                raise ValueError(f"bias {tuple(b.shape)} does not match weights {tuple(w.shape)}")
-            b = _bf16_matrix(b, "bias").contiguous()
-            b = b if b.data_ptr() % 16 == 0 else b.clone()
-        biases.append(b)
+    if bias is not None:
+        bias = _bias(bias, w)
+    if bias_up is not None:
+        bias_up = _bias(bias_up, w)
     ld_res = n
     if residual is not None:
         if residual.shape != lead + (n,):
@@ -518,7 +521,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
         check(lib().hsmoe_linear(ptr(x), _row_stride(x), m, k, ptr(w), ptr(w_up), ldw, group, n,
                                  None if order is None else ptr(order.offsets),
-                                 1 if order is None else order.n_experts, ptr(biases[0]), ptr(biases[1]), ptr(residual),
+                                 1 if order is None else order.n_experts, ptr(bias), ptr(bias_up), ptr(residual),
                                  ld_res, code, limit, kind, ptr(out), ptr(pre), ptr(ws), nbytes, stream_ptr(dev)),
               "hsmoe_linear")
     return (out, pre) if want_pre else out

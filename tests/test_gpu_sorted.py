@@ -48,6 +48,7 @@ SORTS = [
     (0, 6, 256, 0.0), (1, 1, 1, 0.0), (1, 6, 256, 0.0), (3, 16, 5, 0.3), (37, 6, 256, 0.5), (341, 6, 256, 0.0),
     (342, 6, 256, 0.1), (1000, 8, 1024, 0.2), (4096, 6, 256, 0.25), (2048, 1, 2, 0.0), (2049, 1, 1, 0.0),
     (700, 3, 64, 1.0), (50001, 6, 129, 0.1),
+    (4096, 8, 64, 0.1), (4097, 8, 1000, 0.1),
 ]
 
 
