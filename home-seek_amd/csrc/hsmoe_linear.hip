@@ -176,19 +176,28 @@ struct Source {
   }
 };
 
-// Which of a stage's loads: all, the first half, the second half.
+// Which of a stage's loads: all, the first or second half of either operand's,
+// one operand's.
+enum { kPartAll, kPartFirst, kPartSecond, kPartRows, kPartCols };
 template <int kValue>
 struct Part {
   static constexpr int value = kValue;
 };
-constexpr Part<-1> kAll;
-constexpr Part<0> kFirst;
-constexpr Part<1> kSecond;
+constexpr Part<kPartAll> kAll;
+constexpr Part<kPartFirst> kFirst;
+constexpr Part<kPartSecond> kSecond;
+constexpr Part<kPartRows> kRowsOnly;
+constexpr Part<kPartCols> kColsOnly;
+
+// kStages_: the stages, or one of these (reduce_turns with two or three stages
+// of the columns' operand).
+constexpr int kTurnsNear = 0, kTurnsFar = -1;
 
 template <int kBR, int kBC, int kWR, int kWC, int kStages_, bool kTR, bool kTC, bool kGated = false>
 struct Tile {
-  static constexpr int kStages = kStages_ == 0 ? 2 : kStages_;
-  static constexpr bool kTurns = kStages_ == 0;
+  static constexpr int kStages = kStages_ <= 0 ? 2 : kStages_;
+  static constexpr bool kTurns = kStages_ <= 0;
+  static constexpr int kColStages = kStages_ == kTurnsFar ? 3 : kStages;
   static constexpr int kWaves = kWR * kWC;
   static constexpr int kThreads = kWaves * 64;
   static constexpr int kFR = kBR / kWR / 16, kFC = kBC / kWC / 16;  // 16 x 16 blocks per wave
@@ -197,23 +206,26 @@ struct Tile {
   using R = Operand<kBR, kWaves, kTR, false, false>;
   using C = Operand<kBC, kWaves, kTC, true, kGated>;
   static constexpr int kStage = R::kBytes + C::kBytes;
+  static constexpr int kLds = kStages * R::kBytes + kColStages * C::kBytes;
   static constexpr int kLoads = R::kLoads + C::kLoads;  // per wave and stage
 
-  // A stage's loads: all of them (part -1), or either half.
+  // Loads of a stage into r_stage and c_stage.
   template <int kPart>
   static __device__ __forceinline__ void load(const Source<R>& rs, int64_t r_first, const Source<C>& cs, int64_t c_first,
-                                              int left, char* stage, int wave) {
-    rs.template load<kPart == 1 ? R::kLoads / 2 : 0, kPart == 0 ? R::kLoads / 2 : R::kLoads>(r_first, left, stage, wave);
-    cs.template load<kPart == 1 ? C::kLoads / 2 : 0, kPart == 0 ? C::kLoads / 2 : C::kLoads>(c_first, left,
-                                                                                              stage + R::kBytes, wave);
+                                              int left, char* r_stage, char* c_stage, int wave) {
+    constexpr bool kHalf0 = kPart == kPartFirst, kHalf1 = kPart == kPartSecond;
+    if constexpr (kPart != kPartCols)
+      rs.template load<kHalf1 ? R::kLoads / 2 : 0, kHalf0 ? R::kLoads / 2 : R::kLoads>(r_first, left, r_stage, wave);
+    if constexpr (kPart != kPartRows)
+      cs.template load<kHalf1 ? C::kLoads / 2 : 0, kHalf0 ? C::kLoads / 2 : C::kLoads>(c_first, left, c_stage, wave);
   }
 
-  static __device__ __forceinline__ void read(const char* stage, int wr, int wc, int kk, int lane, bf16x8 (&c)[kFC],
-                                              bf16x8 (&r)[kFR]) {
+  static __device__ __forceinline__ void read(const char* r_stage, const char* c_stage, int wr, int wc, int kk, int lane,
+                                              bf16x8 (&c)[kFC], bf16x8 (&r)[kFR]) {
 #pragma unroll
-    for (int j = 0; j < kFC; ++j) c[j] = C::frag(stage + R::kBytes, wc * kFC * 16, j, kk, lane);
+    for (int j = 0; j < kFC; ++j) c[j] = C::frag(c_stage, wc * kFC * 16, j, kk, lane);
 #pragma unroll
-    for (int i = 0; i < kFR; ++i) r[i] = R::frag(stage, wr * kFR * 16, i, kk, lane);
+    for (int i = 0; i < kFR; ++i) r[i] = R::frag(r_stage, wr * kFR * 16, i, kk, lane);
   }
   static __device__ __forceinline__ void product(const bf16x8 (&c)[kFC], const bf16x8 (&r)[kFR],
                                                  f32x4 (&acc)[kFR][kFC]) {
@@ -227,7 +239,7 @@ struct Tile {
 #pragma unroll
     for (int kk = 0; kk < kBK / 32; ++kk) {
       bf16x8 c[kFC], r[kFR];
-      read(stage, wr, wc, kk, lane, c, r);
+      read(stage, stage + R::kBytes, wr, wc, kk, lane, c, r);
       product(c, r, acc);
     }
   }
@@ -239,15 +251,18 @@ struct Tile {
 // products may come later), then all meet: the stage is whole, and nobody reads
 // the one that is loaded next.
 template <typename T, typename Load>
-__device__ __forceinline__ void reduce_stages(const char* lds, int steps, int wr, int wc, int lane, const Load& load,
+__device__ __forceinline__ void reduce_stages(char* lds, int steps, int wr, int wc, int lane, const Load& load,
                                               f32x4 (&acc)[T::kFR][T::kFC]) {
   static_assert(T::kStages == 2, "a stage in use, a stage on its way");
-  if (steps > 0) load(0, 0, kAll);
+  auto fill = [&](int s, int slot, auto part) {
+    load(s, lds + slot * T::kStage, lds + slot * T::kStage + T::R::kBytes, part);
+  };
+  if (steps > 0) fill(0, 0, kAll);
   for (int s = 0; s < steps; ++s) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + 1 < steps) load(s + 1, (s + 1) & 1, kAll);
+    if (s + 1 < steps) fill(s + 1, (s + 1) & 1, kAll);
     T::multiply(lds + (s & 1) * T::kStage, wr, wc, lane, acc);
   }
 }
@@ -258,7 +273,7 @@ __device__ __forceinline__ void reduce_stages(const char* lds, int steps, int wr
 // before it is done, so the wait and the barrier for it come in mid-stage; the
 // place of the stage that is loaded was read to its end before the last barrier.
 template <typename T, typename Load>
-__device__ __forceinline__ void reduce_ahead(const char* lds, int steps, int wr, int wc, int lane, const Load& load,
+__device__ __forceinline__ void reduce_ahead(char* lds, int steps, int wr, int wc, int lane, const Load& load,
                                              f32x4 (&acc)[T::kFR][T::kFC]) {
   constexpr int S = T::kStages, kHalf = T::kLoads / 2;
   static_assert(S >= 3 && T::kLoads % 2 == 0, "a stage is waited for while two others are in use");
@@ -276,6 +291,9 @@ __device__ __forceinline__ void reduce_ahead(const char* lds, int steps, int wr,
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
   };
+  auto fill = [&](int s, int slot, auto part) {
+    load(s, lds + slot * T::kStage, lds + slot * T::kStage + T::R::kBytes, part);
+  };
   auto mix = [&]() {  // the order of what stands between two barriers
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -285,19 +303,23 @@ __device__ __forceinline__ void reduce_ahead(const char* lds, int steps, int wr,
     }
   };
   if (steps == 0) return;
-  for (int s = 0; s < S - 1; ++s) load(s, s, kAll);
+  for (int s = 0; s < S - 1; ++s) fill(s, s, kAll);
   wait(true);
-  T::read(lds, wr, wc, 0, lane, c[0], r[0]);
+  auto read = [&](int slot, int kk) {
+    const char* stage = lds + slot * T::kStage;
+    T::read(stage, stage + T::R::kBytes, wr, wc, kk, lane, c[kk], r[kk]);
+  };
+  read(0, 0);
   int at = 0, next = S - 1;
   for (int s = 0; s < steps; ++s) {
     const int after = at + 1 == S ? 0 : at + 1;
-    load(s + S - 1, next, kFirst);
-    T::read(lds + at * T::kStage, wr, wc, 1, lane, c[1], r[1]);
+    fill(s + S - 1, next, kFirst);
+    read(at, 1);
     T::product(c[0], r[0], acc);
     mix();
     wait(false);
-    load(s + S - 1, next, kSecond);
-    T::read(lds + after * T::kStage, wr, wc, 0, lane, c[0], r[0]);
+    fill(s + S - 1, next, kSecond);
+    read(after, 0);
     T::product(c[1], r[1], acc);
     mix();
     at = after;
@@ -313,15 +335,24 @@ __device__ __forceinline__ void reduce_ahead(const char* lds, int steps, int wr,
 //   read 0, load / multiply 1 of the stage before;  multiply 0 / read 0, load;
 //   read 1 / multiply 0;  multiply 1 / read 1
 // so both have read a stage when the first half starts on the next but one,
-// which goes into its place, and a stage's loads have two turns at least
-// between their issue and the wait for them at the end of the last turn.
+// which goes into its place: a stage's loads have two turns at least between
+// their issue and the wait for them at the end of the last turn.
+// Three stages of the columns' operand (kTurnsFar, for matrices that are read
+// once): its loads are issued a stage earlier, behind the rows' of the stage
+// before, and the wait leaves them in flight (loads return in order); stages
+// beyond the last are loaded too, from nowhere, to keep the count.  Experts of
+// 192 rows: 273 -> 258 us (w), 289 -> 272 (dx); a dense product of 4096^3, which
+// finds w in the caches, 110 -> 118.
 template <typename T, typename Load>
-__device__ __forceinline__ void reduce_turns(const char* lds, int steps, int rows, int wave, int wr, int wc, int lane,
+__device__ __forceinline__ void reduce_turns(char* lds, int steps, int rows, int wave, int wr, int wc, int lane,
                                              const Load& load, f32x4 (&acc)[T::kFR][T::kFC]) {
-  static_assert(T::kWaves == 8 && T::kStages == 2, "two waves per SIMD, two stages");
+  static_assert(T::kWaves == 8, "two waves per SIMD");
   const bool second = wave >= 4;
   bf16x8 c[T::kFC], r[T::kFR];
-  auto read = [&](int s, int kk) { T::read(lds + (s & 1) * T::kStage, wr, wc, kk, lane, c, r); };
+  char* const c_lds = lds + 2 * T::R::kBytes;
+  auto load_rows = [&](int s) { load(s, lds + (s & 1) * T::R::kBytes, c_lds, kRowsOnly); };
+  auto load_cols = [&](int s, int slot) { load(s, lds, c_lds + slot * T::C::kBytes, kColsOnly); };
+  constexpr bool kAhead = T::kColStages == 3;
   // (a wave without rows in the tile only keeps the turns; skipping half of its
   // blocks too costs the registers of a second copy of the products)
   const bool live = rows > wr * T::kFR * 16;
@@ -330,29 +361,41 @@ __device__ __forceinline__ void reduce_turns(const char* lds, int steps, int row
     if (live) T::product(c, r, acc);
     __builtin_amdgcn_s_setprio(0);
   };
-  auto turn = [&](bool loads) {  // ends a turn; loads: the wave's own loads are in LDS
-    if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  auto turn = [&](bool loads) {  // ends a turn; loads: the next stage, as far as the wave loads it, is in LDS
+    if (loads) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kAhead ? T::C::kLoads : 0) : "memory");
     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
   };
-  if (steps > 0) load(0, 0, kAll);
+  if (steps == 0) return;
+  load_cols(0, 0);
+  load_rows(0);
+  if (kAhead) load_cols(1, 1);
   turn(true);
   if (second) turn(false);
+  int at = 0;  // s modulo the columns' stages
   for (int s = 0; s < steps; ++s) {
-    read(s, 0);
-    if (s + 1 < steps) load(s + 1, (s + 1) & 1, kAll);
+    const char* rs = lds + (s & 1) * T::R::kBytes;
+    const char* cs = c_lds + at * T::C::kBytes;
+    const int before = at == 0 ? T::kColStages - 1 : at - 1;  // the stage that was read to its end
+    T::read(rs, cs, wr, wc, 0, lane, c, r);
+    if (kAhead || s + 1 < steps) {
+      load_rows(s + 1);
+      load_cols(s + T::kColStages - 1, before);
+    }
     turn(false);
     multiply();
     turn(false);
-    read(s, 1);
+    T::read(rs, cs, wr, wc, 1, lane, c, r);
     turn(second);
     multiply();
     turn(!second);
+    at = at == T::kColStages - 1 ? 0 : at + 1;
   }
   if (!second) turn(false);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may reach LDS after the workgroup's end
 }
 
 // ---------------------------------------------------------------- groups
@@ -442,7 +485,7 @@ __device__ __forceinline__ bool place_tile(int b, int row_tiles, int col_tiles, 
 }
 
 template <typename T, typename Load>
-__device__ __forceinline__ void reduce(const char* lds, int steps, int rows, int wave, int wr, int wc, int lane,
+__device__ __forceinline__ void reduce(char* lds, int steps, int rows, int wave, int wr, int wc, int lane,
                                        const Load& load, f32x4 (&acc)[T::kFR][T::kFC]) {
   if constexpr (T::kTurns)
     reduce_turns<T>(lds, steps, rows, wave, wr, wc, lane, load, acc);
@@ -637,7 +680,7 @@ __device__ __forceinline__ void clear8(const LinearParams& p, int64_t m, int64_t
 template <int kBR, int kBC, int kWR, int kWC, int kStages, bool kGated>
 __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) linear_kernel(LinearParams p) {
   using T = Tile<kBR, kBC, kWR, kWC, kStages, false, false, kGated>;
-  __shared__ __align__(1024) char lds[T::kStages * T::kStage];
+  __shared__ __align__(1024) char lds[T::kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kCols = kGated ? kBC / 2 : kBC;  // output columns per tile
   const TileScan scan = scan_tiles<kBR>(p.offsets, p.n_groups, p.n_rows, lane);
@@ -667,11 +710,12 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   xs.open(p.x + sp.row * p.ldx, nullptr, p.ldx, rows, p.k * 2, wave, lane);
   Source<typename T::C> ws;
   ws.open(p.w[0] + wo, p.w[1] + wo, p.ldw, cols, p.k * 2, wave, lane);
-  auto load = [&](int s, int slot, auto part) {
+  auto load = [&](int s, char* r_stage, char* c_stage, auto part) {
     const int at = s + turned < steps.count ? s + turned : s + turned - steps.count;
     const int first = (steps.first + at) * kBK;
     T::template load<decltype(part)::value>(xs, first, ws, first, s < steps.count ? (int)p.k - first : 0,
-                                            lds + slot * T::kStage, wave);
+                                            r_stage, c_stage,
+                                            wave);
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
@@ -920,7 +964,7 @@ __device__ __forceinline__ void store_tile(char* out, int64_t width, int64_t row
 template <int kBR, int kBC, int kWR, int kWC, int kStages>
 __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) linear_grad_input_kernel(LinearGradParams p) {
   using T = Tile<kBR, kBC, kWR, kWC, kStages, false, true>;
-  __shared__ __align__(1024) char lds[T::kStages * T::kStage];
+  __shared__ __align__(1024) char lds[T::kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const TileScan scan = scan_tiles<kBR>(p.offsets, p.n_groups, p.n_rows, lane);
   int rt, ct;
@@ -942,11 +986,12 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   Source<typename T::C> ws;
   const int64_t wo = sp.group * p.w_group + c0 * 2;
   ws.open(p.w[0] + wo, nullptr, p.ldw, 0, cols * 2, wave, lane);
-  auto load = [&](int s, int slot, auto part) {
+  auto load = [&](int s, char* r_stage, char* c_stage, auto part) {
     const int step = steps.first + s, mat = step >= per ? 1 : 0, first = (step - mat * per) * kBK;
     ws.base[0] = (mat ? p.w[1] : p.w[0]) + wo;
     T::template load<decltype(part)::value>(zs, mat * p.n + first, ws, first, s < steps.count ? (int)p.n - first : 0,
-                                            lds + slot * T::kStage, wave);
+                                            r_stage, c_stage,
+                                            wave);
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
@@ -960,7 +1005,7 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
 template <int kBR, int kBC, int kWR, int kWC, int kStages>
 __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) linear_grad_weight_kernel(LinearGradParams p) {
   using T = Tile<kBR, kBC, kWR, kWC, kStages, true, true>;
-  __shared__ __align__(1024) char lds[T::kStages * T::kStage];
+  __shared__ __align__(1024) char lds[T::kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row_tiles = (int)((p.n + kBR - 1) / kBR), col_tiles = (int)((p.k + kBC - 1) / kBC);
   int rt, ct;
@@ -976,10 +1021,11 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   zs.open(p.dz + first * p.ldz + (mat * p.n + n0) * 2, nullptr, p.ldz, 0, nrow * 2, wave, lane);
   Source<typename T::C> xs;
   xs.open(p.x + first * p.ldx + c0 * 2, nullptr, p.ldx, 0, ncol * 2, wave, lane);
-  auto load = [&](int s, int slot, auto part) {
+  auto load = [&](int s, char* r_stage, char* c_stage, auto part) {
     const int first_step = (steps.first + s) * kBK;
     T::template load<decltype(part)::value>(zs, first_step, xs, first_step, s < steps.count ? (int)count - first_step : 0,
-                                            lds + slot * T::kStage, wave);
+                                            r_stage, c_stage,
+                                            wave);
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x4 acc[T::kFR][T::kFC] = {};
@@ -1347,7 +1393,8 @@ extern "C" int hsmoe_linear(const void* x, int64_t x_row_stride, int64_t m, int6
   p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
   hipStream_t st = (hipStream_t)stream;
   if (plan.tile == kNarrow) return launch_narrow(p, st);
-  if (plan.tile == 0) return launch_linear<256, 256, 2, 4, 0>(p, st);
+  if (plan.tile == 0 && offsets) return launch_linear<256, 256, 2, 4, kTurnsFar>(p, st);
+  if (plan.tile == 0) return launch_linear<256, 256, 2, 4, kTurnsNear>(p, st);
   if (plan.tile == 1) return launch_linear<128, 128, 2, 2, 4>(p, st);
   if (plan.tile == 2) return launch_linear<64, 128, 2, 2, 4>(p, st);
   return launch_linear<128, 128, 2, 2, 2>(p, st);
@@ -1442,7 +1489,8 @@ extern "C" int hsmoe_linear_grad_input(const void* dz, int64_t dz_row_stride, in
   if (int rc = check_workspace("hsmoe_linear_grad_input", plan, workspace, workspace_bytes)) return rc;
   p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  if (plan.tile == 0) return launch_grad_input<256, 256, 2, 4, 0>(p, st);
+  if (plan.tile == 0 && offsets) return launch_grad_input<256, 256, 2, 4, kTurnsFar>(p, st);
+  if (plan.tile == 0) return launch_grad_input<256, 256, 2, 4, kTurnsNear>(p, st);
   if (plan.tile == 1) return launch_grad_input<128, 128, 2, 2, 4>(p, st);
   if (plan.tile == 2) return launch_grad_input<64, 128, 2, 2, 4>(p, st);
   return launch_grad_input<128, 128, 2, 2, 2>(p, st);
@@ -1474,6 +1522,6 @@ extern "C" int hsmoe_linear_grad_weight(const void* dz, int64_t dz_row_stride, c
   if (int rc = check_workspace("hsmoe_linear_grad_weight", plan, workspace, workspace_bytes)) return rc;
   p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  if (plan.tile == 0) return launch_grad_weight<256, 256, 2, 4, 0>(p, st);
+  if (plan.tile == 0) return launch_grad_weight<256, 256, 2, 4, kTurnsNear>(p, st);
   return launch_grad_weight<128, 128, 2, 2, 4>(p, st);
 }
