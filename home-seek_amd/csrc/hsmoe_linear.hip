@@ -267,11 +267,11 @@ __device__ __forceinline__ void reduce_stages(char* lds, int steps, int wr, int 
   }
 }
 
-// The reduction with one wave per SIMD, three stages or more: operands of the next 32
-// reduction steps are read, and half a stage's loads are issued, between the
-// products of the current ones.  A stage's first half is read before the stage
-// before it is done, so the wait and the barrier for it come in mid-stage; the
-// place of the stage that is loaded was read to its end before the last barrier.
+// The reduction with three stages or more: operands of the next 32 reduction
+// steps are read, and half a stage's loads are issued, between the products of
+// the current ones.  A stage's first half is read before the stage before it is
+// done, so the wait and the barrier for it come in mid-stage; the place of the
+// stage that is loaded was read to its end before the last barrier.
 template <typename T, typename Load>
 __device__ __forceinline__ void reduce_ahead(char* lds, int steps, int wr, int wc, int lane, const Load& load,
                                              f32x4 (&acc)[T::kFR][T::kFC]) {
@@ -1205,10 +1205,11 @@ constexpr int kNarrow = -1;
 // The tiles, with what a round of workgroups (one or two per CU) takes for 64
 // reduction steps and for the rest (first loads, epilogue), in us with every CU
 // at work, and the rate at which they stream matrices that are read once:
-//   256 x 256, turns of eight waves        1.30 + 14, 4.7 TB/s
+//   256 x 256, turns of eight waves        1.36 + 14, 4.7 TB/s
 //   128 x 128, 4 stages                    0.62 + 7,  5.4 TB/s
 //   64 x 128, 4 stages                     0.44 + 5,  5.3 TB/s
 //   128 x 128, 2 stages, two per CU        1.15 + 10, 5.8 TB/s
+//   256 x 128, 3 stages, eight waves       0.83 + 10, 4.7 TB/s
 // (swiglu's two matrices, in tiles of half the columns: 0.87 of that.)  The
 // kernel for few rows streams w at 5.3 TB/s less 3% per row.  What takes the
 // least time by these figures is taken; a split reduction costs the fp32 sums'
@@ -1217,10 +1218,12 @@ struct TileCost {
   int rows, cols, per_cu;
   double step, rest, rate;  // us, us, bytes per us
 };
-constexpr TileCost kTiles[] = {{256, 256, 1, 1.30, 14.0, 4.7e6},
+constexpr TileCost kTiles[] = {{256, 256, 1, 1.36, 14.0, 4.7e6},
                                {128, 128, 1, 0.62, 7.0, 5.4e6},
                                {64, 128, 1, 0.44, 5.0, 5.3e6},
-                               {128, 128, 2, 1.15, 10.0, 5.8e6}};
+                               {128, 128, 2, 1.15, 10.0, 5.8e6},
+                               {256, 128, 1, 0.83, 10.0, 4.7e6}};
+constexpr int kAllTiles = 5, kGatedTiles = 4;  // (the last one does not hold swiglu's two sums in its registers)
 
 // rows: of the output, in groups of which at most `active` have any (one: dense);
 // cols: tiles' columns (twice the output's for swiglu); bytes: of the groups'
@@ -1255,7 +1258,8 @@ Plan plan_linear(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
   const double rows = (double)m / (double)active, bytes = 2.0 * active * n * mats * k;
   double tiled;
   const Plan plan = plan_tiles((double)m, (double)active, n * mats, (k + kBK - 1) / kBK,
-                               mats == 2 ? bytes / 0.87 : bytes, (double)m * n * mats, 0, 4, tiled);
+                               mats == 2 ? bytes / 0.87 : bytes, (double)m * n * mats, 0,
+                               mats == 2 ? kGatedTiles : kAllTiles, tiled);
   const double narrow = 2.0 + bytes / 5.3e6 * (1.0 + 0.03 * rows);
   return rows <= kNarrowRows && narrow < tiled ? Plan{kNarrow, 1, 0} : plan;
 }
@@ -1263,7 +1267,7 @@ Plan plan_grad_input(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats
   const int64_t active = n_groups < m ? n_groups : m;
   double us;
   return plan_tiles((double)m, (double)active, k, (n + kBK - 1) / kBK * mats, 2.0 * active * n * mats * k, (double)m * k,
-                    0, 4, us);
+                    0, kAllTiles, us);
 }
 // (both operands transposed: no tile of 64 rows)
 Plan plan_grad_weight(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
@@ -1282,19 +1286,19 @@ int check_workspace(const char* what, const Plan& plan, const void* ws, size_t b
 
 unsigned join_grid(int64_t values) { return (unsigned)((values / 8 + 255) / 256); }
 
-template <int kBR, int kBC, int kWR, int kWC, int kStages>
-int launch_linear(const LinearParams& p, hipStream_t st) {
-  const bool gated = p.act == HSMOE_ACT_SWIGLU;
+template <int kBR, int kBC, int kWR, int kWC, int kStages, bool kGated>
+int launch_linear_as(const LinearParams& p, hipStream_t st) {
   const int64_t row_tiles = max_row_tiles(p.n_rows, kBR, p.offsets, p.n_groups) * p.splits;
-  const unsigned grid = tile_grid(row_tiles, p.n, gated ? kBC / 2 : kBC);
+  const unsigned grid = tile_grid(row_tiles, p.n, kGated ? kBC / 2 : kBC);
   if (!grid) return fail(HSMOE_ERR_SHAPE, "hsmoe_linear: too many tiles");
-  const dim3 block(kWR * kWC * 64);
-  if (gated)
-    hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, kStages, true>), dim3(grid), block, 0, st, p);
-  else
-    hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, kStages, false>), dim3(grid), block, 0, st, p);
+  hipLaunchKernelGGL((linear_kernel<kBR, kBC, kWR, kWC, kStages, kGated>), dim3(grid), dim3(kWR * kWC * 64), 0, st, p);
   if (p.part) hipLaunchKernelGGL(linear_join_kernel, dim3(join_grid(p.n_rows * p.n)), dim3(256), 0, st, p);
   return check_launch("hsmoe_linear");
+}
+template <int kBR, int kBC, int kWR, int kWC, int kStages>
+int launch_linear(const LinearParams& p, hipStream_t st) {
+  if (p.act == HSMOE_ACT_SWIGLU) return launch_linear_as<kBR, kBC, kWR, kWC, kStages, true>(p, st);
+  return launch_linear_as<kBR, kBC, kWR, kWC, kStages, false>(p, st);
 }
 
 int launch_narrow(const LinearParams& p, hipStream_t st) {
@@ -1397,7 +1401,8 @@ extern "C" int hsmoe_linear(const void* x, int64_t x_row_stride, int64_t m, int6
   if (plan.tile == 0) return launch_linear<256, 256, 2, 4, kTurnsNear>(p, st);
   if (plan.tile == 1) return launch_linear<128, 128, 2, 2, 4>(p, st);
   if (plan.tile == 2) return launch_linear<64, 128, 2, 2, 4>(p, st);
-  return launch_linear<128, 128, 2, 2, 2>(p, st);
+  if (plan.tile == 3) return launch_linear<128, 128, 2, 2, 2>(p, st);
+  return launch_linear_as<256, 128, 4, 2, 3, false>(p, st);
 }
 
 extern "C" size_t hsmoe_linear_act_grad_workspace_size(int64_t m, int64_t n, int64_t n_groups, int act) {
@@ -1493,7 +1498,8 @@ extern "C" int hsmoe_linear_grad_input(const void* dz, int64_t dz_row_stride, in
   if (plan.tile == 0) return launch_grad_input<256, 256, 2, 4, kTurnsNear>(p, st);
   if (plan.tile == 1) return launch_grad_input<128, 128, 2, 2, 4>(p, st);
   if (plan.tile == 2) return launch_grad_input<64, 128, 2, 2, 4>(p, st);
-  return launch_grad_input<128, 128, 2, 2, 2>(p, st);
+  if (plan.tile == 3) return launch_grad_input<128, 128, 2, 2, 2>(p, st);
+  return launch_grad_input<256, 128, 4, 2, 3>(p, st);
 }
 
 extern "C" int hsmoe_linear_grad_weight(const void* dz, int64_t dz_row_stride, const void* x, int64_t x_row_stride,
