@@ -37,11 +37,13 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 // 16 bytes per lane from global memory to LDS, lane l's to dst + 16 l.  Written
 // out because the compiler waits for every such load it knows of before each
 // ds_read_b64_tr_b16, whatever it reads; the waits are reduce_*'s.  No register
-// is written: the load takes its address when it is issued.
+// is written: the load takes its address when it is issued.  (s_nop 4: a vector
+// instruction may have written the resource's scalar registers, v_readfirstlane
+// for one; a memory instruction may read them five wait states later.)
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void lds_load16(i32x4 r, uint32_t off, const char* dst) {
   const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)dst;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(at), "v"(off), "s"(r)
                : "memory", "m0");
