@@ -433,6 +433,8 @@ def _bf16_matrix(t: torch.Tensor, what: str) -> torch.Tensor:
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t, or a contiguous copy where its rows are not 16-byte aligned ones of consecutive elements."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t  # (a row that is no multiple of 8 values is refused below)
     if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for s in t.stride()[:-1]):
         return t.contiguous() if not t.is_contiguous() else t.clone()
     if t.dim() > 1 and t.shape[-2] > 1 and t.stride(-2) < t.shape[-1]:
@@ -514,7 +516,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
         residual = _linear_rows(residual, "residual", n, None)
         ld_res = _row_stride(residual)
     kind = _row_kind(out_dtype, "the output")
-    out = torch.empty(lead + (n,), dtype=out_dtype, device=dev)
+    out = torch.empty((m, n) if len(lead) == 1 else lead + (n,), dtype=out_dtype, device=dev)
     pre = torch.empty(lead + (2 * n if act == "swiglu" else n,), dtype=torch.bfloat16, device=dev) if want_pre else None
     with _on(dev):
         nbytes = lib().hsmoe_linear_workspace_size(m, n, k, 1 if order is None else order.n_experts, code)

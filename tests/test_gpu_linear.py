@@ -100,7 +100,8 @@ def check_forward(dev, m, n, k, act, order=None, lead=(), with_bias=True, with_r
 SHAPES = [(1, 8, 8), (1, 4096, 4096), (3, 64, 72), (5, 1000, 520), (8, 2048, 1024), (16, 256, 64), (17, 136, 4096),
           (31, 520, 2048), (33, 4096, 128), (64, 72, 1000), (100, 264, 136), (127, 128, 64), (129, 1288, 200),
           (500, 2048, 512), (1000, 504, 1032), (2049, 4096, 256), (4093, 2056, 64),
-          (4100, 4104, 72)]  # the last one: more than 256 tiles of 256 x 256
+          (4100, 4104, 72),  # more than 256 tiles of 256 x 256
+          (1500, 4096, 136), (1900, 2048, 136)]  # tiles of 256 x 128; of 128 x 128, two per CU, for swiglu
 
 
 @pytest.mark.parametrize("act", [None, "silu", "swiglu"])
@@ -285,7 +286,8 @@ def check_grad(dev, m, n, k, act, order=None, lead=()):
 
 @pytest.mark.parametrize("act", [None, "silu", "swiglu"])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (1, 1024, 512), (3, 64, 72), (17, 136, 264), (64, 256, 128), (65, 72, 1000),
-                                   (130, 520, 136), (500, 512, 512), (1001, 264, 520), (300, 2048, 4096), (4100, 72, 4104), (72, 4104, 4104)])
+                                   (130, 520, 136), (500, 512, 512), (1001, 264, 520), (300, 2048, 4096), (4100, 72, 4104), (72, 4104, 4104),
+                                   (1500, 136, 4096), (2000, 1024, 1024)])
 def test_dense_gradient(dev, m, n, k, act):
     check_grad(dev, m, n, k, act)
 
@@ -366,6 +368,59 @@ def test_deterministic_and_replayed(dev):
         torch.cuda.synchronize()
         for a, b in zip(outs, step()):
             assert torch.equal(a, b)
+
+
+def test_matrices_that_are_read_once(dev):
+    """64 experts of 2048 x 4096 with a few rows each: the kernels for which w's stream is what counts."""
+    e, n, k = 64, 2048, 4096
+    w = ints(dev, 1, (e, n, k))
+    for m, top_k in ((40, 2), (700, 2), (3000, 2)):
+        order = some_order(dev, m, top_k, e, m)
+        x, d = ints(dev, 2, (m * top_k, k), top=1), ints(dev, 3, (m * top_k, n), top=1)
+        out, dx = ops.linear(x, w, order=order), ops.linear_grad(d, x, w, order=order, need_w=False).x
+        for i, a, b in spans(order, m * top_k):
+            if b > a:
+                assert torch.equal(out[a:b], (x[a:b].double() @ w[i].double().T).to(F32).to(BF16))
+                assert torch.equal(dx[a:b], (d[a:b].double() @ w[i].double()).to(F32).to(BF16))
+
+
+def test_two_graphs_at_once(dev):
+    """Products whose reduction is split hand their sums through a workspace: each call's own, so that graphs of
+    several streams may run together."""
+    m, n, k = 64, 4096, 4096
+    w = ints(dev, 1, (n, k))
+    runs = []
+    for seed in (2, 3):
+        x, d = ints(dev, seed, (m, k)), ints(dev, seed + 5, (m, n))
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            ops.linear(x, w)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outs = [(ops.linear(x, w), ops.linear_grad(d, x, w, need_bias=True)) for _ in range(4)]
+        # x and d stay alive with the graph that reads them
+        runs.append((stream, graph, outs, ops.linear(x, w), ops.linear_grad(d, x, w, need_bias=True), x, d))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for stream, graph, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, _, outs, y, g, *_ in runs:
+            for out, grad in outs:
+                assert torch.equal(out, y)
+                assert all(torch.equal(a, b) for a, b in zip(grad[:3], g[:3]))
+
+
+def test_offsets_beyond_the_rows_are_cut(dev):
+    """An order that does not come from moe_sort: what its offsets say beyond the rows that there are counts for nothing."""
+    x, w, d = ints(dev, 1, (4, 64)), ints(dev, 2, (2, 8, 64)), ints(dev, 3, (4, 8))
+    good = ops.ExpertOrder(*(torch.tensor(t, dtype=torch.int32, device=dev) for t in ([0, 2, 4], [0, 1, 2, 3], [[0, 1], [2, 3]])))
+    far = good._replace(offsets=torch.tensor([-7, 2, 1 << 30], dtype=torch.int32, device=dev))
+    assert torch.equal(ops.linear(x, w, order=far), ops.linear(x, w, order=good))
+    for a, b in zip(ops.linear_grad(d, x, w, order=far, need_bias=True), ops.linear_grad(d, x, w, order=good, need_bias=True)):
+        assert a is None and b is None or torch.equal(a, b)
 
 
 def test_weights_beyond_32_bits(dev):

@@ -83,6 +83,21 @@ def test_sort_of_one_expert_and_int32_ids(dev):
     assert all(torch.equal(s, t) for s, t in zip(a, b))
 
 
+def test_ids_of_any_size_are_no_experts(dev):
+    idx = torch.tensor([[1 << 40, 0], [-(1 << 40), (1 << 32) + 1], [1, -1]], device=dev)
+    order = ops.moe_sort(idx, 2)
+    assert order.offsets.tolist() == [0, 1, 2] and order.pairs.tolist() == [1, 4, -1, -1, -1, -1]
+    assert order.rows.tolist() == [[-1, 0], [-1, -1], [1, -1]]
+
+
+def test_a_row_number_that_is_none_counts_as_dropped(dev):
+    order = ops.moe_sort(torch.tensor([[0, 1], [1, 0]], device=dev), 2)
+    wild = order._replace(rows=torch.tensor([[0, 1 << 30], [-5, 1]], dtype=torch.int32, device=dev))
+    rows, w = torch.randn(4, 64, device=dev), torch.ones(2, 2, device=dev)
+    assert torch.equal(ops.moe_combine(rows, wild, w), rows[:2])
+    assert ops.moe_combine_grad(rows[:2], rows, wild, w)[1][0, 1] == 0
+
+
 ROWS = [(1, 6, 256, 4096, 0.0), (5, 6, 256, 4096, 0.4), (37, 3, 9, 72, 0.2), (33, 16, 40, 1001, 0.5), (200, 9, 64, 520, 0.1),
         (3, 2, 4, 1, 0.0), (700, 6, 64, 2048, 1.0), (2, 1, 3, 16392, 0.0)]
 
