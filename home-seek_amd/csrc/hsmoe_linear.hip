@@ -20,7 +20,6 @@ constexpr int kMaxGroups = 1024;
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) char lds_char;
 
 __device__ __forceinline__ int64_t imin64(int64_t a, int64_t b) { return a < b ? a : b; }
 
@@ -435,6 +434,8 @@ __device__ __forceinline__ TileScan scan_tiles(const int* offsets, int n_groups,
       tiles += b > a ? (int)((b - a + kBR - 1) / kBR) : 0;
     }
   }
+  // (a launch has 2^22 at most; groups that overlap could name more than an int counts)
+  tiles = tiles < 1 << 24 ? tiles : 1 << 24;
   int v = tiles;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {

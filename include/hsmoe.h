@@ -369,9 +369,11 @@ int hsmoe_moe_combine_grad(const void* d_out_dev, int out_kind, const void* rows
  * (both for w_up too); out [m, n] bf16 or fp32 (out_kind), contiguous.  NULL: no
  * bias, residual, pre.  offsets int32 [n_groups + 1]: group g is rows offsets[g]
  * .. offsets[g + 1] - 1; rows from offsets[n_groups] on are zeros (no bias, no
- * residual); NULL: n_groups = 1, all rows.  limit > 0 (INFINITY: none), read for
+ * residual); NULL: n_groups = 1, all rows.  They rise from offsets[0] = 0; others
+ * lead nowhere outside the tensors, but leave rows undefined.  limit > 0 (INFINITY: none), read for
  * swiglu only.  n and k multiples of 8, rows 16-byte aligned, row strides below
- * 2^22, n_groups <= 1024, m < 2^31 - 1024.  Few rows: the reduction may be shared
+ * 2^22, n_groups <= 1024, m < 2^31 - 1024, and at most 2^22 tiles of 64 x 64
+ * results (a group's last may be partly empty).  Few rows: the reduction may be shared
  * by several workgroups per tile, whose sums go through the workspace (any
  * contents; hsmoe_linear_workspace_size bytes, 0 for most shapes). */
 #define HSMOE_ACT_NONE 0

@@ -423,6 +423,19 @@ def test_offsets_beyond_the_rows_are_cut(dev):
         assert a is None and b is None or torch.equal(a, b)
 
 
+@pytest.mark.parametrize("m", [4, 40, 1000])
+def test_groups_that_overlap_stay_inside(dev, m):
+    """Offsets that rise and fall, which no sort gives: rows are undefined then, what is summed per group is not."""
+    x, w = ints(dev, 1, (m, 64)), ints(dev, 2, (3, 8, 64))
+    off = torch.tensor([0, m, 0, m], dtype=torch.int32, device=dev)  # groups 0 and 2 have all rows, group 1 none
+    order = ops.ExpertOrder(off, torch.arange(m, dtype=torch.int32, device=dev), torch.arange(m, dtype=torch.int32, device=dev)[:, None].contiguous())
+    assert ops.linear(x, w, order=order).shape == (m, 8)
+    grad = ops.linear_grad(ints(dev, 3, (m, 8)), x, w, order=order)
+    assert not bool(grad.w[1].any())
+    for g in (0, 2):
+        assert torch.equal(grad.w[g], ops.linear_grad(ints(dev, 3, (m, 8)), x, w[g], need_x=False).w)
+
+
 def test_weights_beyond_32_bits(dev):
     """Expert matrices that lie beyond 2^32 bytes."""
     e, n, k = 40, 8192, 8192  # 5.4 GB
