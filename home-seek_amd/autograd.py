@@ -87,6 +87,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """ops.linear with its gradient (for x, w, bias, residual, w_up, bias_up).  The gradient of an fp32 result is
     rounded to bf16 on its way in: the matrix cores take bf16."""
+    if not torch.is_grad_enabled():  # (a Function is asked for gradients there all the same: no sums kept for them)
+        return ops.linear(x, w, bias, residual, act, w_up, bias_up, limit, order, out_dtype)
     return _Linear.apply(x, w, bias, residual, w_up, bias_up, act, limit, order, out_dtype)
 
 

@@ -46,6 +46,46 @@ def test_only_what_is_needed(dev):
     assert not autograd.linear(x, w.detach()).requires_grad
 
 
+def test_without_gradients_no_sums_are_kept(dev, monkeypatch):
+    x, w = rnd(dev, 1, (4, 64)), leaf(rnd(dev, 2, (8, 64)))
+    kept, plain = [], ops.linear
+    monkeypatch.setattr(ops, "linear", lambda *a, **kw: (kept.append(kw.get("want_pre", False)), plain(*a, **kw))[1])
+    a = autograd.linear(x, w, act="silu")
+    with torch.no_grad():
+        b = autograd.linear(x, w, act="silu")
+    assert a.requires_grad and not b.requires_grad and torch.equal(a, b) and kept == [True, False]
+
+
+def test_one_matrix_for_both_weights_and_for_all_experts(dev):
+    order = ops.moe_sort(torch.tensor([[0, 2], [2, 1], [0, 0]], device=dev), 3)
+    x, w = rnd(dev, 1, (6, 64)), leaf(rnd(dev, 2, (72, 64)))
+    each = w.expand(3, 72, 64)
+    out = autograd.linear(x, each, act="swiglu", w_up=each, limit=3.0, order=order)
+    d = rnd(dev, 3, out.shape)
+    out.backward(d)
+    wide = w.detach().expand(3, 72, 64).contiguous()
+    want, pre = ops.linear(x, wide, act="swiglu", w_up=wide, limit=3.0, order=order, want_pre=True)
+    g = ops.linear_grad(d, x, wide, "swiglu", pre, wide, 3.0, order)
+    assert torch.equal(out, want)
+    # torch adds the six bf16 gradients: five sums, each off by half a step of at most the sum of the sizes
+    size = (g.w.double().abs() + g.w_up.double().abs()).sum(0)
+    assert bool(((w.grad.double() - (g.w.double() + g.w_up.double()).sum(0)).abs() <= 5 * 1.02 * 2.0 ** -8 * size).all())
+
+
+def test_no_tokens_and_bf16_weights(dev):
+    e, d, i = 3, 64, 72
+    w1, w3, w2 = leaf(rnd(dev, 4, (e, i, d))), leaf(rnd(dev, 5, (e, i, d))), leaf(rnd(dev, 6, (e, d, i)))
+    for m in (0, 5):
+        x, tw = leaf(rnd(dev, 1, (m, d))), leaf(rnd(dev, 2, (m, 2)))
+        idx = torch.arange(2 * m, device=dev).reshape(m, 2) % e
+        out = autograd.moe_ffn(x, idx, tw, w1, w3, w2)
+        grads = torch.autograd.grad(out.float().sum(), (x, tw, w1, w3, w2))
+        assert out.shape == (m, d) and out.dtype == BF16
+        for g, t in zip(grads, (x, tw, w1, w3, w2)):
+            assert g.shape == t.shape and g.dtype == BF16
+            assert bool(g.any()) == (m > 0 and g.numel() > 0)
+
+
 @pytest.mark.parametrize("drop", [0.0, 0.4])
 def test_moe_ffn_backward(dev, drop):
     m, k, e, d, i = 40, 3, 9, 128, 72
