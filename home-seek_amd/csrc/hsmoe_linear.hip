@@ -96,7 +96,10 @@ struct Operand {
     const int r = place(i, wave, lane);
     return kGated ? (r >> 5) * 16 + (r & 15) : r;
   }
-  static __device__ __forceinline__ bool second(int i, int wave) { return kGated && ((wave * kLoads + i) >> 1 & 1); }
+  // Two loads per wave: a wave loads one matrix, which Source::open makes its
+  // first (a choice at each load: 49 instead of 36 us, 500 rows, 2 x 4096 x 4096).
+  static constexpr bool kOneMatrix = kGated && kLoads == 2;
+  static __device__ __forceinline__ bool second(int i) { return kGated && !kOneMatrix && (i >> 1 & 1); }
 
   // The MFMA operand of block j of a wave whose rows begin at row0 (a multiple
   // of 32): reduction steps 32 kk + 8 (lane / 16) ..+7 of 16 rows.  kGated:
@@ -147,8 +150,9 @@ struct Source {
   // contiguous: `rows` rows of `bytes` each; transposed: steps of `bytes` each
   __device__ __forceinline__ void open(const char* p, const char* second, int64_t ld_, int rows, int64_t bytes, int wave,
                                        int lane) {
-    base[0] = p;
-    base[1] = second;
+    const bool odd = Op::kOneMatrix && (wave & 1);
+    base[0] = odd ? second : p;
+    base[1] = odd ? p : second;
     ld = (uint32_t)ld_;
     width = Op::kTransposed ? (uint32_t)bytes : (uint32_t)(rows - 1) * ld + (uint32_t)bytes;
 #pragma unroll
@@ -170,7 +174,7 @@ struct Source {
       const uint32_t k = (uint32_t)first * 2, far[2] = {past(edge[0], left), past(edge[1], left)};
 #pragma unroll
       for (int i = kFrom; i < kTo; ++i) {
-        const i32x4 r = lds_buf(Op::second(i, wave) ? base[1] : base[0], width);
+        const i32x4 r = lds_buf(Op::second(i) ? base[1] : base[0], width);
         lds_load16(r, (at[i] + k) | far[i & 1], stage + (wave * Op::kLoads + i) * 1024);
       }
     }
@@ -1055,7 +1059,9 @@ __global__ void __launch_bounds__(256) linear_grad_join_kernel(LinearGradParams 
 }
 
 // dz = d_out act'(pre) and the column sums of dz over the rows of a group (the
-// bias's gradient), from the unrounded values.  A workgroup has 256 columns and
+// bias's gradient), from the unrounded values.  dz itself is rounded to bf16, as
+// pre is: the matrix cores, to which it goes twice, take bf16, and its error of
+// half a step is that of every other factor of those sums.  A workgroup has 256 columns and
 // a share of a group's rows: 32 threads of 8 columns, 8 rows at a time; the
 // shares' sums go to `part` [shares][n_groups][n * mats] and are added in order
 // by a second launch (one share: straight to the result).
@@ -1207,25 +1213,26 @@ constexpr int kNarrow = -1;
 
 // The tiles, with what a round of workgroups (one or two per CU) takes for 64
 // reduction steps and for the rest (first loads, epilogue), in us with every CU
-// at work, and the rate at which they stream matrices that are read once:
-//   256 x 256, turns of eight waves        1.36 + 14, 4.7 TB/s
-//   128 x 128, 4 stages                    0.62 + 7,  5.4 TB/s
-//   64 x 128, 4 stages                     0.44 + 5,  5.3 TB/s
-//   128 x 128, 2 stages, two per CU        1.15 + 10, 5.8 TB/s
-//   256 x 128, 3 stages, eight waves       0.83 + 10, 4.7 TB/s
-// (swiglu's two matrices, in tiles of half the columns: 0.87 of that.)  The
+// at work, the part of a step's time that is left with few at work, and the rate
+// at which they stream matrices that are read once:
+//   256 x 256, turns of eight waves        1.45 + 16, 0.8, 4.7 TB/s
+//   128 x 128, 4 stages, eight waves       0.52 + 6.5, 0.6, 5.4 TB/s (four waves: 0.56 + 7)
+//   64 x 128, 4 stages, four waves         0.35 + 6,  0.8, 5.3 TB/s
+//   128 x 128, 2 stages, two per CU        1.02 + 8,  0.4, 5.8 TB/s
+//   256 x 128, 3 stages, eight waves       0.79 + 9,  0.6, 4.7 TB/s
+// (swiglu's two matrices, in tiles of half the columns: 0.87 of that rate.)  The
 // kernel for few rows streams w at 5.3 TB/s less 3% per row.  What takes the
 // least time by these figures is taken; a split reduction costs the fp32 sums'
 // way to memory and back and a launch.
 struct TileCost {
   int rows, cols, per_cu;
-  double step, rest, rate;  // us, us, bytes per us
+  double step, rest, few, rate;  // us, us, 1, bytes per us
 };
-constexpr TileCost kTiles[] = {{256, 256, 1, 1.36, 14.0, 4.7e6},
-                               {128, 128, 1, 0.62, 7.0, 5.4e6},
-                               {64, 128, 1, 0.44, 5.0, 5.3e6},
-                               {128, 128, 2, 1.15, 10.0, 5.8e6},
-                               {256, 128, 1, 0.83, 10.0, 4.7e6}};
+constexpr TileCost kTiles[] = {{256, 256, 1, 1.45, 16.0, 0.8, 4.7e6},
+                               {128, 128, 1, 0.52, 6.5, 0.6, 5.4e6},
+                               {64, 128, 1, 0.35, 6.0, 0.8, 5.3e6},
+                               {128, 128, 2, 1.02, 8.0, 0.4, 5.8e6},
+                               {256, 128, 1, 0.79, 9.0, 0.6, 4.7e6}};
 constexpr int kAllTiles = 5, kGatedTiles = 4;  // (the last one does not hold swiglu's two sums in its registers)
 
 // rows: of the output, in groups of which at most `active` have any (one: dense);
@@ -1244,9 +1251,10 @@ Plan plan_tiles(double rows, double active, int64_t cols, int64_t steps, double 
     for (int s = 1; s <= 16; s *= 2) {
       const int64_t per = (steps + s - 1) / s;
       if (s > 1 && (per < 4 || (steps + per - 1) / per != s)) continue;
-      double us = __builtin_ceil(tiles * s / (cus * c.per_cu)) * (per * c.step + c.rest);
+      const double fill = tiles * s / (cus * c.per_cu), rounds = __builtin_ceil(fill);
+      double us = rounds * (per * c.step * (c.few + (1.0 - c.few) * fill / rounds) + c.rest);
       if (us < bytes / c.rate) us = bytes / c.rate;
-      if (s > 1) us += 4.0 + s * sums * 8.0 / 5e6;
+      if (s > 1) us += 2.5 + s * sums * 8.0 / 5e6;
       if (us < least) {
         least = us;
         best = {t, s, s > 1 ? (size_t)(s * sums * 4.0) : 0};
@@ -1402,7 +1410,7 @@ extern "C" int hsmoe_linear(const void* x, int64_t x_row_stride, int64_t m, int6
   if (plan.tile == kNarrow) return launch_narrow(p, st);
   if (plan.tile == 0 && offsets) return launch_linear<256, 256, 2, 4, kTurnsFar>(p, st);
   if (plan.tile == 0) return launch_linear<256, 256, 2, 4, kTurnsNear>(p, st);
-  if (plan.tile == 1) return launch_linear<128, 128, 2, 2, 4>(p, st);
+  if (plan.tile == 1) return launch_linear<128, 128, 4, 2, 4>(p, st);
   if (plan.tile == 2) return launch_linear<64, 128, 2, 2, 4>(p, st);
   if (plan.tile == 3) return launch_linear<128, 128, 2, 2, 2>(p, st);
   return launch_linear_as<256, 128, 4, 2, 3, false>(p, st);
@@ -1499,7 +1507,7 @@ extern "C" int hsmoe_linear_grad_input(const void* dz, int64_t dz_row_stride, in
   hipStream_t st = (hipStream_t)stream;
   if (plan.tile == 0 && offsets) return launch_grad_input<256, 256, 2, 4, kTurnsFar>(p, st);
   if (plan.tile == 0) return launch_grad_input<256, 256, 2, 4, kTurnsNear>(p, st);
-  if (plan.tile == 1) return launch_grad_input<128, 128, 2, 2, 4>(p, st);
+  if (plan.tile == 1) return launch_grad_input<128, 128, 4, 2, 4>(p, st);
   if (plan.tile == 2) return launch_grad_input<64, 128, 2, 2, 4>(p, st);
   if (plan.tile == 3) return launch_grad_input<128, 128, 2, 2, 2>(p, st);
   return launch_grad_input<256, 128, 4, 2, 3>(p, st);
@@ -1532,5 +1540,5 @@ extern "C" int hsmoe_linear_grad_weight(const void* dz, int64_t dz_row_stride, c
   p.splits = plan.splits, p.part = plan.bytes ? (float*)workspace : nullptr;
   hipStream_t st = (hipStream_t)stream;
   if (plan.tile == 0) return launch_grad_weight<256, 256, 2, 4, kTurnsNear>(p, st);
-  return launch_grad_weight<128, 128, 2, 2, 4>(p, st);
+  return launch_grad_weight<128, 128, 4, 2, 4>(p, st);
 }
