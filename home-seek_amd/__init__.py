@@ -8,6 +8,7 @@ __graft_entry__.package()).  Modules mirror the reference's operator API:
   engine         HomeSeekMoEEngine: loaders, _forward_ffn, _mtp_verify_batched
   expert_store   HbmExpertStore: all experts resident in HBM
   ops            thin torch wrappers over the C ABI (include/hsmoe.h)
+  autograd       the bf16 expert layer with its gradients: linear, moe_ffn
 The compute runs in libhsmoe.so (csrc/, hand-written HIP for gfx950); there is
 no CPU or Triton fallback.
 """
