@@ -1214,37 +1214,37 @@ constexpr int kNarrow = -1;
 // The tiles, with what a round of workgroups (one or two per CU) takes for 64
 // reduction steps and for the rest (first loads, epilogue), in us with every CU
 // at work, the part of a step's time that is left with few at work, and the rate
-// at which they stream matrices that are read once:
-//   256 x 256, turns of eight waves        1.45 + 16, 0.8, 4.7 TB/s
-//   128 x 128, 4 stages, eight waves       0.52 + 6.5, 0.6, 5.4 TB/s (four waves: 0.56 + 7)
-//   64 x 128, 4 stages, four waves         0.35 + 6,  0.8, 5.3 TB/s
-//   128 x 128, 2 stages, two per CU        1.02 + 8,  0.4, 5.8 TB/s
-//   256 x 128, 3 stages, eight waves       0.79 + 9,  0.6, 4.7 TB/s
-// (swiglu's two matrices, in tiles of half the columns: 0.87 of that rate.)  The
-// kernel for few rows streams w at 5.3 TB/s less 3% per row.  What takes the
+// at which they stream matrices that are read once (swiglu's two):
+//   256 x 256, turns of eight waves        1.45 + 16,  0.8, 5.0 (5.1) TB/s
+//   128 x 128, 4 stages, eight waves       0.52 + 6.5, 0.6, 4.4 (4.6) TB/s (four waves: 0.56 + 7)
+//   64 x 128, 4 stages, four waves         0.35 + 6,   0.8, 4.3 (4.5) TB/s
+//   128 x 128, 2 stages, two per CU        1.02 + 8,   0.4, 5.7 (4.8) TB/s
+//   256 x 128, 3 stages, eight waves       0.79 + 9,   0.6, 3.9 TB/s
+// The kernel for few rows streams w at 5.3 TB/s less 3% per row.  What takes the
 // least time by these figures is taken; a split reduction costs the fp32 sums'
 // way to memory and back and a launch.
 struct TileCost {
   int rows, cols, per_cu;
-  double step, rest, few, rate;  // us, us, 1, bytes per us
+  double step, rest, few, rate, rate_two;  // us, us, 1, bytes per us
 };
-constexpr TileCost kTiles[] = {{256, 256, 1, 1.45, 16.0, 0.8, 4.7e6},
-                               {128, 128, 1, 0.52, 6.5, 0.6, 5.4e6},
-                               {64, 128, 1, 0.35, 6.0, 0.8, 5.3e6},
-                               {128, 128, 2, 1.02, 8.0, 0.4, 5.8e6},
-                               {256, 128, 1, 0.79, 9.0, 0.6, 4.7e6}};
+constexpr TileCost kTiles[] = {{256, 256, 1, 1.45, 16.0, 0.8, 5.0e6, 5.1e6},
+                               {128, 128, 1, 0.52, 6.5, 0.6, 4.4e6, 4.6e6},
+                               {64, 128, 1, 0.35, 6.0, 0.8, 4.3e6, 4.5e6},
+                               {128, 128, 2, 1.02, 8.0, 0.4, 5.7e6, 4.8e6},
+                               {256, 128, 1, 0.79, 9.0, 0.6, 3.9e6, 3.9e6}};
 constexpr int kAllTiles = 5, kGatedTiles = 4;  // (the last one does not hold swiglu's two sums in its registers)
 
 // rows: of the output, in groups of which at most `active` have any (one: dense);
-// cols: tiles' columns (twice the output's for swiglu); bytes: of the groups'
+// cols: tiles' columns (twice the output's for swiglu: two); bytes: of the groups'
 // matrices; sums: fp32 values of one part.
-Plan plan_tiles(double rows, double active, int64_t cols, int64_t steps, double bytes, double sums, int tiles_from,
-                int tiles_to, double& least) {
+Plan plan_tiles(double rows, double active, int64_t cols, int64_t steps, double bytes, bool two, double sums, int n_tiles,
+                double& least) {
   const double cus = device_cus();
-  Plan best{tiles_from, 1, 0};
+  Plan best{0, 1, 0};
   least = 1e30;
-  for (int t = tiles_from; t < tiles_to; ++t) {
+  for (int t = 0; t < n_tiles; ++t) {
     const TileCost& c = kTiles[t];
+    // groups end inside a tile: half a tile more for each on average
     double row_tiles = active <= 1 ? __builtin_ceil(rows / c.rows) : rows / c.rows + 0.5 * active;
     if (row_tiles < active) row_tiles = active;
     const double tiles = row_tiles * (double)((cols + c.cols - 1) / c.cols);
@@ -1253,7 +1253,8 @@ Plan plan_tiles(double rows, double active, int64_t cols, int64_t steps, double 
       if (s > 1 && (per < 4 || (steps + per - 1) / per != s)) continue;
       const double fill = tiles * s / (cus * c.per_cu), rounds = __builtin_ceil(fill);
       double us = rounds * (per * c.step * (c.few + (1.0 - c.few) * fill / rounds) + c.rest);
-      if (us < bytes / c.rate) us = bytes / c.rate;
+      const double stream = bytes / (two ? c.rate_two : c.rate);
+      if (us < stream) us = stream;
       if (s > 1) us += 2.5 + s * sums * 8.0 / 5e6;
       if (us < least) {
         least = us;
@@ -1268,24 +1269,23 @@ Plan plan_linear(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
   const int64_t active = n_groups < m ? n_groups : m, mats = act == HSMOE_ACT_SWIGLU ? 2 : 1;
   const double rows = (double)m / (double)active, bytes = 2.0 * active * n * mats * k;
   double tiled;
-  const Plan plan = plan_tiles((double)m, (double)active, n * mats, (k + kBK - 1) / kBK,
-                               mats == 2 ? bytes / 0.87 : bytes, (double)m * n * mats, 0,
-                               mats == 2 ? kGatedTiles : kAllTiles, tiled);
+  const Plan plan = plan_tiles((double)m, (double)active, n * mats, (k + kBK - 1) / kBK, bytes, mats == 2,
+                               (double)m * n * mats, mats == 2 ? kGatedTiles : kAllTiles, tiled);
   const double narrow = 2.0 + bytes / 5.3e6 * (1.0 + 0.03 * rows);
   return rows <= kNarrowRows && narrow < tiled ? Plan{kNarrow, 1, 0} : plan;
 }
 Plan plan_grad_input(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
   const int64_t active = n_groups < m ? n_groups : m;
   double us;
-  return plan_tiles((double)m, (double)active, k, (n + kBK - 1) / kBK * mats, 2.0 * active * n * mats * k, (double)m * k,
-                    0, kAllTiles, us);
+  return plan_tiles((double)m, (double)active, k, (n + kBK - 1) / kBK * mats, 2.0 * active * n * mats * k, false,
+                    (double)m * k, kAllTiles, us);
 }
 // (both operands transposed: no tile of 64 rows)
 Plan plan_grad_weight(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
   const int64_t rows = (m + n_groups - 1) / n_groups;
   double us;
-  return plan_tiles((double)n, 1, k * n_groups * mats, (rows + kBK - 1) / kBK, 0, (double)n_groups * mats * n * k, 0, 2,
-                    us);
+  return plan_tiles((double)n, 1, k * n_groups * mats, (rows + kBK - 1) / kBK, 0, false,
+                    (double)n_groups * mats * n * k, 2, us);
 }
 
 int check_workspace(const char* what, const Plan& plan, const void* ws, size_t bytes) {

@@ -101,7 +101,9 @@ SHAPES = [(1, 8, 8), (1, 4096, 4096), (3, 64, 72), (5, 1000, 520), (8, 2048, 102
           (31, 520, 2048), (33, 4096, 128), (64, 72, 1000), (100, 264, 136), (127, 128, 64), (129, 1288, 200),
           (500, 2048, 512), (1000, 504, 1032), (2049, 4096, 256), (4093, 2056, 64),
           (4100, 4104, 72),  # more than 256 tiles of 256 x 256
-          (1500, 4096, 136), (1900, 2048, 136)]  # tiles of 256 x 128; of 128 x 128, two per CU, for swiglu
+          # every tile, whole and with its reduction split, for one matrix and for swiglu's two
+          (1500, 4096, 136), (1900, 2048, 136), (200, 4104, 136), (500, 4104, 136), (2000, 4104, 136), (2500, 2056, 520),
+          (3001, 136, 4104)]
 
 
 @pytest.mark.parametrize("act", [None, "silu", "swiglu"])
@@ -119,7 +121,9 @@ def test_dense_without_the_options(dev, m, act, with_bias, with_res, out_dtype):
 
 GROUPS = [(1, 6, 256, 64, 128, 0.0), (8, 6, 256, 512, 512, 0.0), (8, 2, 3, 72, 200, 0.5), (40, 4, 16, 264, 72, 0.3),
           (37, 16, 5, 520, 136, 0.1), (300, 6, 64, 136, 64, 0.2), (512, 6, 8, 512, 256, 0.0), (700, 3, 1, 256, 128, 0.4),
-          (50, 2, 1024, 8, 8, 0.0), (90, 3, 7, 64, 64, 1.0), (1500, 4, 20, 1032, 328, 0.1), (1200, 4, 12, 2056, 136, 0.0), (1200, 4, 12, 136, 2056, 0.0)]
+          (50, 2, 1024, 8, 8, 0.0), (90, 3, 7, 64, 64, 1.0), (1500, 4, 20, 1032, 328, 0.1), (1200, 4, 12, 2056, 136, 0.0), (1200, 4, 12, 136, 2056, 0.0),
+          (750, 2, 16, 1032, 136, 0.1), (750, 2, 8, 4104, 136, 0.1), (1250, 2, 3, 2056, 520, 0.1), (750, 2, 8, 136, 4104, 0.1),
+          (1250, 2, 3, 520, 2056, 0.1), (750, 2, 8, 2056, 136, 0.1), (1000, 2, 3, 136, 2056, 0.1), (100, 2, 16, 4104, 1032, 0.1)]
 
 
 @pytest.mark.parametrize("act", [None, "silu", "swiglu"])
@@ -287,7 +291,8 @@ def check_grad(dev, m, n, k, act, order=None, lead=()):
 @pytest.mark.parametrize("act", [None, "silu", "swiglu"])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 8), (1, 1024, 512), (3, 64, 72), (17, 136, 264), (64, 256, 128), (65, 72, 1000),
                                    (130, 520, 136), (500, 512, 512), (1001, 264, 520), (300, 2048, 4096), (4100, 72, 4104), (72, 4104, 4104),
-                                   (1500, 136, 4096), (2000, 1024, 1024)])
+                                   (1500, 136, 4096), (2000, 1024, 1024), (500, 136, 4104), (2000, 136, 4104),
+                                   (2500, 520, 2056), (3001, 136, 2056), (500, 4104, 4104)])
 def test_dense_gradient(dev, m, n, k, act):
     check_grad(dev, m, n, k, act)
 
