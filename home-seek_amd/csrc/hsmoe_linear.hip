@@ -528,16 +528,22 @@ struct LinearParams {
   int splits;
 };
 
-// From t = exp(-z) by the hardware's exp2 and reciprocal (1 ulp each).  A finite
-// exponent stops at 125, so that the result is small there and not 0 (0 times an
-// infinite up value would be NaN); that of -inf is 0.  kFine: the product with log2(e) as a head
-// and what its rounding left, which keeps t good to 3 ulp; without it the error
-// of t is |z| 2^-24, nothing beside the half step of a bf16 result.
+// A gate as sigmoid() and the products with it take it: finite values below -86 as
+// -86.  Their sigmoid is a number that fp32 does not hold, 2^-124 there: with the
+// gate at -86 too, z sigmoid(z) stays below 2^-117 however far the gate is (with
+// z itself: -7 at -3e38), and not 0 (0 times an infinite up value would be NaN).
+// -inf and NaN stay.
+__device__ __forceinline__ float near_gate(float z) { return z > -__builtin_inff() ? __builtin_fmaxf(z, -86.0f) : z; }
+
+// Of a near_gate, from t = exp(-z) by the hardware's exp2 and reciprocal (1 ulp
+// each).  kFine: the product with log2(e) as a head and what its rounding left,
+// which keeps t good to 3 ulp; without it the error of t is |z| 2^-24, nothing
+// beside the half step of a bf16 result.
 template <bool kFine>
 __device__ __forceinline__ float sigmoid(float z) {
   const float kLog2e = 1.4426950408889634f, kLog2eLow = 1.9259629911e-8f;
   const float h = -z * kLog2e;
-  float t = __builtin_amdgcn_exp2f(h < __builtin_inff() ? __builtin_fminf(h, 125.0f) : h);
+  float t = __builtin_amdgcn_exp2f(h);
   if (kFine) {
     const float rest = __builtin_fmaf(-z, kLog2eLow, __builtin_fmaf(-z, kLog2e, -h));  // NaN for infinities: 0.5 then
     t = __builtin_fmaf(t, __builtin_fminf(rest, 0.5f) * 0.6931471805599453f, t);
@@ -584,9 +590,10 @@ __device__ __forceinline__ Row8 activate(const LinearParams& p, const Row8& z, c
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     if (p.act == HSMOE_ACT_SILU) {
-      y.v[i] = z.v[i] * sigmoid<kFine>(z.v[i]);
+      const float g = near_gate(z.v[i]);
+      y.v[i] = g * sigmoid<kFine>(g);
     } else {
-      const float g = clamp_top(z.v[i], p.limit);
+      const float g = near_gate(clamp_top(z.v[i], p.limit));
       y.v[i] = g * sigmoid<kFine>(g) * clamp_both(zu.v[i], p.limit);
     }
   }
@@ -659,9 +666,10 @@ __device__ __forceinline__ void finish1(const LinearParams& p, int group, int64_
   }
   float y = z;
   if (p.act == HSMOE_ACT_SILU) {
-    y = z * sigmoid<true>(z);
+    const float g = near_gate(z);
+    y = g * sigmoid<true>(g);
   } else if (p.act == HSMOE_ACT_SWIGLU) {
-    const float g = clamp_top(z, p.limit);
+    const float g = near_gate(clamp_top(z, p.limit));
     y = g * sigmoid<true>(g) * clamp_both(zu, p.limit);
   }
   if (!none && p.residual) y += bf(p.residual + m * p.ld_res, n);
@@ -1113,12 +1121,12 @@ __global__ void __launch_bounds__(kActThreads) act_grad_kernel(ActGradParams p) 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if (kMats == 2) {
-          const float g = clamp_top(z.v[i], p.limit), s = sigmoid<kSums>(g), gs = g * s;
+          const float g = near_gate(clamp_top(z.v[i], p.limit)), s = sigmoid<kSums>(g), gs = g * s;
           o[0].v[i] = z.v[i] > p.limit ? 0.0f : d.v[i] * clamp_both(zu.v[i], p.limit) * (s + gs * (1.0f - s));
           o[kMats - 1].v[i] = zu.v[i] > p.limit || zu.v[i] < -p.limit ? 0.0f : d.v[i] * gs;
         } else if (p.act == HSMOE_ACT_SILU) {
-          const float s = sigmoid<kSums>(z.v[i]);
-          o[0].v[i] = d.v[i] * (s + z.v[i] * s * (1.0f - s));
+          const float g = near_gate(z.v[i]), s = sigmoid<kSums>(g);
+          o[0].v[i] = d.v[i] * (s + g * s * (1.0f - s));
         } else {
           o[0].v[i] = d.v[i];
         }
