@@ -7,6 +7,7 @@ Under graph capture, capture the forward and the backward pass together, and let
 go of every eager graph that reaches the same leaves first: torch ties a leaf's
 gradient accumulation to the stream of the first graph that used it, and a
 captured backward pass that meets an eager one's ends the process.
+Second derivatives and forward-mode ones are refused by torch.
 """
 from __future__ import annotations
 
@@ -22,8 +23,8 @@ __all__ = ["linear", "moe_gather", "moe_combine", "moe_ffn"]
 
 class _Linear(Function):
     @staticmethod
-    def forward(ctx, x, w, bias, residual, w_up, bias_up, act, limit, order, out_dtype):
-        need = any(ctx.needs_input_grad)
+    def forward(ctx, x, w, bias, residual, w_up, bias_up, act, limit, order, out_dtype, grad_enabled):
+        need = grad_enabled and any(ctx.needs_input_grad)  # (needs_input_grad says yes under no_grad too)
         out = ops.linear(x, w, bias, residual, act, w_up, bias_up, limit, order, out_dtype, want_pre=need and act is not None)
         out, pre = out if isinstance(out, tuple) else (out, None)
         ctx.save_for_backward(x, w, w_up, pre)
@@ -43,7 +44,7 @@ class _Linear(Function):
         d_res = None
         if need[3]:  # rows of no expert have no residual either
             d_res = d_out if ctx.order is None else _cleared_behind(d_out, ctx.order)
-        return (g.x, g.w if need[1] else None, db[0], d_res, g.w_up if need[4] else None, db[1], None, None, None, None)
+        return (g.x, g.w if need[1] else None, db[0], d_res, g.w_up if need[4] else None, db[1], None, None, None, None, None)
 
 
 def _cleared_behind(rows: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
@@ -87,9 +88,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None, r
            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """ops.linear with its gradient (for x, w, bias, residual, w_up, bias_up).  The gradient of an fp32 result is
     rounded to bf16 on its way in: the matrix cores take bf16."""
-    if not torch.is_grad_enabled():  # (a Function is asked for gradients there all the same: no sums kept for them)
-        return ops.linear(x, w, bias, residual, act, w_up, bias_up, limit, order, out_dtype)
-    return _Linear.apply(x, w, bias, residual, w_up, bias_up, act, limit, order, out_dtype)
+    # (a Function under no_grad too: it refuses forward-mode tangents, which stay on there)
+    return _Linear.apply(x, w, bias, residual, w_up, bias_up, act, limit, order, out_dtype, torch.is_grad_enabled())
 
 
 def moe_gather(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
