@@ -21,29 +21,36 @@ from .ops import ExpertOrder
 __all__ = ["linear", "moe_gather", "moe_combine", "moe_ffn"]
 
 
+# The order's tensors are saved as the others are, so that torch notices a change
+# of one before the backward pass has read it.
+def _saved_order(tensors: list) -> ExpertOrder | None:
+    return ExpertOrder(*tensors) if tensors else None
+
+
 class _Linear(Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, w_up, bias_up, act, limit, order, out_dtype, grad_enabled):
         need = grad_enabled and any(ctx.needs_input_grad)  # (needs_input_grad says yes under no_grad too)
         out = ops.linear(x, w, bias, residual, act, w_up, bias_up, limit, order, out_dtype, want_pre=need and act is not None)
         out, pre = out if isinstance(out, tuple) else (out, None)
-        ctx.save_for_backward(x, w, w_up, pre)
-        ctx.act, ctx.limit, ctx.order = act, limit, order
+        ctx.save_for_backward(x, w, w_up, pre, *(order or ()))
+        ctx.act, ctx.limit = act, limit
         ctx.bias_dtypes = [None if b is None else b.dtype for b in (bias, bias_up)]
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        x, w, w_up, pre = ctx.saved_tensors
+        x, w, w_up, pre, *order = ctx.saved_tensors
+        order = _saved_order(order)
         need = ctx.needs_input_grad
         d_out = d_out.to(torch.bfloat16)
-        g = ops.linear_grad(d_out, x, w, ctx.act, pre, w_up, ctx.limit, ctx.order, need_x=need[0], need_w=need[1] or need[4],
+        g = ops.linear_grad(d_out, x, w, ctx.act, pre, w_up, ctx.limit, order, need_x=need[0], need_w=need[1] or need[4],
                             need_bias=need[2] or need[5])
         db = [b.to(t) if b is not None and t is not None else None for b, t in zip((g.bias, g.bias_up), ctx.bias_dtypes)]
         d_res = None
         if need[3]:  # rows of no expert have no residual either
-            d_res = d_out if ctx.order is None else _cleared_behind(d_out, ctx.order)
+            d_res = d_out if order is None else _cleared_behind(d_out, order)
         return (g.x, g.w if need[1] else None, db[0], d_res, g.w_up if need[4] else None, db[1], None, None, None, None, None)
 
 
@@ -54,31 +61,30 @@ def _cleared_behind(rows: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
 class _Gather(Function):
     @staticmethod
     def forward(ctx, x, order):
-        ctx.order = order
+        ctx.save_for_backward(*order)
         return ops.moe_gather(x, order)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_rows):
-        return ops.moe_combine(d_rows, ctx.order), None
+        return ops.moe_combine(d_rows, _saved_order(ctx.saved_tensors)), None
 
 
 class _Combine(Function):
     @staticmethod
     def forward(ctx, rows, order, topk_w, residual, out_dtype):
         out = ops.moe_combine(rows, order, topk_w, residual, out_dtype)
-        ctx.save_for_backward(rows, topk_w)
-        ctx.order = order
+        ctx.save_for_backward(rows, topk_w, *order)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        rows, topk_w = ctx.saved_tensors
+        rows, topk_w, *order = ctx.saved_tensors
         need = ctx.needs_input_grad
         d_rows = d_w = None
         if need[0] or need[2]:
-            d_rows, d_w = ops.moe_combine_grad(d_out, rows, ctx.order, topk_w, need_rows=need[0], need_w=need[2])
+            d_rows, d_w = ops.moe_combine_grad(d_out, rows, _saved_order(order), topk_w, need_rows=need[0], need_w=need[2])
         return d_rows, None, None if d_w is None else d_w.to(topk_w.dtype), d_out if need[3] else None, None
 
 

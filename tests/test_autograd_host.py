@@ -49,3 +49,49 @@ def test_no_sums_are_kept_where_no_gradient_can_be_asked_for(plain_linear):
     assert plain_linear == [True, False, False, False]
     assert y.requires_grad and not any(t.requires_grad for t in (a, b, c))
     assert all(torch.equal(y, t) for t in (a, b, c))
+
+
+def order_of(rows):
+    """An order of `rows` single-slot tokens in one expert."""
+    at = torch.arange(rows, dtype=torch.int32)
+    return ops.ExpertOrder(torch.tensor([0, rows], dtype=torch.int32), at.clone(), at.clone()[:, None].contiguous())
+
+
+@pytest.fixture()
+def plain_rows(plain_linear, monkeypatch):
+    monkeypatch.setattr(ops, "moe_gather", lambda x, order: x.detach().clone())
+    monkeypatch.setattr(ops, "moe_combine", lambda rows, order, w=None, residual=None, out_dtype=None: rows.detach().clone())
+    monkeypatch.setattr(ops, "moe_combine_grad", lambda d, rows, order, w=None, need_rows=True, need_w=True:
+                        (d if need_rows else None, w if need_w else None))
+    monkeypatch.setattr(ops, "linear_grad", lambda d, x, w, *a, **kw:
+                        ops.LinearGrad(torch.zeros_like(x), torch.zeros_like(w), None, None, None))
+
+
+CALLS = {
+    "linear": lambda x, w, order: autograd.linear(x, w, order=order),
+    "moe_gather": lambda x, w, order: autograd.moe_gather(x, order),
+    "moe_combine": lambda x, w, order: autograd.moe_combine(x, order),
+}
+
+
+@pytest.mark.parametrize("what", CALLS)
+def test_an_order_that_changes_before_the_backward_pass_is_refused(plain_rows, what):
+    """As any tensor that a backward pass reads: its gradients would be those of another order."""
+    for i in range(3):
+        x, w, order = torch.randn(4, 8).to(BF16).requires_grad_(), torch.randn(16, 8).to(BF16), order_of(4)
+        y = CALLS[what](x, w, order)
+        y.sum().backward()
+        assert x.grad.shape == x.shape
+        y = CALLS[what](x, w, order)
+        order[i].add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_a_function_keeps_its_own_order(plain_rows, monkeypatch):
+    """The order that the backward pass hands on is the forward call's."""
+    seen = []
+    monkeypatch.setattr(ops, "moe_combine", lambda rows, order, *a: (seen.append(order), rows.detach().clone())[1])
+    x, order = torch.randn(4, 8).requires_grad_(), order_of(4)
+    autograd.moe_gather(x, order).sum().backward()
+    assert isinstance(seen[0], ops.ExpertOrder) and all(torch.equal(a, b) for a, b in zip(seen[0], order))
