@@ -22,6 +22,9 @@ OUT_BF16 = 1
 ACT_NONE = 0
 ACT_SILU = 1
 ACT_SWIGLU = 2
+LINEAR_OUT = 0
+LINEAR_DX = 1
+LINEAR_DW = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -89,6 +92,7 @@ _SIGNATURES = {
     "hsmoe_linear": (_int, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _i64,
                             _c_void_p, _c_void_p, _c_void_p, _i64, _int, _f32, _int, _c_void_p, _c_void_p,
                             _c_void_p, _size, _c_void_p]),
+    "hsmoe_linear_plan": (_int, [_int, _i64, _i64, _i64, _i64, _int, _c_void_p]),
     "hsmoe_linear_workspace_size": (_size, [_i64, _i64, _i64, _i64, _int]),
     "hsmoe_linear_grad_workspace_size": (_size, [_i64, _i64, _i64, _i64, _int]),
     "hsmoe_linear_act_grad_workspace_size": (_size, [_i64, _i64, _i64, _int]),

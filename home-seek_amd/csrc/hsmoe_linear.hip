@@ -1368,6 +1368,27 @@ int act_shares(int64_t m, int64_t n, int64_t n_groups) {
 
 using namespace hsmoe;
 
+// The rule's answer for a product, as the entry points ask for it below.
+extern "C" int hsmoe_linear_plan(int product, int64_t m, int64_t n, int64_t k, int64_t n_groups, int act, int32_t plan[4]) {
+  if (!plan) return fail(HSMOE_ERR_ARG, "hsmoe_linear_plan: null pointer");
+  if (m < 1 || n < 1 || k < 1 || n_groups < 1) return fail(HSMOE_ERR_ARG, "hsmoe_linear_plan: bad counts");
+  if (act != HSMOE_ACT_NONE && act != HSMOE_ACT_SILU && act != HSMOE_ACT_SWIGLU)
+    return fail(HSMOE_ERR_ARG, "hsmoe_linear_plan: bad activation %d", act);
+  const int mats = act == HSMOE_ACT_SWIGLU ? 2 : 1;
+  Plan p{};
+  if (product == HSMOE_LINEAR_OUT) p = plan_linear(m, n, k, n_groups, act);
+  else if (product == HSMOE_LINEAR_DX) p = plan_grad_input(m, n, k, n_groups, mats);
+  else if (product == HSMOE_LINEAR_DW) p = plan_grad_weight(m, n, k, n_groups, mats);
+  else return fail(HSMOE_ERR_ARG, "hsmoe_linear_plan: bad product %d", product);
+  if (p.tile == kNarrow) {
+    plan[0] = plan[1] = kNarrowRows, plan[2] = 2, plan[3] = 1;
+  } else {
+    const TileCost& c = kTiles[p.tile];
+    plan[0] = c.rows, plan[1] = c.cols, plan[2] = c.per_cu, plan[3] = p.splits;
+  }
+  return HSMOE_OK;
+}
+
 extern "C" size_t hsmoe_linear_workspace_size(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
   return m < 1 || n < 1 || k < 1 || n_groups < 1 ? 0 : plan_linear(m, n, k, n_groups, act).bytes;
 }

@@ -412,6 +412,15 @@ int hsmoe_linear_grad_weight(const void* dz_dev, int64_t dz_row_stride, const vo
                              int out_kind, void* dw_dev, void* dw_up_dev, void* workspace_dev, size_t workspace_bytes,
                              hsmoe_stream_t stream);
 
+/* How the calls above do a product of these sizes on the current device: plan =
+ * {rows and columns of a tile (16 x 16: the kernel for few rows), workgroups of it
+ * per CU, parts of the reduction}.  For measurements and tests; the results do not
+ * depend on it but for the order of fp32 sums. */
+#define HSMOE_LINEAR_OUT 0
+#define HSMOE_LINEAR_DX 1
+#define HSMOE_LINEAR_DW 2
+int hsmoe_linear_plan(int product, int64_t m, int64_t n, int64_t k, int64_t n_groups, int act, int32_t plan[4]);
+
 /* ---------------------------------------------------------------------------
  * lm_head logits + greedy argmax + longest-prefix draft acceptance.
  * Replaces the logits / acceptance loop of _mtp_verify_batched
