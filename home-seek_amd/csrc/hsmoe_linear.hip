@@ -1241,21 +1241,30 @@ constexpr TileCost kTiles[] = {{256, 256, 1, 1.45, 16.0, 0.8, 5.0e6, 5.1e6},
                                {128, 128, 2, 1.02, 8.0, 0.4, 5.7e6, 4.8e6},
                                {256, 128, 1, 0.79, 9.0, 0.6, 3.9e6, 3.9e6}};
 constexpr int kAllTiles = 5, kGatedTiles = 4;  // (the last one does not hold swiglu's two sums in its registers)
+// The same for the weights' gradients, whose experts often have one or two steps
+// and whose tiles often end at the matrix's edge: what a round takes beside its
+// steps is less there, and the results go out at 3 TB/s.  Over 800 shapes (1 to
+// 16384 rows, up to 256 experts, 32 to 4400 columns either way) the choice by
+// these takes 0.6% more than the best tile in the mean and 1.35 times at most;
+// the 256 x 256 one alone takes 60% more in the mean, the 128 x 128 one 20%.
+constexpr TileCost kWeightTiles[] = {{256, 256, 1, 1.9, 4.0, 0.65, 3.0e6, 3.0e6},
+                                     {128, 128, 1, 0.61, 3.0, 0.72, 3.0e6, 3.0e6}};
 
 // rows: of the output, in groups of which at most `active` have any (one: dense);
-// cols: tiles' columns (twice the output's for swiglu: two); bytes: of the groups'
-// matrices; sums: fp32 values of one part.
-Plan plan_tiles(double rows, double active, int64_t cols, int64_t steps, double bytes, bool two, double sums, int n_tiles,
-                double& least) {
+// cols: tiles' columns (twice the output's for swiglu: two); outputs: as many of
+// them, each tiled for itself; bytes: of the groups' matrices; sums: fp32 values
+// of one part; table: the tiles to choose from.
+Plan plan_tiles(double rows, double active, int64_t cols, int64_t outputs, int64_t steps, double bytes, bool two,
+                double sums, const TileCost* table, int n_tiles, double& least) {
   const double cus = device_cus();
   Plan best{0, 1, 0};
   least = 1e30;
   for (int t = 0; t < n_tiles; ++t) {
-    const TileCost& c = kTiles[t];
+    const TileCost& c = table[t];
     // groups end inside a tile: half a tile more for each on average
     double row_tiles = active <= 1 ? __builtin_ceil(rows / c.rows) : rows / c.rows + 0.5 * active;
     if (row_tiles < active) row_tiles = active;
-    const double tiles = row_tiles * (double)((cols + c.cols - 1) / c.cols);
+    const double tiles = row_tiles * (double)((cols + c.cols - 1) / c.cols * outputs);
     for (int s = 1; s <= 16; s *= 2) {
       const int64_t per = (steps + s - 1) / s;
       if (s > 1 && (per < 4 || (steps + per - 1) / per != s)) continue;
@@ -1277,23 +1286,24 @@ Plan plan_linear(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
   const int64_t active = n_groups < m ? n_groups : m, mats = act == HSMOE_ACT_SWIGLU ? 2 : 1;
   const double rows = (double)m / (double)active, bytes = 2.0 * active * n * mats * k;
   double tiled;
-  const Plan plan = plan_tiles((double)m, (double)active, n * mats, (k + kBK - 1) / kBK, bytes, mats == 2,
-                               (double)m * n * mats, mats == 2 ? kGatedTiles : kAllTiles, tiled);
+  const Plan plan = plan_tiles((double)m, (double)active, n * mats, 1, (k + kBK - 1) / kBK, bytes, mats == 2,
+                               (double)m * n * mats, kTiles, mats == 2 ? kGatedTiles : kAllTiles, tiled);
   const double narrow = 2.0 + bytes / 5.3e6 * (1.0 + 0.03 * rows);
   return rows <= kNarrowRows && narrow < tiled ? Plan{kNarrow, 1, 0} : plan;
 }
 Plan plan_grad_input(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
   const int64_t active = n_groups < m ? n_groups : m;
   double us;
-  return plan_tiles((double)m, (double)active, k, (n + kBK - 1) / kBK * mats, 2.0 * active * n * mats * k, false,
-                    (double)m * k, kAllTiles, us);
+  return plan_tiles((double)m, (double)active, k, 1, (n + kBK - 1) / kBK * mats, 2.0 * active * n * mats * k, false,
+                    (double)m * k, kTiles, kAllTiles, us);
 }
 // (both operands transposed: no tile of 64 rows)
 Plan plan_grad_weight(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {
   const int64_t rows = (m + n_groups - 1) / n_groups;
+  const double values = (double)n_groups * mats * n * k;
   double us;
-  return plan_tiles((double)n, 1, k * n_groups * mats, (rows + kBK - 1) / kBK, 0, false,
-                    (double)n_groups * mats * n * k, 2, us);
+  return plan_tiles((double)n, 1, k, n_groups * mats, (rows + kBK - 1) / kBK, 2.0 * values, false, values, kWeightTiles, 2,
+                    us);
 }
 
 int check_workspace(const char* what, const Plan& plan, const void* ws, size_t bytes) {

@@ -69,3 +69,18 @@ def test_every_way_is_tested():
         if way(*args) not in tested:
             missing.setdefault(way(*args), args)
     assert not missing, missing
+
+
+def test_the_weights_gradients_are_tiled_each_for_itself():
+    """One expert's columns that end inside a tile leave its rest empty: widths of as many whole tiles of 128 cost
+    the same (but for the sums of a split reduction), and so have the same tile."""
+    rng = random.Random(5)
+    wrong = []
+    for _ in range(20000):
+        m, n, groups = rng.randint(1, 4000), 8 * rng.randint(1, 512), rng.randint(2, 256)
+        k, act = 8 * rng.randint(1, 512), rng.choice((_lib.ACT_NONE, _lib.ACT_SWIGLU))
+        a, b = plan(DW, m, n, k, groups, act), plan(DW, m, n, (k + 127) // 128 * 128, groups, act)
+        if a[3] == b[3] == 1 and a != b:
+            wrong.append((m, n, k, groups, act, a, b))
+    assert not wrong, (len(wrong), wrong[:3])
+    assert plan(DW, 50, 352, 64, 205)[:2] == (128, 128)  # not 410 tiles of 256 x 256, each three quarters empty
