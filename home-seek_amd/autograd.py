@@ -3,6 +3,8 @@ torch.autograd functions, and moe_ffn, the routed SwiGLU experts made of them.
 
 The gradients are the ops' own (linear_grad, moe_combine_grad): weights' and
 rows' in bf16, routing weights' in fp32, biases' rounded to the bias's dtype.
+Between the ops everything is bf16, as between torch's: the activations, the
+experts' results, the sums kept for the backward pass and their gradients.
 Under graph capture, capture the forward and the backward pass together, and let
 go of every eager graph that reaches the same leaves first: torch ties a leaf's
 gradient accumulation to the stream of the first graph that used it, and a

@@ -1069,10 +1069,12 @@ __global__ void __launch_bounds__(256) linear_grad_join_kernel(LinearGradParams 
 // dz = d_out act'(pre) and the column sums of dz over the rows of a group (the
 // bias's gradient), from the unrounded values.  dz itself is rounded to bf16, as
 // pre is: the matrix cores, to which it goes twice, take bf16, and its error of
-// half a step is that of every other factor of those sums.  A workgroup has 256 columns and
-// a share of a group's rows: 32 threads of 8 columns, 8 rows at a time; the
-// shares' sums go to `part` [shares][n_groups][n * mats] and are added in order
-// by a second launch (one share: straight to the result).
+// half a step is that of every other factor of those sums.  What the limit cuts
+// off goes by pre as it is kept, rounded (hsmoe.h says what that means at the
+// limit).  A workgroup has 256 columns and a share of a group's rows: 32 threads
+// of 8 columns, 8 rows at a time; the shares' sums go to `part`
+// [shares][n_groups][n * mats] and are added in order by a second launch (one
+// share: straight to the result).
 struct ActGradParams {
   const uint16_t* d_out;  // [n_rows][n]
   const uint16_t* pre;    // [n_rows][n * mats], NULL without an activation

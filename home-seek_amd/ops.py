@@ -545,6 +545,10 @@ def linear_grad(d_out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str 
     """The gradient of linear(x, w, ...) for d_out [..., N] (bf16): x in bf16, the
     weights in w_dtype (bf16 or fp32), the biases in fp32; the residual's is d_out.
     pre: what linear(want_pre=True) returned (not needed without an activation).
+    Behind an activation d_out y'(pre) goes to the products rounded to bf16, half a
+    step (2^-8) of each term; the biases' gradients are summed before that.  What the
+    limit cuts off is decided on pre: a sum beyond the limit that rounds onto it (up
+    to 10.03 at limit 10) has a gradient though linear cut it.
     With `order`, an expert without rows has gradient zero, and so have the rows
     behind the last sorted one (hsmoe_linear_act_grad, _grad_input, _grad_weight)."""
     dev = require_cuda(d_out, x, w, w_up, pre, *(order or ()))

@@ -389,7 +389,10 @@ int hsmoe_linear(const void* x_dev, int64_t x_row_stride, int64_t m, int64_t k, 
 /* The gradient of hsmoe_linear in three parts (the residual's is d_out).
  *   act_grad:    dz = d_out y'(pre) in bf16 ([m, n], or [m, 2 n] for swiglu) and
  *                d_bias[g] = sum of dz over the rows of g, fp32, from the unrounded
- *                values.  y' is 0 for what the limit cuts off.  dz, d_bias,
+ *                values.  y' is 0 where pre lies beyond the limit: the cut is
+ *                decided on the bf16 sums, so that one beyond the limit by less
+ *                than half a bf16 step, which rounds onto it (up to 10.03 at limit
+ *                10), is cut by hsmoe_linear and has a gradient here.  dz, d_bias,
  *                d_bias_up may be NULL; pre is not read for HSMOE_ACT_NONE
  *                (there dz is d_out).  Rows of no group are not written.
  *   grad_input:  dx = dz w (+ dz_up w_up), bf16 [m, k]; rows of no group zeros
