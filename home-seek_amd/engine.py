@@ -54,6 +54,11 @@ class HomeSeekMoEEngine:
         # and optionally both "e_proj.weight" and "h_proj.weight" (bf16 [D, D])
         if mtp_weights is not None and ("e_proj.weight" in mtp_weights) != ("h_proj.weight" in mtp_weights):
             raise ValueError("the MTP block has both projections (e_proj.weight, h_proj.weight) or none")
+        d = config.hidden_size
+        for key in ("e_proj.weight", "h_proj.weight"):
+            w = (mtp_weights or {}).get(key)
+            if w is not None and (w.dtype != torch.bfloat16 or w.shape != (d, d)):
+                raise ValueError(f"{key} must be bf16 [{d}, {d}], got {w.dtype} {list(w.shape)}")
         self._mtp_weights = mtp_weights
         self.store = store
         self.device = store.device
