@@ -1230,9 +1230,10 @@ constexpr int kNarrow = -1;
 //   64 x 128, 4 stages, four waves         0.35 + 6,   0.8, 4.3 (4.5) TB/s
 //   128 x 128, 2 stages, two per CU        1.02 + 8,   0.4, 5.7 (4.8) TB/s
 //   256 x 128, 3 stages, eight waves       0.79 + 9,   0.6, 3.9 TB/s
-// The kernel for few rows streams w at 5.3 TB/s less 3% per row.  What takes the
-// least time by these figures is taken; a split reduction costs the fp32 sums'
-// way to memory and back and a launch.
+// The kernel for few rows streams w at 5.3 TB/s less 3% per row, and takes 2.2 us
+// for a tile of 16 of w's rows however short they are.  What takes the least time
+// by these figures is taken; a split reduction costs the fp32 sums' way to memory
+// and back and a launch.
 struct TileCost {
   int rows, cols, per_cu;
   double step, rest, few, rate, rate_two;  // us, us, 1, bytes per us
@@ -1290,7 +1291,8 @@ Plan plan_linear(int64_t m, int64_t n, int64_t k, int64_t n_groups, int act) {
   double tiled;
   const Plan plan = plan_tiles((double)m, (double)active, n * mats, 1, (k + kBK - 1) / kBK, bytes, mats == 2,
                                (double)m * n * mats, kTiles, mats == 2 ? kGatedTiles : kAllTiles, tiled);
-  const double narrow = 2.0 + bytes / 5.3e6 * (1.0 + 0.03 * rows);
+  const double passes = (double)active * ((n * mats + 15) / 16) / (2.0 * device_cus()), stream = bytes / 5.3e6 * (1.0 + 0.03 * rows);
+  const double narrow = 2.0 + (stream > 2.2 * passes ? stream : 2.2 * passes);
   return rows <= kNarrowRows && narrow < tiled ? Plan{kNarrow, 1, 0} : plan;
 }
 Plan plan_grad_input(int64_t m, int64_t n, int64_t k, int64_t n_groups, int mats) {

@@ -84,3 +84,12 @@ def test_the_weights_gradients_are_tiled_each_for_itself():
             wrong.append((m, n, k, groups, act, a, b))
     assert not wrong, (len(wrong), wrong[:3])
     assert plan(DW, 50, 352, 64, 205)[:2] == (128, 128)  # not 410 tiles of 256 x 256, each three quarters empty
+
+
+def test_few_rows_of_many_experts_with_short_reductions_take_tiles():
+    """The kernel for few rows goes through w in tiles of 16 rows, 2.2 us each however short: 48 of them in a row per
+    workgroup take 109 us where 128 x 128 tiles take 39."""
+    assert plan(OUT, 49, 4024, 104, 156, _lib.ACT_SWIGLU) == (128, 128, 2, 1)
+    assert plan(OUT, 127, 440, 72, 108, _lib.ACT_SWIGLU) == (128, 128, 2, 1)
+    for long in ((48, 2048, 4096, 256, _lib.ACT_SWIGLU), (1, 4096, 4096), (6, 2048, 4096, 256), (6, 4352, 664, 86)):
+        assert plan(OUT, *long)[:2] == (16, 16), long
