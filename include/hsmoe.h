@@ -355,9 +355,9 @@ int hsmoe_moe_combine_grad(const void* d_out_dev, int out_kind, const void* rows
 /* ---------------------------------------------------------------------------
  * Matrix product with bias, activation and residual in its epilogue, dense or
  * with one matrix per group of rows (the experts, over rows sorted by
- * hsmoe_moe_sort), for bf16 weights.  The reference has torch's linear here
- * (fused_moe.py:573-598 for the shared expert, one expert at a time in
- * _forward_legacy fused_moe.py:458-551) and no gradients.
+ * hsmoe_moe_sort), for bf16 weights.  The reference calls torch's linear for
+ * such products (fused_moe.py:573-598, one expert at a time in _forward_legacy
+ * fused_moe.py:458-551, engine.py:1864-1872) and has no gradients.
  *   z[r]   = x[r] w[g]^T + bias[g]                  g: the group of row r
  *   zu[r]  = x[r] w_up[g]^T + bias_up[g]            (HSMOE_ACT_SWIGLU only)
  *   y      = z | z sigmoid(z) | min(z, L) sigmoid(min(z, L)) clamp(zu, -L, L)
