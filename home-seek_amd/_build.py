@@ -30,10 +30,10 @@ HIP_FLAGS = [
     f"-I{CSRC}",
 ]
 
-# Flags of one source.  hsmoe_linear: matrix sums in ordinary registers; left to
+# Flags of one source.  hsmoe_linear, hsmoe_fp4: matrix sums in ordinary registers; left to
 # itself the compiler keeps them in the accumulation file and, in kernels of one
 # wave per SIMD, moves 64 of them back and forth in every pass of the loop.
-SOURCE_FLAGS = {"hsmoe_linear": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("hsmoe_linear", "hsmoe_fp4")}
 
 
 def _compile(src: Path) -> Path:

@@ -22,6 +22,7 @@ OUT_BF16 = 1
 ACT_NONE = 0
 ACT_SILU = 1
 ACT_SWIGLU = 2
+ROWS_FP4 = 2
 LINEAR_OUT = 0
 LINEAR_DX = 1
 LINEAR_DW = 2
@@ -102,6 +103,10 @@ _SIGNATURES = {
                                        _c_void_p, _i64, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_linear_grad_weight": (_int, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _int,
                                         _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "hsmoe_fp4_quant": (_int, [_c_void_p, _i64, _int, _i64, _i64, _c_void_p, _c_void_p, _c_void_p]),
+    "hsmoe_fp4_linear_workspace_size": (_size, [_i64, _i64, _i64, _int]),
+    "hsmoe_fp4_linear": (_int, [_c_void_p, _int, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int,
+                                _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_lm_head_workspace_size": (_size, [_i64, _i64]),
     "hsmoe_lm_head_accept": (_int, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p, _c_void_p, _size, _c_void_p]),

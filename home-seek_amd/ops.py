@@ -23,7 +23,7 @@ __all__ = [
     "clear_moe_layer_status", "check_moe_layer_status", "lm_head_accept", "expert_table", "shared_entry",
     "dequant_blocked", "xor_checksum", "MAX_DECODE_TOKENS", "MAX_LAYER_EXPERTS", "embed_add_rms_norm", "mtp_input",
     "decode_step_record", "ExpertOrder", "moe_sort", "moe_gather", "moe_combine", "moe_combine_grad",
-    "linear", "linear_grad", "LinearGrad",
+    "linear", "linear_grad", "LinearGrad", "fp4_quant", "fp4_linear",
 ]
 
 MAX_DECODE_TOKENS = 8
@@ -600,6 +600,85 @@ def linear_grad(d_out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str 
                                                  kind, ptr(dw[0]), ptr(dw[1]), ptr(ws), nbytes, stream_ptr(dev)),
                   "hsmoe_linear_grad_weight")
     return LinearGrad(dx, dw[0], db[0], dw[1], db[1])
+
+
+def _fp4_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
+    """x [..., K] as rows [M, K] that the kernels can read, their kind and the distance between them."""
+    kind = _row_kind(x.dtype, what)
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] % 32:
+        raise ValueError(f"{what} {tuple(x.shape)} must have rows of a multiple of 32 values")
+    k = x.shape[-1]
+    x = x if x.dim() == 2 else x.reshape(-1, k)
+    unit = 16 // x.element_size()
+    if x.data_ptr() % 16 or x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) < k or x.stride(0) % unit)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, kind, _row_stride(x)
+
+
+def _fp4_operand(codes: torch.Tensor, scale: torch.Tensor, what: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """Packed codes [..., K/2] with E8M0 scales [..., K/32], contiguous and 16-byte aligned."""
+    if codes.dtype not in (torch.int8, torch.uint8):
+        raise TypeError(f"{what}: packed FP4 must be int8/uint8, got {codes.dtype}")
+    if scale is None or scale.dtype != torch.float8_e8m0fnu:
+        raise TypeError(f"{what}: the scales must be float8_e8m0fnu, got {None if scale is None else scale.dtype}")
+    if codes.dim() < 1 or codes.shape[-1] < 16 or codes.shape[-1] % 16:
+        raise ValueError(f"{what} {tuple(codes.shape)} must hold a multiple of 32 values per row")
+    want = tuple(codes.shape[:-1]) + (codes.shape[-1] // 16,)
+    if tuple(scale.shape) != want:
+        raise ValueError(f"{what}: scale shape {tuple(scale.shape)} does not match {want}")
+    codes, scale = codes.contiguous(), scale.view(torch.uint8).contiguous()
+    codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
+    return codes, scale if scale.data_ptr() % 16 == 0 else scale.clone()
+
+
+def fp4_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(packed e2m1 int8 [..., K/2], E8M0 scales [..., K/32]) of x [..., K] (bf16 or
+    fp32, K a multiple of 32): the experts' own format, what fp4_dequant_bf16 reads.
+    A scale is the smallest power of two with which the block's largest magnitude is
+    at most 6, a code the nearest one, ties to even; a block with an infinity or a NaN
+    becomes NaN (hsmoe_fp4_quant)."""
+    dev = require_cuda(x)
+    lead, k = x.shape[:-1], x.shape[-1] if x.dim() else 0
+    x, kind, stride = _fp4_rows(x, "x")
+    packed = torch.empty(lead + (k // 2,), dtype=torch.int8, device=dev)
+    scale = torch.empty(lead + (k // 32,), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        check(lib().hsmoe_fp4_quant(ptr(x), stride, kind, x.shape[0], k, ptr(packed), ptr(scale), stream_ptr(dev)),
+              "hsmoe_fp4_quant")
+    return packed, scale.view(torch.float8_e8m0fnu)
+
+
+def fp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x w^T with both operands in 4 bits (hsmoe_fp4_linear): w packed [N, K/2] with
+    w_scale [N, K/32], x [..., K] bf16 or fp32, quantised as fp4_quant does on the way,
+    or packed [..., K/2] with x_scale [..., K/32] -> [..., N] bf16 or fp32.  Sums in
+    fp32.  K must be a multiple of 32, N of 8.  There is no gradient."""
+    dev = require_cuda(x, w, w_scale, x_scale)
+    if w.dim() != 2:
+        raise ValueError("w must be 2-D [N, K/2]")
+    w, w_scale = _fp4_operand(w, w_scale, "w")
+    n, k = w.shape[0], w.shape[1] * 2
+    out_kind = _row_kind(out_dtype, "the output")
+    if x_scale is not None:
+        if x.dim() < 1 or x.shape[-1] != k // 2:
+            raise ValueError(f"x {tuple(x.shape)} does not have packed rows of {k} values")
+        lead = x.shape[:-1]
+        x, x_scale = _fp4_operand(x, x_scale, "x")
+        m, kind, stride = x.numel() // (k // 2), _lib.ROWS_FP4, 0
+    else:
+        if x.dim() < 1 or x.shape[-1] != k:
+            raise ValueError(f"x {tuple(x.shape)} does not have rows of {k}")
+        lead = x.shape[:-1]
+        x, kind, stride = _fp4_rows(x, "x")
+        m = x.shape[0]
+    out = torch.empty(lead + (n,), dtype=out_dtype, device=dev)
+    with _on(dev):
+        nbytes = lib().hsmoe_fp4_linear_workspace_size(m, n, k, kind)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
+        check(lib().hsmoe_fp4_linear(ptr(x), kind, stride, ptr(x_scale), m, k, ptr(w), ptr(w_scale), n, out_kind,
+                                     ptr(out), ptr(ws), nbytes, stream_ptr(dev)), "hsmoe_fp4_linear")
+    return out
 
 
 def moe_decode_stage(stage: int, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,

@@ -425,6 +425,36 @@ int hsmoe_linear_grad_weight(const void* dz_dev, int64_t dz_row_stride, const vo
 int hsmoe_linear_plan(int product, int64_t m, int64_t n, int64_t k, int64_t n_groups, int act, int32_t plan[4]);
 
 /* ---------------------------------------------------------------------------
+ * Microscaled 4-bit floating point in the experts' own format (e2m1 codes, low
+ * nibble first, with one E8M0 power of two per 32 values of a row): quantisation,
+ * what the reference's offline quantiser does (_fp4.py:113-255,
+ * quantize_weights.py:1-199), and the product of two quantised operands, which it
+ * does not have.
+ *
+ * hsmoe_fp4_quant: x [m, k] rows (HSMOE_OUT_BF16 or HSMOE_OUT_F32, x_row_stride
+ * values apart) -> codes uint8 [m, k / 2] and scales uint8 [m, k / 32].  A block's
+ * scale is the smallest power of two with which its largest magnitude is at most
+ * 6 (2^-127 at least, exponent byte 0), so that nothing saturates; a value's code
+ * is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it, ties to the even code, with the
+ * value's sign.  A block with an infinity or a NaN has exponent byte 255: NaN.
+ * k a multiple of 32 below 2^22, rows 16-byte aligned; m may be 0. */
+int hsmoe_fp4_quant(const void* x_dev, int64_t x_row_stride, int row_kind, int64_t m, int64_t k, void* codes_dev,
+                    void* scale_dev, hsmoe_stream_t stream);
+
+/* out[r] = xq[r] wq^T: x quantised as above in the call (x_kind HSMOE_OUT_BF16 or
+ * HSMOE_OUT_F32), or given quantised (HSMOE_ROWS_FP4: contiguous codes [m, k / 2]
+ * and x_scale [m, k / 32]; x_row_stride is not read), by w codes [n, k / 2] and
+ * w_scale [n, k / 32].  Sums in fp32, one rounding to out [m, n] (bf16 or fp32,
+ * out_kind).  k a multiple of 32, n of 8; operands 16-byte aligned.  The workspace
+ * (hsmoe_fp4_linear_workspace_size bytes, any contents) holds x's codes and the
+ * scales in another order; one call at a time.  Deterministic. */
+#define HSMOE_ROWS_FP4 2
+size_t hsmoe_fp4_linear_workspace_size(int64_t m, int64_t n, int64_t k, int x_kind);
+int hsmoe_fp4_linear(const void* x_dev, int x_kind, int64_t x_row_stride, const void* x_scale_dev, int64_t m,
+                     int64_t k, const void* w_dev, const void* w_scale_dev, int64_t n, int out_kind, void* out_dev,
+                     void* workspace_dev, size_t workspace_bytes, hsmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * lm_head logits + greedy argmax + longest-prefix draft acceptance.
  * Replaces the logits / acceptance loop of _mtp_verify_batched
  * (reference src/home_seek/inference_engine/engine.py:2480-2497) and the greedy
