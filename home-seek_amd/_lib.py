@@ -23,6 +23,10 @@ ACT_NONE = 0
 ACT_SILU = 1
 ACT_SWIGLU = 2
 ROWS_FP4 = 2
+GATE_NONE = 0
+GATE_CHANNEL = 1
+GATE_TOKEN = 2
+GATE_FULL = 3
 LINEAR_OUT = 0
 LINEAR_DX = 1
 LINEAR_DW = 2
@@ -40,6 +44,12 @@ class NormTail(ctypes.Structure):
     """hsmoe_norm_tail: the next layer's residual adds + RMSNorm ending a layer launch."""
     _fields_ = [("h_dev", _c_void_p), ("residual_dev", _c_void_p), ("weight_dev", _c_void_p), ("eps", _f32),
                 ("h_out_dev", _c_void_p), ("norm_out_dev", _c_void_p)]
+
+
+class BlockNormSpec(ctypes.Structure):
+    """hsmoe_block_norm_spec: weights, gate and types of hsmoe_block_norm."""
+    _fields_ = [("post_w_dev", _c_void_p), ("pre_w_dev", _c_void_p), ("gate_dev", _c_void_p), ("row_kind", _int),
+                ("stream_kind", _int), ("weight_kind", _int), ("gate_kind", _int), ("gate_form", _int)]
 
 
 # name -> (restype, argtypes); mirrors include/hsmoe.h
@@ -113,6 +123,10 @@ _SIGNATURES = {
     "hsmoe_rms_norm": (_int, [_c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p, _c_void_p]),
     "hsmoe_add_rms_norm": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p,
                                   _c_void_p, _c_void_p]),
+    "hsmoe_block_norm": (_int, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _f32, _f32, _c_void_p, _c_void_p, _c_void_p]),
+    "hsmoe_block_norm_grad_workspace_size": (_size, [_i64, _i64]),
+    "hsmoe_block_norm_grad": (_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _f32, _f32,
+                                     _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_embed_add_rms_norm": (_int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _f32,
                                         _c_void_p, _c_void_p, _c_void_p]),
     "hsmoe_mtp_input": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,

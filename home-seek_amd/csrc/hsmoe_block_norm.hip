@@ -1,0 +1,545 @@
+// What stands between two blocks of a residual network: the norm after the block,
+// its gate and residual scale, the add to the stream, and the norm before the next
+// block, in one pass, and the gradient of it all.
+//   u  = post_w * f r1,  r1 = 1 / sqrt(mean(f^2) + eps)     (without post_w: u = f)
+//   h' = h + scale * gate * u                                rounded to the stream's type
+//   n  = pre_w * h' r2,  r2 = 1 / sqrt(mean(h'^2) + eps)    (without pre_w: none)
+// The norm before the next block is that of the stream as it is held (rounded), so
+// that the gradient, which has h' only, is that of the same function.  Gradient:
+//   g   = pre_w dn;  dH = dh' + r2 (g - h' r2^2 mean(g h'));  d_pre = sum_rows dn h' r2
+//   dt  = scale dH;  d_gate = dt u (summed over what the gate is broadcast to)
+//   du  = dt gate;   d_post = sum_rows du f r1
+//   df  = r1 (post_w du - f r1^2 mean(post_w du f))         (without post_w: du)
+// Sums in fp32.  All of it is bound by HBM; few rows by the latency of two sums
+// over a row, one after the other.
+#include "hsmoe_common.h"
+#include "hsmoe_internal.h"
+
+namespace hsmoe {
+namespace {
+
+constexpr int kMaxD = 16384;
+enum { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateFull = 3 };
+
+struct BlockNormParams {
+  const void *f, *h;             // [m][d]; h: the stream before (forward), after the block (gradient)
+  const void *post_w, *pre_w;    // [d] or NULL
+  const void* gate;              // [d], [m], [m][d] or NULL
+  void *h_out, *n_out;           // forward
+  const void *d_h, *d_n;         // gradient: [m][d] each, NULL for zeros
+  void *d_f, *d_x;               // [m][d] of f and of the stream; NULL where not wanted
+  void* d_gate;                  // kGateFull: [m][d]; kGateToken: fp32 [m]
+  float* part;                   // fp32 [workgroups][3][d]: sums of d_pre, d_post, d_gate (kGateChannel)
+  int64_t m;
+  int d, gate_kind;
+  bool w_f32, gate_f32;          // weights and gate of fp32 (else bf16)
+  bool sum_pre, sum_post, sum_gate;
+  float scale, eps;
+};
+
+// Eight values of a row at a time.
+struct V8 {
+  float v[8];
+};
+// (row: values before the row, the same for a workgroup's threads where they share
+// it, so that an address is a scalar base and a 32-bit offset)
+template <bool kF32>
+__device__ __forceinline__ const char* place(const void* base, int64_t row, uint32_t col) {
+  return (const char*)base + row * (kF32 ? 4 : 2) + col * (uint32_t)(kF32 ? 4 : 2);
+}
+template <bool kF32>
+__device__ __forceinline__ V8 read8(const void* base, int64_t row, uint32_t col) {
+  V8 r;
+  const char* p = place<kF32>(base, row, col);
+  if (kF32) {
+    const uint4 a = ldg<uint4>(p), b = ldg<uint4>(p + 16);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(w[i]);
+  } else {
+    const uint4 a = ldg<uint4>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[2 * i] = __uint_as_float(w[i] << 16), r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  return r;
+}
+__device__ __forceinline__ V8 read8(const void* base, int64_t row, uint32_t col, bool f32) {
+  return f32 ? read8<true>(base, row, col) : read8<false>(base, row, col);
+}
+template <bool kF32>
+__device__ __forceinline__ void write8(void* base, int64_t row, uint32_t col, const V8& r) {
+  char* at = const_cast<char*>(place<kF32>(base, row, col));
+  if (kF32) {
+    float4* p = reinterpret_cast<float4*>(at);
+    p[0] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
+    p[1] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16_bits(r.v[2 * i]) | f32_to_bf16_bits(r.v[2 * i + 1]) << 16;
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <bool kF32>
+__device__ __forceinline__ V8 rounded8(const V8& r) {
+  if (kF32) return r;
+  V8 o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o.v[i] = bf16_bits_to_f32(f32_to_bf16_bits(r.v[i]));
+  return o;
+}
+__device__ __forceinline__ V8 ones8() { return V8{{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f}}; }
+
+__device__ __forceinline__ float inv_rms(float sum, int d, float eps) {
+  return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)d), eps)));
+}
+
+// kLanes threads share a row: 8 .. 64 of a wave (a workgroup of 256 then takes
+// several rows at a time), or all of a workgroup (0), up to 1024 threads.  kC: a
+// thread's chunks of eight columns, kLanes (the workgroup) apart.
+// Sums over the row's threads, in a fixed order; every thread gets them.
+template <int kLanes, int kN>
+__device__ __forceinline__ void row_sum(float (&s)[kN], float (*mem)[16], int threads) {
+  constexpr int kWave = kLanes ? kLanes : 64;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s[i] += __shfl_xor(s[i], off, 64);
+  if (kLanes == 0) {
+    const int waves = threads >> 6, wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < kN; ++i) mem[i][wave] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      s[i] = 0.0f;
+      for (int w = 0; w < waves; ++w) s[i] += mem[i][w];
+    }
+  }
+}
+
+template <int kLanes, int kC, bool kF32, bool kS32>
+__global__ void __launch_bounds__(kLanes ? 256 : 1024) block_norm_kernel(BlockNormParams p) {
+  __shared__ float mem[2][1][16];
+  const int threads = kLanes ? kLanes : (int)blockDim.x;
+  const int t = kLanes ? threadIdx.x % kLanes : threadIdx.x;
+  const int64_t row = kLanes ? (int64_t)blockIdx.x * (256 / (kLanes ? kLanes : 1)) + threadIdx.x / (kLanes ? kLanes : 1) : blockIdx.x;
+  const bool live = row < p.m;
+  const int64_t base = (live ? row : 0) * p.d;
+  V8 f[kC], h[kC], gate[kC], wa[kC], wb[kC];
+  bool in[kC];
+  float token = 1.0f;
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const uint32_t col = (t + c * threads) * 8;
+    in[c] = live && col < (uint32_t)p.d;
+    f[c] = h[c] = V8{}, gate[c] = wa[c] = wb[c] = ones8();
+    if (!in[c]) continue;
+    f[c] = read8<kF32>(p.f, base, col);
+    h[c] = read8<kS32>(p.h, base, col);
+    if (p.gate_kind == kGateFull) gate[c] = read8(p.gate, base, col, p.gate_f32);
+    if (p.gate_kind == kGateChannel) gate[c] = read8(p.gate, 0, col, p.gate_f32);
+    if (p.post_w) wa[c] = read8(p.post_w, 0, col, p.w_f32);
+    if (p.pre_w) wb[c] = read8(p.pre_w, 0, col, p.w_f32);
+  }
+  if (p.gate_kind == kGateToken && live)
+    token = p.gate_f32 ? ((const float*)p.gate)[row] : bf16_bits_to_f32(((const uint16_t*)p.gate)[row]);
+  float r1 = 1.0f;
+  if (p.post_w) {
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[0] = __fmaf_rn(f[c].v[i], f[c].v[i], s[0]);
+    row_sum<kLanes, 1>(s, mem[0], threads);
+    r1 = inv_rms(s[0], p.d, p.eps);
+  }
+  float s[1] = {0.0f};
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const uint32_t col = (t + c * threads) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float u = f[c].v[i] * r1 * wa[c].v[i];
+      h[c].v[i] = __fmaf_rn(p.scale, token * gate[c].v[i] * u, h[c].v[i]);
+    }
+    h[c] = rounded8<kS32>(h[c]);
+    if (in[c]) write8<kS32>(p.h_out, base, col, h[c]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[0] = __fmaf_rn(in[c] ? h[c].v[i] : 0.0f, h[c].v[i], s[0]);
+  }
+  if (!p.pre_w) return;
+  row_sum<kLanes, 1>(s, mem[1], threads);
+  const float r2 = inv_rms(s[0], p.d, p.eps);
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const uint32_t col = (t + c * threads) * 8;
+    V8 n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n.v[i] = h[c].v[i] * r2 * wb[c].v[i];
+    if (in[c]) write8<kF32>(p.n_out, base, col, n);
+  }
+}
+
+// Eight values as they lie in memory.
+template <bool kF32>
+struct Raw8 {
+  uint32_t w[kF32 ? 8 : 4];
+  __device__ __forceinline__ float at(int i) const {
+    if (kF32) return __uint_as_float(w[i]);
+    return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
+  }
+};
+template <bool kF32>
+__device__ __forceinline__ Raw8<kF32> raw8(const void* base, int64_t row, uint32_t col) {
+  Raw8<kF32> r;
+  const char* p = place<kF32>(base, row, col);
+#pragma unroll
+  for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+    const uint4 a = ldg<uint4>(p + 16 * i);
+    r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
+  }
+  return r;
+}
+
+// The compiler unpacks it again behind this, instead of keeping eight floats over a sum.
+template <bool kF32>
+__device__ __forceinline__ void unpack_later(Raw8<kF32>& r) {
+#pragma unroll
+  for (int i = 0; i < (kF32 ? 8 : 4); ++i) asm volatile("" : "+v"(r.w[i]));
+}
+
+// No load moves over this.
+__device__ __forceinline__ void apart() { asm volatile("" ::: "memory"); }
+
+// The gradient.  A workgroup goes through every gridDim-th row (group of rows),
+// the next one's loads on their way while one is worked on, and keeps its columns'
+// part of the weights' gradients in registers; they leave once at its end, as one
+// row of `part`, and a second kernel adds the workgroups' rows in their order.
+template <int kLanes, int kC, int kMax, bool kF32, bool kS32>
+__global__ void __launch_bounds__(kMax) block_norm_grad_kernel(BlockNormParams p) {
+  __shared__ float mem[2][5][16];
+  __shared__ float sums[kLanes ? 256 * 8 * kC : 1];
+  constexpr int kRows = kLanes ? 256 / (kLanes ? kLanes : 1) : 1;  // at a time
+  const int threads = kLanes ? kLanes : (int)blockDim.x;
+  const int t = kLanes ? threadIdx.x % kLanes : threadIdx.x;
+  const int mine = kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0;
+  struct Row {
+    Raw8<kF32> f[kC], dn[kC];
+    Raw8<kS32> h[kC], dh[kC];
+  };
+  auto load = [&](int64_t row) {
+    Row r = {};
+    if (row >= p.m) return r;
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const uint32_t col = (t + c * threads) * 8;
+      if (col >= (uint32_t)p.d) continue;
+      r.f[c] = raw8<kF32>(p.f, row * p.d, col);
+      if (p.d_h) r.dh[c] = raw8<kS32>(p.d_h, row * p.d, col);
+      if (p.d_n) r.h[c] = raw8<kS32>(p.h, row * p.d, col), r.dn[c] = raw8<kF32>(p.d_n, row * p.d, col);
+    }
+    return r;
+  };
+  const int64_t stride = (int64_t)gridDim.x * kRows;
+  int64_t first = (int64_t)blockIdx.x * kRows;
+  // wide rows: the weights are read again for every row, and for the widest no row
+  // is loaded ahead, for the registers
+  constexpr bool kLean = kC > 1, kAhead = kC < 4;
+  Row next = kAhead ? load(first + mine) : Row{};
+  V8 a_pre[kC] = {}, a_post[kC] = {}, a_gate[kC] = {}, gate[kC], wa[kC], wb[kC];
+  auto read_post = [&](int c) {
+    const uint32_t col = (t + c * threads) * 8;
+    gate[c] = wa[c] = ones8();
+    if (col >= (uint32_t)p.d) return;
+    if (p.gate_kind == kGateChannel) gate[c] = read8(p.gate, 0, col, p.gate_f32);
+    if (p.post_w) wa[c] = read8(p.post_w, 0, col, p.w_f32);
+  };
+  auto read_pre = [&](int c) {
+    const uint32_t col = (t + c * threads) * 8;
+    wb[c] = p.d_n && col < (uint32_t)p.d ? read8(p.pre_w, 0, col, p.w_f32) : ones8();
+  };
+  if (!kLean)
+#pragma unroll
+    for (int c = 0; c < kC; ++c) read_post(c), read_pre(c);
+  for (; first < p.m; first += stride) {
+    const int64_t row = first + mine;
+    const bool live = row < p.m;
+    const int64_t base = (live ? row : 0) * p.d;
+    Row r = kAhead ? next : load(row);
+    if (kAhead) next = load(row + stride);
+    float token = 1.0f;
+    if (p.gate_kind == kGateToken && live)
+      token = p.gate_f32 ? ((const float*)p.gate)[row] : bf16_bits_to_f32(((const uint16_t*)p.gate)[row]);
+    if (!kLean && p.gate_kind == kGateFull)
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint32_t col = (t + c * threads) * 8;
+        if (live && col < (uint32_t)p.d) gate[c] = read8(p.gate, base, col, p.gate_f32);
+      }
+    float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      if (kLean) apart(), read_pre(c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = r.f[c].at(i), h = r.h[c].at(i);
+        s[0] = __fmaf_rn(f, f, s[0]);
+        s[1] = __fmaf_rn(h, h, s[1]);
+        s[2] = __fmaf_rn(r.dn[c].at(i) * wb[c].v[i], h, s[2]);
+      }
+    }
+    row_sum<kLanes, 3>(s, mem[0], threads);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) unpack_later(r.f[c]), unpack_later(r.h[c]), unpack_later(r.dn[c]);
+    const float r1 = p.post_w ? inv_rms(s[0], p.d, p.eps) : 1.0f;
+    const float r2 = p.d_n ? inv_rms(s[1], p.d, p.eps) : 0.0f;
+    const float m2 = s[2] / (float)p.d * r2 * r2;  // r2^2 mean(g h')
+    float q[2] = {0.0f, 0.0f};                     // sum of post_w du f, and of dt u
+    V8 df[kC];
+#pragma unroll
+    for (int c = 0; c < kC; ++c) {
+      const uint32_t col = (t + c * threads) * 8;
+      V8 dx, dg;
+      if (kLean) {
+        apart(), read_pre(c), read_post(c);
+        if (p.gate_kind == kGateFull && live && col < (uint32_t)p.d) gate[c] = read8(p.gate, base, col, p.gate_f32);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = r.h[c].at(i), g = r.dn[c].at(i), f = r.f[c].at(i);
+        a_pre[c].v[i] = __fmaf_rn(g, x * r2, a_pre[c].v[i]);
+        dx.v[i] = __fmaf_rn(r2, __fmaf_rn(-x, m2, g * wb[c].v[i]), r.dh[c].at(i));
+        const float dt = p.scale * dx.v[i];
+        const float y = f * r1;
+        dg.v[i] = dt * (y * wa[c].v[i]);
+        const float du = dt * (token * gate[c].v[i]);
+        a_gate[c].v[i] += dg.v[i];
+        a_post[c].v[i] = __fmaf_rn(du, y, a_post[c].v[i]);
+        df[c].v[i] = du * wa[c].v[i];
+        q[0] = __fmaf_rn(df[c].v[i], f, q[0]);
+        q[1] += dg.v[i];
+      }
+      if (live && col < (uint32_t)p.d) {
+        if (p.d_x) write8<kS32>(p.d_x, base, col, dx);
+        if (p.gate_kind == kGateFull && p.d_gate) {
+          if (p.gate_f32) write8<true>(p.d_gate, base, col, dg);
+          else write8<false>(p.d_gate, base, col, dg);
+        }
+      }
+    }
+    row_sum<kLanes, 2>(q, mem[1], threads);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) unpack_later(r.f[c]);
+    if (p.gate_kind == kGateToken && p.d_gate && live && t == 0) ((float*)p.d_gate)[row] = q[1];
+    if (p.d_f) {
+      const float m1 = p.post_w ? q[0] / (float)p.d * r1 * r1 : 0.0f;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint32_t col = (t + c * threads) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) df[c].v[i] = r1 * __fmaf_rn(-r.f[c].at(i), m1, df[c].v[i]);
+        if (live && col < (uint32_t)p.d) write8<kF32>(p.d_f, base, col, df[c]);
+      }
+    }
+  }
+  if (!p.part) return;
+  float* out = p.part + (int64_t)blockIdx.x * 3 * p.d;
+  auto leave = [&](const V8 (&a)[kC], float* to) {
+    if (kLanes == 0) {
+#pragma unroll
+      for (int c = 0; c < kC; ++c) {
+        const uint32_t col = (t + c * threads) * 8;
+        if (col < (uint32_t)p.d) write8<true>(to, 0, col, a[c]);
+      }
+    } else {  // the rows' groups in their order
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[(mine * kC + c) * 8 * threads + i * threads + t] = a[c].v[i];
+      __syncthreads();
+      if (mine == 0)
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          const uint32_t col = (t + c * threads) * 8;
+          V8 v = {};
+          for (int g = 0; g < kRows; ++g)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v.v[i] += sums[(g * kC + c) * 8 * threads + i * threads + t];
+          if (col < (uint32_t)p.d) write8<true>(to, 0, col, v);
+        }
+    }
+  };
+  if (p.sum_pre) leave(a_pre, out);
+  if (p.sum_post) leave(a_post, out + p.d);
+  if (p.sum_gate) leave(a_gate, out + 2 * p.d);
+}
+
+// Column sums of the workgroups' rows: 64 columns per workgroup, its 16 waves a
+// sixteenth of the rows each, joined in wave order.
+constexpr int kJoinWaves = 16;
+struct JoinParams {
+  const float* part;
+  float* out[3];
+  int rows[3];  // 0: a gradient of zeros
+  int d;
+};
+__global__ void __launch_bounds__(kJoinWaves * 64) block_norm_join_kernel(JoinParams p) {
+  __shared__ float mem[kJoinWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t col = blockIdx.x * 64 + lane, which = blockIdx.y;
+  if (!p.out[which]) return;
+  const int rows = p.rows[which], per = (rows + kJoinWaves - 1) / kJoinWaves;
+  const int r0 = wave * per, r1 = r0 + per < rows ? r0 + per : rows;
+  float s = 0.0f;
+  if (col < (uint32_t)p.d)
+#pragma unroll 8
+    for (int r = r0; r < r1; ++r) s += p.part[((int64_t)r * 3 + which) * p.d + col];
+  mem[wave][lane] = s;
+  __syncthreads();
+  if (wave || col >= (uint32_t)p.d) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWaves; ++w) s += mem[w][lane];
+  p.out[which][col] = s;
+}
+
+// How rows are shared out: threads per row (8 .. 64 of a wave, 0: the workgroup's),
+// threads of a workgroup, its rows at a time, a thread's chunks of eight columns.
+struct Shape {
+  int lanes, threads, rows, chunks;
+};
+Shape shape_of(int64_t d, bool grad) {
+  const int chunks = (int)(d / 8);
+  if (chunks <= 8) return {8, 256, 32, 1};
+  if (chunks <= 16) return {16, 256, 16, 1};
+  if (chunks <= 32) return {32, 256, 8, 1};
+  if (chunks <= 64) return {64, 256, 4, 1};
+  const int per = !grad ? 2 : chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
+  return {0, ((chunks + per - 1) / per + 63) / 64 * 64, 1, per};
+}
+// Workgroups of the gradient: with weights' gradients to sum, what the CUs hold
+// (each leaves a row of sums); else one per row group.
+int64_t grad_groups(int64_t m, const Shape& s, bool sums) {
+  const int64_t all = (m + s.rows - 1) / s.rows, some = (s.chunks > 1 ? 1 : 2) * (int64_t)device_cus();
+  return sums && all > some ? some : all;
+}
+
+template <bool kGrad, bool kF32, bool kS32>
+void launch(const Shape& s, int64_t grid, const BlockNormParams& p, hipStream_t st) {
+  const dim3 g((unsigned)grid), b(s.threads);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, st, p); };
+  if constexpr (kGrad) {
+    if (s.lanes == 8) return go(block_norm_grad_kernel<8, 1, 256, kF32, kS32>);
+    if (s.lanes == 16) return go(block_norm_grad_kernel<16, 1, 256, kF32, kS32>);
+    if (s.lanes == 32) return go(block_norm_grad_kernel<32, 1, 256, kF32, kS32>);
+    if (s.lanes == 64) return go(block_norm_grad_kernel<64, 1, 256, kF32, kS32>);
+    if (s.chunks == 1) return go(block_norm_grad_kernel<0, 1, 512, kF32, kS32>);
+    if (s.chunks == 2) return go(block_norm_grad_kernel<0, 2, 512, kF32, kS32>);
+    return go(block_norm_grad_kernel<0, 4, 512, kF32, kS32>);
+  } else {
+    if (s.lanes == 8) return go(block_norm_kernel<8, 1, kF32, kS32>);
+    if (s.lanes == 16) return go(block_norm_kernel<16, 1, kF32, kS32>);
+    if (s.lanes == 32) return go(block_norm_kernel<32, 1, kF32, kS32>);
+    if (s.lanes == 64) return go(block_norm_kernel<64, 1, kF32, kS32>);
+    return go(block_norm_kernel<0, 2, kF32, kS32>);
+  }
+}
+template <bool kGrad>
+void launch_kinds(const Shape& s, int64_t grid, bool f32, bool s32, const BlockNormParams& p, hipStream_t st) {
+  if (f32 && s32)
+    launch<kGrad, true, true>(s, grid, p, st);
+  else if (f32)
+    launch<kGrad, true, false>(s, grid, p, st);
+  else if (s32)
+    launch<kGrad, false, true>(s, grid, p, st);
+  else
+    launch<kGrad, false, false>(s, grid, p, st);
+}
+
+bool kind_ok(int k) { return k == HSMOE_OUT_F32 || k == HSMOE_OUT_BF16; }
+int check_norm(const char* who, int64_t m, int64_t d, float eps, const hsmoe_block_norm_spec* n) {
+  if (!n || m < 0 || d < 1 || !(eps >= 0.0f) || !kind_ok(n->row_kind) || !kind_ok(n->stream_kind) || !kind_ok(n->weight_kind) ||
+      !kind_ok(n->gate_kind) || n->gate_form < kGateNone || n->gate_form > kGateFull ||
+      (n->gate_form == kGateNone && n->gate_dev) || (n->gate_form != kGateNone && !n->gate_dev && m > 0))
+    return fail(HSMOE_ERR_ARG, "%s: bad arguments", who);
+  if (d % 8 != 0 || d > kMaxD) return fail(HSMOE_ERR_SHAPE, "%s: d must be a multiple of 8 and at most %d", who, kMaxD);
+  if (m >= (1ll << 31)) return fail(HSMOE_ERR_SHAPE, "%s: m must be below 2^31", who);
+  if (!aligned(n->post_w_dev, 16) || !aligned(n->pre_w_dev, 16) || !aligned(n->gate_dev, n->gate_form == kGateToken ? 4 : 16))
+    return fail(HSMOE_ERR_SHAPE, "%s: weights and gates must be 16-byte aligned", who);
+  return HSMOE_OK;
+}
+BlockNormParams params_of(int64_t m, int64_t d, float scale, float eps, const hsmoe_block_norm_spec* n) {
+  BlockNormParams p{};
+  p.post_w = n->post_w_dev, p.pre_w = n->pre_w_dev, p.gate = n->gate_dev;
+  p.m = m, p.d = (int)d, p.gate_kind = n->gate_form;
+  p.w_f32 = n->weight_kind == HSMOE_OUT_F32, p.gate_f32 = n->gate_kind == HSMOE_OUT_F32;
+  p.scale = scale, p.eps = eps;
+  return p;
+}
+
+}  // namespace
+}  // namespace hsmoe
+
+using namespace hsmoe;
+
+extern "C" int hsmoe_block_norm(const void* f, const void* h, int64_t m, int64_t d, const hsmoe_block_norm_spec* spec,
+                                float scale, float eps, void* h_out, void* n_out, hsmoe_stream_t stream) {
+  const char* who = "hsmoe_block_norm";
+  if (int rc = check_norm(who, m, d, eps, spec)) return rc;
+  if (m == 0) return HSMOE_OK;
+  if (!f || !h || !h_out || (spec->pre_w_dev != nullptr) != (n_out != nullptr)) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
+  if (!aligned(f, 16) || !aligned(h, 16) || !aligned(h_out, 16) || !aligned(n_out, 16))
+    return fail(HSMOE_ERR_SHAPE, "%s: rows must be 16-byte aligned", who);
+  BlockNormParams p = params_of(m, d, scale, eps, spec);
+  p.f = f, p.h = h, p.h_out = h_out, p.n_out = n_out;
+  const Shape s = shape_of(d, false);
+  launch_kinds<false>(s, (m + s.rows - 1) / s.rows, spec->row_kind == HSMOE_OUT_F32, spec->stream_kind == HSMOE_OUT_F32, p,
+                      (hipStream_t)stream);
+  return check_launch(who);
+}
+
+extern "C" size_t hsmoe_block_norm_grad_workspace_size(int64_t m, int64_t d) {
+  if (m < 1 || d < 8 || d > kMaxD) return 0;
+  return (size_t)grad_groups(m, shape_of(d, true), true) * 3 * d * sizeof(float);
+}
+
+extern "C" int hsmoe_block_norm_grad(const void* d_h, const void* d_n, const void* f, const void* h_out, int64_t m,
+                                     int64_t d, const hsmoe_block_norm_spec* spec, float scale, float eps, void* d_f,
+                                     void* d_x, float* d_post, void* d_gate, float* d_pre, void* workspace,
+                                     size_t workspace_bytes, hsmoe_stream_t stream) {
+  const char* who = "hsmoe_block_norm_grad";
+  if (int rc = check_norm(who, m, d, eps, spec)) return rc;
+  if ((d_post && !spec->post_w_dev) || (d_pre && !spec->pre_w_dev) || (d_gate && spec->gate_form == kGateNone) || (d_n && !spec->pre_w_dev))
+    return fail(HSMOE_ERR_ARG, "%s: the gradient of what is not there", who);
+  if (m > 0 && !d_h && !d_n) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
+  const bool sum_gate = d_gate && spec->gate_form == kGateChannel;
+  const bool sums = d_post || d_pre || sum_gate;
+  if (m > 0 && (!f || (d_n && !h_out))) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
+  const void* rows[] = {d_h, d_n, f, h_out, d_f, d_x};
+  for (const void* q : rows)
+    if (!aligned(q, 16)) return fail(HSMOE_ERR_SHAPE, "%s: rows must be 16-byte aligned", who);
+  if (!aligned(d_gate, spec->gate_form == kGateFull ? 16 : 4) || !aligned(d_post, 4) || !aligned(d_pre, 4))
+    return fail(HSMOE_ERR_SHAPE, "%s: misaligned gradients", who);
+  const Shape s = shape_of(d, true);
+  const int64_t groups = m > 0 ? grad_groups(m, s, sums) : 0;
+  const size_t need = sums ? (size_t)groups * 3 * d * sizeof(float) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return fail(HSMOE_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, need);
+  if (need && !aligned(workspace, 16)) return fail(HSMOE_ERR_SHAPE, "%s: misaligned workspace", who);
+  BlockNormParams p = params_of(m, d, scale, eps, spec);
+  p.d_h = d_h, p.d_n = d_n, p.f = f, p.h = h_out;
+  p.d_f = d_f, p.d_x = d_x, p.d_gate = sum_gate ? nullptr : d_gate;
+  p.part = sums ? (float*)workspace : nullptr;
+  p.sum_pre = d_pre && d_n, p.sum_post = d_post, p.sum_gate = sum_gate;
+  hipStream_t st = (hipStream_t)stream;
+  if (groups)
+    launch_kinds<true>(s, groups, spec->row_kind == HSMOE_OUT_F32, spec->stream_kind == HSMOE_OUT_F32, p, st);
+  if (sums) {
+    const int g = (int)groups;
+    const JoinParams j{(const float*)workspace, {d_pre, d_post, sum_gate ? (float*)d_gate : nullptr}, {d_n ? g : 0, g, g}, (int)d};
+    hipLaunchKernelGGL(block_norm_join_kernel, dim3((unsigned)((d + 63) / 64), 3), dim3(kJoinWaves * 64), 0, st, j);
+  }
+  return check_launch(who);
+}

@@ -24,6 +24,7 @@ __all__ = [
     "dequant_blocked", "xor_checksum", "MAX_DECODE_TOKENS", "MAX_LAYER_EXPERTS", "embed_add_rms_norm", "mtp_input",
     "decode_step_record", "ExpertOrder", "moe_sort", "moe_gather", "moe_combine", "moe_combine_grad",
     "linear", "linear_grad", "LinearGrad", "fp4_quant", "fp4_linear",
+    "block_norm", "block_norm_grad", "BlockNormGrad",
 ]
 
 MAX_DECODE_TOKENS = 8
@@ -944,6 +945,111 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, add: torch.Tensor | None
     check(lib().hsmoe_add_rms_norm(ptr(x2), ptr(add), ptr(residual), ptr(w), x2.shape[0], d, eps, ptr(h), ptr(out),
                                    stream_ptr(dev)), "hsmoe_add_rms_norm")
     return (None if h is None else h.reshape(shape)), out.reshape(shape)
+
+
+def _packed16(t: torch.Tensor) -> torch.Tensor:
+    """t, contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _block_norm_spec(f: torch.Tensor, stream: torch.dtype, post_w, gate, pre_w):
+    """(hsmoe_block_norm_spec, what it points to) for rows f [..., D]."""
+    d = f.shape[-1] if f.dim() else 0
+    if d < 8 or d % 8:
+        raise ValueError(f"rows {tuple(f.shape)} must have a multiple of 8 values")
+    spec = _lib.BlockNormSpec(row_kind=_row_kind(f.dtype, "f"), stream_kind=_row_kind(stream, "the stream"))
+    ws = [w for w in (post_w, pre_w) if w is not None]
+    for w in ws:
+        if tuple(w.shape) != (d,):
+            raise ValueError(f"norm weights must be [{d}], got {tuple(w.shape)}")
+    kinds = [_row_kind(w.dtype, "norm weights") for w in ws]
+    both = torch.float32 if len(set(kinds)) == 2 else None  # one kind for both
+    post_w, pre_w = (None if w is None else _packed16(w if both is None else w.to(both)) for w in (post_w, pre_w))
+    spec.weight_kind = _lib.OUT_F32 if both is not None else kinds[0] if kinds else _lib.OUT_BF16
+    if gate is not None:
+        spec.gate_kind = _row_kind(gate.dtype, "the gate")
+        if tuple(gate.shape) == (d,):
+            spec.gate_form = _lib.GATE_CHANNEL
+        elif gate.shape == f.shape:
+            spec.gate_form = _lib.GATE_FULL
+        elif gate.shape == f.shape[:-1] + (1,):
+            spec.gate_form = _lib.GATE_TOKEN
+        else:
+            raise ValueError(f"a gate must be [{d}], {tuple(f.shape[:-1] + (1,))} or {tuple(f.shape)}, got {tuple(gate.shape)}")
+        gate = _packed16(gate)
+    spec.post_w_dev, spec.pre_w_dev, spec.gate_dev = ptr(post_w), ptr(pre_w), ptr(gate)
+    return spec, (post_w, pre_w, gate)
+
+
+def block_norm(f: torch.Tensor, h: torch.Tensor, post_w: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+               scale: float = 1.0, pre_w: torch.Tensor | None = None, eps: float = 1e-6):
+    """What stands between two blocks (hsmoe_block_norm): for a block's result f
+    [..., D] and the stream h [..., D] before it
+      h' = h + scale * gate * RMSNorm(f, post_w)     (without post_w: f as it is)
+      n  = RMSNorm(h', pre_w)                        (None without pre_w)
+    -> (h', n): h' of h's dtype, n of f's, of the rounded h'.  gate: [D], [..., 1] or
+    [..., D].  Every tensor bf16 or fp32; D a multiple of 8 up to 16384."""
+    dev = require_cuda(f, h, post_w, gate, pre_w)
+    if h.shape != f.shape:
+        raise ValueError(f"the stream {tuple(h.shape)} does not match f {tuple(f.shape)}")
+    spec, keep = _block_norm_spec(f, h.dtype, post_w, gate, pre_w)
+    d = f.shape[-1]
+    f, h = _packed16(f), _packed16(h)
+    out = torch.empty(f.shape, dtype=h.dtype, device=dev)
+    n = None if pre_w is None else torch.empty(f.shape, dtype=f.dtype, device=dev)
+    with _on(dev):
+        check(lib().hsmoe_block_norm(ptr(f), ptr(h), f.numel() // d, d, ctypes.addressof(spec), scale, eps, ptr(out), ptr(n),
+                                     stream_ptr(dev)), "hsmoe_block_norm")
+    return out, n
+
+
+class BlockNormGrad(NamedTuple):
+    """The gradient of block_norm; None where there is nothing or it is not needed."""
+    f: torch.Tensor | None
+    h: torch.Tensor | None
+    post_w: torch.Tensor | None
+    gate: torch.Tensor | None
+    pre_w: torch.Tensor | None
+
+
+def block_norm_grad(d_h: torch.Tensor | None, d_n: torch.Tensor | None, f: torch.Tensor, h_out: torch.Tensor,
+                    post_w: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+                    pre_w: torch.Tensor | None = None, eps: float = 1e-6,
+                    need: tuple[bool, bool, bool, bool, bool] = (True,) * 5) -> BlockNormGrad:
+    """The gradient of block_norm(f, h, ...) for d_h of its first result h_out and d_n of
+    its second (either None: zeros): f and h in their dtypes, a gate [..., D] in its own,
+    the norms' weights and a gate that is broadcast in fp32 (hsmoe_block_norm_grad).
+    need: which of them."""
+    dev = require_cuda(d_h, d_n, f, h_out, post_w, gate, pre_w)
+    spec, keep = _block_norm_spec(f, h_out.dtype, post_w, gate, pre_w)
+    for t, what, dtype in ((h_out, "h_out", h_out.dtype), (d_h, "d_h", h_out.dtype), (d_n, "d_n", f.dtype)):
+        if t is not None and (t.shape != f.shape or t.dtype != dtype):
+            raise ValueError(f"{what} must be {tuple(f.shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+    if d_n is not None and pre_w is None:
+        raise ValueError("d_n goes with pre_w")
+    if d_h is None and d_n is None:
+        raise ValueError("the gradient of neither result is given")
+    d = f.shape[-1]
+    m = f.numel() // d
+    f, h_out = _packed16(f), _packed16(h_out)
+    d_h, d_n = (None if t is None else _packed16(t) for t in (d_h, d_n))
+    new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev)
+    d_f = new(f.shape, f.dtype) if need[0] else None
+    d_x = new(f.shape, h_out.dtype) if need[1] else None
+    d_post = new((d,), torch.float32) if need[2] and post_w is not None else None
+    d_gate = None
+    if need[3] and gate is not None:
+        d_gate = new(gate.shape, gate.dtype if spec.gate_form == _lib.GATE_FULL else torch.float32)
+    d_pre = new((d,), torch.float32) if need[4] and pre_w is not None else None
+    with _on(dev):
+        sums = d_post is not None or d_pre is not None or (d_gate is not None and spec.gate_form == _lib.GATE_CHANNEL)
+        nbytes = lib().hsmoe_block_norm_grad_workspace_size(m, d) if sums else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
+        check(lib().hsmoe_block_norm_grad(ptr(d_h), ptr(d_n), ptr(f), ptr(h_out), m, d, ctypes.addressof(spec), scale, eps,
+                                          ptr(d_f), ptr(d_x), ptr(d_post), ptr(d_gate), ptr(d_pre), ptr(ws), nbytes,
+                                          stream_ptr(dev)), "hsmoe_block_norm_grad")
+    return BlockNormGrad(d_f, d_x, d_post, d_gate, d_pre)
 
 
 def _bf16_row(t: torch.Tensor, d: int, what: str) -> torch.Tensor:

@@ -491,6 +491,43 @@ int hsmoe_rms_norm(const void* x_dev, const void* w_dev, int64_t rows, int64_t d
 int hsmoe_add_rms_norm(const void* x_dev, const void* add_dev, const void* res_dev, const void* w_dev, int64_t rows,
                        int64_t d, float eps, void* h_out_dev, void* out_dev, hsmoe_stream_t stream);
 
+/* What stands between two blocks f of a residual network with the stream h: the
+ * norm after the block, its gate and residual scale, the add to the stream, and the
+ * norm before the next block, in one launch (the reference's _forward_layer has the
+ * plain form of it, engine.py:2653-2690, without gradients):
+ *   u = post_w f / rms(f)      (post_w NULL: u = f)      rms(v) = sqrt(mean(v^2) + eps)
+ *   h_out = h + scale gate u   (gate NULL: 1), rounded to the stream's type
+ *   n_out = pre_w h_out / rms(h_out)   (pre_w NULL: n_out NULL), of the rounded h_out
+ * f, n_out [m, d] of row_kind, h, h_out [m, d] of stream_kind, post_w, pre_w [d] of
+ * weight_kind, each HSMOE_OUT_F32 or HSMOE_OUT_BF16; gate of gate_kind: [d], [m] or
+ * [m, d] by gate_form.  Sums in fp32.  h_out may be h, n_out may be f.  d a multiple
+ * of 8 up to 16384, rows contiguous and 16-byte aligned, eps >= 0; m may be 0. */
+#define HSMOE_GATE_NONE 0
+#define HSMOE_GATE_CHANNEL 1
+#define HSMOE_GATE_TOKEN 2
+#define HSMOE_GATE_FULL 3
+typedef struct {
+  const void* post_w_dev;
+  const void* pre_w_dev;
+  const void* gate_dev;
+  int row_kind, stream_kind, weight_kind, gate_kind, gate_form;
+} hsmoe_block_norm_spec;
+int hsmoe_block_norm(const void* f_dev, const void* h_dev, int64_t m, int64_t d, const hsmoe_block_norm_spec* spec,
+                     float scale, float eps, void* h_out_dev, void* n_out_dev, hsmoe_stream_t stream);
+
+/* The gradient of hsmoe_block_norm for d_h of h_out (stream_kind) and d_n of n_out
+ * (row_kind), either NULL for zeros, from f and h_out:
+ *   d_f [m, d] of row_kind, d_x [m, d] of stream_kind (h's), d_post, d_pre fp32 [d],
+ *   d_gate: HSMOE_GATE_FULL [m, d] of gate_kind, HSMOE_GATE_TOKEN fp32 [m],
+ *   HSMOE_GATE_CHANNEL fp32 [d]; NULL for what is not wanted.
+ * d_x may be d_h, d_f may be f or d_n (of its kind).  Deterministic (no atomics); the workspace, of any
+ * contents, is needed for d_post, d_pre and a channel's d_gate. */
+size_t hsmoe_block_norm_grad_workspace_size(int64_t m, int64_t d);
+int hsmoe_block_norm_grad(const void* d_h_dev, const void* d_n_dev, const void* f_dev, const void* h_out_dev, int64_t m,
+                          int64_t d, const hsmoe_block_norm_spec* spec, float scale, float eps, void* d_f_dev,
+                          void* d_x_dev, float* d_post_dev, void* d_gate_dev, float* d_pre_dev, void* workspace_dev,
+                          size_t workspace_bytes, hsmoe_stream_t stream);
+
 /* The first layer's input of a forward: the token embedding lookup
  * (engine.py:2475 and 2814, self.embed[ids].to(bfloat16)) followed by hsmoe_add_rms_norm with
  * no add: row r of x is row ids[r] of table [vocab, d] (an id outside
