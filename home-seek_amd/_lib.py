@@ -23,6 +23,8 @@ ACT_NONE = 0
 ACT_SILU = 1
 ACT_SWIGLU = 2
 ROWS_FP4 = 2
+IDS_I32 = 0
+IDS_I64 = 1
 GATE_NONE = 0
 GATE_CHANNEL = 1
 GATE_TOKEN = 2
@@ -129,6 +131,10 @@ _SIGNATURES = {
                                      _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_embed_add_rms_norm": (_int, [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _f32,
                                         _c_void_p, _c_void_p, _c_void_p]),
+    "hsmoe_embed": (_int, [_c_void_p, _int, _i64, _c_void_p, _i64, _int, _i64, _i64, _f32, _int, _c_void_p, _c_void_p]),
+    "hsmoe_embed_grad_workspace_size": (_size, [_i64, _i64]),
+    "hsmoe_embed_grad": (_int, [_c_void_p, _i64, _int, _c_void_p, _int, _i64, _i64, _i64, _f32, _int, _c_void_p, _i64, _int,
+                                _c_void_p, _size, _c_void_p]),
     "hsmoe_mtp_input": (_int, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                _i64, _f32, _c_void_p, _c_void_p, _c_void_p]),
     "hsmoe_decode_step_record": (_int, [_c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,

@@ -1,0 +1,473 @@
+// Embedding lookup with a scale, and its gradient.
+//   out[t] = scale * table[ids[t]]               (a row of zeros for an id outside the table)
+//   d_table[v] = scale * sum of d_out[t] over the tokens t with ids[t] = v
+// The gradient sorts the tokens by id, stably, so that every row's terms are added
+// in the order of the tokens, and cuts the sorted tokens into chunks of 32, so that
+// a word that makes up much of a batch is summed by many workgroups: a run of equal
+// ids inside a chunk is a row of the table; the ends of chunks that share a run leave
+// fp32 sums, which a second launch adds in their order.  All of it is bound by HBM:
+// the table's rows that are written, most of them zeros.
+#include <algorithm>
+
+#include "hsmoe_common.h"
+#include "hsmoe_internal.h"
+
+namespace hsmoe {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kChunk = 32;           // sorted tokens per chunk
+constexpr int kSortThreads = 1024;
+constexpr int kSortTokens = 64;      // tokens that a sorting workgroup places
+constexpr int64_t kSortByRank = 16384;  // tokens up to which every token's place is counted out
+
+// The id of token t, -1 outside the table.
+__device__ __forceinline__ int id_of(const void* ids, bool wide, int64_t t, int64_t vocab) {
+  const int64_t v = wide ? ((const int64_t*)ids)[t] : (int64_t)((const int32_t*)ids)[t];
+  return v >= 0 && v < vocab ? (int)v : -1;
+}
+
+template <bool kF32>
+__device__ __forceinline__ float value(const void* p, int64_t at) {
+  return kF32 ? ((const float*)p)[at] : bf16_bits_to_f32(((const uint16_t*)p)[at]);
+}
+template <bool kF32>
+__device__ __forceinline__ void put(void* p, int64_t at, float v) {
+  if (kF32) ((float*)p)[at] = v;
+  else ((uint16_t*)p)[at] = (uint16_t)f32_to_bf16_bits(v);
+}
+
+// kVec values of a row at a time: 8 where rows are 16-byte aligned, else one.
+template <int kVec>
+struct Vals {
+  float v[kVec];
+};
+template <int kVec, bool kF32>
+__device__ __forceinline__ Vals<kVec> read(const void* base, int64_t at) {
+  Vals<kVec> r;
+  if constexpr (kVec == 1) {
+    r.v[0] = value<kF32>(base, at);
+  } else if constexpr (kF32) {
+    const char* p = (const char*)base + at * 4;
+    const uint4 a = ldg<uint4>(p), b = ldg<uint4>(p + 16);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(w[i]);
+  } else {
+    const uint4 a = ldg<uint4>((const char*)base + at * 2);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[2 * i] = __uint_as_float(w[i] << 16), r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  return r;
+}
+template <int kVec, bool kF32>
+__device__ __forceinline__ void write(void* base, int64_t at, const Vals<kVec>& r) {
+  if constexpr (kVec == 1) {
+    put<kF32>(base, at, r.v[0]);
+  } else if constexpr (kF32) {
+    float4* p = reinterpret_cast<float4*>((float*)base + at);
+    p[0] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
+    p[1] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16_bits(r.v[2 * i]) | f32_to_bf16_bits(r.v[2 * i + 1]) << 16;
+    *reinterpret_cast<uint4*>((uint16_t*)base + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ---------------------------------------------------------------- lookup
+struct EmbedParams {
+  const void* ids;
+  const void* table;
+  void* out;
+  int64_t m, vocab, d, ld;  // ld: values between the table's rows
+  bool wide;
+  int shift;                // 2^shift threads per row
+  float scale;
+};
+template <int kVec, bool kF32, bool kOutF32>
+__global__ void __launch_bounds__(kThreads) embed_kernel(EmbedParams p) {
+  const int lanes = 1 << p.shift;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
+  if (row >= p.m) return;
+  const int id = id_of(p.ids, p.wide, row, p.vocab);
+  const int64_t from = (int64_t)(id < 0 ? 0 : id) * p.ld, to = row * p.d;
+  constexpr int kAhead = 2;
+  for (int64_t c = (int64_t)(threadIdx.x & (lanes - 1)) * kVec; c < p.d; c += (int64_t)kAhead * lanes * kVec) {
+    Vals<kVec> v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t at = c + (int64_t)i * lanes * kVec;
+      v[i] = id >= 0 && at < p.d ? read<kVec, kF32>(p.table, from + at) : Vals<kVec>{};
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t at = c + (int64_t)i * lanes * kVec;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[i].v[j] = id >= 0 ? v[i].v[j] * p.scale : 0.0f;
+      if (at < p.d) write<kVec, kOutF32>(p.out, to + at, v[i]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradient
+// The tokens by (id, t): sorted_id[r] and token[r], ids outside the table left out
+// and the rest of sorted_id -1.  A token's place is the number of tokens with a
+// smaller id, or the same and before it: m^2 comparisons, for 16384 tokens 2^28 of
+// them, which the chip does in the time of one of the launches that a radix sort
+// needs.  A workgroup places 64 tokens, its 16 waves each counting a sixteenth of
+// all.  The first `sorters` workgroups do that; the others meanwhile clear the table's
+// gradient, which is written once more than needed where a token falls, but waits
+// for no order.
+struct SortParams {
+  const void* ids;
+  int64_t m, vocab;
+  bool wide;
+  int sorters;
+  int *sorted_id, *token;
+  char* clear;
+  int64_t clear_bytes;
+};
+__device__ __forceinline__ void clear_part(char* p, int64_t bytes, int64_t part, int64_t parts) {
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+  const int64_t head = bytes < (-(intptr_t)p & 15) ? bytes : (-(intptr_t)p & 15), words = (bytes - head) / 16;
+  if (part == 0) {
+    for (int64_t i = threadIdx.x; i < head; i += kSortThreads) p[i] = 0;
+    for (int64_t i = head + words * 16 + threadIdx.x; i < bytes; i += kSortThreads) p[i] = 0;
+  }
+  u32x4* w = reinterpret_cast<u32x4*>(p + head);
+  for (int64_t i = part * kSortThreads + threadIdx.x; i < words; i += parts * kSortThreads) __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, w + i);
+}
+__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p) {
+  if ((int)blockIdx.x >= p.sorters) {
+    clear_part(p.clear, p.clear_bytes, (int)blockIdx.x - p.sorters, (int)gridDim.x - p.sorters);
+    return;
+  }
+  __shared__ int ids[kSortByRank];
+  __shared__ int counts[kSortThreads / 64][kSortTokens], valid[kSortThreads / 64];
+  const int m = (int)p.m, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int live = 0;
+  for (int i = threadIdx.x; i < m; i += kSortThreads) {
+    const int v = id_of(p.ids, p.wide, i, p.vocab);
+    ids[i] = v < 0 ? 0x7fffffff : v;
+    live += v >= 0;
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) live += __shfl_xor(live, off, 64);
+  if (lane == 0) valid[wave] = live;
+  __syncthreads();
+  const int t0 = blockIdx.x * kSortTokens, t = t0 + lane;
+  const int mine = t < m ? ids[t] : 0x7fffffff;
+  // this wave's share of all tokens; those before the 64 count if not above, those behind if below
+  const int per = ((m + kSortThreads / 64 - 1) / (kSortThreads / 64) + 3) & ~3;
+  const int a = wave * per, b = a + per < m ? a + per : m;
+  int n = 0;
+  auto count = [&](int from, int to, int limit) {  // ids below limit
+#pragma unroll 16
+    for (int i = from; i < to; ++i) n += ids[i] < limit;
+  };
+  const int c = a > t0 ? a : t0, e = t0 + kSortTokens < b ? t0 + kSortTokens : b;
+  count(a, b < t0 ? b : t0, mine == 0x7fffffff ? mine : mine + 1);
+  for (int i = c; i < e; ++i) n += ids[i] < mine || (ids[i] == mine && i < t);
+  count(a > t0 + kSortTokens ? a : t0 + kSortTokens, b, mine);
+  counts[wave][lane] = n;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kSortThreads / 64; ++w) total += valid[w];
+  if (wave) return;
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < kSortThreads / 64; ++w) n += counts[w][lane];
+  if (t < m && mine != 0x7fffffff) p.sorted_id[n] = mine, p.token[n] = t;
+  if (t < m && t >= total) p.sorted_id[t] = -1;
+}
+__global__ void __launch_bounds__(kSortThreads) embed_clear_kernel(char* p, int64_t bytes) {
+  clear_part(p, bytes, blockIdx.x, gridDim.x);
+}
+
+// More tokens: digits of ten bits, lowest first, each sorted by hsmoe_moe_sort.
+// digit_kernel: the digit of what the pass before has put in row r (token r in the
+// first pass), -1 where there is none.
+__global__ void __launch_bounds__(kThreads) embed_digit_kernel(const void* ids, bool wide, int64_t m, int64_t vocab, const int* order,
+                                                               int shift, int64_t* digit) {
+  const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (r >= m) return;
+  const int64_t t = order ? order[r] : r;
+  const int id = t < 0 ? -1 : id_of(ids, wide, t, vocab);
+  digit[r] = id < 0 ? -1 : (id >> shift) & 1023;
+}
+// order <- what this pass puts in row r
+__global__ void __launch_bounds__(kThreads) embed_order_kernel(const int* pairs, const int* before, int64_t m, int* order) {
+  const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (r >= m) return;
+  const int q = pairs[r];
+  order[r] = q < 0 ? -1 : before ? before[q] : q;
+}
+__global__ void __launch_bounds__(kThreads) embed_sorted_kernel(const void* ids, bool wide, int64_t m, int64_t vocab, const int* order,
+                                                                int* sorted_id) {
+  const int64_t r = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (r < m) sorted_id[r] = order[r] < 0 ? -1 : id_of(ids, wide, order[r], vocab);
+}
+
+struct SumParams {
+  const void* d_out;
+  const int *sorted_id, *token;
+  void* d_table;
+  float* part;          // fp32 [chunks][2][d]: a chunk's first run, if the chunk before has its beginning, and its last, if it goes on
+  int64_t m, d, ld, ld_out;  // ld: values between the table's rows, ld_out: between d_out's
+  int64_t chunks;
+  int shift, slabs;     // 2^shift threads per chunk, `slabs` times that many vectors cover a row
+  bool add;
+  float scale;
+};
+template <int kVec, bool kOutF32>
+__device__ __forceinline__ void finish(const SumParams& p, int id, int64_t col, const Vals<kVec>& s) {
+  const int64_t at = (int64_t)id * p.ld + col;
+  Vals<kVec> v;
+  if (p.add) {
+    const Vals<kVec> old = read<kVec, kOutF32>(p.d_table, at);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v.v[i] = __fmaf_rn(p.scale, s.v[i], old.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v.v[i] = p.scale * s.v[i];
+  }
+  write<kVec, kOutF32>(p.d_table, at, v);
+}
+template <int kVec>
+__device__ __forceinline__ void leave(float* to, const Vals<kVec>& s) {
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) to[i] = s.v[i];
+}
+
+// Sums of the runs of a chunk, for kVec columns per thread.
+template <int kVec, bool kF32, bool kOutF32>
+__global__ void __launch_bounds__(kThreads) embed_sum_kernel(SumParams p) {
+  const int lanes = 1 << p.shift;
+  const int64_t chunk = (int64_t)(blockIdx.x / p.slabs) * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
+  const int64_t col = ((int64_t)(blockIdx.x % p.slabs) * lanes + (threadIdx.x & (lanes - 1))) * kVec;
+  if (chunk >= p.chunks || col >= p.d) return;
+  const int64_t r0 = chunk * kChunk, r1 = r0 + kChunk < p.m ? r0 + kChunk : p.m;
+  int id = p.sorted_id[r0];
+  if (id < 0) return;
+  bool open = chunk > 0 && p.sorted_id[r0 - 1] == id;  // the run began before the chunk
+  const int after = r1 < p.m ? p.sorted_id[r1] : -1;
+  float* part = p.part + chunk * 2 * p.d + col;
+  Vals<kVec> s = {};
+  constexpr int kAhead = 8;
+  for (int64_t r = r0; r < r1; r += kAhead) {
+    int ids[kAhead];
+    Vals<kVec> v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      ids[i] = r + i < r1 ? p.sorted_id[r + i] : -1;
+      v[i] = ids[i] >= 0 ? read<kVec, kF32>(p.d_out, (int64_t)p.token[r + i] * p.ld_out + col) : Vals<kVec>{};
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (ids[i] < 0) continue;
+      if (ids[i] != id) {  // the run before is done
+        if (open) leave<kVec>(part, s);
+        else finish<kVec, kOutF32>(p, id, col, s);
+        open = false, id = ids[i], s = Vals<kVec>{};
+      }
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) s.v[j] += v[i].v[j];
+    }
+  }
+  // the last run: goes on in the next chunk, or ends here
+  if (after == id) leave<kVec>(part + (open ? 0 : p.d), s);
+  else if (open) leave<kVec>(part, s);
+  else finish<kVec, kOutF32>(p, id, col, s);
+}
+
+// Runs over several chunks: the chunk where one begins adds what the next ones left.
+template <int kVec, bool kOutF32>
+__global__ void __launch_bounds__(kThreads) embed_join_kernel(SumParams p) {
+  const int lanes = 1 << p.shift;
+  const int64_t chunk = (int64_t)(blockIdx.x / p.slabs) * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
+  const int64_t col = ((int64_t)(blockIdx.x % p.slabs) * lanes + (threadIdx.x & (lanes - 1))) * kVec;
+  const int64_t r0 = chunk * kChunk, r1 = r0 + kChunk;
+  if (chunk >= p.chunks || col >= p.d || r1 >= p.m) return;
+  const int id = p.sorted_id[r1];
+  if (id < 0 || p.sorted_id[r1 - 1] != id) return;                            // nothing goes on
+  if (p.sorted_id[r0] == id && chunk > 0 && p.sorted_id[r0 - 1] == id) return;  // it began earlier
+  const float* part = p.part + chunk * 2 * p.d + col;
+  Vals<kVec> s = {};
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) s.v[j] = part[p.d + j];
+  constexpr int kAhead = 16;
+  for (int64_t c = chunk + 1; c < p.chunks; c += kAhead) {
+    bool on[kAhead];  // equal ids lie together: true up to the run's end
+    Vals<kVec> v[kAhead] = {};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      on[i] = c + i < p.chunks && p.sorted_id[(c + i) * kChunk] == id;
+      if (on[i]) v[i] = read<kVec, true>(p.part, (c + i) * 2 * p.d + col);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) s.v[j] += on[i] ? v[i].v[j] : 0.0f;
+    if (!on[kAhead - 1]) break;
+  }
+  finish<kVec, kOutF32>(p, id, col, s);
+}
+
+// ---------------------------------------------------------------- host
+int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+// Threads per row: a power of two of them that covers d in vectors, up to a workgroup.
+int shift_for(int64_t vectors) {
+  int s = 0;
+  while (s < 8 && (1ll << s) < vectors) ++s;
+  return s;
+}
+
+struct GradSpace {
+  int64_t ids, token, order, digit, offsets, pairs, rows, sort, sort_bytes, part, bytes;
+};
+GradSpace space_of(int64_t m, int64_t d) {
+  GradSpace s{};
+  const int64_t n = up(m * 4, 256);
+  s.ids = 0, s.token = n, s.bytes = 2 * n;
+  if (m > kSortByRank) {
+    s.order = s.bytes, s.digit = s.order + n, s.offsets = s.digit + 2 * n, s.pairs = s.offsets + up(1025 * 4, 256);
+    s.rows = s.pairs + n, s.sort = s.rows + n;
+    s.sort_bytes = (int64_t)hsmoe_moe_sort_workspace_size(m, 1, 1024);
+    s.bytes = s.sort + up(s.sort_bytes, 256);
+  }
+  s.part = s.bytes;
+  s.bytes += (m + kChunk - 1) / kChunk * 2 * d * 4;
+  return s;
+}
+
+bool kind_ok(int k) { return k == HSMOE_OUT_F32 || k == HSMOE_OUT_BF16; }
+int check_embed(const char* who, const void* ids, int id_kind, int64_t m, int64_t vocab, int64_t d, int64_t ld, int a, int b) {
+  if (m < 0 || vocab < 1 || d < 1 || ld < d || !kind_ok(a) || !kind_ok(b) || (id_kind != HSMOE_IDS_I32 && id_kind != HSMOE_IDS_I64))
+    return fail(HSMOE_ERR_ARG, "%s: bad arguments", who);
+  if (m >= (1ll << 31) || vocab >= (1ll << 30) || d >= (1 << 23) || ld >= (1ll << 31))
+    return fail(HSMOE_ERR_SHAPE, "%s: sizes beyond 2^31 tokens, 2^30 rows or 2^23 columns", who);
+  if (m > 0 && !ids) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
+  if (!aligned(ids, id_kind == HSMOE_IDS_I64 ? 8 : 4)) return fail(HSMOE_ERR_SHAPE, "%s: misaligned ids", who);
+  return HSMOE_OK;
+}
+int size_of(int kind) { return kind == HSMOE_OUT_F32 ? 4 : 2; }
+bool rows16(const void* p, int64_t ld, int kind) { return aligned(p, 16) && ld * size_of(kind) % 16 == 0; }
+
+template <bool kSum, int kVec, bool kF32, bool kOutF32>
+void launch_grad(const SumParams& p, hipStream_t st) {
+  const int64_t per = kThreads >> p.shift;
+  const dim3 grid((unsigned)((p.chunks + per - 1) / per * p.slabs));
+  if constexpr (kSum)
+    hipLaunchKernelGGL((embed_sum_kernel<kVec, kF32, kOutF32>), grid, dim3(kThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL((embed_join_kernel<kVec, kOutF32>), grid, dim3(kThreads), 0, st, p);
+}
+template <bool kSum, int kVec>
+void launch_grad(const SumParams& p, bool f32, bool out_f32, hipStream_t st) {
+  if (f32 && out_f32) launch_grad<kSum, kVec, true, true>(p, st);
+  else if (f32) launch_grad<kSum, kVec, true, false>(p, st);
+  else if (out_f32) launch_grad<kSum, kVec, false, true>(p, st);
+  else launch_grad<kSum, kVec, false, false>(p, st);
+}
+
+}  // namespace
+}  // namespace hsmoe
+
+using namespace hsmoe;
+
+extern "C" int hsmoe_embed(const void* ids, int id_kind, int64_t m, const void* table, int64_t table_row_stride,
+                           int table_kind, int64_t vocab, int64_t d, float scale, int out_kind, void* out,
+                           hsmoe_stream_t stream) {
+  const char* who = "hsmoe_embed";
+  if (int rc = check_embed(who, ids, id_kind, m, vocab, d, table_row_stride, table_kind, out_kind)) return rc;
+  if (m == 0) return HSMOE_OK;
+  if (!table || !out) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
+  if (!aligned(table, size_of(table_kind)) || !aligned(out, size_of(out_kind))) return fail(HSMOE_ERR_SHAPE, "%s: misaligned rows", who);
+  EmbedParams p{ids, table, out, m, vocab, d, table_row_stride, id_kind == HSMOE_IDS_I64, 0, scale};
+  const bool vec = d % 8 == 0 && rows16(table, table_row_stride, table_kind) && rows16(out, d, out_kind);
+  p.shift = shift_for(vec ? (d / 8 + 1) / 2 : (d + 1) / 2);
+  const int64_t per = kThreads >> p.shift;
+  const dim3 grid((unsigned)((m + per - 1) / per)), block(kThreads);
+  hipStream_t st = (hipStream_t)stream;
+  const bool f = table_kind == HSMOE_OUT_F32, o = out_kind == HSMOE_OUT_F32;
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p); };
+  if (vec) f ? (o ? go(embed_kernel<8, true, true>) : go(embed_kernel<8, true, false>))
+             : (o ? go(embed_kernel<8, false, true>) : go(embed_kernel<8, false, false>));
+  else f ? (o ? go(embed_kernel<1, true, true>) : go(embed_kernel<1, true, false>))
+         : (o ? go(embed_kernel<1, false, true>) : go(embed_kernel<1, false, false>));
+  return check_launch(who);
+}
+
+extern "C" size_t hsmoe_embed_grad_workspace_size(int64_t m, int64_t d) {
+  return m < 1 || d < 1 ? 0 : (size_t)space_of(m, d).bytes;
+}
+
+extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_kind, const void* ids, int id_kind,
+                                int64_t m, int64_t vocab, int64_t d, float scale, int add, void* d_table,
+                                int64_t table_row_stride, int table_kind, void* workspace, size_t workspace_bytes,
+                                hsmoe_stream_t stream) {
+  const char* who = "hsmoe_embed_grad";
+  if (int rc = check_embed(who, ids, id_kind, m, vocab, d, table_row_stride, table_kind, d_kind)) return rc;
+  if (m >= (1 << 24)) return fail(HSMOE_ERR_SHAPE, "%s: 2^24 tokens and more", who);
+  if (!d_table || (m > 0 && (!d_out || d_row_stride < d)) || (add != 0 && add != 1) || (!add && table_row_stride != d))
+    return fail(HSMOE_ERR_ARG, "%s: bad arguments", who);
+  if (!aligned(d_table, size_of(table_kind)) || !aligned(d_out, size_of(d_kind))) return fail(HSMOE_ERR_SHAPE, "%s: misaligned rows", who);
+  const GradSpace sp = m > 0 ? space_of(m, d) : GradSpace{};
+  if (m > 0 && (!workspace || workspace_bytes < (size_t)sp.bytes))
+    return fail(HSMOE_ERR_WORKSPACE, "%s: workspace of %lld bytes needed", who, (long long)sp.bytes);
+  if (!aligned(workspace, 16)) return fail(HSMOE_ERR_SHAPE, "%s: misaligned workspace", who);
+  hipStream_t st = (hipStream_t)stream;
+  char* mem = (char*)workspace;
+  const bool wide = id_kind == HSMOE_IDS_I64;
+  int *sorted_id = (int*)(mem + sp.ids), *token = (int*)(mem + sp.token);
+  const int64_t bytes = add ? 0 : vocab * d * size_of(table_kind);
+  const int64_t fill = bytes ? std::min<int64_t>(2 * device_cus(), (bytes + 65535) / 65536) : 0;
+  if (m == 0) {
+    if (!fill) return HSMOE_OK;
+    hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)fill), dim3(kSortThreads), 0, st, (char*)d_table, bytes);
+    return check_launch(who);
+  }
+  if (m <= kSortByRank) {
+    SortParams s{ids, m, vocab, wide, (int)((m + kSortTokens - 1) / kSortTokens), sorted_id, token, (char*)d_table, bytes};
+    hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(s.sorters + fill)), dim3(kSortThreads), 0, st, s);
+  } else {
+    if (fill) hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)fill), dim3(kSortThreads), 0, st, (char*)d_table, bytes);
+    const dim3 grid((unsigned)((m + kThreads - 1) / kThreads)), block(kThreads);
+    int *order = (int*)(mem + sp.order), *pairs = (int*)(mem + sp.pairs);
+    int64_t* digit = (int64_t*)(mem + sp.digit);
+    const int* before = nullptr;
+    int* after = token;  // passes write token and order in turn
+    for (int shift = 0; shift == 0 || (vocab - 1) >> shift; shift += 10) {
+      hipLaunchKernelGGL(embed_digit_kernel, grid, block, 0, st, ids, wide, m, vocab, before, shift, digit);
+      if (int rc = hsmoe_moe_sort(digit, m, 1, 1024, (int32_t*)(mem + sp.offsets), pairs, (int32_t*)(mem + sp.rows), mem + sp.sort,
+                                  (size_t)sp.sort_bytes, stream))
+        return rc;
+      hipLaunchKernelGGL(embed_order_kernel, grid, block, 0, st, pairs, before, m, after);
+      before = after;
+      after = after == token ? order : token;
+    }
+    hipLaunchKernelGGL(embed_sorted_kernel, grid, block, 0, st, ids, wide, m, vocab, before, sorted_id);
+    token = const_cast<int*>(before);
+  }
+  SumParams p{};
+  p.d_out = d_out, p.sorted_id = sorted_id, p.token = token, p.d_table = d_table, p.part = (float*)(mem + sp.part);
+  p.m = m, p.d = d, p.ld = table_row_stride, p.ld_out = d_row_stride, p.chunks = (m + kChunk - 1) / kChunk;
+  p.add = add, p.scale = scale;
+  const bool vec = d % 8 == 0 && rows16(d_out, d_row_stride, d_kind) && rows16(d_table, table_row_stride, table_kind);
+  const int64_t vectors = vec ? d / 8 : d;
+  p.shift = shift_for(vectors);
+  p.slabs = (int)((vectors + (1ll << p.shift) - 1) >> p.shift);
+  const bool f = d_kind == HSMOE_OUT_F32, o = table_kind == HSMOE_OUT_F32;
+  if (vec) launch_grad<true, 8>(p, f, o, st);
+  else launch_grad<true, 1>(p, f, o, st);
+  if (p.chunks > 1) {
+    if (vec) launch_grad<false, 8>(p, f, o, st);
+    else launch_grad<false, 1>(p, f, o, st);
+  }
+  return check_launch(who);
+}

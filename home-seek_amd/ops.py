@@ -25,6 +25,7 @@ __all__ = [
     "decode_step_record", "ExpertOrder", "moe_sort", "moe_gather", "moe_combine", "moe_combine_grad",
     "linear", "linear_grad", "LinearGrad", "fp4_quant", "fp4_linear",
     "block_norm", "block_norm_grad", "BlockNormGrad",
+    "embed", "embed_grad",
 ]
 
 MAX_DECODE_TOKENS = 8
@@ -1078,6 +1079,72 @@ def embed_add_rms_norm(ids: torch.Tensor, table: torch.Tensor, weight: torch.Ten
                                          ptr(out), stream_ptr(dev)), "hsmoe_embed_add_rms_norm")
     shape = tuple(ids.shape) + (d,)
     return h.reshape(shape), out.reshape(shape)
+
+
+def _token_ids(ids: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """ids, contiguous int32 or int64, and their kind."""
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+        raise TypeError(f"ids must be integers, got {ids.dtype}")
+    if ids.dtype != torch.int32:
+        ids = ids.to(torch.int64)
+    return ids.contiguous(), _lib.IDS_I32 if ids.dtype == torch.int32 else _lib.IDS_I64
+
+
+def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """scale * table[ids] (hsmoe_embed): ids of any shape and integer type, table [V, D]
+    bf16 or fp32 -> [*ids.shape, D] of out_dtype (the table's when None); an id outside
+    [0, V) gives a row of zeros, as in embed_add_rms_norm."""
+    dev = require_cuda(ids, table)
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"the embedding table must be [V, D], got {tuple(table.shape)}")
+    kind = _row_kind(table.dtype, "the embedding table")
+    out_kind = kind if out_dtype is None else _row_kind(out_dtype, "the output")
+    vocab, d = table.shape
+    if (d > 1 and table.stride(1) != 1) or (vocab > 1 and table.stride(0) < d):
+        table = table.contiguous()
+    lead = ids.shape
+    ids, id_kind = _token_ids(ids)
+    out = torch.empty(lead + (d,), dtype=table.dtype if out_dtype is None else out_dtype, device=dev)
+    with _on(dev):
+        check(lib().hsmoe_embed(ptr(ids), id_kind, ids.numel(), ptr(table), max(table.stride(0), d), kind, vocab, d, scale,
+                                out_kind, ptr(out), stream_ptr(dev)), "hsmoe_embed")
+    return out
+
+
+def embed_grad(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float = 1.0,
+               out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of embed's table for d_out [*ids.shape, D] (bf16 or fp32): [vocab, D]
+    of out_dtype (d_out's when None), with zeros in rows that no id names
+    (hsmoe_embed_grad).  With out [vocab, D] (bf16 or fp32; rows may be apart) it is
+    added to that instead, in the rows that ids name, and out is returned."""
+    dev = require_cuda(d_out, ids, out)
+    kind = _row_kind(d_out.dtype, "d_out")
+    if d_out.shape[:-1] != ids.shape or d_out.dim() != ids.dim() + 1 or d_out.shape[-1] < 1:
+        raise ValueError(f"d_out {tuple(d_out.shape)} does not match ids {tuple(ids.shape)}")
+    d = d_out.shape[-1]
+    vocab = int(vocab)
+    if vocab < 1:
+        raise ValueError("the table must have rows")
+    if out is not None:
+        if out_dtype is not None and out_dtype != out.dtype:
+            raise TypeError("out_dtype is out's where out is given")
+        if tuple(out.shape) != (vocab, d) or (d > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < d):
+            raise ValueError(f"out must be [{vocab}, {d}] with rows of consecutive values, got {tuple(out.shape)}, "
+                             f"strides {out.stride()}")
+    table = torch.empty(vocab, d, dtype=out_dtype or d_out.dtype, device=dev) if out is None else out
+    out_kind = _row_kind(table.dtype, "the table's gradient")
+    d_out = d_out.reshape(-1, d)
+    if (d > 1 and d_out.stride(1) != 1) or (d_out.shape[0] > 1 and d_out.stride(0) < d):
+        d_out = d_out.contiguous()
+    ids, id_kind = _token_ids(ids)
+    m = ids.numel()
+    with _on(dev):
+        nbytes = lib().hsmoe_embed_grad_workspace_size(m, d)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
+        check(lib().hsmoe_embed_grad(ptr(d_out), max(d_out.stride(0), d), kind, ptr(ids), id_kind, m, vocab, d, scale,
+                                     0 if out is None else 1, ptr(table), max(table.stride(0), d), out_kind, ptr(ws), nbytes,
+                                     stream_ptr(dev)), "hsmoe_embed_grad")
+    return table
 
 
 def mtp_input(tok: torch.Tensor, embed: torch.Tensor, h_prev: torch.Tensor, enorm: torch.Tensor,

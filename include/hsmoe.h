@@ -538,6 +538,28 @@ int hsmoe_embed_add_rms_norm(const int64_t* ids_dev, int64_t rows, const void* t
                              const void* res_dev, const void* w_dev, int64_t d, float eps, void* h_out_dev,
                              void* out_dev, hsmoe_stream_t stream);
 
+/* The embedding lookup alone, and its gradient (the reference's lookup is
+ * self.embed[ids], engine.py:2475 and 2814; it has no gradient).
+ *   hsmoe_embed:      out[t] = scale * table[ids[t]]  (zeros for an id outside [0, vocab))
+ *   hsmoe_embed_grad: d_table[v] = scale * sum of d_out[t] over the t with ids[t] = v
+ * ids int32 or int64 (id_kind); table and d_table [vocab, d], rows table_row_stride
+ * values apart, of table_kind; out [m, d] contiguous, of out_kind; d_out [m, d] of
+ * d_kind; kinds HSMOE_OUT_F32 or HSMOE_OUT_BF16.  Sums in fp32, in the order of the
+ * tokens within chunks of 32 of them and of the chunks, rounded once: deterministic.
+ * add 0: every row of d_table (table_row_stride = d) is written, those that no token
+ * names with zeros; add 1: the sums are added to the rows that tokens name, the others are left.
+ * m < 2^31 (2^24 for the gradient, 0 included), vocab < 2^30, d < 2^23; any d (rows
+ * that are 16-byte aligned move in 16-byte vectors).  The workspace (any contents)
+ * holds hsmoe_embed_grad_workspace_size bytes. */
+#define HSMOE_IDS_I32 0
+#define HSMOE_IDS_I64 1
+int hsmoe_embed(const void* ids_dev, int id_kind, int64_t m, const void* table_dev, int64_t table_row_stride,
+                int table_kind, int64_t vocab, int64_t d, float scale, int out_kind, void* out_dev, hsmoe_stream_t stream);
+size_t hsmoe_embed_grad_workspace_size(int64_t m, int64_t d);
+int hsmoe_embed_grad(const void* d_out_dev, int64_t d_row_stride, int d_kind, const void* ids_dev, int id_kind, int64_t m,
+                     int64_t vocab, int64_t d, float scale, int add, void* d_table_dev, int64_t table_row_stride,
+                     int table_kind, void* workspace_dev, size_t workspace_bytes, hsmoe_stream_t stream);
+
 /* The MTP block's input for one draft token (the data flow of the reference's
  * draft step, engine.py:2251-2339, without its attention and projections):
  *   e = RMSNorm(embed[tok[0]]) * enorm_w;  g = RMSNorm(h_prev) * hnorm_w;
