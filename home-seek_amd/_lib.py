@@ -115,6 +115,10 @@ _SIGNATURES = {
                                        _c_void_p, _i64, _c_void_p, _c_void_p, _size, _c_void_p]),
     "hsmoe_linear_grad_weight": (_int, [_c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p, _i64, _int,
                                         _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "hsmoe_grad_norm_workspace_size": (_size, [_i64]),
+    "hsmoe_grad_norm": (_int, [_i64, _c_void_p, _c_void_p, _c_void_p, ctypes.c_double, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "hsmoe_clip_grads": (_int, [_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, ctypes.c_double, _f32, _c_void_p,
+                                _c_void_p, _size, _c_void_p]),
     "hsmoe_fp4_quant": (_int, [_c_void_p, _i64, _int, _i64, _i64, _c_void_p, _c_void_p, _c_void_p]),
     "hsmoe_fp4_linear_workspace_size": (_size, [_i64, _i64, _i64, _int]),
     "hsmoe_fp4_linear": (_int, [_c_void_p, _int, _i64, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int,

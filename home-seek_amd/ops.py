@@ -25,7 +25,7 @@ __all__ = [
     "decode_step_record", "ExpertOrder", "moe_sort", "moe_gather", "moe_combine", "moe_combine_grad",
     "linear", "linear_grad", "LinearGrad", "fp4_quant", "fp4_linear",
     "block_norm", "block_norm_grad", "BlockNormGrad",
-    "embed", "embed_grad",
+    "embed", "embed_grad", "grad_norm", "clip_grads",
 ]
 
 MAX_DECODE_TOKENS = 8
@@ -602,6 +602,75 @@ def linear_grad(d_out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str 
                                                  kind, ptr(dw[0]), ptr(dw[1]), ptr(ws), nbytes, stream_ptr(dev)),
                   "hsmoe_linear_grad_weight")
     return LinearGrad(dx, dw[0], db[0], dw[1], db[1])
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """t's values fill their memory, in some order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for stride, size in sorted((stride, size) for size, stride in zip(t.shape, t.stride()) if size != 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _tensor_list(grads, what: str) -> tuple[array.array, array.array, array.array]:
+    """Addresses, counts and kinds of tensors, as the entry points read them."""
+    for t in grads:
+        if not _dense(t):
+            raise ValueError(f"{what} must fill their memory, got {tuple(t.shape)} with strides {t.stride()}")
+    return (array.array("Q", [t.data_ptr() for t in grads]), array.array("q", [t.numel() for t in grads]),
+            array.array("i", [_row_kind(t.dtype, what) for t in grads]))
+
+
+def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
+    grads = list(grads)
+    if not grads:
+        raise ValueError("no gradients are given")
+    dev = require_cuda(*grads)
+    ins, counts, kinds = _tensor_list(grads, "gradients")
+    outs = out_kinds = None
+    if max_norm is not None:
+        outs, out_kinds = ins, kinds
+        if out is not None:
+            out = list(out)
+            require_cuda(grads[0], *out)
+            if len(out) != len(grads):
+                raise ValueError(f"{len(out)} outputs for {len(grads)} gradients")
+            for g, o in zip(grads, out):
+                if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+                    raise ValueError(f"an output must have its gradient's shape and strides, got {tuple(o.shape)}, {o.stride()} for "
+                                     f"{tuple(g.shape)}, {g.stride()}")
+            outs, _, out_kinds = _tensor_list(out, "outputs")
+    at = lambda a: a.buffer_info()[0]
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nbytes = lib().hsmoe_grad_norm_workspace_size(len(grads))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the call's own, as in moe_sort
+    with _on(dev):
+        if max_norm is None:
+            check(lib().hsmoe_grad_norm(len(grads), at(ins), at(counts), at(kinds), norm_type, ptr(norm), ptr(ws), nbytes,
+                                        stream_ptr(dev)), "hsmoe_grad_norm")
+        else:
+            check(lib().hsmoe_clip_grads(len(grads), at(ins), at(counts), at(kinds), at(outs), at(out_kinds), norm_type, max_norm,
+                                         ptr(norm), ptr(ws), nbytes, stream_ptr(dev)), "hsmoe_clip_grads")
+    return norm
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all values of a list of tensors (bf16 or fp32, any shapes, on one
+    device) together, as an fp32 scalar on the device (hsmoe_grad_norm): norm_type 2,
+    summed in 64 bits, or float("inf"), the largest magnitude."""
+    return _clip(grads, None, float(norm_type), None)
+
+
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """Multiplies a list of gradients by min(1, max_norm / (norm + 1e-6)), in place or into
+    the tensors of out (bf16 or fp32, of their shapes), and returns their norm before that, as
+    grad_norm (hsmoe_clip_grads).  Nothing waits for the device.  A NaN anywhere makes all of them NaN.  Tensors may
+    not overlap: one that is given twice is refused."""
+    return _clip(grads, float(max_norm), float(norm_type), out)
 
 
 def _fp4_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:

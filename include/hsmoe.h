@@ -425,6 +425,27 @@ int hsmoe_linear_grad_weight(const void* dz_dev, int64_t dz_row_stride, const vo
 int hsmoe_linear_plan(int product, int64_t m, int64_t n, int64_t k, int64_t n_groups, int act, int32_t plan[4]);
 
 /* ---------------------------------------------------------------------------
+ * The norm of many tensors together, and gradients cut down to a limit on it (no
+ * reference counterpart: it does not train).
+ *   norm = (sum of x^2 over all values)^(1/2) for norm_type 2, max |x| for INFINITY
+ *   out  = x * min(1, max_norm / (norm + 1e-6))
+ * n tensors of counts[i] values of kinds[i] (HSMOE_OUT_F32 or HSMOE_OUT_BF16), any
+ * alignment of a value; outs[i] of out_kinds[i] may be the tensor itself (in its
+ * kind), and else overlaps none of the others.  The arrays lie in host memory and are
+ * read before the call returns.  norm_out fp32 [1] on the device.  Squares and sums in
+ * 64 bits; a NaN anywhere makes the norm and every output NaN, an infinity makes the
+ * outputs 0 (NaN where it is).  Deterministic, nothing waits for the device.  n = 0
+ * and empty tensors are allowed.  The workspace (any contents) holds
+ * hsmoe_grad_norm_workspace_size bytes for both. */
+size_t hsmoe_grad_norm_workspace_size(int64_t n);
+int hsmoe_grad_norm(int64_t n, const void* const* tensors_dev, const int64_t* counts, const int32_t* kinds,
+                    double norm_type, float* norm_out_dev, void* workspace_dev, size_t workspace_bytes,
+                    hsmoe_stream_t stream);
+int hsmoe_clip_grads(int64_t n, const void* const* tensors_dev, const int64_t* counts, const int32_t* kinds,
+                     void* const* outs_dev, const int32_t* out_kinds, double norm_type, float max_norm,
+                     float* norm_out_dev, void* workspace_dev, size_t workspace_bytes, hsmoe_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Microscaled 4-bit floating point in the experts' own format (e2m1 codes, low
  * nibble first, with one E8M0 power of two per 32 values of a row): quantisation,
  * what the reference's offline quantiser does (_fp4.py:113-255,
