@@ -1,8 +1,10 @@
 """The bf16 expert layer for training: ops.linear, moe_gather and moe_combine as
-torch.autograd functions, and moe_ffn, the routed SwiGLU experts made of them.
+torch.autograd functions, moe_ffn, the routed SwiGLU experts made of them, and what
+stands around it: the embedding lookup and the norms between two blocks.
 
-The gradients are the ops' own (linear_grad, moe_combine_grad): weights' and
-rows' in bf16, routing weights' in fp32, biases' rounded to the bias's dtype.
+The gradients are the ops' own (linear_grad, moe_combine_grad, embed_grad,
+block_norm_grad): weights' and rows' in bf16, routing weights' in fp32, biases',
+norms' weights' and broadcast gates' rounded to their tensor's dtype.
 Between the ops everything is bf16, as between torch's: the activations, the
 experts' results, the sums kept for the backward pass and their gradients.
 Under graph capture, capture the forward and the backward pass together, and let
@@ -20,7 +22,7 @@ from torch.autograd.function import once_differentiable
 from . import ops
 from .ops import ExpertOrder
 
-__all__ = ["linear", "moe_gather", "moe_combine", "moe_ffn"]
+__all__ = ["linear", "moe_gather", "moe_combine", "moe_ffn", "embed", "block_norm"]
 
 
 # The order's tensors are saved as the others are, so that torch notices a change
@@ -119,3 +121,49 @@ def moe_ffn(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, w1: t
     order = ops.moe_sort(topk_idx, w1.shape[0])
     a = linear(moe_gather(x, order), w1, act="swiglu", w_up=w3, limit=limit, order=order)
     return moe_combine(linear(a, w2, order=order), order, topk_w, residual)
+
+
+class _Embed(Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, out_dtype):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.vocab, ctx.dtype = scale, table.shape[0], table.dtype
+        return ops.embed(ids, table, scale, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        ids, = ctx.saved_tensors
+        return None, ops.embed_grad(d_out, ids, ctx.vocab, ctx.scale, ctx.dtype), None, None
+
+
+class _BlockNorm(Function):
+    @staticmethod
+    def forward(ctx, f, h, post_w, gate, pre_w, scale, eps):
+        ctx.set_materialize_grads(False)  # a result that is not used has no gradient to be read
+        out, n = ops.block_norm(f, h, post_w, gate, scale, pre_w, eps)
+        ctx.save_for_backward(f, out, post_w, gate, pre_w)
+        ctx.scale, ctx.eps = scale, eps
+        return out, n
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_h, d_n):
+        f, out, post_w, gate, pre_w = ctx.saved_tensors
+        if d_h is None and d_n is None:
+            return (None,) * 7
+        g = ops.block_norm_grad(d_h, d_n, f, out, post_w, gate, ctx.scale, pre_w, ctx.eps, need=ctx.needs_input_grad[:5])
+        like = lambda d, t: None if d is None else d.to(t.dtype)
+        return g.f, g.h, like(g.post_w, post_w), like(g.gate, gate), like(g.pre_w, pre_w), None, None
+
+
+def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """ops.embed with its gradient (for the table, in its dtype, every row written; a training loop
+    that keeps a gradient buffer of its own adds to it with ops.embed_grad(..., out=))."""
+    return _Embed.apply(ids, table, scale, out_dtype)
+
+
+def block_norm(f: torch.Tensor, h: torch.Tensor, post_w: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+               scale: float = 1.0, pre_w: torch.Tensor | None = None, eps: float = 1e-6):
+    """ops.block_norm with its gradient (for f, h, the norms' weights and the gate) -> (h', n)."""
+    return _BlockNorm.apply(f, h, post_w, gate, pre_w, scale, eps)

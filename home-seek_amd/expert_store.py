@@ -161,6 +161,20 @@ class HbmExpertStore:
         return ops.xor_checksum(self.buf if region is None else region)
 
     # ------------------------------------------------------------ fill
+    def put_expert(self, layer: int, eid: int, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor) -> None:
+        """Quantises an expert's weights (bf16 or fp32: w1, w3 [I, D], w2 [D, I], as autograd.moe_ffn
+        trains them) into its record (hsmoe_fp4_quant); an absent expert is there afterwards.
+        Graphs captured over the store read the new weights."""
+        views = self.expert_views(layer, eid)
+        for name, w, shape in (("w1", w1, (self.i, self.d)), ("w3", w3, (self.i, self.d)), ("w2", w2, (self.d, self.i))):
+            if tuple(w.shape) != shape:
+                raise ValueError(f"{name} must be {list(shape)}, got {tuple(w.shape)}")
+        for w, codes, scale in zip((w1, w3, w2), views[0::2], views[1::2]):
+            ops.fp4_quant(w.detach(), out=(codes, scale))
+        if (layer, eid) in self._absent:
+            self._absent.discard((layer, eid))
+            self._tables.pop(layer, None)
+
     def fill_synthetic(self, seed: int, layers=None) -> None:
         """Fills experts (and shared experts) with the seeded synthetic weights."""
         for layer in (range(self.n_layers) if layers is None else layers):

@@ -604,6 +604,17 @@ def linear_grad(d_out: torch.Tensor, x: torch.Tensor, w: torch.Tensor, act: str 
     return LinearGrad(dx, dw[0], db[0], dw[1], db[1])
 
 
+def _written(*tensors: torch.Tensor) -> None:
+    """Tells autograd that a kernel has written these, which a caller gave."""
+    torch.autograd.graph.increment_version(tensors)
+
+
+def _writable(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} is part of a gradient's graph: it is written under torch.no_grad() only")
+    return t
+
+
 def _dense(t: torch.Tensor) -> bool:
     """t's values fill their memory, in some order of its dimensions."""
     if t.is_contiguous():
@@ -634,6 +645,7 @@ def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
     outs = out_kinds = None
     if max_norm is not None:
         outs, out_kinds = ins, kinds
+        written = grads
         if out is not None:
             out = list(out)
             require_cuda(grads[0], *out)
@@ -644,6 +656,9 @@ def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
                     raise ValueError(f"an output must have its gradient's shape and strides, got {tuple(o.shape)}, {o.stride()} for "
                                      f"{tuple(g.shape)}, {g.stride()}")
             outs, _, out_kinds = _tensor_list(out, "outputs")
+            written = out
+        for t in written:
+            _writable(t, "a gradient that is clipped")
     at = lambda a: a.buffer_info()[0]
     norm = torch.empty((), dtype=torch.float32, device=dev)
     nbytes = lib().hsmoe_grad_norm_workspace_size(len(grads))
@@ -655,6 +670,7 @@ def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
         else:
             check(lib().hsmoe_clip_grads(len(grads), at(ins), at(counts), at(kinds), at(outs), at(out_kinds), norm_type, max_norm,
                                          ptr(norm), ptr(ws), nbytes, stream_ptr(dev)), "hsmoe_clip_grads")
+            _written(*written)
     return norm
 
 
@@ -702,21 +718,33 @@ def _fp4_operand(codes: torch.Tensor, scale: torch.Tensor, what: str) -> tuple[t
     return codes, scale if scale.data_ptr() % 16 == 0 else scale.clone()
 
 
-def fp4_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+def fp4_quant(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(packed e2m1 int8 [..., K/2], E8M0 scales [..., K/32]) of x [..., K] (bf16 or
     fp32, K a multiple of 32): the experts' own format, what fp4_dequant_bf16 reads.
-    A scale is the smallest power of two with which the block's largest magnitude is
+    out: contiguous tensors of these shapes to write to.  A scale is the smallest power of two with which the block's largest magnitude is
     at most 6, a code the nearest one, ties to even; a block with an infinity or a NaN
     becomes NaN (hsmoe_fp4_quant)."""
     dev = require_cuda(x)
     lead, k = x.shape[:-1], x.shape[-1] if x.dim() else 0
     x, kind, stride = _fp4_rows(x, "x")
-    packed = torch.empty(lead + (k // 2,), dtype=torch.int8, device=dev)
-    scale = torch.empty(lead + (k // 32,), dtype=torch.uint8, device=dev)
+    shapes = lead + (k // 2,), lead + (k // 32,)
+    written = out is not None
+    if out is None:
+        out = (torch.empty(shapes[0], dtype=torch.int8, device=dev),
+               torch.empty(shapes[1], dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu))
+    else:
+        require_cuda(x, *out)
+        if out[0].dtype not in (torch.int8, torch.uint8) or out[1].dtype != torch.float8_e8m0fnu:
+            raise TypeError(f"fp4_quant writes int8 codes and float8_e8m0fnu scales, not {out[0].dtype}, {out[1].dtype}")
+        if (tuple(out[0].shape), tuple(out[1].shape)) != shapes or not (out[0].is_contiguous() and out[1].is_contiguous()):
+            raise ValueError(f"fp4_quant writes contiguous {shapes[0]} codes and {shapes[1]} scales")
+    packed, scale = out
     with _on(dev):
         check(lib().hsmoe_fp4_quant(ptr(x), stride, kind, x.shape[0], k, ptr(packed), ptr(scale), stream_ptr(dev)),
               "hsmoe_fp4_quant")
-    return packed, scale.view(torch.float8_e8m0fnu)
+    if written:
+        _written(packed, scale)
+    return packed, scale
 
 
 def fp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale: torch.Tensor | None = None,
@@ -1200,6 +1228,7 @@ def embed_grad(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float 
         if tuple(out.shape) != (vocab, d) or (d > 1 and out.stride(1) != 1) or (vocab > 1 and out.stride(0) < d):
             raise ValueError(f"out must be [{vocab}, {d}] with rows of consecutive values, got {tuple(out.shape)}, "
                              f"strides {out.stride()}")
+        _writable(out, "out")
     table = torch.empty(vocab, d, dtype=out_dtype or d_out.dtype, device=dev) if out is None else out
     out_kind = _row_kind(table.dtype, "the table's gradient")
     d_out = d_out.reshape(-1, d)
@@ -1213,6 +1242,8 @@ def embed_grad(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float 
         check(lib().hsmoe_embed_grad(ptr(d_out), max(d_out.stride(0), d), kind, ptr(ids), id_kind, m, vocab, d, scale,
                                      0 if out is None else 1, ptr(table), max(table.stride(0), d), out_kind, ptr(ws), nbytes,
                                      stream_ptr(dev)), "hsmoe_embed_grad")
+    if out is not None:
+        _written(out)
     return table
 
 
