@@ -102,20 +102,23 @@ __device__ __forceinline__ Factor factor(double norm, float max_norm) {
 struct Vals {
   float v[8];
 };
+// Eight values as they lie in memory.
 template <bool kF32>
-__device__ __forceinline__ Vals read8(const void* base, int64_t at) {
-  Vals r;
+struct Raw {
+  uint32_t w[kF32 ? 8 : 4] = {};
+  __device__ __forceinline__ float at(int i) const {
+    if (kF32) return __uint_as_float(w[i]);
+    return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
+  }
+};
+template <bool kF32>
+__device__ __forceinline__ Raw<kF32> read8(const void* base, int64_t at) {
+  Raw<kF32> r;
   const char* p = (const char*)base + at * (kF32 ? 4 : 2);
-  const uint4 a = ldg<uint4>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-  if (kF32) {
-    const uint4 b = ldg<uint4>(p + 16);
-    const uint32_t u[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = __uint_as_float(w[i]), r.v[4 + i] = __uint_as_float(u[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[2 * i] = __uint_as_float(w[i] << 16), r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+    const uint4 a = ldg<uint4>(p + 16 * i);
+    r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
   }
   return r;
 }
@@ -150,13 +153,13 @@ __device__ __forceinline__ void take_part(const void* in, int64_t a, int64_t b, 
     constexpr int kAhead = (kF32 ? 2 : 4) * (kN == kThreads ? 2 : 1);
     const int64_t whole = a + (b - a) / 8 * 8;
     for (int64_t i = a + (int64_t)threadIdx.x * 8; i < whole; i += (int64_t)kAhead * kN * 8) {
-      Vals v[kAhead];
+      Raw<kF32> v[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j] = i + (int64_t)j * kN * 8 < whole ? read8<kF32>(in, i + (int64_t)j * kN * 8) : Vals{};
+      for (int j = 0; j < kAhead; ++j) v[j] = i + (int64_t)j * kN * 8 < whole ? read8<kF32>(in, i + (int64_t)j * kN * 8) : Raw<kF32>{};
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s.take(v[j].v[k]);
+        for (int k = 0; k < 8; ++k) s.take(v[j].at(k));
     }
     done = whole;
   }
@@ -169,14 +172,15 @@ __device__ __forceinline__ void scale_part(const void* in, void* out, int64_t a,
     constexpr int kAhead = (kF32 ? 2 : 4) * (kN == kThreads ? 2 : 1);
     const int64_t whole = a + (b - a) / 8 * 8;
     for (int64_t i = a + (int64_t)threadIdx.x * 8; i < whole; i += (int64_t)kAhead * kN * 8) {
-      Vals v[kAhead];
+      Raw<kF32> v[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j] = i + (int64_t)j * kN * 8 < whole ? read8<kF32>(in, i + (int64_t)j * kN * 8) : Vals{};
+      for (int j = 0; j < kAhead; ++j) v[j] = i + (int64_t)j * kN * 8 < whole ? read8<kF32>(in, i + (int64_t)j * kN * 8) : Raw<kF32>{};
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
+        Vals o;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[j].v[k] = v[j].v[k] * c.a * c.b;
-        if (i + (int64_t)j * kN * 8 < whole) write8<kO32>(out, i + (int64_t)j * kN * 8, v[j]);
+        for (int k = 0; k < 8; ++k) o.v[k] = v[j].at(k) * c.a * c.b;
+        if (i + (int64_t)j * kN * 8 < whole) write8<kO32>(out, i + (int64_t)j * kN * 8, o);
       }
     }
     done = whole;

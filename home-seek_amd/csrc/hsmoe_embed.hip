@@ -18,8 +18,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kChunk = 32;           // sorted tokens per chunk
 constexpr int kSortThreads = 1024;
-constexpr int kSortTokens = 64;      // tokens that a sorting workgroup places
-constexpr int64_t kSortByRank = 16384;  // tokens up to which every token's place is counted out
+constexpr int64_t kSortByRank = 65536;  // tokens up to which places are found by bisection
+constexpr uint32_t kNoId = 1u << 30;    // an id outside the table, above all others
 
 // The id of token t, -1 outside the table.
 __device__ __forceinline__ int id_of(const void* ids, bool wide, int64_t t, int64_t vocab) {
@@ -58,6 +58,31 @@ __device__ __forceinline__ Vals<kVec> read(const void* base, int64_t at) {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.v[2 * i] = __uint_as_float(w[i] << 16), r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  return r;
+}
+// As they lie in memory.
+template <int kVec, bool kF32>
+struct Raw {
+  uint32_t w[kVec == 1 ? 1 : kF32 ? 8 : 4];
+  __device__ __forceinline__ float at(int i) const {
+    if (kF32) return __uint_as_float(w[i]);
+    if (kVec == 1) return __uint_as_float(w[0] << 16);
+    return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
+  }
+};
+template <int kVec, bool kF32>
+__device__ __forceinline__ Raw<kVec, kF32> fetch(const void* base, int64_t at) {
+  Raw<kVec, kF32> r;
+  const char* p = (const char*)base + at * (kF32 ? 4 : 2);
+  if constexpr (kVec == 1) {
+    r.w[0] = kF32 ? *(const uint32_t*)p : *(const uint16_t*)p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+      const uint4 a = ldg<uint4>(p + 16 * i);
+      r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
+    }
   }
   return r;
 }
@@ -113,20 +138,20 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedParams p) {
 }
 
 // ---------------------------------------------------------------- gradient
-// The tokens by (id, t): sorted_id[r] and token[r], ids outside the table left out
-// and the rest of sorted_id -1.  A token's place is the number of tokens with a
-// smaller id, or the same and before it: m^2 comparisons, for 16384 tokens 2^28 of
-// them, which the chip does in the time of one of the launches that a radix sort
-// needs.  A workgroup places 64 tokens, its 16 waves each counting a sixteenth of
-// all.  The first `sorters` workgroups do that; the others meanwhile clear the table's
-// gradient, which is written once more than needed where a token falls, but waits
-// for no order.
+// The tokens by (id, t): sorted_id[r] and token[r], those with an id outside the
+// table last with sorted_id -1.  First every 1024 tokens by themselves, by a workgroup
+// each, while other workgroups clear the table's gradient (which is written once
+// more than needed where a token falls, but waits for no order): 16381 tokens are
+// sorted long before a gigabyte is cleared.  Then a token's place is its place in its own
+// 1024 plus, for each of the others, the number of smaller ids there (or equal ones, if
+// they come before it), found by bisection in LDS.
 struct SortParams {
   const void* ids;
   int64_t m, vocab;
   bool wide;
   int sorters;
-  int *sorted_id, *token;
+  int *sorted_id, *token;   // what is sorted in the end
+  int *part_id, *part_token;  // by 1024
   char* clear;
   int64_t clear_bytes;
 };
@@ -145,44 +170,71 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p) 
     clear_part(p.clear, p.clear_bytes, (int)blockIdx.x - p.sorters, (int)gridDim.x - p.sorters);
     return;
   }
-  __shared__ int ids[kSortByRank];
-  __shared__ int counts[kSortThreads / 64][kSortTokens], valid[kSortThreads / 64];
-  const int m = (int)p.m, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int live = 0;
-  for (int i = threadIdx.x; i < m; i += kSortThreads) {
-    const int v = id_of(p.ids, p.wide, i, p.vocab);
-    ids[i] = v < 0 ? 0x7fffffff : v;
-    live += v >= 0;
+  __shared__ unsigned long long mem[kSortThreads];
+  const int i = threadIdx.x;
+  const int64_t t = (int64_t)blockIdx.x * kSortThreads + i;
+  const int id = t < p.m ? id_of(p.ids, p.wide, t, p.vocab) : -1;
+  // bitonic, on (id, place): no two are the same, so the result is the stable sort's
+  unsigned long long key = (unsigned long long)(id < 0 ? kNoId : (uint32_t)id) << 10 | (unsigned)i;
+  for (int size = 2; size <= kSortThreads; size *= 2)
+    for (int step = size / 2; step > 0; step /= 2) {
+      unsigned long long other;
+      if (step >= 64) {
+        __syncthreads();
+        mem[i] = key;
+        __syncthreads();
+        other = mem[i ^ step];
+      } else {
+        other = (unsigned long long)__shfl_xor((long long)key, step, 64);
+      }
+      const bool up = !(i & size), low = !(i & step);
+      key = (key < other) == (up == low) ? key : other;
+    }
+  const uint32_t v = (uint32_t)(key >> 10);
+  const int64_t from = (int64_t)blockIdx.x * kSortThreads + (int)(key & 1023);
+  if (t < p.m) {  // (places behind the last token sort behind all others)
+    const bool one = p.sorters == 1;
+    (one ? p.sorted_id : p.part_id)[t] = one && v == kNoId ? -1 : (int)v;
+    (one ? p.token : p.part_token)[t] = (int)from;
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) live += __shfl_xor(live, off, 64);
-  if (lane == 0) valid[wave] = live;
-  __syncthreads();
-  const int t0 = blockIdx.x * kSortTokens, t = t0 + lane;
-  const int mine = t < m ? ids[t] : 0x7fffffff;
-  // this wave's share of all tokens; those before the 64 count if not above, those behind if below
-  const int per = ((m + kSortThreads / 64 - 1) / (kSortThreads / 64) + 3) & ~3;
-  const int a = wave * per, b = a + per < m ? a + per : m;
+}
+
+// 64 tokens per workgroup, a wave for each of 16 sorted parts at a time.
+__global__ void __launch_bounds__(kSortThreads) embed_rank_kernel(SortParams p) {
+  __shared__ int ids[kSortThreads * 16];
+  __shared__ int counts[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m = (int)p.m, parts = p.sorters, t = blockIdx.x * 64 + lane, own = t / kSortThreads;
+  const int id = t < m ? p.part_id[t] : 0;
   int n = 0;
-  auto count = [&](int from, int to, int limit) {  // ids below limit
-#pragma unroll 16
-    for (int i = from; i < to; ++i) n += ids[i] < limit;
-  };
-  const int c = a > t0 ? a : t0, e = t0 + kSortTokens < b ? t0 + kSortTokens : b;
-  count(a, b < t0 ? b : t0, mine == 0x7fffffff ? mine : mine + 1);
-  for (int i = c; i < e; ++i) n += ids[i] < mine || (ids[i] == mine && i < t);
-  count(a > t0 + kSortTokens ? a : t0 + kSortTokens, b, mine);
+  for (int p0 = 0; p0 < parts; p0 += 16) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kSortThreads * 16; i += kSortThreads) {
+      const int at = p0 * kSortThreads + i;
+      ids[i] = at < m ? p.part_id[at] : (int)kNoId;
+    }
+    __syncthreads();
+    const int part = p0 + wave;
+    if (part < parts && part != own) {
+      // the number of ids below id, or not above it in an earlier part
+      const int limit = part < own ? id + 1 : id;  // (of kNoId: 2^30 + 1)
+      int lo = 0;
+#pragma unroll
+      for (int step = kSortThreads / 2; step > 0; step /= 2)
+        if (ids[wave * kSortThreads + lo + step - 1] < limit) lo += step;
+      if (ids[wave * kSortThreads + lo] < limit) ++lo;  // (lo <= 1023 so far)
+      const int there = m - part * kSortThreads;
+      n += lo < there ? lo : there;
+    }
+  }
   counts[wave][lane] = n;
   __syncthreads();
-  int total = 0;
+  if (wave || t >= m) return;
+  n = t % kSortThreads;
 #pragma unroll
-  for (int w = 0; w < kSortThreads / 64; ++w) total += valid[w];
-  if (wave) return;
-  n = 0;
-#pragma unroll
-  for (int w = 0; w < kSortThreads / 64; ++w) n += counts[w][lane];
-  if (t < m && mine != 0x7fffffff) p.sorted_id[n] = mine, p.token[n] = t;
-  if (t < m && t >= total) p.sorted_id[t] = -1;
+  for (int w = 0; w < 16; ++w) n += counts[w][lane];
+  p.sorted_id[n] = (uint32_t)id == kNoId ? -1 : id;
+  p.token[n] = p.part_token[t];
 }
 __global__ void __launch_bounds__(kSortThreads) embed_clear_kernel(char* p, int64_t bytes) {
   clear_part(p, bytes, blockIdx.x, gridDim.x);
@@ -243,76 +295,98 @@ __device__ __forceinline__ void leave(float* to, const Vals<kVec>& s) {
   for (int i = 0; i < kVec; ++i) to[i] = s.v[i];
 }
 
-// Sums of the runs of a chunk, for kVec columns per thread.
+// Sums of the runs of a chunk, for kVec columns per thread.  The chunk's ids and
+// tokens are read once; then eight rows are on their way at a time.
 template <int kVec, bool kF32, bool kOutF32>
 __global__ void __launch_bounds__(kThreads) embed_sum_kernel(SumParams p) {
-  const int lanes = 1 << p.shift;
-  const int64_t chunk = (int64_t)(blockIdx.x / p.slabs) * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
+  __shared__ int2 mem[kThreads / 8][kChunk + 1];  // (id, token) of the workgroup's chunks, and the id behind each
+  __shared__ int before[kThreads / 8];
+  const int lanes = 1 << p.shift, per = kThreads >> p.shift, mine = threadIdx.x >> p.shift;
+  const int64_t c0 = (int64_t)(blockIdx.x / p.slabs) * per;
+  const int64_t chunk = c0 + mine;
+  for (int i = threadIdx.x; i < per * (kChunk + 1); i += kThreads) {
+    const int64_t r = (c0 + i / (kChunk + 1)) * kChunk + i % (kChunk + 1);
+    mem[i / (kChunk + 1)][i % (kChunk + 1)] = r < p.m ? make_int2(p.sorted_id[r], p.token[r]) : make_int2(-1, 0);
+  }
+  for (int i = threadIdx.x; i < per; i += kThreads) {
+    const int64_t r = (c0 + i) * kChunk - 1;
+    before[i] = r >= 0 && r < p.m ? p.sorted_id[r] : -1;
+  }
+  __syncthreads();
   const int64_t col = ((int64_t)(blockIdx.x % p.slabs) * lanes + (threadIdx.x & (lanes - 1))) * kVec;
   if (chunk >= p.chunks || col >= p.d) return;
-  const int64_t r0 = chunk * kChunk, r1 = r0 + kChunk < p.m ? r0 + kChunk : p.m;
-  int id = p.sorted_id[r0];
+  int id = mem[mine][0].x;
   if (id < 0) return;
-  bool open = chunk > 0 && p.sorted_id[r0 - 1] == id;  // the run began before the chunk
-  const int after = r1 < p.m ? p.sorted_id[r1] : -1;
+  bool open = before[mine] == id;  // the run began before the chunk
   float* part = p.part + chunk * 2 * p.d + col;
   Vals<kVec> s = {};
   constexpr int kAhead = 8;
-  for (int64_t r = r0; r < r1; r += kAhead) {
-    int ids[kAhead];
-    Vals<kVec> v[kAhead];
+  for (int r = 0; r < kChunk; r += kAhead) {
+    if (mem[mine][r].x < 0) break;
+    Raw<kVec, kF32> v[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      ids[i] = r + i < r1 ? p.sorted_id[r + i] : -1;
-      v[i] = ids[i] >= 0 ? read<kVec, kF32>(p.d_out, (int64_t)p.token[r + i] * p.ld_out + col) : Vals<kVec>{};
+      const int2 e = mem[mine][r + i];
+      v[i] = fetch<kVec, kF32>(p.d_out, (int64_t)(e.x < 0 ? mem[mine][r].y : e.y) * p.ld_out + col);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (ids[i] < 0) continue;
-      if (ids[i] != id) {  // the run before is done
+      const int next = mem[mine][r + i].x;
+      if (next < 0) continue;
+      if (next != id) {  // the run before is done
         if (open) leave<kVec>(part, s);
         else finish<kVec, kOutF32>(p, id, col, s);
-        open = false, id = ids[i], s = Vals<kVec>{};
+        open = false, id = next, s = Vals<kVec>{};
       }
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) s.v[j] += v[i].v[j];
+      for (int j = 0; j < kVec; ++j) s.v[j] += v[i].at(j);
     }
   }
   // the last run: goes on in the next chunk, or ends here
-  if (after == id) leave<kVec>(part + (open ? 0 : p.d), s);
+  if (mem[mine][kChunk].x == id) leave<kVec>(part + (open ? 0 : p.d), s);
   else if (open) leave<kVec>(part, s);
   else finish<kVec, kOutF32>(p, id, col, s);
 }
 
 // Runs over several chunks: the chunk where one begins adds what the next ones left.
+// A wave or more per chunk; its lanes look for the run's end 64 chunks at a time.
 template <int kVec, bool kOutF32>
 __global__ void __launch_bounds__(kThreads) embed_join_kernel(SumParams p) {
   const int lanes = 1 << p.shift;
   const int64_t chunk = (int64_t)(blockIdx.x / p.slabs) * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
   const int64_t col = ((int64_t)(blockIdx.x % p.slabs) * lanes + (threadIdx.x & (lanes - 1))) * kVec;
   const int64_t r0 = chunk * kChunk, r1 = r0 + kChunk;
-  if (chunk >= p.chunks || col >= p.d || r1 >= p.m) return;
-  const int id = p.sorted_id[r1];
-  if (id < 0 || p.sorted_id[r1 - 1] != id) return;                            // nothing goes on
-  if (p.sorted_id[r0] == id && chunk > 0 && p.sorted_id[r0 - 1] == id) return;  // it began earlier
-  const float* part = p.part + chunk * 2 * p.d + col;
-  Vals<kVec> s = {};
+  if (chunk >= p.chunks || r1 >= p.m) return;
+  const int id = p.sorted_id[r1], last = p.sorted_id[r1 - 1], first = p.sorted_id[r0], before = r0 > 0 ? p.sorted_id[r0 - 1] : -1;
+  if (id < 0 || last != id) return;             // nothing goes on
+  if (first == id && before == id) return;  // it began earlier
+  int64_t end = chunk + 1;                      // the first chunk that does not begin with the run
+  for (bool on = true; on;) {
+    const int64_t c = end + (threadIdx.x & 63);
+    const uint64_t other = __ballot(!(c < p.chunks && p.sorted_id[c * kChunk] == id));
+    on = other == 0;
+    end += on ? 64 : __builtin_ctzll(other);
+  }
+  if (col >= p.d) return;
+  const float* part = p.part + col;
+  Vals<kVec> s;
 #pragma unroll
-  for (int j = 0; j < kVec; ++j) s.v[j] = part[p.d + j];
-  constexpr int kAhead = 16;
-  for (int64_t c = chunk + 1; c < p.chunks; c += kAhead) {
-    bool on[kAhead];  // equal ids lie together: true up to the run's end
-    Vals<kVec> v[kAhead] = {};
+  for (int j = 0; j < kVec; ++j) s.v[j] = part[(chunk * 2 + 1) * p.d + j];
+  int64_t c = chunk + 1;
+  constexpr int kAhead = 8;
+  for (; c + kAhead <= end; c += kAhead) {
+    Raw<kVec, true> v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      on[i] = c + i < p.chunks && p.sorted_id[(c + i) * kChunk] == id;
-      if (on[i]) v[i] = read<kVec, true>(p.part, (c + i) * 2 * p.d + col);
-    }
+    for (int i = 0; i < kAhead; ++i) v[i] = fetch<kVec, true>(part, (c + i) * 2 * p.d);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) s.v[j] += on[i] ? v[i].v[j] : 0.0f;
-    if (!on[kAhead - 1]) break;
+      for (int j = 0; j < kVec; ++j) s.v[j] += v[i].at(j);
+  }
+  for (; c < end; ++c) {
+    const Raw<kVec, true> v = fetch<kVec, true>(part, c * 2 * p.d);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) s.v[j] += v.at(j);
   }
   finish<kVec, kOutF32>(p, id, col, s);
 }
@@ -328,13 +402,15 @@ int shift_for(int64_t vectors) {
 }
 
 struct GradSpace {
-  int64_t ids, token, order, digit, offsets, pairs, rows, sort, sort_bytes, part, bytes;
+  int64_t ids, token, part_id, part_token, order, digit, offsets, pairs, rows, sort, sort_bytes, part, bytes;
 };
 GradSpace space_of(int64_t m, int64_t d) {
   GradSpace s{};
   const int64_t n = up(m * 4, 256);
   s.ids = 0, s.token = n, s.bytes = 2 * n;
-  if (m > kSortByRank) {
+  if (m > kSortThreads && m <= kSortByRank) {
+    s.part_id = s.bytes, s.part_token = s.bytes + n, s.bytes += 2 * n;
+  } else if (m > kSortByRank) {
     s.order = s.bytes, s.digit = s.order + n, s.offsets = s.digit + 2 * n, s.pairs = s.offsets + up(1025 * 4, 256);
     s.rows = s.pairs + n, s.sort = s.rows + n;
     s.sort_bytes = (int64_t)hsmoe_moe_sort_workspace_size(m, 1, 1024);
@@ -433,8 +509,10 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
     return check_launch(who);
   }
   if (m <= kSortByRank) {
-    SortParams s{ids, m, vocab, wide, (int)((m + kSortTokens - 1) / kSortTokens), sorted_id, token, (char*)d_table, bytes};
+    const SortParams s{ids, m, vocab, wide, (int)((m + kSortThreads - 1) / kSortThreads), sorted_id, token, (int*)(mem + sp.part_id),
+                       (int*)(mem + sp.part_token), (char*)d_table, bytes};
     hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(s.sorters + fill)), dim3(kSortThreads), 0, st, s);
+    if (s.sorters > 1) hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((m + 63) / 64)), dim3(kSortThreads), 0, st, s);
   } else {
     if (fill) hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)fill), dim3(kSortThreads), 0, st, (char*)d_table, bytes);
     const dim3 grid((unsigned)((m + kThreads - 1) / kThreads)), block(kThreads);
@@ -460,12 +538,14 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
   p.add = add, p.scale = scale;
   const bool vec = d % 8 == 0 && rows16(d_out, d_row_stride, d_kind) && rows16(d_table, table_row_stride, table_kind);
   const int64_t vectors = vec ? d / 8 : d;
-  p.shift = shift_for(vectors);
+  p.shift = std::max(shift_for(vectors), 3);
   p.slabs = (int)((vectors + (1ll << p.shift) - 1) >> p.shift);
   const bool f = d_kind == HSMOE_OUT_F32, o = table_kind == HSMOE_OUT_F32;
   if (vec) launch_grad<true, 8>(p, f, o, st);
   else launch_grad<true, 1>(p, f, o, st);
   if (p.chunks > 1) {
+    p.shift = std::max(p.shift, 6);
+    p.slabs = (int)((vectors + (1ll << p.shift) - 1) >> p.shift);
     if (vec) launch_grad<false, 8>(p, f, o, st);
     else launch_grad<false, 1>(p, f, o, st);
   }
