@@ -34,51 +34,70 @@ struct BlockNormParams {
   int d, gate_kind;
   bool w_f32, gate_f32;          // weights and gate of fp32 (else bf16)
   bool sum_pre, sum_post, sum_gate;
-  float scale, eps;
+  float scale, eps, per;         // per: 1 / d
 };
 
 // Eight values of a row at a time.
 struct V8 {
   float v[8];
 };
-// (row: values before the row, the same for a workgroup's threads where they share
-// it, so that an address is a scalar base and a 32-bit offset)
+// Eight values as they lie in memory.
 template <bool kF32>
-__device__ __forceinline__ const char* place(const void* base, int64_t row, uint32_t col) {
-  return (const char*)base + row * (kF32 ? 4 : 2) + col * (uint32_t)(kF32 ? 4 : 2);
+struct Raw8 {
+  uint32_t w[kF32 ? 8 : 4];
+  __device__ __forceinline__ float at(int i) const {
+    if (kF32) return __uint_as_float(w[i]);
+    return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
+  }
+};
+
+// Rows through a buffer resource over those that a workgroup takes at a time, a
+// thread's place in them a 32-bit offset in values: one register instead of an
+// address per tensor, and beyond the rows and columns reads give zeros and writes
+// go nowhere.
+constexpr uint32_t kNowhere = 0x0ffffff0u;
+template <bool kF32>
+__device__ __forceinline__ BufRsrc rows_buf(const void* base, int64_t first, int64_t left, int64_t d) {
+  constexpr int64_t kSize = kF32 ? 4 : 2;
+  return make_buf((uint64_t)base + (uint64_t)(first * d * kSize), left > 0 && base ? (uint32_t)(left * d * kSize) : 0u);
 }
 template <bool kF32>
-__device__ __forceinline__ V8 read8(const void* base, int64_t row, uint32_t col) {
-  V8 r;
-  const char* p = place<kF32>(base, row, col);
-  if (kF32) {
-    const uint4 a = ldg<uint4>(p), b = ldg<uint4>(p + 16);
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+__device__ __forceinline__ Raw8<kF32> raw8(BufRsrc buf, uint32_t at) {
+  Raw8<kF32> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(w[i]);
-  } else {
-    const uint4 a = ldg<uint4>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[2 * i] = __uint_as_float(w[i] << 16), r.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
+    const uint4 a = bload128(buf, at * (kF32 ? 4 : 2) + 16 * i);
+    r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
   }
   return r;
 }
-__device__ __forceinline__ V8 read8(const void* base, int64_t row, uint32_t col, bool f32) {
-  return f32 ? read8<true>(base, row, col) : read8<false>(base, row, col);
+template <bool kF32>
+__device__ __forceinline__ V8 read8(BufRsrc buf, uint32_t at) {
+  const Raw8<kF32> r = raw8<kF32>(buf, at);
+  V8 v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v.v[i] = r.at(i);
+  return v;
+}
+// Rows of either kind, decided at run time.
+__device__ __forceinline__ V8 read8(const void* base, int64_t first, int64_t left, int64_t d, uint32_t at, bool f32) {
+  return f32 ? read8<true>(rows_buf<true>(base, first, left, d), at) : read8<false>(rows_buf<false>(base, first, left, d), at);
+}
+__device__ __forceinline__ void store16(BufRsrc buf, uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+  __builtin_amdgcn_raw_buffer_store_b128(u32x4{a, b, c, d}, buf, (int)at, 0, 0);
 }
 template <bool kF32>
-__device__ __forceinline__ void write8(void* base, int64_t row, uint32_t col, const V8& r) {
-  char* at = const_cast<char*>(place<kF32>(base, row, col));
+__device__ __forceinline__ void write8(BufRsrc buf, uint32_t at, const V8& r) {
   if (kF32) {
-    float4* p = reinterpret_cast<float4*>(at);
-    p[0] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
-    p[1] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+      store16(buf, at * 4 + i * 4, __float_as_uint(r.v[i]), __float_as_uint(r.v[i + 1]), __float_as_uint(r.v[i + 2]), __float_as_uint(r.v[i + 3]));
   } else {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16_bits(r.v[2 * i]) | f32_to_bf16_bits(r.v[2 * i + 1]) << 16;
-    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    store16(buf, at * 2, w[0], w[1], w[2], w[3]);
   }
 }
 template <bool kF32>
@@ -91,61 +110,75 @@ __device__ __forceinline__ V8 rounded8(const V8& r) {
 }
 __device__ __forceinline__ V8 ones8() { return V8{{1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f}}; }
 
-__device__ __forceinline__ float inv_rms(float sum, int d, float eps) {
-  return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sum, (float)d), eps)));
+__device__ __forceinline__ float inv_rms(float sum, float per, float eps) {
+  return __fdiv_rn(1.0f, __fsqrt_rn(__fmaf_rn(sum, per, eps)));
+}
+
+// Sums over 8, 16, 32 or 64 lanes, in every one of them, in a fixed order: within
+// sixteen by DPP, beyond by reading a lane of each.
+template <int kCtrl>
+__device__ __forceinline__ float moved(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += moved<0xB1>(v);                       // lane ^ 1
+  v += moved<0x4E>(v);                       // lane ^ 2
+  v += moved<0x141>(v);                      // the other four of eight
+  if (kLanes >= 16) v += moved<0x140>(v);    // the other eight of sixteen
+  if (kLanes == 32) v += __shfl_xor(v, 16, 64);
+  if (kLanes == 64) v = (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+  return v;
 }
 
 // kLanes threads share a row: 8 .. 64 of a wave (a workgroup of 256 then takes
 // several rows at a time), or all of a workgroup (0), up to 1024 threads.  kC: a
 // thread's chunks of eight columns, kLanes (the workgroup) apart.
-// Sums over the row's threads, in a fixed order; every thread gets them.
+// Sums over the row's threads; every thread gets them.
 template <int kLanes, int kN>
 __device__ __forceinline__ void row_sum(float (&s)[kN], float (*mem)[16], int threads) {
-  constexpr int kWave = kLanes ? kLanes : 64;
 #pragma unroll
-  for (int off = 1; off < kWave; off <<= 1)
-#pragma unroll
-    for (int i = 0; i < kN; ++i) s[i] += __shfl_xor(s[i], off, 64);
+  for (int i = 0; i < kN; ++i) s[i] = lanes_sum<kLanes ? kLanes : 64>(s[i]);
   if (kLanes == 0) {
-    const int waves = threads >> 6, wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0)
+    const int waves = threads >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (lane == 0)
 #pragma unroll
       for (int i = 0; i < kN; ++i) mem[i][wave] = s[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      s[i] = 0.0f;
-      for (int w = 0; w < waves; ++w) s[i] += mem[i][w];
-    }
+    for (int i = 0; i < kN; ++i) s[i] = lanes_sum<16>(lane % 16 < waves ? mem[i][lane % 16] : 0.0f);
   }
 }
 
 template <int kLanes, int kC, bool kF32, bool kS32>
 __global__ void __launch_bounds__(kLanes ? 256 : 1024) block_norm_kernel(BlockNormParams p) {
   __shared__ float mem[2][1][16];
+  constexpr int kRows = kLanes ? 256 / (kLanes ? kLanes : 1) : 1;
   const int threads = kLanes ? kLanes : (int)blockDim.x;
   const int t = kLanes ? threadIdx.x % kLanes : threadIdx.x;
-  const int64_t row = kLanes ? (int64_t)blockIdx.x * (256 / (kLanes ? kLanes : 1)) + threadIdx.x / (kLanes ? kLanes : 1) : blockIdx.x;
-  const bool live = row < p.m;
-  const int64_t base = (live ? row : 0) * p.d;
+  const int mine = kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0;
+  const int64_t first = (int64_t)blockIdx.x * kRows, left = p.m - first < kRows ? p.m - first : kRows;
+  const bool live = mine < left;
   V8 f[kC], h[kC], gate[kC], wa[kC], wb[kC];
-  bool in[kC];
+  uint32_t at[kC];
   float token = 1.0f;
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
-    const uint32_t col = (t + c * threads) * 8;
-    in[c] = live && col < (uint32_t)p.d;
-    f[c] = h[c] = V8{}, gate[c] = wa[c] = wb[c] = ones8();
-    if (!in[c]) continue;
-    f[c] = read8<kF32>(p.f, base, col);
-    h[c] = read8<kS32>(p.h, base, col);
-    if (p.gate_kind == kGateFull) gate[c] = read8(p.gate, base, col, p.gate_f32);
-    if (p.gate_kind == kGateChannel) gate[c] = read8(p.gate, 0, col, p.gate_f32);
-    if (p.post_w) wa[c] = read8(p.post_w, 0, col, p.w_f32);
-    if (p.pre_w) wb[c] = read8(p.pre_w, 0, col, p.w_f32);
+    const uint32_t col = (uint32_t)(t + c * threads) * 8;
+    const bool in = col < (uint32_t)p.d;
+    at[c] = live && in ? (uint32_t)(mine * p.d) + col : kNowhere;
+    gate[c] = wa[c] = wb[c] = ones8();
+    f[c] = read8<kF32>(rows_buf<kF32>(p.f, first, left, p.d), at[c]);
+    h[c] = read8<kS32>(rows_buf<kS32>(p.h, first, left, p.d), at[c]);
+    const uint32_t wcol = in ? col : kNowhere;
+    if (p.gate_kind == kGateFull) gate[c] = read8(p.gate, first, left, p.d, at[c], p.gate_f32);
+    if (p.gate_kind == kGateChannel) gate[c] = read8(p.gate, 0, 1, p.d, wcol, p.gate_f32);
+    if (p.post_w) wa[c] = read8(p.post_w, 0, 1, p.d, wcol, p.w_f32);
+    if (p.pre_w) wb[c] = read8(p.pre_w, 0, 1, p.d, wcol, p.w_f32);
   }
   if (p.gate_kind == kGateToken && live)
-    token = p.gate_f32 ? ((const float*)p.gate)[row] : bf16_bits_to_f32(((const uint16_t*)p.gate)[row]);
+    token = p.gate_f32 ? ((const float*)p.gate)[first + mine] : bf16_bits_to_f32(((const uint16_t*)p.gate)[first + mine]);
   float r1 = 1.0f;
   if (p.post_w) {
     float s[1] = {0.0f};
@@ -154,54 +187,54 @@ __global__ void __launch_bounds__(kLanes ? 256 : 1024) block_norm_kernel(BlockNo
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[0] = __fmaf_rn(f[c].v[i], f[c].v[i], s[0]);
     row_sum<kLanes, 1>(s, mem[0], threads);
-    r1 = inv_rms(s[0], p.d, p.eps);
+    r1 = inv_rms(s[0], p.per, p.eps);
   }
   float s[1] = {0.0f};
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
-    const uint32_t col = (t + c * threads) * 8;
+    const bool in = at[c] != kNowhere;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float u = f[c].v[i] * r1 * wa[c].v[i];
       h[c].v[i] = __fmaf_rn(p.scale, token * gate[c].v[i] * u, h[c].v[i]);
     }
     h[c] = rounded8<kS32>(h[c]);
-    if (in[c]) write8<kS32>(p.h_out, base, col, h[c]);
+    write8<kS32>(rows_buf<kS32>(p.h_out, first, left, p.d), at[c], h[c]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[0] = __fmaf_rn(in[c] ? h[c].v[i] : 0.0f, h[c].v[i], s[0]);
+    for (int i = 0; i < 8; ++i) s[0] = __fmaf_rn(in ? h[c].v[i] : 0.0f, h[c].v[i], s[0]);
   }
   if (!p.pre_w) return;
   row_sum<kLanes, 1>(s, mem[1], threads);
-  const float r2 = inv_rms(s[0], p.d, p.eps);
+  const float r2 = inv_rms(s[0], p.per, p.eps);
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
-    const uint32_t col = (t + c * threads) * 8;
     V8 n;
 #pragma unroll
     for (int i = 0; i < 8; ++i) n.v[i] = h[c].v[i] * r2 * wb[c].v[i];
-    if (in[c]) write8<kF32>(p.n_out, base, col, n);
+    write8<kF32>(rows_buf<kF32>(p.n_out, first, left, p.d), at[c], n);
   }
 }
 
-// Eight values as they lie in memory.
-template <bool kF32>
-struct Raw8 {
-  uint32_t w[kF32 ? 8 : 4];
-  __device__ __forceinline__ float at(int i) const {
-    if (kF32) return __uint_as_float(w[i]);
-    return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : __uint_as_float(w[i >> 1] << 16);
-  }
-};
-template <bool kF32>
-__device__ __forceinline__ Raw8<kF32> raw8(const void* base, int64_t row, uint32_t col) {
-  Raw8<kF32> r;
-  const char* p = place<kF32>(base, row, col);
+// Ones, and weights of either kind (bf16 ones as fp32 where kW32).
+template <bool kW32>
+__device__ __forceinline__ Raw8<kW32> ones() {
+  Raw8<kW32> r;
 #pragma unroll
-  for (int i = 0; i < (kF32 ? 2 : 1); ++i) {
-    const uint4 a = ldg<uint4>(p + 16 * i);
-    r.w[4 * i] = a.x, r.w[4 * i + 1] = a.y, r.w[4 * i + 2] = a.z, r.w[4 * i + 3] = a.w;
-  }
+  for (int i = 0; i < (kW32 ? 8 : 4); ++i) r.w[i] = kW32 ? 0x3f800000u : 0x3f803f80u;
   return r;
+}
+template <bool kW32>
+__device__ __forceinline__ Raw8<kW32> weights8(const void* base, int64_t first, int64_t left, int64_t d, uint32_t at, bool f32) {
+  if constexpr (kW32) {
+    if (f32) return raw8<true>(rows_buf<true>(base, first, left, d), at);
+    const Raw8<false> b = raw8<false>(rows_buf<false>(base, first, left, d), at);
+    Raw8<true> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = __float_as_uint(b.at(i));
+    return r;
+  } else {
+    return raw8<false>(rows_buf<false>(base, first, left, d), at);
+  }
 }
 
 // The compiler unpacks it again behind this, instead of keeping eight floats over a sum.
@@ -218,28 +251,35 @@ __device__ __forceinline__ void apart() { asm volatile("" ::: "memory"); }
 // the next one's loads on their way while one is worked on, and keeps its columns'
 // part of the weights' gradients in registers; they leave once at its end, as one
 // row of `part`, and a second kernel adds the workgroups' rows in their order.
-template <int kLanes, int kC, int kMax, bool kF32, bool kS32>
-__global__ void __launch_bounds__(kMax) block_norm_grad_kernel(BlockNormParams p) {
+template <int kLanes, int kC, int kMax, bool kF32, bool kS32, bool kW32>
+__global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_norm_grad_kernel(BlockNormParams p) {
   __shared__ float mem[2][5][16];
   __shared__ float sums[kLanes ? 256 * 8 * kC : 1];
   constexpr int kRows = kLanes ? 256 / (kLanes ? kLanes : 1) : 1;  // at a time
   const int threads = kLanes ? kLanes : (int)blockDim.x;
   const int t = kLanes ? threadIdx.x % kLanes : threadIdx.x;
   const int mine = kLanes ? threadIdx.x / (kLanes ? kLanes : 1) : 0;
+  uint32_t at[kC], wcol[kC];  // the thread's places in the rows, and in the weights
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    const uint32_t col = (uint32_t)(t + c * threads) * 8;
+    wcol[c] = col < (uint32_t)p.d ? col : kNowhere;
+    at[c] = col < (uint32_t)p.d ? (uint32_t)(mine * p.d) + col : kNowhere;
+  }
+  auto left_at = [&](int64_t first) { return p.m - first < kRows ? p.m - first : (int64_t)kRows; };
   struct Row {
     Raw8<kF32> f[kC], dn[kC];
     Raw8<kS32> h[kC], dh[kC];
   };
-  auto load = [&](int64_t row) {
-    Row r = {};
-    if (row >= p.m) return r;
+  auto load = [&](int64_t first) {  // (zeros of what is not there)
+    const int64_t left = left_at(first);
+    Row r;
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const uint32_t col = (t + c * threads) * 8;
-      if (col >= (uint32_t)p.d) continue;
-      r.f[c] = raw8<kF32>(p.f, row * p.d, col);
-      if (p.d_h) r.dh[c] = raw8<kS32>(p.d_h, row * p.d, col);
-      if (p.d_n) r.h[c] = raw8<kS32>(p.h, row * p.d, col), r.dn[c] = raw8<kF32>(p.d_n, row * p.d, col);
+      r.f[c] = raw8<kF32>(rows_buf<kF32>(p.f, first, left, p.d), at[c]);
+      r.dh[c] = raw8<kS32>(rows_buf<kS32>(p.d_h, first, left, p.d), at[c]);
+      r.h[c] = raw8<kS32>(rows_buf<kS32>(p.d_n ? p.h : nullptr, first, left, p.d), at[c]);
+      r.dn[c] = raw8<kF32>(rows_buf<kF32>(p.d_n, first, left, p.d), at[c]);
     }
     return r;
   };
@@ -248,37 +288,33 @@ __global__ void __launch_bounds__(kMax) block_norm_grad_kernel(BlockNormParams p
   // wide rows: the weights are read again for every row, and for the widest no row
   // is loaded ahead, for the registers
   constexpr bool kLean = kC > 1, kAhead = kC < 4;
-  Row next = kAhead ? load(first + mine) : Row{};
-  V8 a_pre[kC] = {}, a_post[kC] = {}, a_gate[kC] = {}, gate[kC], wa[kC], wb[kC];
+  Row next;
+  if (kAhead) next = load(first);
+  V8 a_pre[kC] = {}, a_post[kC] = {}, a_gate[kC] = {};
+  Raw8<kW32> gate[kC], wa[kC], wb[kC];
   auto read_post = [&](int c) {
-    const uint32_t col = (t + c * threads) * 8;
-    gate[c] = wa[c] = ones8();
-    if (col >= (uint32_t)p.d) return;
-    if (p.gate_kind == kGateChannel) gate[c] = read8(p.gate, 0, col, p.gate_f32);
-    if (p.post_w) wa[c] = read8(p.post_w, 0, col, p.w_f32);
+    gate[c] = p.gate_kind == kGateChannel ? weights8<kW32>(p.gate, 0, 1, p.d, wcol[c], p.gate_f32) : ones<kW32>();
+    wa[c] = p.post_w ? weights8<kW32>(p.post_w, 0, 1, p.d, wcol[c], p.w_f32) : ones<kW32>();
   };
-  auto read_pre = [&](int c) {
-    const uint32_t col = (t + c * threads) * 8;
-    wb[c] = p.d_n && col < (uint32_t)p.d ? read8(p.pre_w, 0, col, p.w_f32) : ones8();
-  };
+  auto read_pre = [&](int c) { wb[c] = p.d_n ? weights8<kW32>(p.pre_w, 0, 1, p.d, wcol[c], p.w_f32) : ones<kW32>(); };
   if (!kLean)
 #pragma unroll
     for (int c = 0; c < kC; ++c) read_post(c), read_pre(c);
   for (; first < p.m; first += stride) {
-    const int64_t row = first + mine;
-    const bool live = row < p.m;
-    const int64_t base = (live ? row : 0) * p.d;
-    Row r = kAhead ? next : load(row);
-    if (kAhead) next = load(row + stride);
+    const int64_t left = left_at(first);
+    const bool live = mine < left;
+    Row r;
+    if (kAhead) r = next, next = load(first + stride);
+    else r = load(first);
     float token = 1.0f;
     if (p.gate_kind == kGateToken && live)
-      token = p.gate_f32 ? ((const float*)p.gate)[row] : bf16_bits_to_f32(((const uint16_t*)p.gate)[row]);
+      token = p.gate_f32 ? ((const float*)p.gate)[first + mine] : bf16_bits_to_f32(((const uint16_t*)p.gate)[first + mine]);
     if (!kLean && p.gate_kind == kGateFull)
 #pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        const uint32_t col = (t + c * threads) * 8;
-        if (live && col < (uint32_t)p.d) gate[c] = read8(p.gate, base, col, p.gate_f32);
-      }
+      for (int c = 0; c < kC; ++c) gate[c] = weights8<kW32>(p.gate, first, left, p.d, at[c], p.gate_f32);
+    if (!kLean)
+#pragma unroll
+      for (int c = 0; c < kC; ++c) unpack_later(wa[c]), unpack_later(wb[c]), unpack_later(gate[c]);
     float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
@@ -288,60 +324,56 @@ __global__ void __launch_bounds__(kMax) block_norm_grad_kernel(BlockNormParams p
         const float f = r.f[c].at(i), h = r.h[c].at(i);
         s[0] = __fmaf_rn(f, f, s[0]);
         s[1] = __fmaf_rn(h, h, s[1]);
-        s[2] = __fmaf_rn(r.dn[c].at(i) * wb[c].v[i], h, s[2]);
+        s[2] = __fmaf_rn(r.dn[c].at(i) * wb[c].at(i), h, s[2]);
       }
     }
     row_sum<kLanes, 3>(s, mem[0], threads);
 #pragma unroll
-    for (int c = 0; c < kC; ++c) unpack_later(r.f[c]), unpack_later(r.h[c]), unpack_later(r.dn[c]);
-    const float r1 = p.post_w ? inv_rms(s[0], p.d, p.eps) : 1.0f;
-    const float r2 = p.d_n ? inv_rms(s[1], p.d, p.eps) : 0.0f;
-    const float m2 = s[2] / (float)p.d * r2 * r2;  // r2^2 mean(g h')
+    for (int c = 0; c < kC; ++c) unpack_later(r.f[c]), unpack_later(r.h[c]), unpack_later(r.dn[c]), unpack_later(wb[c]);
+    const float r1 = p.post_w ? inv_rms(s[0], p.per, p.eps) : 1.0f;
+    const float r2 = p.d_n ? inv_rms(s[1], p.per, p.eps) : 0.0f;
+    const float m2 = s[2] * p.per * r2 * r2;  // r2^2 mean(g h')
     float q[2] = {0.0f, 0.0f};                     // sum of post_w du f, and of dt u
     V8 df[kC];
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      const uint32_t col = (t + c * threads) * 8;
       V8 dx, dg;
       if (kLean) {
         apart(), read_pre(c), read_post(c);
-        if (p.gate_kind == kGateFull && live && col < (uint32_t)p.d) gate[c] = read8(p.gate, base, col, p.gate_f32);
+        if (p.gate_kind == kGateFull) gate[c] = weights8<kW32>(p.gate, first, left, p.d, at[c], p.gate_f32);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = r.h[c].at(i), g = r.dn[c].at(i), f = r.f[c].at(i);
         a_pre[c].v[i] = __fmaf_rn(g, x * r2, a_pre[c].v[i]);
-        dx.v[i] = __fmaf_rn(r2, __fmaf_rn(-x, m2, g * wb[c].v[i]), r.dh[c].at(i));
+        dx.v[i] = __fmaf_rn(r2, __fmaf_rn(-x, m2, g * wb[c].at(i)), r.dh[c].at(i));
         const float dt = p.scale * dx.v[i];
         const float y = f * r1;
-        dg.v[i] = dt * (y * wa[c].v[i]);
-        const float du = dt * (token * gate[c].v[i]);
+        dg.v[i] = dt * (y * wa[c].at(i));
+        const float du = dt * (token * gate[c].at(i));
         a_gate[c].v[i] += dg.v[i];
         a_post[c].v[i] = __fmaf_rn(du, y, a_post[c].v[i]);
-        df[c].v[i] = du * wa[c].v[i];
+        df[c].v[i] = du * wa[c].at(i);
         q[0] = __fmaf_rn(df[c].v[i], f, q[0]);
         q[1] += dg.v[i];
       }
-      if (live && col < (uint32_t)p.d) {
-        if (p.d_x) write8<kS32>(p.d_x, base, col, dx);
-        if (p.gate_kind == kGateFull && p.d_gate) {
-          if (p.gate_f32) write8<true>(p.d_gate, base, col, dg);
-          else write8<false>(p.d_gate, base, col, dg);
-        }
+      if (p.d_x) write8<kS32>(rows_buf<kS32>(p.d_x, first, left, p.d), at[c], dx);
+      if (p.gate_kind == kGateFull && p.d_gate) {
+        if (p.gate_f32) write8<true>(rows_buf<true>(p.d_gate, first, left, p.d), at[c], dg);
+        else write8<false>(rows_buf<false>(p.d_gate, first, left, p.d), at[c], dg);
       }
     }
     row_sum<kLanes, 2>(q, mem[1], threads);
 #pragma unroll
     for (int c = 0; c < kC; ++c) unpack_later(r.f[c]);
-    if (p.gate_kind == kGateToken && p.d_gate && live && t == 0) ((float*)p.d_gate)[row] = q[1];
+    if (p.gate_kind == kGateToken && p.d_gate && live && t == 0) ((float*)p.d_gate)[first + mine] = q[1];
     if (p.d_f) {
-      const float m1 = p.post_w ? q[0] / (float)p.d * r1 * r1 : 0.0f;
+      const float m1 = p.post_w ? q[0] * p.per * r1 * r1 : 0.0f;
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
-        const uint32_t col = (t + c * threads) * 8;
-#pragma unroll
+  #pragma unroll
         for (int i = 0; i < 8; ++i) df[c].v[i] = r1 * __fmaf_rn(-r.f[c].at(i), m1, df[c].v[i]);
-        if (live && col < (uint32_t)p.d) write8<kF32>(p.d_f, base, col, df[c]);
+        write8<kF32>(rows_buf<kF32>(p.d_f, first, left, p.d), at[c], df[c]);
       }
     }
   }
@@ -351,8 +383,7 @@ __global__ void __launch_bounds__(kMax) block_norm_grad_kernel(BlockNormParams p
     if (kLanes == 0) {
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
-        const uint32_t col = (t + c * threads) * 8;
-        if (col < (uint32_t)p.d) write8<true>(to, 0, col, a[c]);
+        write8<true>(rows_buf<true>(to, 0, 1, p.d), wcol[c], a[c]);
       }
     } else {  // the rows' groups in their order
       __syncthreads();
@@ -364,12 +395,11 @@ __global__ void __launch_bounds__(kMax) block_norm_grad_kernel(BlockNormParams p
       if (mine == 0)
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-          const uint32_t col = (t + c * threads) * 8;
-          V8 v = {};
+            V8 v = {};
           for (int g = 0; g < kRows; ++g)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v.v[i] += sums[(g * kC + c) * 8 * threads + i * threads + t];
-          if (col < (uint32_t)p.d) write8<true>(to, 0, col, v);
+          write8<true>(rows_buf<true>(to, 0, 1, p.d), wcol[c], v);
         }
     }
   };
@@ -427,18 +457,18 @@ int64_t grad_groups(int64_t m, const Shape& s, bool sums) {
   return sums && all > some ? some : all;
 }
 
-template <bool kGrad, bool kF32, bool kS32>
+template <bool kGrad, bool kF32, bool kS32, bool kW32>
 void launch(const Shape& s, int64_t grid, const BlockNormParams& p, hipStream_t st) {
   const dim3 g((unsigned)grid), b(s.threads);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, st, p); };
   if constexpr (kGrad) {
-    if (s.lanes == 8) return go(block_norm_grad_kernel<8, 1, 256, kF32, kS32>);
-    if (s.lanes == 16) return go(block_norm_grad_kernel<16, 1, 256, kF32, kS32>);
-    if (s.lanes == 32) return go(block_norm_grad_kernel<32, 1, 256, kF32, kS32>);
-    if (s.lanes == 64) return go(block_norm_grad_kernel<64, 1, 256, kF32, kS32>);
-    if (s.chunks == 1) return go(block_norm_grad_kernel<0, 1, 512, kF32, kS32>);
-    if (s.chunks == 2) return go(block_norm_grad_kernel<0, 2, 512, kF32, kS32>);
-    return go(block_norm_grad_kernel<0, 4, 512, kF32, kS32>);
+    if (s.lanes == 8) return go(block_norm_grad_kernel<8, 1, 256, kF32, kS32, kW32>);
+    if (s.lanes == 16) return go(block_norm_grad_kernel<16, 1, 256, kF32, kS32, kW32>);
+    if (s.lanes == 32) return go(block_norm_grad_kernel<32, 1, 256, kF32, kS32, kW32>);
+    if (s.lanes == 64) return go(block_norm_grad_kernel<64, 1, 256, kF32, kS32, kW32>);
+    if (s.chunks == 1) return go(block_norm_grad_kernel<0, 1, 512, kF32, kS32, kW32>);
+    if (s.chunks == 2) return go(block_norm_grad_kernel<0, 2, 512, kF32, kS32, kW32>);
+    return go(block_norm_grad_kernel<0, 4, 512, kF32, kS32, kW32>);
   } else {
     if (s.lanes == 8) return go(block_norm_kernel<8, 1, kF32, kS32>);
     if (s.lanes == 16) return go(block_norm_kernel<16, 1, kF32, kS32>);
@@ -447,16 +477,24 @@ void launch(const Shape& s, int64_t grid, const BlockNormParams& p, hipStream_t 
     return go(block_norm_kernel<0, 2, kF32, kS32>);
   }
 }
+template <bool kGrad, bool kW32>
+void launch_rows(const Shape& s, int64_t grid, bool f32, bool s32, const BlockNormParams& p, hipStream_t st) {
+  if (f32 && s32)
+    launch<kGrad, true, true, kW32>(s, grid, p, st);
+  else if (f32)
+    launch<kGrad, true, false, kW32>(s, grid, p, st);
+  else if (s32)
+    launch<kGrad, false, true, kW32>(s, grid, p, st);
+  else
+    launch<kGrad, false, false, kW32>(s, grid, p, st);
+}
 template <bool kGrad>
 void launch_kinds(const Shape& s, int64_t grid, bool f32, bool s32, const BlockNormParams& p, hipStream_t st) {
-  if (f32 && s32)
-    launch<kGrad, true, true>(s, grid, p, st);
-  else if (f32)
-    launch<kGrad, true, false>(s, grid, p, st);
-  else if (s32)
-    launch<kGrad, false, true>(s, grid, p, st);
+  // (the forward pass reads weights of either kind as they come)
+  if (kGrad && ((p.w_f32 && (p.post_w || p.pre_w)) || (p.gate_f32 && (p.gate_kind == kGateChannel || p.gate_kind == kGateFull))))
+    launch_rows<kGrad, kGrad>(s, grid, f32, s32, p, st);
   else
-    launch<kGrad, false, false>(s, grid, p, st);
+    launch_rows<kGrad, false>(s, grid, f32, s32, p, st);
 }
 
 bool kind_ok(int k) { return k == HSMOE_OUT_F32 || k == HSMOE_OUT_BF16; }
@@ -476,7 +514,7 @@ BlockNormParams params_of(int64_t m, int64_t d, float scale, float eps, const hs
   p.post_w = n->post_w_dev, p.pre_w = n->pre_w_dev, p.gate = n->gate_dev;
   p.m = m, p.d = (int)d, p.gate_kind = n->gate_form;
   p.w_f32 = n->weight_kind == HSMOE_OUT_F32, p.gate_f32 = n->gate_kind == HSMOE_OUT_F32;
-  p.scale = scale, p.eps = eps;
+  p.scale = scale, p.eps = eps, p.per = 1.0f / (float)d;
   return p;
 }
 
