@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
   int64_t first = (int64_t)blockIdx.x * kRows;
   // wide rows: the weights are read again for every row, and for the widest no row
   // is loaded ahead, for the registers
-  constexpr bool kLean = kC > 1, kAhead = kC < 4;
+  constexpr bool kLean = kC > 1, kAhead = kLanes != 0;
   Row next;
   if (kAhead) next = load(first);
   V8 a_pre[kC] = {}, a_post[kC] = {}, a_gate[kC] = {};

@@ -206,9 +206,13 @@ __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c, int sa, int s
 // stage is 256 values of both operands: [row][128 bytes] with a row's 16-byte chunk
 // c at place c ^ (row / 2 % 8), loaded straight to LDS, then the scales' words.
 // Instruction s takes chunk 4 h + s of a row in lanes of half h.
-template <int kBR, int kBC, int kWR, int kWC, int kStages>
+// kStages_ 0: two stages, eight waves in turns.
+template <int kBR, int kBC, int kWR, int kWC, int kStages_>
 struct Fp4Tile {
+  static constexpr bool kTurns = kStages_ == 0;
+  static constexpr int kStages = kTurns ? 2 : kStages_;
   static constexpr int kWaves = kWR * kWC, kThreads = kWaves * 64;
+  static_assert(!kTurns || kWaves == 8, "two waves per SIMD");
   static constexpr int kFR = kBR / kWR / 32, kFC = kBC / kWC / 32;
   static constexpr int kRowsBytes = kBR * 128, kColsBytes = kBC * 128, kScaleBytes = (kBR + kBC) * 8;
   static constexpr int kStage = kRowsBytes + kColsBytes + kScaleBytes;
@@ -252,9 +256,10 @@ struct Fp4Source {
   }
 };
 
-template <int kBR, int kBC, int kWR, int kWC, int kStages>
+template <int kBR, int kBC, int kWR, int kWC, int kStages_>
 __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) fp4_tile_kernel(Fp4Params p) {
-  using T = Fp4Tile<kBR, kBC, kWR, kWC, kStages>;
+  using T = Fp4Tile<kBR, kBC, kWR, kWC, kStages_>;
+  constexpr int kStages = T::kStages;
   __shared__ __align__(1024) char lds[T::kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int rt, ct;
@@ -284,41 +289,94 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   };
   const int wr = wave / kWC, wc = wave % kWC;
   f32x16 acc[T::kFR][T::kFC] = {};
-  for (int s = 0; s < kStages - 1; ++s) load(s, s);
-  int at = 0, next = kStages - 1;
-  for (int s = 0; s < steps; ++s) {
-    // stage s is whole when every wave's loads of it are, and nobody reads the one
-    // before any more; stages beyond the last are loaded from nowhere, for the count
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * T::kLoads) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    load(s + kStages - 1, next);
-    const char* stage = lds + at * T::kStage;
+  int sr[T::kFR], sc[T::kFC];
+  auto read_scales = [&](const char* stage) {
     const char* scales = stage + T::kRowsBytes + T::kColsBytes;
-    int sr[T::kFR], sc[T::kFC];
 #pragma unroll
     for (int i = 0; i < T::kFR; ++i) sr[i] = *reinterpret_cast<const int*>(scales + (wr * T::kFR + i) * 256 + lane * 4);
 #pragma unroll
     for (int j = 0; j < T::kFC; ++j)
       sc[j] = *reinterpret_cast<const int*>(scales + kBR * 8 + (wc * T::kFC + j) * 256 + lane * 4);
-    auto step = [&](auto byte) {
-      constexpr int kByte = decltype(byte)::value;
-      i32x4 r[T::kFR], c[T::kFC];
+  };
+  auto read = [&](const char* stage, int step, i32x4 (&r)[T::kFR], i32x4 (&c)[T::kFC]) {
 #pragma unroll
-      for (int j = 0; j < T::kFC; ++j) c[j] = T::frag(stage + T::kRowsBytes, (wc * T::kFC + j) * 32, kByte, lane);
+    for (int j = 0; j < T::kFC; ++j) c[j] = T::frag(stage + T::kRowsBytes, (wc * T::kFC + j) * 32, step, lane);
 #pragma unroll
-      for (int i = 0; i < T::kFR; ++i) r[i] = T::frag(stage, (wr * T::kFR + i) * 32, kByte, lane);
+    for (int i = 0; i < T::kFR; ++i) r[i] = T::frag(stage, (wr * T::kFR + i) * 32, step, lane);
+  };
+  auto multiply = [&](auto step, const i32x4 (&r)[T::kFR], const i32x4 (&c)[T::kFC]) {
+    constexpr int kByte = decltype(step)::value;
 #pragma unroll
-      for (int i = 0; i < T::kFR; ++i)
+    for (int i = 0; i < T::kFR; ++i)
 #pragma unroll
-        for (int j = 0; j < T::kFC; ++j) acc[i][j] = mfma32<kByte>(c[j], r[i], acc[i][j], sc[j], sr[i]);
+      for (int j = 0; j < T::kFC; ++j) acc[i][j] = mfma32<kByte>(c[j], r[i], acc[i][j], sc[j], sr[i]);
+  };
+  constexpr std::integral_constant<int, 0> k0;
+  constexpr std::integral_constant<int, 1> k1;
+  constexpr std::integral_constant<int, 2> k2;
+  constexpr std::integral_constant<int, 3> k3;
+  if constexpr (T::kTurns) {
+    // Two waves share a SIMD (w and w + 4): one half's waves read half a stage's
+    // operands, and issue the next stage's loads, while the other half's multiply,
+    // with a barrier between the turns; the second half is one turn behind.  Both
+    // have read a stage when the first half starts on the next but one, which goes
+    // into its place; a stage's loads have two turns at least before they are
+    // waited for at the end of the last.
+    const bool second = wave >= 4;
+    i32x4 r[2][T::kFR], c[2][T::kFC];
+    auto turn = [&](bool loads) {  // ends a turn; loads: what the wave loads of the next stage is in LDS
+      if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
     };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 3>{});
-    at = at + 1 == kStages ? 0 : at + 1;
-    next = next + 1 == kStages ? 0 : next + 1;
+    load(0, 0);
+    turn(true);
+    if (second) turn(false);
+    for (int s = 0; s < steps; ++s) {
+      const char* stage = lds + (s & 1) * T::kStage;
+      read_scales(stage);
+      read(stage, 0, r[0], c[0]);
+      read(stage, 1, r[1], c[1]);
+      if (s + 1 < steps) load(s + 1, (s + 1) & 1);
+      turn(false);
+      __builtin_amdgcn_s_setprio(1);
+      multiply(k0, r[0], c[0]);
+      multiply(k1, r[1], c[1]);
+      __builtin_amdgcn_s_setprio(0);
+      turn(false);
+      read(stage, 2, r[0], c[0]);
+      read(stage, 3, r[1], c[1]);
+      turn(second);
+      __builtin_amdgcn_s_setprio(1);
+      multiply(k2, r[0], c[0]);
+      multiply(k3, r[1], c[1]);
+      __builtin_amdgcn_s_setprio(0);
+      turn(!second);
+    }
+    if (!second) turn(false);
+  } else {
+    for (int s = 0; s < kStages - 1; ++s) load(s, s);
+    int at = 0, next = kStages - 1;
+    for (int s = 0; s < steps; ++s) {
+      // stage s is whole when every wave's loads of it are, and nobody reads the one
+      // before any more; stages beyond the last are loaded from nowhere, for the count
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * T::kLoads) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      load(s + kStages - 1, next);
+      const char* stage = lds + at * T::kStage;
+      i32x4 r[T::kFR], c[T::kFC];
+      read_scales(stage);
+      read(stage, 0, r, c), multiply(k0, r, c);
+      read(stage, 1, r, c), multiply(k1, r, c);
+      read(stage, 2, r, c), multiply(k2, r, c);
+      read(stage, 3, r, c), multiply(k3, r, c);
+      at = at + 1 == kStages ? 0 : at + 1;
+      next = next + 1 == kStages ? 0 : next + 1;
+    }
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no load may reach LDS once it is used for the results
   __syncthreads();
@@ -659,7 +717,7 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   else
     hipLaunchKernelGGL((fp4_ready_kernel<kRowsF32>), grid, block, 0, st, q, dx, dw, first);
   if (plan.tile == 0)
-    launch_tile<256, 256, 2, 4, 2>(p, st);
+    launch_tile<256, 256, 2, 4, 0>(p, st);
   else if (plan.tile == 1)
     launch_tile<128, 128, 2, 2, 2>(p, st);
   else
