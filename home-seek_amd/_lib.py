@@ -201,17 +201,24 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_devices: dict[int, torch.device] = {}
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
-    dev = None
+    index = None
     for t in tensors:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise HsmoeError(f"tensor on {t.device} passed to a GPU kernel; the HIP path has no CPU fallback")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise HsmoeError(f"tensors on different devices ({dev} and {t.device})")
-    if dev is None:
+        at = t.get_device()
+        if index is None:
+            index = at
+        elif at != index:
+            raise HsmoeError(f"tensors on different devices (cuda:{index} and cuda:{at})")
+    if index is None:
         raise HsmoeError("no device tensor given")
+    dev = _devices.get(index)
+    if dev is None:
+        dev = _devices[index] = torch.device("cuda", index)
     return dev

@@ -10,6 +10,7 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -285,6 +286,27 @@ _NO_GUARD = contextlib.nullcontext()
 def _on(dev: torch.device):
     """Makes dev the current device around a launch (its stream belongs to it)."""
     return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _run(dev: torch.device, fn, *args) -> None:
+    """An entry point with its last argument, the device's current stream, and that device the current one
+    (1 us less than _on, stream_ptr and check by themselves)."""
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, fn.__name__)
+
+
+def _space(dev: torch.device, nbytes: int) -> torch.Tensor | None:
+    """A workspace of the call's own, as in moe_sort."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
 def _row_kind(dtype: torch.dtype, what: str) -> int:
@@ -627,50 +649,47 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _tensor_list(grads, what: str) -> tuple[array.array, array.array, array.array]:
-    """Addresses, counts and kinds of tensors, as the entry points read them."""
-    for t in grads:
-        if not _dense(t):
-            raise ValueError(f"{what} must fill their memory, got {tuple(t.shape)} with strides {t.stride()}")
-    return (array.array("Q", [t.data_ptr() for t in grads]), array.array("q", [t.numel() for t in grads]),
-            array.array("i", [_row_kind(t.dtype, what) for t in grads]))
-
-
 def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
     grads = list(grads)
-    if not grads:
+    n = len(grads)
+    if not n:
         raise ValueError("no gradients are given")
-    dev = require_cuda(*grads)
-    ins, counts, kinds = _tensor_list(grads, "gradients")
-    outs = out_kinds = None
-    if max_norm is not None:
-        outs, out_kinds = ins, kinds
-        written = grads
-        if out is not None:
-            out = list(out)
-            require_cuda(grads[0], *out)
-            if len(out) != len(grads):
-                raise ValueError(f"{len(out)} outputs for {len(grads)} gradients")
-            for g, o in zip(grads, out):
-                if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                    raise ValueError(f"an output must have its gradient's shape and strides, got {tuple(o.shape)}, {o.stride()} for "
-                                     f"{tuple(g.shape)}, {g.stride()}")
-            outs, _, out_kinds = _tensor_list(out, "outputs")
-            written = out
-        for t in written:
-            _writable(t, "a gradient that is clipped")
+    outs = grads if out is None else list(out)
+    dev = require_cuda(*grads) if outs is grads else require_cuda(*grads, *outs)
+    if len(outs) != n:
+        raise ValueError(f"{len(outs)} outputs for {n} gradients")
+    for t in outs if max_norm is not None else ():
+        _writable(t, "a gradient that is clipped")
+    for g, o in zip(grads, outs):
+        if not g.is_contiguous() and not _dense(g):
+            raise ValueError(f"gradients must fill their memory, got {tuple(g.shape)} with strides {g.stride()}")
+        if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
+            raise ValueError(f"an output must have its gradient's shape and strides, got {tuple(o.shape)}, {o.stride()} for "
+                             f"{tuple(g.shape)}, {g.stride()}")
+    # addresses, counts and kinds, as the entry points read them
+    kind = _ROW_KINDS.get
+    ins, counts = array.array("Q", [g.data_ptr() for g in grads]), array.array("q", [g.numel() for g in grads])
+    kinds = [kind(g.dtype) for g in grads]
+    if None in kinds:
+        _row_kind(grads[kinds.index(None)].dtype, "gradients")
+    kinds = array.array("i", kinds)
     at = lambda a: a.buffer_info()[0]
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = lib().hsmoe_grad_norm_workspace_size(len(grads))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the call's own, as in moe_sort
-    with _on(dev):
-        if max_norm is None:
-            check(lib().hsmoe_grad_norm(len(grads), at(ins), at(counts), at(kinds), norm_type, ptr(norm), ptr(ws), nbytes,
-                                        stream_ptr(dev)), "hsmoe_grad_norm")
-        else:
-            check(lib().hsmoe_clip_grads(len(grads), at(ins), at(counts), at(kinds), at(outs), at(out_kinds), norm_type, max_norm,
-                                         ptr(norm), ptr(ws), nbytes, stream_ptr(dev)), "hsmoe_clip_grads")
-            _written(*written)
+    L = lib()
+    nbytes = L.hsmoe_grad_norm_workspace_size(n)
+    ws = _space(dev, nbytes)
+    if max_norm is None:
+        _run(dev, L.hsmoe_grad_norm, n, at(ins), at(counts), at(kinds), norm_type, norm.data_ptr(), ws.data_ptr(), nbytes)
+        return norm
+    out_ins, out_kinds = ins, kinds
+    if outs is not grads:
+        out_ins, out_kinds = array.array("Q", [o.data_ptr() for o in outs]), [kind(o.dtype) for o in outs]
+        if None in out_kinds:
+            _row_kind(outs[out_kinds.index(None)].dtype, "outputs")
+        out_kinds = array.array("i", out_kinds)
+    _run(dev, L.hsmoe_clip_grads, n, at(ins), at(counts), at(kinds), at(out_ins), at(out_kinds), norm_type, max_norm, norm.data_ptr(),
+         ws.data_ptr(), nbytes)
+    _written(*outs)
     return norm
 
 
@@ -689,33 +708,37 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
     return _clip(grads, float(max_norm), float(norm_type), out)
 
 
-def _fp4_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
-    """x [..., K] as rows [M, K] that the kernels can read, their kind and the distance between them."""
-    kind = _row_kind(x.dtype, what)
-    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] % 32:
-        raise ValueError(f"{what} {tuple(x.shape)} must have rows of a multiple of 32 values")
-    k = x.shape[-1]
-    x = x if x.dim() == 2 else x.reshape(-1, k)
+def _fp4_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
+    """x [..., K] as rows [M, K] that the kernels can read, their kind, number and distance."""
+    kind = _ROW_KINDS.get(x.dtype)
+    if kind is None:
+        _row_kind(x.dtype, what)
+    shape = x.shape
+    k = shape[-1] if shape else 0
+    if k < 1 or k % 32:
+        raise ValueError(f"{what} {tuple(shape)} must have rows of a multiple of 32 values")
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, kind, x.numel() // k, k
+    x = x if len(shape) == 2 else x.reshape(-1, k)
     unit = 16 // x.element_size()
     if x.data_ptr() % 16 or x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) < k or x.stride(0) % unit)):
         x = x.clone(memory_format=torch.contiguous_format)
-    return x, kind, _row_stride(x)
+    return x, kind, x.shape[0], _row_stride(x)
 
 
 def _fp4_operand(codes: torch.Tensor, scale: torch.Tensor, what: str) -> tuple[torch.Tensor, torch.Tensor]:
     """Packed codes [..., K/2] with E8M0 scales [..., K/32], contiguous and 16-byte aligned."""
-    if codes.dtype not in (torch.int8, torch.uint8):
+    if codes.dtype is not torch.int8 and codes.dtype is not torch.uint8:
         raise TypeError(f"{what}: packed FP4 must be int8/uint8, got {codes.dtype}")
-    if scale is None or scale.dtype != torch.float8_e8m0fnu:
+    if scale is None or scale.dtype is not torch.float8_e8m0fnu:
         raise TypeError(f"{what}: the scales must be float8_e8m0fnu, got {None if scale is None else scale.dtype}")
-    if codes.dim() < 1 or codes.shape[-1] < 16 or codes.shape[-1] % 16:
-        raise ValueError(f"{what} {tuple(codes.shape)} must hold a multiple of 32 values per row")
-    want = tuple(codes.shape[:-1]) + (codes.shape[-1] // 16,)
-    if tuple(scale.shape) != want:
-        raise ValueError(f"{what}: scale shape {tuple(scale.shape)} does not match {want}")
-    codes, scale = codes.contiguous(), scale.view(torch.uint8).contiguous()
-    codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
-    return codes, scale if scale.data_ptr() % 16 == 0 else scale.clone()
+    shape = codes.shape
+    if not shape or shape[-1] < 16 or shape[-1] % 16:
+        raise ValueError(f"{what} {tuple(shape)} must hold a multiple of 32 values per row")
+    want = shape[:-1] + (shape[-1] // 16,)
+    if scale.shape != want:
+        raise ValueError(f"{what}: scale shape {tuple(scale.shape)} does not match {tuple(want)}")
+    return _packed16(codes), _packed16(scale)
 
 
 def fp4_quant(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -725,13 +748,13 @@ def fp4_quant(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = N
     at most 6, a code the nearest one, ties to even; a block with an infinity or a NaN
     becomes NaN (hsmoe_fp4_quant)."""
     dev = require_cuda(x)
-    lead, k = x.shape[:-1], x.shape[-1] if x.dim() else 0
-    x, kind, stride = _fp4_rows(x, "x")
-    shapes = lead + (k // 2,), lead + (k // 32,)
+    shape = x.shape
+    x, kind, m, stride = _fp4_rows(x, "x")
+    k = shape[-1]
+    shapes = shape[:-1] + (k // 2,), shape[:-1] + (k // 32,)
     written = out is not None
     if out is None:
-        out = (torch.empty(shapes[0], dtype=torch.int8, device=dev),
-               torch.empty(shapes[1], dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu))
+        out = (torch.empty(shapes[0], dtype=torch.int8, device=dev), torch.empty(shapes[1], dtype=torch.float8_e8m0fnu, device=dev))
     else:
         require_cuda(x, *out)
         if out[0].dtype not in (torch.int8, torch.uint8) or out[1].dtype != torch.float8_e8m0fnu:
@@ -739,9 +762,7 @@ def fp4_quant(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = N
         if (tuple(out[0].shape), tuple(out[1].shape)) != shapes or not (out[0].is_contiguous() and out[1].is_contiguous()):
             raise ValueError(f"fp4_quant writes contiguous {shapes[0]} codes and {shapes[1]} scales")
     packed, scale = out
-    with _on(dev):
-        check(lib().hsmoe_fp4_quant(ptr(x), stride, kind, x.shape[0], k, ptr(packed), ptr(scale), stream_ptr(dev)),
-              "hsmoe_fp4_quant")
+    _run(dev, lib().hsmoe_fp4_quant, x.data_ptr(), stride, kind, m, k, packed.data_ptr(), scale.data_ptr())
     if written:
         _written(packed, scale)
     return packed, scale
@@ -754,29 +775,29 @@ def fp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale:
     or packed [..., K/2] with x_scale [..., K/32] -> [..., N] bf16 or fp32.  Sums in
     fp32.  K must be a multiple of 32, N of 8.  There is no gradient."""
     dev = require_cuda(x, w, w_scale, x_scale)
+    w, w_scale = _fp4_operand(w, w_scale, "w")
     if w.dim() != 2:
         raise ValueError("w must be 2-D [N, K/2]")
-    w, w_scale = _fp4_operand(w, w_scale, "w")
-    n, k = w.shape[0], w.shape[1] * 2
-    out_kind = _row_kind(out_dtype, "the output")
-    if x_scale is not None:
-        if x.dim() < 1 or x.shape[-1] != k // 2:
-            raise ValueError(f"x {tuple(x.shape)} does not have packed rows of {k} values")
-        lead = x.shape[:-1]
-        x, x_scale = _fp4_operand(x, x_scale, "x")
-        m, kind, stride = x.numel() // (k // 2), _lib.ROWS_FP4, 0
+    n, k = w.shape
+    k *= 2
+    out_kind = _ROW_KINDS.get(out_dtype)
+    if out_kind is None:
+        _row_kind(out_dtype, "the output")
+    shape = x.shape
+    if not shape or shape[-1] != (k if x_scale is None else k // 2):
+        raise ValueError(f"x {tuple(shape)} does not have {'rows' if x_scale is None else 'packed rows'} of {k} values")
+    if x_scale is None:
+        x, kind, m, stride = _fp4_rows(x, "x")
+        scales = None
     else:
-        if x.dim() < 1 or x.shape[-1] != k:
-            raise ValueError(f"x {tuple(x.shape)} does not have rows of {k}")
-        lead = x.shape[:-1]
-        x, kind, stride = _fp4_rows(x, "x")
-        m = x.shape[0]
-    out = torch.empty(lead + (n,), dtype=out_dtype, device=dev)
-    with _on(dev):
-        nbytes = lib().hsmoe_fp4_linear_workspace_size(m, n, k, kind)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
-        check(lib().hsmoe_fp4_linear(ptr(x), kind, stride, ptr(x_scale), m, k, ptr(w), ptr(w_scale), n, out_kind,
-                                     ptr(out), ptr(ws), nbytes, stream_ptr(dev)), "hsmoe_fp4_linear")
+        x, x_scale = _fp4_operand(x, x_scale, "x")
+        m, kind, stride, scales = x.numel() // (k // 2), _lib.ROWS_FP4, 0, x_scale.data_ptr()
+    out = torch.empty(shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    L = lib()
+    nbytes = L.hsmoe_fp4_linear_workspace_size(m, n, k, kind)
+    ws = _space(dev, nbytes)
+    _run(dev, L.hsmoe_fp4_linear, x.data_ptr(), kind, stride, scales, m, k, w.data_ptr(), w_scale.data_ptr(), n, out_kind,
+         out.data_ptr(), ptr(ws), nbytes)
     return out
 
 
@@ -1051,33 +1072,43 @@ def _packed16(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+_BLOCK_NORM_SPEC = struct.Struct("3P5i4x")  # hsmoe_block_norm_spec
+
+
 def _block_norm_spec(f: torch.Tensor, stream: torch.dtype, post_w, gate, pre_w):
-    """(hsmoe_block_norm_spec, what it points to) for rows f [..., D]."""
-    d = f.shape[-1] if f.dim() else 0
+    """(hsmoe_block_norm_spec, its gate's form, the tensors that it points to) for rows f [..., D]."""
+    shape = f.shape
+    d = shape[-1] if shape else 0
     if d < 8 or d % 8:
-        raise ValueError(f"rows {tuple(f.shape)} must have a multiple of 8 values")
-    spec = _lib.BlockNormSpec(row_kind=_row_kind(f.dtype, "f"), stream_kind=_row_kind(stream, "the stream"))
-    ws = [w for w in (post_w, pre_w) if w is not None]
-    for w in ws:
-        if tuple(w.shape) != (d,):
+        raise ValueError(f"rows {tuple(shape)} must have a multiple of 8 values")
+    rows, held = _row_kind(f.dtype, "f"), _row_kind(stream, "the stream")
+    row = shape[-1:]
+    for w in (post_w, pre_w):
+        if w is not None and w.shape != row:
             raise ValueError(f"norm weights must be [{d}], got {tuple(w.shape)}")
-    kinds = [_row_kind(w.dtype, "norm weights") for w in ws]
-    both = torch.float32 if len(set(kinds)) == 2 else None  # one kind for both
-    post_w, pre_w = (None if w is None else _packed16(w if both is None else w.to(both)) for w in (post_w, pre_w))
-    spec.weight_kind = _lib.OUT_F32 if both is not None else kinds[0] if kinds else _lib.OUT_BF16
+    if post_w is not None and pre_w is not None and post_w.dtype != pre_w.dtype:  # one kind for both
+        _row_kind(post_w.dtype, "norm weights"), _row_kind(pre_w.dtype, "norm weights")
+        post_w, pre_w = post_w.float(), pre_w.float()
+    weights, a, b, g, gates, form = _lib.OUT_BF16, 0, 0, 0, _lib.OUT_BF16, _lib.GATE_NONE
+    if post_w is not None:
+        weights, post_w = _row_kind(post_w.dtype, "norm weights"), _packed16(post_w)
+        a = post_w.data_ptr()
+    if pre_w is not None:
+        weights, pre_w = _row_kind(pre_w.dtype, "norm weights"), _packed16(pre_w)
+        b = pre_w.data_ptr()
     if gate is not None:
-        spec.gate_kind = _row_kind(gate.dtype, "the gate")
-        if tuple(gate.shape) == (d,):
-            spec.gate_form = _lib.GATE_CHANNEL
-        elif gate.shape == f.shape:
-            spec.gate_form = _lib.GATE_FULL
-        elif gate.shape == f.shape[:-1] + (1,):
-            spec.gate_form = _lib.GATE_TOKEN
+        gates, at = _row_kind(gate.dtype, "the gate"), gate.shape
+        if at == row:
+            form = _lib.GATE_CHANNEL
+        elif at == shape:
+            form = _lib.GATE_FULL
+        elif at == shape[:-1] + (1,):
+            form = _lib.GATE_TOKEN
         else:
-            raise ValueError(f"a gate must be [{d}], {tuple(f.shape[:-1] + (1,))} or {tuple(f.shape)}, got {tuple(gate.shape)}")
+            raise ValueError(f"a gate must be [{d}], {tuple(shape[:-1] + (1,))} or {tuple(shape)}, got {tuple(at)}")
         gate = _packed16(gate)
-    spec.post_w_dev, spec.pre_w_dev, spec.gate_dev = ptr(post_w), ptr(pre_w), ptr(gate)
-    return spec, (post_w, pre_w, gate)
+        g = gate.data_ptr()
+    return _BLOCK_NORM_SPEC.pack(a, b, g, rows, held, weights, gates, form), form, (post_w, pre_w, gate)
 
 
 def block_norm(f: torch.Tensor, h: torch.Tensor, post_w: torch.Tensor | None = None, gate: torch.Tensor | None = None,
@@ -1089,16 +1120,15 @@ def block_norm(f: torch.Tensor, h: torch.Tensor, post_w: torch.Tensor | None = N
     -> (h', n): h' of h's dtype, n of f's, of the rounded h'.  gate: [D], [..., 1] or
     [..., D].  Every tensor bf16 or fp32; D a multiple of 8 up to 16384."""
     dev = require_cuda(f, h, post_w, gate, pre_w)
-    if h.shape != f.shape:
-        raise ValueError(f"the stream {tuple(h.shape)} does not match f {tuple(f.shape)}")
-    spec, keep = _block_norm_spec(f, h.dtype, post_w, gate, pre_w)
-    d = f.shape[-1]
+    shape = f.shape
+    if h.shape != shape:
+        raise ValueError(f"the stream {tuple(h.shape)} does not match f {tuple(shape)}")
+    spec, _, keep = _block_norm_spec(f, h.dtype, post_w, gate, pre_w)
+    d = shape[-1]
     f, h = _packed16(f), _packed16(h)
-    out = torch.empty(f.shape, dtype=h.dtype, device=dev)
-    n = None if pre_w is None else torch.empty(f.shape, dtype=f.dtype, device=dev)
-    with _on(dev):
-        check(lib().hsmoe_block_norm(ptr(f), ptr(h), f.numel() // d, d, ctypes.addressof(spec), scale, eps, ptr(out), ptr(n),
-                                     stream_ptr(dev)), "hsmoe_block_norm")
+    out = torch.empty_like(h)
+    n = None if pre_w is None else torch.empty_like(f)
+    _run(dev, lib().hsmoe_block_norm, f.data_ptr(), h.data_ptr(), f.numel() // d, d, spec, scale, eps, out.data_ptr(), ptr(n))
     return out, n
 
 
@@ -1120,33 +1150,33 @@ def block_norm_grad(d_h: torch.Tensor | None, d_n: torch.Tensor | None, f: torch
     the norms' weights and a gate that is broadcast in fp32 (hsmoe_block_norm_grad).
     need: which of them."""
     dev = require_cuda(d_h, d_n, f, h_out, post_w, gate, pre_w)
-    spec, keep = _block_norm_spec(f, h_out.dtype, post_w, gate, pre_w)
+    spec, form, keep = _block_norm_spec(f, h_out.dtype, post_w, gate, pre_w)
+    shape = f.shape
     for t, what, dtype in ((h_out, "h_out", h_out.dtype), (d_h, "d_h", h_out.dtype), (d_n, "d_n", f.dtype)):
-        if t is not None and (t.shape != f.shape or t.dtype != dtype):
-            raise ValueError(f"{what} must be {tuple(f.shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
+        if t is not None and (t.shape != shape or t.dtype != dtype):
+            raise ValueError(f"{what} must be {tuple(shape)} in {dtype}, got {tuple(t.shape)} in {t.dtype}")
     if d_n is not None and pre_w is None:
         raise ValueError("d_n goes with pre_w")
     if d_h is None and d_n is None:
         raise ValueError("the gradient of neither result is given")
-    d = f.shape[-1]
+    d = shape[-1]
     m = f.numel() // d
     f, h_out = _packed16(f), _packed16(h_out)
     d_h, d_n = (None if t is None else _packed16(t) for t in (d_h, d_n))
     new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev)
-    d_f = new(f.shape, f.dtype) if need[0] else None
-    d_x = new(f.shape, h_out.dtype) if need[1] else None
+    d_f = torch.empty_like(f) if need[0] else None
+    d_x = torch.empty_like(h_out) if need[1] else None
     d_post = new((d,), torch.float32) if need[2] and post_w is not None else None
     d_gate = None
     if need[3] and gate is not None:
-        d_gate = new(gate.shape, gate.dtype if spec.gate_form == _lib.GATE_FULL else torch.float32)
+        d_gate = new(gate.shape, gate.dtype if form == _lib.GATE_FULL else torch.float32)
     d_pre = new((d,), torch.float32) if need[4] and pre_w is not None else None
-    with _on(dev):
-        sums = d_post is not None or d_pre is not None or (d_gate is not None and spec.gate_form == _lib.GATE_CHANNEL)
-        nbytes = lib().hsmoe_block_norm_grad_workspace_size(m, d) if sums else 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
-        check(lib().hsmoe_block_norm_grad(ptr(d_h), ptr(d_n), ptr(f), ptr(h_out), m, d, ctypes.addressof(spec), scale, eps,
-                                          ptr(d_f), ptr(d_x), ptr(d_post), ptr(d_gate), ptr(d_pre), ptr(ws), nbytes,
-                                          stream_ptr(dev)), "hsmoe_block_norm_grad")
+    L = lib()
+    sums = d_post is not None or d_pre is not None or (d_gate is not None and form == _lib.GATE_CHANNEL)
+    nbytes = L.hsmoe_block_norm_grad_workspace_size(m, d) if sums else 0
+    ws = _space(dev, nbytes)
+    _run(dev, L.hsmoe_block_norm_grad, ptr(d_h), ptr(d_n), f.data_ptr(), h_out.data_ptr(), m, d, spec, scale, eps, ptr(d_f), ptr(d_x),
+         ptr(d_post), ptr(d_gate), ptr(d_pre), ptr(ws), nbytes)
     return BlockNormGrad(d_f, d_x, d_post, d_gate, d_pre)
 
 
@@ -1178,13 +1208,17 @@ def embed_add_rms_norm(ids: torch.Tensor, table: torch.Tensor, weight: torch.Ten
     return h.reshape(shape), out.reshape(shape)
 
 
+_ID_KINDS = {torch.int64: _lib.IDS_I64, torch.int32: _lib.IDS_I32}
+
+
 def _token_ids(ids: torch.Tensor) -> tuple[torch.Tensor, int]:
     """ids, contiguous int32 or int64, and their kind."""
-    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
-        raise TypeError(f"ids must be integers, got {ids.dtype}")
-    if ids.dtype != torch.int32:
-        ids = ids.to(torch.int64)
-    return ids.contiguous(), _lib.IDS_I32 if ids.dtype == torch.int32 else _lib.IDS_I64
+    kind = _ID_KINDS.get(ids.dtype)
+    if kind is None:
+        if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+            raise TypeError(f"ids must be integers, got {ids.dtype}")
+        ids, kind = ids.to(torch.int64), _lib.IDS_I64
+    return ids.contiguous(), kind
 
 
 def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out_dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -1192,19 +1226,21 @@ def embed(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out_dtype:
     bf16 or fp32 -> [*ids.shape, D] of out_dtype (the table's when None); an id outside
     [0, V) gives a row of zeros, as in embed_add_rms_norm."""
     dev = require_cuda(ids, table)
-    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
-        raise ValueError(f"the embedding table must be [V, D], got {tuple(table.shape)}")
+    shape = table.shape
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+        raise ValueError(f"the embedding table must be [V, D], got {tuple(shape)}")
     kind = _row_kind(table.dtype, "the embedding table")
     out_kind = kind if out_dtype is None else _row_kind(out_dtype, "the output")
-    vocab, d = table.shape
-    if (d > 1 and table.stride(1) != 1) or (vocab > 1 and table.stride(0) < d):
-        table = table.contiguous()
-    lead = ids.shape
+    vocab, d = shape
+    ld = d
+    if not table.is_contiguous():
+        ld = max(table.stride(0), d)
+        if (d > 1 and table.stride(1) != 1) or (vocab > 1 and table.stride(0) < d):
+            table, ld = table.contiguous(), d
+    out = torch.empty(ids.shape + (d,), dtype=table.dtype if out_dtype is None else out_dtype, device=dev)
     ids, id_kind = _token_ids(ids)
-    out = torch.empty(lead + (d,), dtype=table.dtype if out_dtype is None else out_dtype, device=dev)
-    with _on(dev):
-        check(lib().hsmoe_embed(ptr(ids), id_kind, ids.numel(), ptr(table), max(table.stride(0), d), kind, vocab, d, scale,
-                                out_kind, ptr(out), stream_ptr(dev)), "hsmoe_embed")
+    _run(dev, lib().hsmoe_embed, ids.data_ptr(), id_kind, ids.numel(), table.data_ptr(), ld, kind, vocab, d, scale, out_kind,
+         out.data_ptr())
     return out
 
 
@@ -1236,12 +1272,11 @@ def embed_grad(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float 
         d_out = d_out.contiguous()
     ids, id_kind = _token_ids(ids)
     m = ids.numel()
-    with _on(dev):
-        nbytes = lib().hsmoe_embed_grad_workspace_size(m, d)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None  # the call's own, as in moe_sort
-        check(lib().hsmoe_embed_grad(ptr(d_out), max(d_out.stride(0), d), kind, ptr(ids), id_kind, m, vocab, d, scale,
-                                     0 if out is None else 1, ptr(table), max(table.stride(0), d), out_kind, ptr(ws), nbytes,
-                                     stream_ptr(dev)), "hsmoe_embed_grad")
+    L = lib()
+    nbytes = L.hsmoe_embed_grad_workspace_size(m, d)
+    ws = _space(dev, nbytes)
+    _run(dev, L.hsmoe_embed_grad, d_out.data_ptr(), max(d_out.stride(0), d), kind, ids.data_ptr(), id_kind, m, vocab, d, scale,
+         0 if out is None else 1, table.data_ptr(), max(table.stride(0), d), out_kind, ptr(ws), nbytes)
     if out is not None:
         _written(out)
     return table
