@@ -96,40 +96,43 @@ struct QuantParams {
   int64_t row_blocks; // dealt words: blocks of 32 rows (0: rows of scales)
 };
 
-// Waves take units of 512 values, four at a time: eight values per lane, 16 bytes
-// in (bf16), 4 out, whole lines both ways.  HBM-bound.
-constexpr int kQuantUnits = 4;
-template <int kKind>
-__device__ __forceinline__ void quant_units(const QuantParams& p, int64_t wave, int lane) {
-  const int64_t u0 = wave * kQuantUnits, total = p.m * p.units;
-  Eight x[kQuantUnits];
-  int64_t row[kQuantUnits], seg[kQuantUnits];
+// A wave takes 512 values of kRows rows: eight values per lane, 16 bytes in (bf16), 4
+// out, whole lines both ways.  HBM-bound; one row per wave where few rows would leave
+// the chip idle.
+template <int kKind, int kRows>
+__device__ __forceinline__ void quant_rows(const QuantParams& p, int64_t row0, int seg, int lane) {
+  if (row0 >= p.m) return;
+  const int64_t at = (int64_t)seg * kUnit + lane * 8;
+  const int rows = p.m - row0 < kRows ? (int)(p.m - row0) : kRows;
+  Eight x[kRows];
 #pragma unroll
-  for (int i = 0; i < kQuantUnits; ++i) {
-    row[i] = (u0 + i) / p.units, seg[i] = (u0 + i) % p.units;
+  for (int i = 0; i < kRows; ++i) {
     x[i] = Eight{};
-    const int64_t at = seg[i] * kUnit + lane * 8;
-    if (u0 + i < total && at < p.k) x[i] = load_eight<kKind>(p.x + row[i] * p.ldx + at * (kKind == kRowsBf16 ? 2 : 4));
+    if (i < rows && at < p.k) x[i] = load_eight<kKind>(p.x + (row0 + i) * p.ldx + at * (kKind == kRowsBf16 ? 2 : 4));
   }
+  uint32_t words[kRows];
+  const int64_t group = (int64_t)seg * 4 + (lane >> 4);  // of four blocks
 #pragma unroll
-  for (int i = 0; i < kQuantUnits; ++i) {
-    if (u0 + i >= total) return;
-    const int64_t at = seg[i] * kUnit + lane * 8;
+  for (int i = 0; i < kRows; ++i) {
     uint32_t e;
     const uint32_t w = quantise8(x[i], e);
-    if (at < p.k) *reinterpret_cast<uint32_t*>(p.codes + row[i] * (p.k / 2) + at / 2) = w;
+    if (i < rows && at < p.k) *reinterpret_cast<uint32_t*>(p.codes + (row0 + i) * (p.k / 2) + at / 2) = w;
     if (at >= p.k) e = 0;  // padding of the words
-    const uint32_t word = gather_exponents(e, lane);
-    const int64_t group = seg[i] * 4 + (lane >> 4);  // of four blocks
-    if (p.row_blocks) {
-      if ((lane & 15) == 0)
-        reinterpret_cast<uint32_t*>(p.scale)[dealt_word(group >> 1, row[i], (int)(group & 1), p.row_blocks)] = word;
-    } else if (p.ld_scale % 4 == 0) {
-      if ((lane & 15) == 0 && group * 4 < p.ld_scale)
-        *reinterpret_cast<uint32_t*>(p.scale + row[i] * p.ld_scale + group * 4) = word;
+    words[i] = gather_exponents(e, lane);
+    if (p.row_blocks || i >= rows) continue;
+    uint8_t* to = p.scale + (row0 + i) * p.ld_scale;
+    if (p.ld_scale % 4 == 0) {
+      if ((lane & 15) == 0 && group * 4 < p.ld_scale) *reinterpret_cast<uint32_t*>(to + group * 4) = words[i];
     } else if ((lane & 3) == 0 && at < p.k) {
-      p.scale[row[i] * p.ld_scale + at / 32] = (uint8_t)e;
+      to[at / 32] = (uint8_t)e;
     }
+  }
+  if (p.row_blocks && (lane & 15) == 0) {  // (rows beyond the last have words too)
+    uint32_t* to = reinterpret_cast<uint32_t*>(p.scale) + dealt_word(group >> 1, row0, (int)(group & 1), p.row_blocks);
+    if constexpr (kRows == 4)
+      *reinterpret_cast<uint4*>(to) = make_uint4(words[0], words[1], words[2], words[3]);
+    else
+      to[0] = words[0];
   }
 }
 
@@ -159,23 +162,26 @@ __device__ __forceinline__ void deal_scales(const DealParams& p, int64_t t) {
 }
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantBlock = kQuantThreads / 64 * kQuantUnits;  // units per workgroup
+constexpr int kQuantWaves = kQuantThreads / 64;
 
-template <int kKind>
+// Workgroups (rows, segment of 512 values).
+template <int kKind, int kRows>
 __global__ void __launch_bounds__(kQuantThreads) fp4_quant_kernel(QuantParams p) {
-  quant_units<kKind>(p, (int64_t)blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
+  quant_rows<kKind, kRows>(p, ((int64_t)blockIdx.x * kQuantWaves + (threadIdx.x >> 6)) * kRows, blockIdx.y, threadIdx.x & 63);
 }
 
 // What a product wants before it: x quantised (kKind < 0: its scales dealt) by the
-// first `quant_blocks` workgroups, the weights' scales dealt by the others.
-template <int kKind>
-__global__ void __launch_bounds__(kQuantThreads) fp4_ready_kernel(QuantParams q, DealParams x, DealParams w, int64_t first_blocks) {
-  if ((int64_t)blockIdx.x >= first_blocks)
-    deal_scales(w, ((int64_t)blockIdx.x - first_blocks) * kQuantThreads + threadIdx.x);
-  else if constexpr (kKind < 0)
+// first `first_blocks` workgroups, the weights' scales dealt by the others.
+template <int kKind, int kRows>
+__global__ void __launch_bounds__(kQuantThreads) fp4_ready_kernel(QuantParams q, DealParams x, DealParams w, uint32_t first_blocks) {
+  if (blockIdx.x >= first_blocks) {
+    deal_scales(w, (int64_t)(blockIdx.x - first_blocks) * kQuantThreads + threadIdx.x);
+  } else if constexpr (kKind < 0) {
     deal_scales(x, (int64_t)blockIdx.x * kQuantThreads + threadIdx.x);
-  else
-    quant_units<kKind>(q, (int64_t)blockIdx.x * (kQuantThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
+  } else {
+    const uint32_t units = (uint32_t)q.units, r = blockIdx.x / units;
+    quant_rows<kKind, kRows>(q, ((int64_t)r * kQuantWaves + (threadIdx.x >> 6)) * kRows, (int)(blockIdx.x - r * units), threadIdx.x & 63);
+  }
 }
 
 // ---------------------------------------------------------------- tiles
@@ -323,6 +329,9 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
     // into its place; a stage's loads have two turns at least before they are
     // waited for at the end of the last.
     const bool second = wave >= 4;
+    // (a wave without rows in the tile only keeps the turns; the branch also keeps the
+    // products between the barriers, where the compiler would move them behind the last)
+    const bool live = rows > wr * T::kFR * 32;
     i32x4 r[2][T::kFR], c[2][T::kFC];
     auto turn = [&](bool loads) {  // ends a turn; loads: what the wave loads of the next stage is in LDS
       if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -343,16 +352,14 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
       if (s + 1 < steps) load(s + 1, (s + 1) & 1);
       turn(false);
       __builtin_amdgcn_s_setprio(1);
-      multiply(k0, r[0], c[0]);
-      multiply(k1, r[1], c[1]);
+      if (live) multiply(k0, r[0], c[0]), multiply(k1, r[1], c[1]);
       __builtin_amdgcn_s_setprio(0);
       turn(false);
       read(stage, 2, r[0], c[0]);
       read(stage, 3, r[1], c[1]);
       turn(second);
       __builtin_amdgcn_s_setprio(1);
-      multiply(k2, r[0], c[0]);
-      multiply(k3, r[1], c[1]);
+      if (live) multiply(k2, r[0], c[0]), multiply(k3, r[1], c[1]);
       __builtin_amdgcn_s_setprio(0);
       turn(!second);
     }
@@ -549,6 +556,24 @@ __global__ void __launch_bounds__(256) fp4_few_kernel(Fp4Params p, const char* x
 // ---------------------------------------------------------------- host
 constexpr int64_t kFewRows = 64;
 
+// Rows per wave and workgroups along the rows of a quantisation.
+bool four_rows(int64_t m, int64_t units) { return m * units >= 8192; }
+int64_t quant_groups(int64_t m, int64_t units) {
+  const int64_t rows = kQuantWaves * (four_rows(m, units) ? 4 : 1);
+  return (m + rows - 1) / rows;
+}
+void launch_quant(const QuantParams& q, bool bf16, hipStream_t st) {
+  const dim3 grid((unsigned)quant_groups(q.m, q.units), (unsigned)q.units), block(kQuantThreads);
+  if (bf16 && four_rows(q.m, q.units))
+    hipLaunchKernelGGL((fp4_quant_kernel<kRowsBf16, 4>), grid, block, 0, st, q);
+  else if (bf16)
+    hipLaunchKernelGGL((fp4_quant_kernel<kRowsBf16, 1>), grid, block, 0, st, q);
+  else if (four_rows(q.m, q.units))
+    hipLaunchKernelGGL((fp4_quant_kernel<kRowsF32, 4>), grid, block, 0, st, q);
+  else
+    hipLaunchKernelGGL((fp4_quant_kernel<kRowsF32, 1>), grid, block, 0, st, q);
+}
+
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 // What a product does and where its workspace keeps what.
@@ -624,13 +649,7 @@ extern "C" int hsmoe_fp4_quant(const void* x, int64_t x_row_stride, int row_kind
   q.x = (const char*)x, q.codes = (char*)codes, q.scale = (uint8_t*)scale;
   q.m = m, q.k = k, q.ldx = x_row_stride * (row_kind == HSMOE_OUT_BF16 ? 2 : 4), q.ld_scale = k / 32;
   q.units = (k + kUnit - 1) / kUnit;
-  const int64_t grid = (m * q.units + kQuantBlock - 1) / kQuantBlock;
-  if (grid >= (1ll << 31)) return fail(HSMOE_ERR_SHAPE, "hsmoe_fp4_quant: more than 2^44 values");
-  hipStream_t st = (hipStream_t)stream;
-  if (row_kind == HSMOE_OUT_BF16)
-    hipLaunchKernelGGL((fp4_quant_kernel<kRowsBf16>), dim3((unsigned)grid), dim3(kQuantThreads), 0, st, q);
-  else
-    hipLaunchKernelGGL((fp4_quant_kernel<kRowsF32>), dim3((unsigned)grid), dim3(kQuantThreads), 0, st, q);
+  launch_quant(q, row_kind == HSMOE_OUT_BF16, (hipStream_t)stream);
   return check_launch("hsmoe_fp4_quant");
 }
 
@@ -683,17 +702,12 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   dx = dw;
   dx.scale = (const uint8_t*)x_scale, dx.words = (uint32_t*)(mem + plan.xs), dx.rows = m, dx.row_blocks = (m + 31) / 32;
   auto deal_blocks = [&](const DealParams& d) { return (d.row_blocks * 32 * d.groups + kQuantThreads - 1) / kQuantThreads; };
-  const int64_t quant_blocks = (m * q.units + kQuantBlock - 1) / kQuantBlock;
   if (plan.few) {
     p.xs = (const uint8_t*)q.scale, p.ld_xs = q.ld_scale;
-    const dim3 grid((unsigned)quant_blocks), block(kQuantThreads);
-    if (packed) {
+    if (packed)
       p.xs = (const uint8_t*)x_scale, p.ld_xs = k / 32;
-    } else if (x_kind == HSMOE_OUT_BF16) {
-      hipLaunchKernelGGL((fp4_quant_kernel<kRowsBf16>), grid, block, 0, st, q);
-    } else {
-      hipLaunchKernelGGL((fp4_quant_kernel<kRowsF32>), grid, block, 0, st, q);
-    }
+    else
+      launch_quant(q, x_kind == HSMOE_OUT_BF16, st);
     if (m <= 16)
       launch_few<1, -1>(p, nullptr, 0, st);
     else if (m <= 32)
@@ -706,16 +720,14 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   }
   p.words = mem + plan.xs, p.x_words = 0, p.w_words = (uint32_t)(plan.ws - plan.xs);
   p.words_bytes = (uint32_t)(plan.bytes - plan.xs);
-  const int64_t first = packed ? deal_blocks(dx) : quant_blocks;
+  const int64_t first = packed ? deal_blocks(dx) : quant_groups(m, q.units) * q.units;
   const int64_t all = first + deal_blocks(dw);
   if (all >= (1ll << 31)) return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
-  const dim3 grid((unsigned)all), block(kQuantThreads);
-  if (packed)
-    hipLaunchKernelGGL((fp4_ready_kernel<-1>), grid, block, 0, st, q, dx, dw, first);
-  else if (x_kind == HSMOE_OUT_BF16)
-    hipLaunchKernelGGL((fp4_ready_kernel<kRowsBf16>), grid, block, 0, st, q, dx, dw, first);
-  else
-    hipLaunchKernelGGL((fp4_ready_kernel<kRowsF32>), grid, block, 0, st, q, dx, dw, first);
+  auto ready = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kQuantThreads), 0, st, q, dx, dw, (uint32_t)first); };
+  const bool bf16 = x_kind == HSMOE_OUT_BF16, four = four_rows(m, q.units);
+  if (packed) ready(fp4_ready_kernel<-1, 1>);
+  else if (bf16) four ? ready(fp4_ready_kernel<kRowsBf16, 4>) : ready(fp4_ready_kernel<kRowsBf16, 1>);
+  else four ? ready(fp4_ready_kernel<kRowsF32, 4>) : ready(fp4_ready_kernel<kRowsF32, 1>);
   if (plan.tile == 0)
     launch_tile<256, 256, 2, 4, 0>(p, st);
   else if (plan.tile == 1)
