@@ -554,6 +554,8 @@ __global__ void __launch_bounds__(256) fp4_few_kernel(Fp4Params p, const char* x
 }
 
 // ---------------------------------------------------------------- host
+// Rows up to which fp4_few_kernel is taken: 33 of them by 4096 x 4096 take 8.9 us with
+// it and 11.1 with tiles, 48 9.4 and 11.0, 64 10.8 and 11.1.
 constexpr int64_t kFewRows = 64;
 
 // Rows per wave and workgroups along the rows of a quantisation.
@@ -596,9 +598,18 @@ Fp4Plan plan_fp4(int64_t m, int64_t n, int64_t k, bool packed) {
     p.ws = p.xs + stages * ((m + 31) / 32) * 256;
     p.bytes = p.ws + stages * ((n + 31) / 32) * 256;
   }
-  auto tiles = [&](int64_t s) { return ((m + s - 1) / s) * ((n + s - 1) / s); };
-  const int cus = device_cus();
-  p.tile = tiles(256) >= cus ? 0 : tiles(128) >= cus ? 1 : 2;
+  // The tile by estimated time: us for k = 4096 on 256 CUs, from the rounds of tiles
+  // that a CU takes (measured, with 4096 columns: 64 x 64 tiles 9 us for a round, 12 for
+  // two at once, then 5 more each; 128 x 128 18, then 10 more each; 256 x 256 36 each.  700
+  // rows: 19, 16 and 30 us; 4096 rows: 76, 46 and 40; 6000 rows: 113, 66 and 72).  Short
+  // reductions keep the order (k = 512, 4096 rows: 31, 19 and 17 us with the quantisation).
+  auto rounds = [&](int64_t s) {
+    const int64_t cus = device_cus();
+    return (((m + s - 1) / s) * ((n + s - 1) / s) + cus - 1) / cus;
+  };
+  const int64_t r64 = rounds(64), r128 = rounds(128), r256 = rounds(256);
+  const double t64 = r64 <= 2 ? 6.5 + 2.6 * r64 : 3.0 + 5.0 * r64, t128 = 7.0 + 9.8 * r128, t256 = 3.0 + 36.0 * r256;
+  p.tile = t256 <= t128 && t256 <= t64 ? 0 : t128 <= t64 ? 1 : 2;
   return p;
 }
 

@@ -119,17 +119,15 @@ class HbmExpertStore:
         """Device uint64 [n_experts, 6] address table of a layer (cached)."""
         t = self._tables.get(layer)
         if t is None:
-            base = self.buf.data_ptr() + layer * self.n_experts * self.expert_bytes
-            rows = []
-            for e in range(self.n_experts):
-                b = base + e * self.expert_bytes
-                if (layer, e) in self._absent:
-                    rows.append([0] * 6)
-                else:
-                    rows.append([b + self._off[n] for n in ("w1", "s1", "w3", "s3", "w2", "s2")])
-            t = torch.tensor(rows, dtype=torch.int64).to(self.device)
+            t = torch.tensor([self._table_row(layer, e) for e in range(self.n_experts)], dtype=torch.int64).to(self.device)
             self._tables[layer] = t
         return t
+
+    def _table_row(self, layer: int, eid: int) -> list[int]:
+        if (layer, eid) in self._absent:
+            return [0] * 6
+        b = self.buf.data_ptr() + self._expert_base(layer, eid)
+        return [b + self._off[n] for n in ("w1", "s1", "w3", "s3", "w2", "s2")]
 
     def shared_entry(self, layer: int) -> torch.Tensor | None:
         if not self.has_shared(layer):
@@ -163,17 +161,23 @@ class HbmExpertStore:
     # ------------------------------------------------------------ fill
     def put_expert(self, layer: int, eid: int, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor) -> None:
         """Quantises an expert's weights (bf16 or fp32: w1, w3 [I, D], w2 [D, I], as autograd.moe_ffn
-        trains them) into its record (hsmoe_fp4_quant); an absent expert is there afterwards.
-        Graphs captured over the store read the new weights."""
+        trains them) into its record (hsmoe_fp4_quant), which is never absent afterwards.  The
+        record and the layer's table stay where they are: graphs captured over them read the new weights."""
         views = self.expert_views(layer, eid)
         for name, w, shape in (("w1", w1, (self.i, self.d)), ("w3", w3, (self.i, self.d)), ("w2", w2, (self.d, self.i))):
             if tuple(w.shape) != shape:
                 raise ValueError(f"{name} must be {list(shape)}, got {tuple(w.shape)}")
+            if w.dtype not in (torch.bfloat16, torch.float32):
+                raise TypeError(f"{name} must be bf16 or fp32, got {w.dtype}")
+            if w.device != self.buf.device:
+                raise ValueError(f"{name} is on {w.device}, the store on {self.buf.device}")
         for w, codes, scale in zip((w1, w3, w2), views[0::2], views[1::2]):
             ops.fp4_quant(w.detach(), out=(codes, scale))
         if (layer, eid) in self._absent:
             self._absent.discard((layer, eid))
-            self._tables.pop(layer, None)
+            t = self._tables.get(layer)
+            if t is not None:
+                t[eid].copy_(torch.tensor(self._table_row(layer, eid), dtype=torch.int64))
 
     def fill_synthetic(self, seed: int, layers=None) -> None:
         """Fills experts (and shared experts) with the seeded synthetic weights."""

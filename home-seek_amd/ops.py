@@ -304,9 +304,14 @@ def _run(dev: torch.device, fn, *args) -> None:
         check(rc, fn.__name__)
 
 
-def _space(dev: torch.device, nbytes: int) -> torch.Tensor | None:
-    """A workspace of the call's own, as in moe_sort."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _space(dev: torch.device, size, *args) -> tuple[torch.Tensor | None, int]:
+    """A workspace of the call's own, as in moe_sort, of size(*args) bytes (which may ask for the device's CUs)."""
+    if torch._C._cuda_getDevice() == dev.index:
+        nbytes = size(*args)
+    else:
+        with torch.cuda.device(dev.index):
+            nbytes = size(*args)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None), nbytes
 
 
 def _row_kind(dtype: torch.dtype, what: str) -> int:
@@ -676,8 +681,7 @@ def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
     at = lambda a: a.buffer_info()[0]
     norm = torch.empty((), dtype=torch.float32, device=dev)
     L = lib()
-    nbytes = L.hsmoe_grad_norm_workspace_size(n)
-    ws = _space(dev, nbytes)
+    ws, nbytes = _space(dev, L.hsmoe_grad_norm_workspace_size, n)
     if max_norm is None:
         _run(dev, L.hsmoe_grad_norm, n, at(ins), at(counts), at(kinds), norm_type, norm.data_ptr(), ws.data_ptr(), nbytes)
         return norm
@@ -794,8 +798,7 @@ def fp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, x_scale:
         m, kind, stride, scales = x.numel() // (k // 2), _lib.ROWS_FP4, 0, x_scale.data_ptr()
     out = torch.empty(shape[:-1] + (n,), dtype=out_dtype, device=dev)
     L = lib()
-    nbytes = L.hsmoe_fp4_linear_workspace_size(m, n, k, kind)
-    ws = _space(dev, nbytes)
+    ws, nbytes = _space(dev, L.hsmoe_fp4_linear_workspace_size, m, n, k, kind)
     _run(dev, L.hsmoe_fp4_linear, x.data_ptr(), kind, stride, scales, m, k, w.data_ptr(), w_scale.data_ptr(), n, out_kind,
          out.data_ptr(), ptr(ws), nbytes)
     return out
@@ -1173,8 +1176,7 @@ def block_norm_grad(d_h: torch.Tensor | None, d_n: torch.Tensor | None, f: torch
     d_pre = new((d,), torch.float32) if need[4] and pre_w is not None else None
     L = lib()
     sums = d_post is not None or d_pre is not None or (d_gate is not None and form == _lib.GATE_CHANNEL)
-    nbytes = L.hsmoe_block_norm_grad_workspace_size(m, d) if sums else 0
-    ws = _space(dev, nbytes)
+    ws, nbytes = _space(dev, L.hsmoe_block_norm_grad_workspace_size, m, d) if sums else (None, 0)
     _run(dev, L.hsmoe_block_norm_grad, ptr(d_h), ptr(d_n), f.data_ptr(), h_out.data_ptr(), m, d, spec, scale, eps, ptr(d_f), ptr(d_x),
          ptr(d_post), ptr(d_gate), ptr(d_pre), ptr(ws), nbytes)
     return BlockNormGrad(d_f, d_x, d_post, d_gate, d_pre)
@@ -1273,8 +1275,7 @@ def embed_grad(d_out: torch.Tensor, ids: torch.Tensor, vocab: int, scale: float 
     ids, id_kind = _token_ids(ids)
     m = ids.numel()
     L = lib()
-    nbytes = L.hsmoe_embed_grad_workspace_size(m, d)
-    ws = _space(dev, nbytes)
+    ws, nbytes = _space(dev, L.hsmoe_embed_grad_workspace_size, m, d)
     _run(dev, L.hsmoe_embed_grad, d_out.data_ptr(), max(d_out.stride(0), d), kind, ids.data_ptr(), id_kind, m, vocab, d, scale,
          0 if out is None else 1, table.data_ptr(), max(table.stride(0), d), out_kind, ptr(ws), nbytes)
     if out is not None:

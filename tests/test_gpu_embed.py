@@ -73,7 +73,7 @@ def test_lookup_and_gradient(dev, m, vocab, d, t):
         assert torch.equal(out[untouched], base[untouched])
 
 
-@pytest.mark.parametrize("m,vocab", ((16385, 1), (20000, 700), (50001, 129280), (40000, 3000000), (17000, 1 << 20), (17001, (1 << 20) + 1)))
+@pytest.mark.parametrize("m,vocab", ((16385, 1), (20000, 700), (65536, 5000), (65537, 5000), (70001, 1 << 20), (70000, (1 << 20) + 1), (66000, 1), (50001, 129280), (40000, 3000000), (17000, 1 << 20), (17001, (1 << 20) + 1)))
 def test_many_tokens(dev, m, vocab):
     ids, d_out = make_ids(dev, m, vocab, m, hot=0.4), normal(dev, 2, (m, 16))
     s, a, n = plain_grad(d_out, ids, vocab)
@@ -141,6 +141,9 @@ def test_shapes_strides_and_kinds_of_ids(dev):
     base = torch.zeros(50, 208, dtype=F32, device=dev)
     ops.embed_grad(d_out, ids, 50, out=base[:, 5:101])  # rows that are apart, not 16-byte aligned
     assert torch.equal(base[:, 5:101].to(BF16), g) and (base[:, :5] == 0).all() and (base[:, 101:] == 0).all()
+    far = torch.tensor([2 ** 32 + 3, -2 ** 40, 3, 2 ** 63 - 1], device=dev)  # beyond 32 bits: no row of the table
+    assert torch.equal(ops.embed(far, table), torch.where((far == 3)[:, None], table[3], 0))
+    assert torch.equal(ops.embed_grad(torch.ones(4, 96, device=dev), far, 50)[:, 0], (torch.arange(50, device=dev) == 3).float())
     assert ops.embed(ids[:0], table).shape == (0, 3, 4, 96)
     assert (ops.embed_grad(d_out[:0], ids[:0], 50) == 0).all()
     assert ops.embed(ids[0, 0, 0], table).shape == (96,)

@@ -171,17 +171,18 @@ def test_products(dev, m, n, k):
     check(ops.fp4_linear(xq32[0], *w, x_scale=xq32[1]), xq32, w, k, BF16)
 
 
-@pytest.mark.parametrize("m,n,k", ((2050, 2056, 96), (2049, 2040, 544), (4097, 4104, 320), (4090, 4000, 1024)))
+@pytest.mark.parametrize("m,n,k", ((2050, 2056, 96), (2049, 2040, 544), (4097, 4104, 320), (4090, 4000, 1024), (3900, 4008, 96), (4095, 4088, 544),
+                                   (7700, 4096, 32)))
 def test_products_of_large_tiles(dev, m, n, k):
     x, w = normal(dev, m, (m, k)), ops.fp4_quant(normal(dev, n, (n, k)))
     check(ops.fp4_linear(x, *w), ops.fp4_quant(x), w, k, BF16)
     check(ops.fp4_linear(x, *w, out_dtype=F32), ops.fp4_quant(x), w, k, F32)
 
 
-@pytest.mark.parametrize("m", (1, 20, 80, 2100))
+@pytest.mark.parametrize("m", (1, 20, 80, 2100, 4000))
 def test_far_exponents(dev, m):
     """Scales over the whole range: sums whose blocks are far apart, results that no output type holds."""
-    n, k = (2056 if m == 2100 else 64), 256
+    n, k = {2100: 2056, 4000: 4096}.get(m, 64), 256
     g = torch.Generator(device=dev).manual_seed(m)
     x = normal(dev, m, (m, k), F32) * torch.exp2(torch.randint(-10, 10, (m, k // 32, 1), generator=g, device=dev).expand(-1, -1, 32).reshape(m, k).float())
     wq = ops.fp4_quant(normal(dev, 9, (n, k)))

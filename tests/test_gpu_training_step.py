@@ -154,9 +154,13 @@ def test_step_clip_and_serve(dev):
     # back into the store, and served: the kernels of the 4-bit experts on what the codes stand for
     store = expert_store.HbmExpertStore(1, E, D, I, dev, with_shared=False)
     store.mark_absent(0, 3)
+    table = store.table(0)
+    assert (table[3] == 0).all() and (table[2] != 0).all()
     for e in range(E):
         store.put_expert(0, e, p["w10"][e], p["w30"][e], p["w20"][e])
-    assert store.has_expert(0, 3)
+    assert store.has_expert(0, 3) and store.table(0) is table and (table != 0).all()
+    fresh = expert_store.HbmExpertStore(1, E, D, I, dev, with_shared=False).table(0)
+    assert torch.equal(table - table[0, 0], fresh - fresh[0, 0])
     x = rnd(dev, 77, (M, D))
     got = ops.moe_prefill(x, idx, w, store.table(0), ops.SCALE_E8M0, None, 10.0, i=I)[0].double()
     held = [[ops.fp4_dequant_bf16(c, s) for c, s in zip(store.expert_views(0, e)[0::2], store.expert_views(0, e)[1::2])] for e in range(E)]
@@ -212,6 +216,9 @@ def test_what_autograd_is_told(dev):
 def test_put_expert_refuses_other_shapes(dev):
     store = expert_store.HbmExpertStore(1, 2, D, I, dev, with_shared=False)
     a, b = rnd(dev, 1, (I, D)), rnd(dev, 2, (D, I))
-    for bad, exc in (((0, 0, a, a, a), ValueError), ((0, 0, b, a, b), ValueError), ((0, 2, a, a, b), IndexError), ((0, 0, a.half(), a, b), TypeError)):
+    for bad, exc in (((0, 0, a, a, a), ValueError), ((0, 0, b, a, b), ValueError), ((0, 2, a, a, b), IndexError), ((0, 0, a, a, b.half()), TypeError),
+                     ((0, 0, a, a.cpu(), b), ValueError)):
+        store.expert_record(0, 0).fill_(7)
         with pytest.raises(exc):
             store.put_expert(*bad)
+        assert (store.expert_record(0, 0) == 7).all()  # nothing is written before everything is looked at
