@@ -666,9 +666,10 @@ def _clip(grads, max_norm: float | None, norm_type: float, out) -> torch.Tensor:
     for t in outs if max_norm is not None else ():
         _writable(t, "a gradient that is clipped")
     for g, o in zip(grads, outs):
-        if not g.is_contiguous() and not _dense(g):
+        plain = g.is_contiguous()
+        if not plain and not _dense(g):
             raise ValueError(f"gradients must fill their memory, got {tuple(g.shape)} with strides {g.stride()}")
-        if o is not g and (o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))):
+        if o is not g and (o.shape != g.shape or (not (plain and o.is_contiguous()) and o.stride() != g.stride())):
             raise ValueError(f"an output must have its gradient's shape and strides, got {tuple(o.shape)}, {o.stride()} for "
                              f"{tuple(g.shape)}, {g.stride()}")
     # addresses, counts and kinds, as the entry points read them
