@@ -6,7 +6,10 @@
 // workgroup leaves its part, and one that adds up the parts (in every workgroup, in
 // one order), and multiplies.  The second goes through the data backwards, so that
 // what the first read last comes out of the caches.  Tensors that are clipped in
-// place and need no clipping are not touched.
+// place and need no clipping are not touched.  Measured: 1.24 GB in 60 tensors, bf16 and
+// fp32, the norm 211 us (5.9 TB/s; reads alone reach 6.5), with the clipped copy 700; 6
+// tensors of 8064 values in all 7.6 us.  More workgroups, or fewer loads on their way,
+// change nothing.
 #include <algorithm>
 #include <cmath>
 #include <vector>

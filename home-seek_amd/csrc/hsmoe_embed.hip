@@ -5,8 +5,11 @@
 // in the order of the tokens, and cuts the sorted tokens into chunks of 32, so that
 // a word that makes up much of a batch is summed by many workgroups: a run of equal
 // ids inside a chunk is a row of the table; the ends of chunks that share a run leave
-// fp32 sums, which a second launch adds in their order.  All of it is bound by HBM:
-// the table's rows that are written, most of them zeros.
+// fp32 sums, which a second launch adds in their order.  All of it is bound by HBM.
+// Measured: 16381 tokens of 4096 bf16 looked up 37 us (5.0 TB/s: the copy's rate); the
+// gradient of a table of 129280 x 4096 230 us: the sort beside 1.06 GB of zeros 166,
+// places 7, sums 38, joins 8.  (Rows that no token names cleared beside the sums, by a
+// flag each, instead of all beside the sort: 235 to 243.)
 #include <algorithm>
 
 #include "hsmoe_common.h"
