@@ -256,7 +256,7 @@ __device__ __forceinline__ void apart() { asm volatile("" ::: "memory"); }
 // their order.
 template <int kLanes, int kC, int kMax, bool kF32, bool kS32, bool kW32>
 __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_norm_grad_kernel(BlockNormParams p) {
-  __shared__ float mem[2][5][16];
+  __shared__ float mem[2][3][16];
   __shared__ float sums[kLanes ? 256 * 8 * kC : 1];
   constexpr int kRows = kLanes ? 256 / (kLanes ? kLanes : 1) : 1;  // at a time
   const int threads = kLanes ? kLanes : (int)blockDim.x;
@@ -336,10 +336,11 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     row_sum<kLanes, 3>(s, mem[0], threads);
 #pragma unroll
     for (int c = 0; c < kC; ++c) unpack_later(r.f[c]), unpack_later(r.h[c]), unpack_later(r.dn[c]), unpack_later(wb[c]);
-    const float r1 = p.post_w ? inv_rms(s[0], p.per, p.eps) : 1.0f;
-    const float r2 = p.d_n ? inv_rms(s[1], p.per, p.eps) : 0.0f;
+    // (a row that is not there adds nothing to the sums, without eps either)
+    const float r1 = !live ? 0.0f : p.post_w ? inv_rms(s[0], p.per, p.eps) : 1.0f;
+    const float r2 = live && p.d_n ? inv_rms(s[1], p.per, p.eps) : 0.0f;
     const float m2 = s[2] * p.per * r2 * r2;  // r2^2 mean(g h')
-    float q[2] = {0.0f, 0.0f};                     // sum of post_w du f, and of dt u
+    float q[2] = {0.0f, 0.0f};                // sum of post_w du f, and of dt u
     V8 df[kC];
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
       const float m1 = p.post_w ? q[0] * p.per * r1 * r1 : 0.0f;
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 8; ++i) df[c].v[i] = r1 * __fmaf_rn(-r.f[c].at(i), m1, df[c].v[i]);
         write8<kF32>(rows_buf<kF32>(p.d_f, first, left, p.d), at[c], df[c]);
       }
@@ -388,9 +389,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
   auto leave = [&](const V8 (&a)[kC], float* to) {
     if (kLanes == 0) {
 #pragma unroll
-      for (int c = 0; c < kC; ++c) {
-        write8<true>(rows_buf<true>(to, 0, 1, p.d), wcol[c], a[c]);
-      }
+      for (int c = 0; c < kC; ++c) write8<true>(rows_buf<true>(to, 0, 1, p.d), wcol[c], a[c]);
     } else {  // the rows' groups in their order
       __syncthreads();
 #pragma unroll
@@ -401,7 +400,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
       if (mine == 0)
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
-            V8 v = {};
+          V8 v = {};
           for (int g = 0; g < kRows; ++g)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v.v[i] += sums[(g * kC + c) * 8 * threads + i * threads + t];

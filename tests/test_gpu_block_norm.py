@@ -178,6 +178,18 @@ def test_rows_of_zeros_infinities_and_nan_stay_rows(dev):
     assert torch.isfinite(g.f[rest]).all() and torch.isfinite(g.f[3:5]).all() and g.f[6].isnan().all()
 
 
+@pytest.mark.parametrize("m,d", ((33, 72), (5, 128), (9, 256), (3, 512), (3, 1024), (1, 64)))
+def test_without_eps(dev, m, d):
+    """Rows beyond the last of a group of rows are zeros to the kernels, and have no rms: they may not reach the sums."""
+    a = make(dev, m, d, BF16, BF16, BF16, "channel", True, True)
+    out, n = ops.block_norm(a["f"], a["h"], a["post_w"], a["gate"], 0.5, a["pre_w"], 0.0)
+    check_forward(a, out, n, 0.5, 0.0)
+    d_h, d_n = normal(dev, 1, (m, d)), normal(dev, 2, (m, d))
+    g = ops.block_norm_grad(d_h, d_n, a["f"], a["h"], a["post_w"], a["gate"], 0.5, a["pre_w"], 0.0)
+    assert all(torch.isfinite(x).all() for x in g)
+    check_grad(a, d_h, d_n, 0.5, 0.0, g)
+
+
 def test_shapes_strides_and_no_rows(dev):
     f, h = normal(dev, 1, (3, 4, 96))[:, :, 16:80], normal(dev, 2, (4, 3, 64), F32).transpose(0, 1)
     w = normal(dev, 3, (128,), BF16, 0.1, 1.0)[::2]
