@@ -209,13 +209,14 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise HsmoeError(f"tensor on {t.device} passed to a GPU kernel; the HIP path has no CPU fallback")
         at = t.get_device()
-        if index is None:
-            index = at
-        elif at != index:
+        if at == index:
+            continue
+        if at < 0 or not t.is_cuda:
+            raise HsmoeError(f"tensor on {t.device} passed to a GPU kernel; the HIP path has no CPU fallback")
+        if index is not None:
             raise HsmoeError(f"tensors on different devices (cuda:{index} and cuda:{at})")
+        index = at
     if index is None:
         raise HsmoeError("no device tensor given")
     dev = _devices.get(index)

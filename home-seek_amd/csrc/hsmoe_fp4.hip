@@ -600,17 +600,17 @@ Fp4Plan plan_fp4(int64_t m, int64_t n, int64_t k, bool packed) {
   p.xs = packed ? 0 : up(m * (k / 2), 256);
   if (p.few) {
     p.ws = p.bytes = packed ? 0 : p.xs + up(m * up(k / 32, 16), 256);
-  } else {
-    p.ws = p.xs + stages * ((m + 31) / 32) * 256;
-    p.bytes = p.ws + stages * ((n + 31) / 32) * 256;
+    return p;
   }
+  p.ws = p.xs + stages * ((m + 31) / 32) * 256;
+  p.bytes = p.ws + stages * ((n + 31) / 32) * 256;
   // The tile by estimated time: us for k = 4096 on 256 CUs, from the rounds of tiles
   // that a CU takes (measured, with 4096 columns: 64 x 64 tiles 9 us for a round, 12 for
   // two at once, then 5 more each; 128 x 128 18, then 10 more each; 256 x 256 36 each.  700
   // rows: 19, 16 and 30 us; 4096 rows: 76, 46 and 40; 6000 rows: 113, 66 and 72).  Short
   // reductions keep the order (k = 512, 4096 rows: 31, 19 and 17 us with the quantisation).
+  const int64_t cus = device_cus();
   auto rounds = [&](int64_t s) {
-    const int64_t cus = device_cus();
     return (((m + s - 1) / s) * ((n + s - 1) / s) + cus - 1) / cus;
   };
   const int64_t r64 = rounds(64), r128 = rounds(128), r256 = rounds(256);
