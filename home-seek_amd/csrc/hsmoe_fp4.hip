@@ -212,10 +212,9 @@ __device__ __forceinline__ f32x4 mfma16(i32x4 a, i32x4 b, f32x4 c, int sa, int s
 // v_mfma_scale_f32_32x32x64.  A stage is 256 values of both operands: [row][128 bytes] with a row's 16-byte chunk
 // c at place c ^ (row / 2 % 8), loaded straight to LDS, then the scales' words.
 // Instruction s takes chunk 4 h + s of a row in lanes of half h.  Measured, 256 x 256
-// tiles by eight waves: 8190 x 4096 x 4096 73 us, 3.7 PFLOP/s, the matrix cores busy 39%
-// of it; 43 us without the products, 59 without the loads.  A loop of these
+// tiles by eight waves: 8190 x 4096 x 4096 72 us, 3.8 PFLOP/s.  A loop of these
 // instructions alone makes 6.2 PFLOP/s of random codes and 8.9 of zeros, and this
-// kernel 3.8 and 4.8 at 8192^3: much of what is left is power.  Two stages without
+// kernel 3.9 and 5.0 at 8192^3: much of what is left is power.  Two stages without
 // turns, and four waves of 128 x 128 with the next operands read ahead, take as long.
 // kStages_ 0: two stages, eight waves in turns.
 template <int kBR, int kBC, int kWR, int kWC, int kStages_>
@@ -327,17 +326,19 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   constexpr std::integral_constant<int, 2> k2;
   constexpr std::integral_constant<int, 3> k3;
   if constexpr (T::kTurns) {
-    // Two waves share a SIMD (w and w + 4): one half's waves read half a stage's
-    // operands, and issue the next stage's loads, while the other half's multiply,
-    // with a barrier between the turns; the second half is one turn behind.  Both
-    // have read a stage when the first half starts on the next but one, which goes
-    // into its place; a stage's loads have two turns at least before they are
-    // waited for at the end of the last.
+    // Two waves share a SIMD (w and w + 4): one half's waves read a stage's operands
+    // while the other half's multiply, with a barrier between the turns; the second
+    // half is one turn behind.  The first half reads stage i in turn 2 i and multiplies in
+    // turn 2 i + 1, the second reads in 2 i + 1 and multiplies in 2 i + 2.  So stage i's
+    // place is free from turn 2 i + 2 on: each half issues its part of stage i + 2 in that
+    // turn and waits for it at the end of turn 2 i + 3, before anybody reads it.
+    // (Half a stage in a turn: 291 us for 282 at 8192^3.  Workgroups that go on to another
+    // tile, its first stage loaded during the last products: 281 to 285.)
     const bool second = wave >= 4;
     // (a wave without rows in the tile only keeps the turns; the branch also keeps the
     // products between the barriers, where the compiler would move them behind the last)
     const bool live = rows > wr * T::kFR * 32;
-    i32x4 r[2][T::kFR], c[2][T::kFC];
+    i32x4 r[4][T::kFR], c[4][T::kFC];
     auto turn = [&](bool loads) {  // ends a turn; loads: what the wave loads of the next stage is in LDS
       if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -348,23 +349,22 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
     };
     load(0, 0);
     turn(true);
-    if (second) turn(false);
+    if (second) {
+      if (steps > 1) load(1, 1);
+      turn(false);
+    }
     for (int s = 0; s < steps; ++s) {
       const char* stage = lds + (s & 1) * T::kStage;
       read_scales(stage);
       read(stage, 0, r[0], c[0]);
       read(stage, 1, r[1], c[1]);
-      if (s + 1 < steps) load(s + 1, (s + 1) & 1);
-      turn(false);
-      __builtin_amdgcn_s_setprio(1);
-      if (live) multiply(k0, r[0], c[0]), multiply(k1, r[1], c[1]);
-      __builtin_amdgcn_s_setprio(0);
-      turn(false);
-      read(stage, 2, r[0], c[0]);
-      read(stage, 3, r[1], c[1]);
+      read(stage, 2, r[2], c[2]);
+      read(stage, 3, r[3], c[3]);
+      if (!second && s + 1 < steps) load(s + 1, (s + 1) & 1);
       turn(second);
+      if (second && s + 2 < steps) load(s + 2, s & 1);
       __builtin_amdgcn_s_setprio(1);
-      if (live) multiply(k2, r[0], c[0]), multiply(k3, r[1], c[1]);
+      if (live) multiply(k0, r[0], c[0]), multiply(k1, r[1], c[1]), multiply(k2, r[2], c[2]), multiply(k3, r[3], c[3]);
       __builtin_amdgcn_s_setprio(0);
       turn(!second);
     }
