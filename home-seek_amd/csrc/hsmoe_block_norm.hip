@@ -15,6 +15,8 @@
 // per channel 46 us (5.8 TB/s), fp32 stream and a full gate 93 us (5.0 TB/s, the rate of
 // a large copy); the gradient 84 us and 5 for the join (4.5 TB/s), with an fp32 stream
 // 4.8 TB/s; three rows 3.9 us.
+#include <algorithm>
+
 #include "hsmoe_common.h"
 #include "hsmoe_internal.h"
 
@@ -459,7 +461,7 @@ Shape shape_of(int64_t d, bool grad) {
 // (each leaves a row of sums); else one per row group.
 int64_t grad_groups(int64_t m, const Shape& s, bool sums) {
   const int64_t all = (m + s.rows - 1) / s.rows, some = (s.chunks > 1 ? 1 : 2) * (int64_t)device_cus();
-  return sums && all > some ? some : all;
+  return sums && all > some ? some : std::min<int64_t>(all, 1 << 22);  // (workgroups go on to further rows)
 }
 
 template <bool kGrad, bool kF32, bool kS32, bool kW32>
@@ -539,6 +541,7 @@ extern "C" int hsmoe_block_norm(const void* f, const void* h, int64_t m, int64_t
   BlockNormParams p = params_of(m, d, scale, eps, spec);
   p.f = f, p.h = h, p.h_out = h_out, p.n_out = n_out;
   const Shape s = shape_of(d, false);
+  if (!grid_fits((m + s.rows - 1) / s.rows, s.threads)) return fail(HSMOE_ERR_SHAPE, "%s: too many rows of this width for one launch", who);
   launch_kinds<false>(s, (m + s.rows - 1) / s.rows, spec->row_kind == HSMOE_OUT_F32, spec->stream_kind == HSMOE_OUT_F32, p,
                       (hipStream_t)stream);
   return check_launch(who);

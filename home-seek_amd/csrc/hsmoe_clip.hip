@@ -298,7 +298,7 @@ int check_tensors(const char* who, const Tensors& t, double norm_type, float max
       return fail(HSMOE_ERR_ARG, "%s: bad arguments", who);
     if (t.counts[i] == 0) continue;
     if (!t.in[i] || (t.out && !t.out[i])) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
-    if (t.counts[i] >= (1ll << 40)) return fail(HSMOE_ERR_SHAPE, "%s: a tensor of 2^40 values and more", who);
+    if (t.counts[i] >= (1ll << 38)) return fail(HSMOE_ERR_SHAPE, "%s: a tensor of 2^38 values and more", who);
     if (!aligned(t.in[i], k == HSMOE_OUT_F32 ? 4 : 2) || (t.out && !aligned(t.out[i], o == HSMOE_OUT_F32 ? 4 : 2)))
       return fail(HSMOE_ERR_SHAPE, "%s: misaligned tensor", who);
     if (!t.out) continue;
@@ -324,15 +324,13 @@ Batch batch_of(const Tensors& t, int64_t& at) {
   for (; at < t.n && b.n < kPer; ++at) {
     const int64_t c = t.counts[at];
     if (c == 0) continue;
-    const uint64_t more = (uint64_t)((c + kChunk - 1) / kChunk);
-    if (chunks + more >= (1ull << 31) && b.n) break;
     const int j = b.n++;
     b.in[j] = t.in[at], b.out[j] = t.out ? t.out[at] : nullptr, b.count[j] = c;
     const bool f = t.kinds[at] == HSMOE_OUT_F32, o = t.out && t.out_kinds[at] == HSMOE_OUT_F32;
     b.flags[j] = (uint8_t)((f ? kInF32 : 0) | (o ? kOutF32 : 0) | (aligned(b.in[j], 16) ? kInVec : 0) | (aligned(b.out[j], 16) ? kOutVec : 0) |
                            (b.in[j] == b.out[j] && f == o ? kSame : 0));
     b.first[j] = (uint32_t)chunks;
-    chunks += more;
+    chunks += (uint64_t)((c + kChunk - 1) / kChunk);  // (kPer tensors of less than 2^38 values: below 2^31)
     b.first[b.n] = (uint32_t)chunks;
   }
   return b;

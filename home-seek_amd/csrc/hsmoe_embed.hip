@@ -488,6 +488,7 @@ extern "C" int hsmoe_embed(const void* ids, int id_kind, int64_t m, const void* 
   const bool vec = d % 8 == 0 && rows16(table, table_row_stride, table_kind) && rows16(out, d, out_kind);
   p.shift = shift_for(vec ? (d / 8 + 1) / 2 : (d + 1) / 2);
   const int64_t per = kThreads >> p.shift;
+  if (!grid_fits((m + per - 1) / per, kThreads)) return fail(HSMOE_ERR_SHAPE, "%s: too many rows of this width for one launch", who);
   const dim3 grid((unsigned)((m + per - 1) / per)), block(kThreads);
   hipStream_t st = (hipStream_t)stream;
   const bool f = table_kind == HSMOE_OUT_F32, o = out_kind == HSMOE_OUT_F32;
@@ -523,7 +524,17 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
   int *sorted_id = (int*)(mem + sp.ids), *token = (int*)(mem + sp.token);
   const int64_t bytes = add ? 0 : vocab * d * size_of(table_kind);
   const int64_t clears = (bytes + kClear * 16 - 1) / (kClear * 16);
-  if (clears >= (1ll << 31) - 128) return fail(HSMOE_ERR_SHAPE, "%s: a gradient of 2^45 bytes and more", who);
+  SumParams p{};
+  p.m = m, p.d = d, p.ld = table_row_stride, p.ld_out = d_row_stride, p.chunks = (m + kChunk - 1) / kChunk;
+  p.add = add, p.scale = scale;
+  const bool vec = d % 8 == 0 && rows16(d_out, d_row_stride, d_kind) && rows16(d_table, table_row_stride, table_kind);
+  const int64_t vectors = vec ? d / 8 : d, join_slabs = (vectors + 63) / 64;
+  p.shift = std::max(shift_for(vectors), 3);
+  p.slabs = (int)((vectors + (1ll << p.shift) - 1) >> p.shift);
+  // (all launches or none: those behind one that fails would take its places from what lies in the workspace)
+  if (!grid_fits(clears + kSortByRank / kSortThreads, kSortThreads) || !grid_fits(p.chunks * p.slabs, kThreads) ||
+      !grid_fits(p.chunks * join_slabs, kJoinThreads))
+    return fail(HSMOE_ERR_SHAPE, "%s: a gradient of 64 GiB, or too many tokens of this width, for one launch", who);
   if (m == 0) {
     if (!clears) return HSMOE_OK;
     hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)clears), dim3(kSortThreads), 0, st, (char*)d_table, bytes);
@@ -553,19 +564,12 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
     hipLaunchKernelGGL(embed_sorted_kernel, grid, block, 0, st, ids, wide, m, vocab, before, sorted_id);
     token = const_cast<int*>(before);
   }
-  SumParams p{};
   p.d_out = d_out, p.sorted_id = sorted_id, p.token = token, p.d_table = d_table, p.part = (float*)(mem + sp.part);
-  p.m = m, p.d = d, p.ld = table_row_stride, p.ld_out = d_row_stride, p.chunks = (m + kChunk - 1) / kChunk;
-  p.add = add, p.scale = scale;
-  const bool vec = d % 8 == 0 && rows16(d_out, d_row_stride, d_kind) && rows16(d_table, table_row_stride, table_kind);
-  const int64_t vectors = vec ? d / 8 : d;
-  p.shift = std::max(shift_for(vectors), 3);
-  p.slabs = (int)((vectors + (1ll << p.shift) - 1) >> p.shift);
   const bool f = d_kind == HSMOE_OUT_F32, o = table_kind == HSMOE_OUT_F32;
   if (vec) launch_grad<true, 8>(p, f, o, st);
   else launch_grad<true, 1>(p, f, o, st);
   if (p.chunks > 1) {
-    p.slabs = (int)((vectors + 63) / 64);
+    p.slabs = (int)join_slabs;
     if (vec) launch_grad<false, 8>(p, f, o, st);
     else launch_grad<false, 1>(p, f, o, st);
   }

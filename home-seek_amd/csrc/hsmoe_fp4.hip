@@ -662,6 +662,8 @@ extern "C" int hsmoe_fp4_quant(const void* x, int64_t x_row_stride, int row_kind
   if (!codes || !scale) return fail(HSMOE_ERR_ARG, "hsmoe_fp4_quant: null pointer");
   if (!aligned(codes, 4) || (k % 128 == 0 && !aligned(scale, 4)))
     return fail(HSMOE_ERR_SHAPE, "hsmoe_fp4_quant: codes and scales must be 4-byte aligned");
+  if (!grid_fits(quant_groups(m, (k + kUnit - 1) / kUnit), kQuantThreads))
+    return fail(HSMOE_ERR_SHAPE, "hsmoe_fp4_quant: too many rows for one launch");
   QuantParams q{};
   q.x = (const char*)x, q.codes = (char*)codes, q.scale = (uint8_t*)scale;
   q.m = m, q.k = k, q.ldx = x_row_stride * (row_kind == HSMOE_OUT_BF16 ? 2 : 4), q.ld_scale = k / 32;
@@ -690,6 +692,7 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   if (!aligned(w, 16) || !aligned(out, 16) || (k % 512 == 0 && (!aligned(w_scale, 16) || (packed && !aligned(x_scale, 16)))))
     return fail(HSMOE_ERR_SHAPE, "%s: operands must be 16-byte aligned", who);
   const Fp4Plan plan = plan_fp4(m, n, k, packed);
+  if (plan.few && !grid_fits((n + 15) / 16, 256)) return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
   if (!plan.few && (plan.bytes - plan.xs >= (1ll << 31) - 1024 || ((m + 63) / 64) * ((n + 63) / 64) >= (1ll << 30)))
     return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
   if (plan.bytes && (!workspace || workspace_bytes < (size_t)plan.bytes))
@@ -739,7 +742,7 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   p.words_bytes = (uint32_t)(plan.bytes - plan.xs);
   const int64_t first = packed ? deal_blocks(dx) : quant_groups(m, q.units) * q.units;
   const int64_t all = first + deal_blocks(dw);
-  if (all >= (1ll << 31)) return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
+  if (!grid_fits(all, kQuantThreads)) return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
   auto ready = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kQuantThreads), 0, st, q, dx, dw, (uint32_t)first); };
   const bool bf16 = x_kind == HSMOE_OUT_BF16, four = four_rows(m, q.units);
   if (packed) ready(fp4_ready_kernel<-1, 1>);

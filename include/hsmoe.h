@@ -569,8 +569,9 @@ int hsmoe_embed_add_rms_norm(const int64_t* ids_dev, int64_t rows, const void* t
  * tokens within chunks of 32 of them and of the chunks, rounded once: deterministic.
  * add 0: every row of d_table (table_row_stride = d) is written, those that no token
  * names with zeros; add 1: the sums are added to the rows that tokens name, the others are left.
- * m < 2^31 (2^24 for the gradient, 0 included), vocab < 2^30, d < 2^23; any d (rows
- * that are 16-byte aligned move in 16-byte vectors).  The workspace (any contents)
+ * m < 2^31 (2^24 for the gradient, 0 included), vocab < 2^30, d < 2^23, and what a
+ * launch holds: 2^24 - 1 rows of more than 2048 values (256 unaligned), a d_table below 64 GiB; any d
+ * (rows that are 16-byte aligned move in 16-byte vectors).  The workspace (any contents)
  * holds hsmoe_embed_grad_workspace_size bytes. */
 #define HSMOE_IDS_I32 0
 #define HSMOE_IDS_I64 1

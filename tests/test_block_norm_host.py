@@ -43,3 +43,7 @@ def test_gradient_rejects_bad_arguments():
         assert grad(**kw) == -2, kw
     need = _lib.lib().hsmoe_block_norm_grad_workspace_size(4, 64)
     assert need == 3 * 64 * 4 and grad(nws=need - 1) == -4 and grad(ws=None) == -4
+
+
+def test_refuses_what_one_launch_does_not_hold():
+    assert forward(m=1 << 24, d=4096) == -2 and forward(m=1 << 29, d=64) == -2

@@ -30,3 +30,12 @@ def test_gradient_rejects_bad_arguments():
     need = _lib.lib().hsmoe_embed_grad_workspace_size(4, 64)
     assert need >= 2 * 64 * 4 and grad(nws=need - 1) == -4 and grad(ws=None) == -4
     assert _lib.lib().hsmoe_embed_grad_workspace_size(0, 64) == 0 and grad(m=0, add=1, ws=None, nws=0, d_out=None, ids=None) == 0
+
+
+def test_refuses_what_one_launch_does_not_hold():
+    # threads of a launch are counted in 32 bits: 2^24 rows by workgroups of 256, 2^22 pieces of 16 KB by 1024
+    wide = dict(d=4096, ld=4096)
+    assert embed(m=1 << 24, **wide) == -2
+    for kw in (dict(vocab=1 << 23, **wide), dict(vocab=(1 << 23) - 1, **wide), dict(m=0, vocab=1 << 23, **wide),
+               dict(m=(1 << 24) - 1, add=1, d=65536, ld=65536, vocab=100)):
+        assert grad(**{"ldd": kw["d"], "nws": 1 << 60, **kw}) == -2, kw

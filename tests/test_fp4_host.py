@@ -35,3 +35,8 @@ def test_linear_rejects_bad_arguments():
     big = dict(m=500, n=2048, k=4096, ld=4096)
     assert need >= 500 * 2048 + 128 * 512 + 128 * 2048
     assert linear(**big, nwork=need - 1) == -4 and linear(**big, work=None) == -4 and linear(**big, work=A + 8) == -2
+
+
+def test_refuses_what_one_launch_does_not_hold():
+    assert quant(m=1 << 28, k=32, ld=32) == -2
+    assert linear(m=1, n=1 << 28, k=32, ld=32) == -2
