@@ -257,7 +257,7 @@ __device__ __forceinline__ void apart() { asm volatile("" ::: "memory"); }
 // its end, as one row of `part`, and a second kernel adds the workgroups' rows in
 // their order.
 template <int kLanes, int kC, int kMax, bool kF32, bool kS32, bool kW32>
-__global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_norm_grad_kernel(BlockNormParams p) {
+__global__ void __launch_bounds__(kMax, kMax >= 512 ? 4 : 2) block_norm_grad_kernel(BlockNormParams p) {
   __shared__ float mem[2][3][16];
   __shared__ float sums[kLanes ? 256 * 8 * kC : 1];
   constexpr int kRows = kLanes ? 256 / (kLanes ? kLanes : 1) : 1;  // at a time
@@ -276,29 +276,33 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     Raw8<kF32> f[kC], dn[kC];
     Raw8<kS32> h[kC], dh[kC];
   };
-  auto load = [&](int64_t first) {  // (zeros of what is not there)
+  auto load_at = [&](Row& r, int c, int64_t first) {  // (zeros of what is not there)
     const int64_t left = left_at(first);
+    r.f[c] = raw8<kF32>(rows_buf<kF32>(p.f, first, left, p.d), at[c]);
+    r.dh[c] = raw8<kS32>(rows_buf<kS32>(p.d_h, first, left, p.d), at[c]);
+    r.h[c] = raw8<kS32>(rows_buf<kS32>(p.d_n ? p.h : nullptr, first, left, p.d), at[c]);
+    r.dn[c] = raw8<kF32>(rows_buf<kF32>(p.d_n, first, left, p.d), at[c]);
+  };
+  auto load = [&](int64_t first) {
     Row r;
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
-      r.f[c] = raw8<kF32>(rows_buf<kF32>(p.f, first, left, p.d), at[c]);
-      r.dh[c] = raw8<kS32>(rows_buf<kS32>(p.d_h, first, left, p.d), at[c]);
-      r.h[c] = raw8<kS32>(rows_buf<kS32>(p.d_n ? p.h : nullptr, first, left, p.d), at[c]);
-      r.dn[c] = raw8<kF32>(rows_buf<kF32>(p.d_n, first, left, p.d), at[c]);
-    }
+    for (int c = 0; c < kC; ++c) load_at(r, c, first);
     return r;
   };
   const int64_t stride = (int64_t)gridDim.x * kRows;
   int64_t first = (int64_t)blockIdx.x * kRows;
-  // Rows of more than 4096: the weights are read again for every row (3.9 TB/s at
-  // 8192; beyond 8192 the sums do not fit the registers: 1.4 TB/s at 16384).  The next
-  // row is loaded ahead where several share a workgroup only: otherwise it costs the
-  // registers with which two workgroups share a CU, which hides more (fp32 rows of 4096:
-  // 129 us with, 85 without).
+  // Rows of more than 8192 (kLean): what is not summed is read again where it is needed,
+  // the row a second and third time, from the caches: kept, it spills (2048 x 16384 bf16
+  // 125 us, 3.2 TB/s, 283 with all of it kept; fp32 with a full gate 267, 4.0 TB/s, and
+  // 441).  The next row is loaded ahead where several share a workgroup only: otherwise
+  // it costs the registers with which two workgroups share a CU, which hides more (fp32
+  // rows of 4096: 129 us with, 85 without).
   constexpr bool kLean = kC > 1, kAhead = kLanes != 0;
   Row next;
   if (kAhead) next = load(first);
-  V8 a_pre[kC] = {}, a_post[kC] = {}, a_gate[kC] = {};
+  // (a_y: the rows' sums of dt y times what of the gate is a row's own; the norm's weight
+  // and a channel's gate are factors of the whole sum)
+  V8 a_pre[kC] = {}, a_y[kC] = {};
   Raw8<kW32> gate[kC], wa[kC], wb[kC];
   auto read_post = [&](int c) {
     gate[c] = p.gate_kind == kGateChannel ? weights8<kW32>(p.gate, 0, 1, p.d, wcol[c], p.gate_f32) : ones<kW32>();
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     const bool live = mine < left;
     Row r;
     if (kAhead) r = next, next = load(first + stride);
-    else r = load(first);
+    else if (!kLean) r = load(first);
     float token = 1.0f;
     if (p.gate_kind == kGateToken && live)
       token = p.gate_f32 ? ((const float*)p.gate)[first + mine] : bf16_bits_to_f32(((const uint16_t*)p.gate)[first + mine]);
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
-      if (kLean) apart(), read_pre(c);
+      if (kLean) apart(), load_at(r, c, first), read_pre(c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float f = r.f[c].at(i), h = r.h[c].at(i);
@@ -337,7 +341,8 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     }
     row_sum<kLanes, 3>(s, mem[0], threads);
 #pragma unroll
-    for (int c = 0; c < kC; ++c) unpack_later(r.f[c]), unpack_later(r.h[c]), unpack_later(r.dn[c]), unpack_later(wb[c]);
+    for (int c = 0; c < kC; ++c)
+      if (!kLean) unpack_later(r.f[c]), unpack_later(r.h[c]), unpack_later(r.dn[c]), unpack_later(wb[c]);
     // (a row that is not there adds nothing to the sums, without eps either)
     const float r1 = !live ? 0.0f : p.post_w ? inv_rms(s[0], p.per, p.eps) : 1.0f;
     const float r2 = live && p.d_n ? inv_rms(s[1], p.per, p.eps) : 0.0f;
@@ -348,7 +353,7 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     for (int c = 0; c < kC; ++c) {
       V8 dx, dg;
       if (kLean) {
-        apart(), read_pre(c), read_post(c);
+        apart(), load_at(r, c, first), read_pre(c), read_post(c);
         if (p.gate_kind == kGateFull) gate[c] = weights8<kW32>(p.gate, first, left, p.d, at[c], p.gate_f32);
       }
 #pragma unroll
@@ -360,11 +365,15 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
         const float y = f * r1;
         dg.v[i] = dt * (y * wa[c].at(i));
         const float du = dt * (token * gate[c].at(i));
-        a_gate[c].v[i] += dg.v[i];
-        a_post[c].v[i] = __fmaf_rn(du, y, a_post[c].v[i]);
+        a_y[c].v[i] = __fmaf_rn(p.gate_kind == kGateFull ? du : dt * token, y, a_y[c].v[i]);
         df[c].v[i] = du * wa[c].at(i);
         q[0] = __fmaf_rn(df[c].v[i], f, q[0]);
         q[1] += dg.v[i];
+      }
+      if (kLean) {  // (the sums are made here, not kept as their terms until the end of the row)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(a_pre[c].v[i]), "+v"(a_y[c].v[i]), "+v"(df[c].v[i]));
+        asm volatile("" : "+v"(q[0]), "+v"(q[1]));
       }
       if (p.d_x) write8<kS32>(rows_buf<kS32>(p.d_x, first, left, p.d), at[c], dx);
       if (p.gate_kind == kGateFull && p.d_gate) {
@@ -374,7 +383,10 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     }
     row_sum<kLanes, 2>(q, mem[1], threads);
 #pragma unroll
-    for (int c = 0; c < kC; ++c) unpack_later(r.f[c]);
+    for (int c = 0; c < kC; ++c) {
+      if (kLean) r.f[c] = raw8<kF32>(rows_buf<kF32>(p.f, first, left, p.d), at[c]);
+      unpack_later(r.f[c]);
+    }
     if (p.gate_kind == kGateToken && p.d_gate && live && t == 0) ((float*)p.d_gate)[first + mine] = q[1];
     if (p.d_f) {
       const float m1 = p.post_w ? q[0] * p.per * r1 * r1 : 0.0f;
@@ -411,8 +423,21 @@ __global__ void __launch_bounds__(kMax, kMax == 512 && kC == 1 ? 4 : 2) block_no
     }
   };
   if (p.sum_pre) leave(a_pre, out);
-  if (p.sum_post) leave(a_post, out + p.d);
-  if (p.sum_gate) leave(a_gate, out + 2 * p.d);
+  if (!p.sum_post && !p.sum_gate) return;
+  V8 v[kC];
+#pragma unroll
+  for (int c = 0; c < kC; ++c) {
+    if (kLean) read_post(c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[c].v[i] = a_y[c].v[i] * wa[c].at(i);
+  }
+  if (p.sum_gate) leave(v, out + 2 * p.d);
+  if (!p.sum_post) return;
+#pragma unroll
+  for (int c = 0; c < kC; ++c)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[c].v[i] = p.gate_kind == kGateChannel ? a_y[c].v[i] * gate[c].at(i) : a_y[c].v[i];
+  leave(v, out + p.d);
 }
 
 // Column sums of the workgroups' rows: 64 columns per workgroup, its 16 waves a
@@ -454,13 +479,13 @@ Shape shape_of(int64_t d, bool grad) {
   if (chunks <= 16) return {16, 256, 16, 1};
   if (chunks <= 32) return {32, 256, 8, 1};
   if (chunks <= 64) return {64, 256, 4, 1};
-  const int per = !grad ? 2 : chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4;
+  const int per = !grad || chunks > 1024 ? 2 : 1;
   return {0, ((chunks + per - 1) / per + 63) / 64 * 64, 1, per};
 }
 // Workgroups of the gradient: with weights' gradients to sum, what the CUs hold
 // (each leaves a row of sums); else one per row group.
 int64_t grad_groups(int64_t m, const Shape& s, bool sums) {
-  const int64_t all = (m + s.rows - 1) / s.rows, some = (s.chunks > 1 ? 1 : 2) * (int64_t)device_cus();
+  const int64_t all = (m + s.rows - 1) / s.rows, some = (s.threads > 512 ? 1 : 2) * (int64_t)device_cus();
   return sums && all > some ? some : std::min<int64_t>(all, 1 << 22);  // (workgroups go on to further rows)
 }
 
@@ -473,9 +498,9 @@ void launch(const Shape& s, int64_t grid, const BlockNormParams& p, hipStream_t 
     if (s.lanes == 16) return go(block_norm_grad_kernel<16, 1, 256, kF32, kS32, kW32>);
     if (s.lanes == 32) return go(block_norm_grad_kernel<32, 1, 256, kF32, kS32, kW32>);
     if (s.lanes == 64) return go(block_norm_grad_kernel<64, 1, 256, kF32, kS32, kW32>);
-    if (s.chunks == 1) return go(block_norm_grad_kernel<0, 1, 512, kF32, kS32, kW32>);
-    if (s.chunks == 2) return go(block_norm_grad_kernel<0, 2, 512, kF32, kS32, kW32>);
-    return go(block_norm_grad_kernel<0, 4, 512, kF32, kS32, kW32>);
+    if (s.threads <= 512) return go(block_norm_grad_kernel<0, 1, 512, kF32, kS32, kW32>);
+    if (s.chunks == 1) return go(block_norm_grad_kernel<0, 1, 1024, kF32, kS32, kW32>);
+    return go(block_norm_grad_kernel<0, 2, 1024, kF32, kS32, kW32>);
   } else {
     if (s.lanes == 8) return go(block_norm_kernel<8, 1, kF32, kS32>);
     if (s.lanes == 16) return go(block_norm_kernel<16, 1, kF32, kS32>);
