@@ -10,7 +10,7 @@ by (M + 2 D + 32) e times that of their terms."""
 import pytest
 import torch
 
-from home_seek_amd import ops
+from home_seek_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +245,30 @@ def test_refusals(dev):
                      (lambda: ops.block_norm(normal(dev, 1, (1, 16392)), normal(dev, 1, (1, 16392))), RuntimeError)):
         with pytest.raises(exc):
             bad()
+
+
+@pytest.mark.parametrize("m,d", ((37, 64), (9, 512), (600, 2056), (300, 8192), (270, 12296)))
+@pytest.mark.parametrize("gate", ("channel", "token", "full"))
+def test_written_over_what_was_read(dev, m, d, gate):
+    """The entry points may write the stream over the stream, n over f, and gradients over d_h and f or d_n."""
+    L = _lib.lib()
+    a = make(dev, m, d, BF16, F32, BF16, gate, True, True)
+    out, n = ops.block_norm(a["f"], a["h"], a["post_w"], a["gate"], 0.5, a["pre_w"])
+    d_h, d_n = normal(dev, 1, (m, d), F32), normal(dev, 2, (m, d))
+    want = ops.block_norm_grad(d_h, d_n, a["f"], out, a["post_w"], a["gate"], 0.5, a["pre_w"])
+    spec, _, keep = ops._block_norm_spec(a["f"], F32, a["post_w"], a["gate"], a["pre_w"])
+    f, h = a["f"].clone(), a["h"].clone()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert L.hsmoe_block_norm(f.data_ptr(), h.data_ptr(), m, d, spec, 0.5, 1e-6, h.data_ptr(), f.data_ptr(), stream) == 0
+    assert torch.equal(h, out) and torch.equal(f, n)
+    nbytes = L.hsmoe_block_norm_grad_workspace_size(m, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    for over_f in (True, False):
+        f, dx, dn = a["f"].clone(), d_h.clone(), d_n.clone()
+        post, pre = torch.empty(d, device=dev), torch.empty(d, device=dev)
+        d_gate = torch.empty_like(want.gate)
+        df = f if over_f else dn
+        assert L.hsmoe_block_norm_grad(dx.data_ptr(), dn.data_ptr(), f.data_ptr(), out.data_ptr(), m, d, spec, 0.5, 1e-6, df.data_ptr(),
+                                       dx.data_ptr(), post.data_ptr(), d_gate.data_ptr(), pre.data_ptr(), ws.data_ptr(), nbytes, stream) == 0
+        for got, ref in ((df, want.f), (dx, want.h), (post, want.post_w), (d_gate, want.gate), (pre, want.pre_w)):
+            assert torch.equal(got, ref)
