@@ -6,10 +6,10 @@
 // a word that makes up much of a batch is summed by many workgroups: a run of equal
 // ids inside a chunk is a row of the table; the ends of chunks that share a run leave
 // fp32 sums, which a second launch adds in their order.  All of it is bound by HBM.
-// Measured: 16381 tokens of 4096 bf16 looked up 37 us (5.0 TB/s: the copy's rate); the
-// gradient of a table of 129280 x 4096 230 us: the sort beside 1.06 GB of zeros 166,
-// places 7, sums 38, joins 8.  (Rows that no token names cleared beside the sums, by a
-// flag each, instead of all beside the sort: 235 to 243.)
+// Measured: 16381 tokens of 4096 bf16 looked up 37 us, with all of them different 44
+// (6.1 TB/s); the gradient of a table of 129280 x 4096 216 us: sort and places beside
+// 1.06 GB of zeros 165, sums 38, joins 8.  (Rows that no token names cleared beside the
+// sums, by a flag each, instead of all before them, took 5 to 13 us longer.)
 #include <algorithm>
 
 #include "hsmoe_common.h"
@@ -113,18 +113,23 @@ struct EmbedParams {
   void* out;
   int64_t m, vocab, d, ld;  // ld: values between the table's rows
   bool wide;
-  int shift;                // 2^shift threads per row
+  int shift;                // 2^shift threads per row ..
+  uint32_t slabs;           // .. and that many workgroups
   float scale;
 };
+// Vectors of a row per thread at a time: 8 KB written by a workgroup (16381 rows of 4096
+// bf16 to fp32, 16 KB by a workgroup 85 us, 8 KB 77; to bf16 8 KB 44, 4 KB 46).
+constexpr int ahead(bool out_f32) { return out_f32 ? 1 : 2; }
 template <int kVec, bool kF32, bool kOutF32>
 __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedParams p) {
+  constexpr int kAhead = ahead(kOutF32);
   const int lanes = 1 << p.shift;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
+  const uint32_t slabs = kVec == 1 ? 1 : p.slabs, group = blockIdx.x / slabs, slab = blockIdx.x - group * slabs;
+  const int64_t row = (int64_t)group * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
   if (row >= p.m) return;
   const int id = id_of(p.ids, p.wide, row, p.vocab);
-  const int64_t from = (int64_t)(id < 0 ? 0 : id) * p.ld, to = row * p.d;
-  constexpr int kAhead = 2;
-  for (int64_t c = (int64_t)(threadIdx.x & (lanes - 1)) * kVec; c < p.d; c += (int64_t)kAhead * lanes * kVec) {
+  const int64_t from = (int64_t)(id < 0 ? 0 : id) * p.ld, to = row * p.d, step = (int64_t)kAhead * lanes * kVec;
+  for (int64_t c = slab * step + (int64_t)(threadIdx.x & (lanes - 1)) * kVec; c < p.d; c += step * slabs) {
     Vals<kVec> v[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -145,8 +150,8 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedParams p) {
 // The tokens by (id, t): sorted_id[r] and token[r], those with an id outside the
 // table last with sorted_id -1.  First every 1024 tokens by themselves, by a workgroup
 // each, while other workgroups clear the table's gradient (which is written once
-// more than needed where a token falls, but waits for no order): 16381 tokens are
-// sorted long before a gigabyte is cleared.  Then a token's place is its place in its own
+// more than needed where a token falls, but waits for no order), the rest of which the
+// next launch clears: 16381 tokens are sorted long before a gigabyte is cleared.  Then a token's place is its place in its own
 // 1024 plus, for each of the others, the number of smaller ids there (or equal ones, if
 // they come before it), found by bisection in LDS.
 struct SortParams {
@@ -157,11 +162,15 @@ struct SortParams {
   int *sorted_id, *token;   // what is sorted in the end
   int *part_id, *part_token;  // by 1024
   char* clear;
-  int64_t clear_bytes;
+  int64_t clear_bytes, early;  // early: pieces cleared beside the first launch
+  int rankers;
 };
-// A workgroup clears 16 KB and ends: 129280 x 4096 bf16 in 165 us, against 200 by 512
-// workgroups that go through all of it side by side, and 154 without a sort beside it.
+// A workgroup clears 16 KB and ends, four pieces of 4 KB that are eight apart: what is
+// written at a time is then one narrow window that moves through the table (129280 x
+// 4096 bf16: 165 us, 175 by 16 KB in a row; 155 by workgroups of one piece each, which
+// the sort's 1024 threads do not allow).
 constexpr int64_t kClear = kSortThreads;  // 16-byte words
+constexpr int64_t kPiece = 256;
 __device__ __forceinline__ void clear_part(char* p, int64_t bytes, int64_t part) {
   typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
   const int64_t to_line = -(intptr_t)p & 15, head = bytes < to_line ? bytes : to_line, words = (bytes - head) / 16;
@@ -169,7 +178,7 @@ __device__ __forceinline__ void clear_part(char* p, int64_t bytes, int64_t part)
     for (int64_t i = threadIdx.x; i < head; i += kSortThreads) p[i] = 0;
     for (int64_t i = head + words * 16 + threadIdx.x; i < bytes; i += kSortThreads) p[i] = 0;
   }
-  const int64_t i = part * kClear + threadIdx.x;
+  const int64_t piece = (part / 8 * (kClear / kPiece) + threadIdx.x / kPiece) * 8 + part % 8, i = piece * kPiece + threadIdx.x % kPiece;
   if (i < words) __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4*>(p + head) + i);
 }
 __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p) {
@@ -208,6 +217,10 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p) 
 
 // 64 tokens per workgroup, a wave for each of 16 sorted parts at a time.
 __global__ void __launch_bounds__(kSortThreads) embed_rank_kernel(SortParams p) {
+  if ((int)blockIdx.x >= p.rankers) {
+    clear_part(p.clear, p.clear_bytes, (int64_t)blockIdx.x - p.rankers + p.early);
+    return;
+  }
   __shared__ int ids[kSortThreads * 16];
   __shared__ int counts[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -484,12 +497,14 @@ extern "C" int hsmoe_embed(const void* ids, int id_kind, int64_t m, const void* 
   if (m == 0) return HSMOE_OK;
   if (!table || !out) return fail(HSMOE_ERR_ARG, "%s: null pointer", who);
   if (!aligned(table, size_of(table_kind)) || !aligned(out, size_of(out_kind))) return fail(HSMOE_ERR_SHAPE, "%s: misaligned rows", who);
-  EmbedParams p{ids, table, out, m, vocab, d, table_row_stride, id_kind == HSMOE_IDS_I64, 0, scale};
+  EmbedParams p{ids, table, out, m, vocab, d, table_row_stride, id_kind == HSMOE_IDS_I64, 0, 1, scale};
   const bool vec = d % 8 == 0 && rows16(table, table_row_stride, table_kind) && rows16(out, d, out_kind);
-  p.shift = shift_for(vec ? (d / 8 + 1) / 2 : (d + 1) / 2);
-  const int64_t per = kThreads >> p.shift;
-  if (!grid_fits((m + per - 1) / per, kThreads)) return fail(HSMOE_ERR_SHAPE, "%s: too many rows of this width for one launch", who);
-  const dim3 grid((unsigned)((m + per - 1) / per)), block(kThreads);
+  const int64_t vectors = vec ? d / 8 : d, each = ahead(out_kind == HSMOE_OUT_F32);
+  p.shift = shift_for((vectors + each - 1) / each);
+  if (vec) p.slabs = (uint32_t)((vectors + each * kThreads - 1) / (each * kThreads));
+  const int64_t per = kThreads >> p.shift, groups = (m + per - 1) / per * p.slabs;
+  if (!grid_fits(groups, kThreads)) return fail(HSMOE_ERR_SHAPE, "%s: too many rows of this width for one launch", who);
+  const dim3 grid((unsigned)groups), block(kThreads);
   hipStream_t st = (hipStream_t)stream;
   const bool f = table_kind == HSMOE_OUT_F32, o = out_kind == HSMOE_OUT_F32;
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p); };
@@ -523,7 +538,7 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
   const bool wide = id_kind == HSMOE_IDS_I64;
   int *sorted_id = (int*)(mem + sp.ids), *token = (int*)(mem + sp.token);
   const int64_t bytes = add ? 0 : vocab * d * size_of(table_kind);
-  const int64_t clears = (bytes + kClear * 16 - 1) / (kClear * 16);
+  const int64_t clears = (bytes + 8 * kClear * 16 - 1) / (8 * kClear * 16) * 8;  // (eight share out their pieces)
   SumParams p{};
   p.m = m, p.d = d, p.ld = table_row_stride, p.ld_out = d_row_stride, p.chunks = (m + kChunk - 1) / kChunk;
   p.add = add, p.scale = scale;
@@ -532,7 +547,7 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
   p.shift = std::max(shift_for(vectors), 3);
   p.slabs = (int)((vectors + (1ll << p.shift) - 1) >> p.shift);
   // (all launches or none: those behind one that fails would take its places from what lies in the workspace)
-  if (!grid_fits(clears + kSortByRank / kSortThreads, kSortThreads) || !grid_fits(p.chunks * p.slabs, kThreads) ||
+  if (!grid_fits(clears + kSortByRank / 64, kSortThreads) || !grid_fits(p.chunks * p.slabs, kThreads) ||
       !grid_fits(p.chunks * join_slabs, kJoinThreads))
     return fail(HSMOE_ERR_SHAPE, "%s: a gradient of 64 GiB, or too many tokens of this width, for one launch", who);
   if (m == 0) {
@@ -541,10 +556,12 @@ extern "C" int hsmoe_embed_grad(const void* d_out, int64_t d_row_stride, int d_k
     return check_launch(who);
   }
   if (m <= kSortByRank) {
-    const SortParams s{ids, m, vocab, wide, (int)((m + kSortThreads - 1) / kSortThreads), sorted_id, token, (int*)(mem + sp.part_id),
-                       (int*)(mem + sp.part_token), (char*)d_table, bytes};
-    hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(s.sorters + clears)), dim3(kSortThreads), 0, st, s);
-    if (s.sorters > 1) hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((m + 63) / 64)), dim3(kSortThreads), 0, st, s);
+    SortParams s{ids, m, vocab, wide, (int)((m + kSortThreads - 1) / kSortThreads), sorted_id, token, (int*)(mem + sp.part_id),
+                 (int*)(mem + sp.part_token), (char*)d_table, bytes, clears, (int)((m + 63) / 64)};
+    if (s.sorters > 1) s.early = clears * 5 / 8;
+    hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(s.sorters + s.early)), dim3(kSortThreads), 0, st, s);
+    if (s.sorters > 1)
+      hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)(s.rankers + clears - s.early)), dim3(kSortThreads), 0, st, s);
   } else {
     if (clears) hipLaunchKernelGGL(embed_clear_kernel, dim3((unsigned)clears), dim3(kSortThreads), 0, st, (char*)d_table, bytes);
     const dim3 grid((unsigned)((m + kThreads - 1) / kThreads)), block(kThreads);
