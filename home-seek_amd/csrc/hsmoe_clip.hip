@@ -7,7 +7,7 @@
 // one order), and multiplies.  The second goes through the data backwards, so that
 // what the first read last comes out of the caches.  Tensors that are clipped in
 // place and need no clipping are not touched.  Measured: 1.24 GB in 60 tensors, bf16 and
-// fp32, the norm 211 us (5.9 TB/s; reads alone reach 6.5), with the clipped copy 700; 6
+// fp32, the norm 211 us (5.9 TB/s; reads alone reach 6.5), with the clipped copy 660; 6
 // tensors of 8064 values in all 7.6 us.  More workgroups, or fewer loads on their way,
 // change nothing.
 #include <algorithm>
@@ -22,7 +22,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 16384;        // values that a workgroup takes at a time
-constexpr int kBlocks = 1024;        // workgroups of a pass at most
+constexpr int kPiece = 2048;         // .. or in piece_kernel, all in all
+constexpr int kBlocks = 1024;        // workgroups of a pass that go through chunks, at most
+constexpr int64_t kMuch = 1 << 24;   // values from which piece_kernel is worth the launch of norm_join_kernel
 constexpr int kPer = 112;            // tensors per launch: their addresses are kernel arguments, so that a captured graph holds them
 constexpr int64_t kSmall = 32768;    // values up to which one workgroup does it all
 constexpr int kSmallThreads = 1024;
@@ -253,10 +255,55 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(Batch t, const Part<kMa
   }
 }
 
+// The norm, and the factor for piece_kernel (NULL: the norm alone).
 template <bool kMax>
-__global__ void __launch_bounds__(kThreads) norm_join_kernel(const Part<kMax>* parts, int n_parts, float* norm_out) {
+__global__ void __launch_bounds__(kThreads) norm_join_kernel(const Part<kMax>* parts, int n_parts, float max_norm, float* norm_out, Factor* f) {
   const double norm = norm_of<kMax>(parts, n_parts);
-  if (threadIdx.x == 0) *norm_out = (float)norm;
+  if (threadIdx.x) return;
+  *norm_out = (float)norm;
+  if (f) *f = factor(norm, max_norm);
+}
+
+// The second pass over much data: a workgroup takes 2048 values and ends, so that
+// what is on its way is one narrow window that moves through the tensors (a copy runs
+// at 6.2 TB/s this way, at 5.4 by workgroups that go through all of it side by side).
+template <bool kF32, bool kO32>
+__device__ __forceinline__ void scale_piece(const void* in, void* out, int64_t a, int64_t b, bool vec, Factor c) {
+  if (vec && b - a == kPiece) {
+    if constexpr (kF32 && kO32) {
+      float4 v[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] = reinterpret_cast<const float4*>((const float*)in + a)[i * kThreads + threadIdx.x];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<float4*>((float*)out + a)[i * kThreads + threadIdx.x] =
+            make_float4(v[i].x * c.a * c.b, v[i].y * c.a * c.b, v[i].z * c.a * c.b, v[i].w * c.a * c.b);
+    } else {
+      const int64_t at = a + (int64_t)threadIdx.x * 8;
+      const Raw<kF32> v = read8<kF32>(in, at);
+      Vals o;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o.v[k] = v.at(k) * c.a * c.b;
+      write8<kO32>(out, at, o);
+    }
+    return;
+  }
+  for (int64_t i = a + threadIdx.x; i < b; i += kThreads) write1<kO32>(out, i, read1<kF32>(in, i) * c.a * c.b);
+}
+__global__ void __launch_bounds__(kThreads) piece_kernel(Batch t, const Factor* factor) {
+  const uint32_t piece = gridDim.x - 1 - blockIdx.x, chunk = piece / (kChunk / kPiece);
+  const int j = tensor_of(t, chunk), flags = t.flags[j];
+  const int64_t a = (int64_t)(chunk - t.first[j]) * kChunk + piece % (kChunk / kPiece) * kPiece;
+  const int64_t b = a + kPiece < t.count[j] ? a + kPiece : t.count[j];
+  const Factor c = *factor;
+  if (a >= b || (c.a == 1.0f && c.b == 1.0f && (flags & kSame))) return;
+  const bool vec = (flags & (kInVec | kOutVec)) == (kInVec | kOutVec);
+  switch (flags & (kInF32 | kOutF32)) {
+    case 0: return scale_piece<false, false>(t.in[j], t.out[j], a, b, vec, c);
+    case kInF32: return scale_piece<true, false>(t.in[j], t.out[j], a, b, vec, c);
+    case kOutF32: return scale_piece<false, true>(t.in[j], t.out[j], a, b, vec, c);
+    default: return scale_piece<true, true>(t.in[j], t.out[j], a, b, vec, c);
+  }
 }
 
 // Few values: one workgroup, one launch.
@@ -336,10 +383,15 @@ Batch batch_of(const Tensors& t, int64_t& at) {
   return b;
 }
 
+size_t parts_bytes(int64_t n) { return (size_t)((n + kPer - 1) / kPer) * kBlocks * sizeof(Part<false>); }
+
 template <bool kMax>
 int run_clip(const char* who, const Tensors& t, float max_norm, float* norm_out, void* workspace, hipStream_t st) {
-  int64_t total = 0, live = 0;
-  for (int64_t i = 0; i < t.n; ++i) total += t.counts[i], live += t.counts[i] > 0;
+  int64_t total = 0, live = 0, moved = 0;
+  for (int64_t i = 0; i < t.n; ++i) {
+    total += t.counts[i], live += t.counts[i] > 0;
+    if (t.out && (t.out[i] != t.in[i] || t.out_kinds[i] != t.kinds[i])) moved += t.counts[i];
+  }
   if (total <= kSmall && live <= kPer) {
     int64_t at = 0;
     const Batch b = batch_of(t, at);
@@ -356,14 +408,22 @@ int run_clip(const char* who, const Tensors& t, float max_norm, float* norm_out,
     hipLaunchKernelGGL((norm_part_kernel<kMax>), dim3(blocks), dim3(kThreads), 0, st, b, parts + n_parts);
     n_parts += blocks;
   }
-  if (!t.out) {
-    hipLaunchKernelGGL((norm_join_kernel<kMax>), dim3(1), dim3(kThreads), 0, st, parts, n_parts, norm_out);
-    return check_launch(who);
-  }
+  // (what is clipped in place often needs no clipping: workgroups that only find that out
+  // would cost 30 us for 1 GB, in 180, and gain 40 in 607 where it does)
+  const bool much = moved >= kMuch;
+  Factor* f = much ? (Factor*)((char*)workspace + parts_bytes(t.n)) : nullptr;
+  if (!t.out || much)
+    hipLaunchKernelGGL((norm_join_kernel<kMax>), dim3(1), dim3(kThreads), 0, st, parts, n_parts, max_norm, norm_out, f);
+  if (!t.out) return check_launch(who);
   for (int64_t at = 0; at < t.n;) {
-    const bool first = at == 0;
+    const bool first = at == 0 && !much;
     const Batch b = batch_of(t, at);
     if (!b.n && !first) continue;
+    const int64_t pieces = (int64_t)b.first[b.n] * (kChunk / kPiece);
+    if (much && grid_fits(pieces, kThreads)) {
+      hipLaunchKernelGGL(piece_kernel, dim3((unsigned)pieces), dim3(kThreads), 0, st, b, f);
+      continue;
+    }
     const int blocks = std::max(1, (int)std::min<uint32_t>(b.first[b.n], kBlocks));
     hipLaunchKernelGGL((scale_kernel<kMax>), dim3(blocks), dim3(kThreads), 0, st, b, parts, n_parts, max_norm, first ? norm_out : nullptr);
   }
@@ -390,7 +450,7 @@ int clip(const char* who, const Tensors& t, double norm_type, float max_norm, fl
 using namespace hsmoe;
 
 extern "C" size_t hsmoe_grad_norm_workspace_size(int64_t n) {
-  return n < 1 ? 0 : (size_t)((n + kPer - 1) / kPer) * kBlocks * sizeof(Part<false>);
+  return n < 1 ? 0 : parts_bytes(n) + sizeof(Factor);
 }
 
 extern "C" int hsmoe_grad_norm(int64_t n, const void* const* tensors, const int64_t* counts, const int32_t* kinds,

@@ -49,6 +49,7 @@ LISTS = {
     "more than a launch": [(411 + i % 7,) for i in range(113)],
     "many": [(1 + 37 * i % 2999,) for i in range(700)],
     "large": [(3000, 4099), (1, 70001), (4096,), (2048, 4096)],
+    "large and more than a launch": [(411 + i % 7,) for i in range(113)] + [(4099, 4097), (16385,)],
 }
 
 
@@ -74,6 +75,17 @@ def test_lists(dev, name, kind):
         for a, b in zip(outs, kept):
             if a.dtype == b.dtype:
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("max_norm", (1.0, 1e9))
+def test_some_in_place(dev, max_norm):
+    base = normal(dev, 1, (9000001,))
+    grads = [base[1:], normal(dev, 2, (9000000,), F32), normal(dev, 3, (40000,)), normal(dev, 4, (70003,), F32)]
+    before = [g.clone() for g in grads]
+    outs = [torch.empty(9000000, dtype=F32, device=dev), torch.empty(9000000, device=dev), grads[2], grads[3]]
+    norm = ops.clip_grads(grads, max_norm, out=outs)
+    check(before, max_norm, 2.0, norm, outs)
+    assert torch.equal(grads[0], before[0]) and torch.equal(grads[1], before[1])
 
 
 @pytest.mark.parametrize("n", (5, 40000))
