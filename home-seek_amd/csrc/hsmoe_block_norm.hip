@@ -12,8 +12,8 @@
 //   df  = r1 (post_w du - f r1^2 mean(post_w du f))         (without post_w: du)
 // Sums in fp32.  All of it is bound by HBM; few rows by the latency of two sums
 // over a row, one after the other.  Measured: 8191 x 4096, rows and stream bf16, a gate
-// per channel 46 us (5.8 TB/s), fp32 stream and a full gate 93 us (5.0 TB/s, the rate of
-// a large copy); the gradient 84 us and 5 for the join (4.5 TB/s), with an fp32 stream
+// per channel 47 us (5.7 TB/s), fp32 stream and a full gate 90 us (5.2 TB/s; a copy by
+// workgroups of 4 KB runs at 6.2, torch's at 5.1); the gradient 84 us and 5 for the join (4.5 TB/s), with an fp32 stream
 // 4.8 TB/s; three rows 3.9 us.
 #include <algorithm>
 
@@ -473,13 +473,15 @@ __global__ void __launch_bounds__(kJoinWaves * 64) block_norm_join_kernel(JoinPa
 struct Shape {
   int lanes, threads, rows, chunks;
 };
-Shape shape_of(int64_t d, bool grad) {
+Shape shape_of(int64_t d) {
   const int chunks = (int)(d / 8);
   if (chunks <= 8) return {8, 256, 32, 1};
   if (chunks <= 16) return {16, 256, 16, 1};
   if (chunks <= 32) return {32, 256, 8, 1};
   if (chunks <= 64) return {64, 256, 4, 1};
-  const int per = !grad || chunks > 1024 ? 2 : 1;
+  // (half the threads with two chunks each take longer: forward 8191 x 4096 51.5 us for 47,
+  // 8191 x 6144 89 for 72)
+  const int per = chunks > 1024 ? 2 : 1;
   return {0, ((chunks + per - 1) / per + 63) / 64 * 64, 1, per};
 }
 // Workgroups of the gradient: with weights' gradients to sum, what the CUs hold
@@ -506,6 +508,7 @@ void launch(const Shape& s, int64_t grid, const BlockNormParams& p, hipStream_t 
     if (s.lanes == 16) return go(block_norm_kernel<16, 1, kF32, kS32>);
     if (s.lanes == 32) return go(block_norm_kernel<32, 1, kF32, kS32>);
     if (s.lanes == 64) return go(block_norm_kernel<64, 1, kF32, kS32>);
+    if (s.chunks == 1) return go(block_norm_kernel<0, 1, kF32, kS32>);
     return go(block_norm_kernel<0, 2, kF32, kS32>);
   }
 }
@@ -565,7 +568,7 @@ extern "C" int hsmoe_block_norm(const void* f, const void* h, int64_t m, int64_t
     return fail(HSMOE_ERR_SHAPE, "%s: rows must be 16-byte aligned", who);
   BlockNormParams p = params_of(m, d, scale, eps, spec);
   p.f = f, p.h = h, p.h_out = h_out, p.n_out = n_out;
-  const Shape s = shape_of(d, false);
+  const Shape s = shape_of(d);
   if (!grid_fits((m + s.rows - 1) / s.rows, s.threads)) return fail(HSMOE_ERR_SHAPE, "%s: too many rows of this width for one launch", who);
   launch_kinds<false>(s, (m + s.rows - 1) / s.rows, spec->row_kind == HSMOE_OUT_F32, spec->stream_kind == HSMOE_OUT_F32, p,
                       (hipStream_t)stream);
@@ -574,7 +577,7 @@ extern "C" int hsmoe_block_norm(const void* f, const void* h, int64_t m, int64_t
 
 extern "C" size_t hsmoe_block_norm_grad_workspace_size(int64_t m, int64_t d) {
   if (m < 1 || d < 8 || d > kMaxD) return 0;
-  return (size_t)grad_groups(m, shape_of(d, true), true) * 3 * d * sizeof(float);
+  return (size_t)grad_groups(m, shape_of(d), true) * 3 * d * sizeof(float);
 }
 
 extern "C" int hsmoe_block_norm_grad(const void* d_h, const void* d_n, const void* f, const void* h_out, int64_t m,
@@ -594,7 +597,7 @@ extern "C" int hsmoe_block_norm_grad(const void* d_h, const void* d_n, const voi
     if (!aligned(q, 16)) return fail(HSMOE_ERR_SHAPE, "%s: rows must be 16-byte aligned", who);
   if (!aligned(d_gate, spec->gate_form == kGateFull ? 16 : 4) || !aligned(d_post, 4) || !aligned(d_pre, 4))
     return fail(HSMOE_ERR_SHAPE, "%s: misaligned gradients", who);
-  const Shape s = shape_of(d, true);
+  const Shape s = shape_of(d);
   const int64_t groups = m > 0 ? grad_groups(m, s, sums) : 0;
   const size_t need = sums ? (size_t)groups * 3 * d * sizeof(float) : 0;
   if (need && (!workspace || workspace_bytes < need)) return fail(HSMOE_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, need);
