@@ -93,6 +93,7 @@ struct QuantParams {
   uint8_t* scale;     // [m][ld_scale], or dealt words
   int64_t m, k, ldx, ld_scale;
   int64_t units;      // waves' units per row
+  int across;         // of a workgroup's waves, so many side by side in a row, the others in further rows
   int64_t row_blocks; // dealt words: blocks of 32 rows (0: rows of scales)
 };
 
@@ -165,10 +166,18 @@ __device__ __forceinline__ void deal_scales(const DealParams& p, int64_t t) {
 constexpr int kQuantThreads = 256;
 constexpr int kQuantWaves = kQuantThreads / 64;
 
-// Workgroups (rows, segment of 512 values).
+// Workgroup b's part: four waves side by side read 4 KB of a row in one piece, and the
+// workgroups go through the rows in the order of memory (65536 x 4096 bf16 149 us with
+// the waves in further rows, 130 so; fp32 8190 x 4096 36 and 29).
+template <int kKind, int kRows>
+__device__ __forceinline__ void quant_group(const QuantParams& p, uint32_t b) {
+  const uint32_t parts = (uint32_t)p.units / p.across, r = b / parts, wave = threadIdx.x >> 6, down = wave / p.across;
+  const int seg = (int)((b - r * parts) * p.across + (wave - down * p.across));
+  quant_rows<kKind, kRows>(p, ((int64_t)r * (kQuantWaves / p.across) + down) * kRows, seg, threadIdx.x & 63);
+}
 template <int kKind, int kRows>
 __global__ void __launch_bounds__(kQuantThreads) fp4_quant_kernel(QuantParams p) {
-  quant_rows<kKind, kRows>(p, ((int64_t)blockIdx.x * kQuantWaves + (threadIdx.x >> 6)) * kRows, blockIdx.y, threadIdx.x & 63);
+  quant_group<kKind, kRows>(p, blockIdx.x);
 }
 
 // What a product wants before it: x quantised (kKind < 0: its scales dealt) by the
@@ -180,8 +189,7 @@ __global__ void __launch_bounds__(kQuantThreads) fp4_ready_kernel(QuantParams q,
   } else if constexpr (kKind < 0) {
     deal_scales(x, (int64_t)blockIdx.x * kQuantThreads + threadIdx.x);
   } else {
-    const uint32_t units = (uint32_t)q.units, r = blockIdx.x / units;
-    quant_rows<kKind, kRows>(q, ((int64_t)r * kQuantWaves + (threadIdx.x >> 6)) * kRows, (int)(blockIdx.x - r * units), threadIdx.x & 63);
+    quant_group<kKind, kRows>(q, blockIdx.x);
   }
 }
 
@@ -564,14 +572,17 @@ __global__ void __launch_bounds__(256) fp4_few_kernel(Fp4Params p, const char* x
 // it and 11.1 with tiles, 48 9.4 and 11.0, 64 10.8 and 11.1.
 constexpr int64_t kFewRows = 64;
 
-// Rows per wave and workgroups along the rows of a quantisation.
+// Rows per wave, waves side by side in a row and workgroups of a quantisation.
 bool four_rows(int64_t m, int64_t units) { return m * units >= 8192; }
-int64_t quant_groups(int64_t m, int64_t units) {
-  const int64_t rows = kQuantWaves * (four_rows(m, units) ? 4 : 1);
-  return (m + rows - 1) / rows;
+// Dealt words of sixteen rows are whole lines, so waves that write them take further rows.
+int waves_across(int64_t units, bool dealt) { return dealt ? 1 : units % 4 == 0 ? 4 : units % 2 == 0 ? 2 : 1; }
+int64_t quant_groups(int64_t m, int64_t units, bool dealt) {
+  const int across = waves_across(units, dealt);
+  const int64_t rows = kQuantWaves / across * (four_rows(m, units) ? 4 : 1);
+  return (m + rows - 1) / rows * (units / across);
 }
 void launch_quant(const QuantParams& q, bool bf16, hipStream_t st) {
-  const dim3 grid((unsigned)quant_groups(q.m, q.units), (unsigned)q.units), block(kQuantThreads);
+  const dim3 grid((unsigned)quant_groups(q.m, q.units, q.row_blocks)), block(kQuantThreads);
   if (bf16 && four_rows(q.m, q.units))
     hipLaunchKernelGGL((fp4_quant_kernel<kRowsBf16, 4>), grid, block, 0, st, q);
   else if (bf16)
@@ -662,12 +673,12 @@ extern "C" int hsmoe_fp4_quant(const void* x, int64_t x_row_stride, int row_kind
   if (!codes || !scale) return fail(HSMOE_ERR_ARG, "hsmoe_fp4_quant: null pointer");
   if (!aligned(codes, 4) || (k % 128 == 0 && !aligned(scale, 4)))
     return fail(HSMOE_ERR_SHAPE, "hsmoe_fp4_quant: codes and scales must be 4-byte aligned");
-  if (!grid_fits(quant_groups(m, (k + kUnit - 1) / kUnit), kQuantThreads))
+  if (!grid_fits(quant_groups(m, (k + kUnit - 1) / kUnit, false), kQuantThreads))
     return fail(HSMOE_ERR_SHAPE, "hsmoe_fp4_quant: too many rows for one launch");
   QuantParams q{};
   q.x = (const char*)x, q.codes = (char*)codes, q.scale = (uint8_t*)scale;
   q.m = m, q.k = k, q.ldx = x_row_stride * (row_kind == HSMOE_OUT_BF16 ? 2 : 4), q.ld_scale = k / 32;
-  q.units = (k + kUnit - 1) / kUnit;
+  q.units = (k + kUnit - 1) / kUnit, q.across = waves_across(q.units, false);
   launch_quant(q, row_kind == HSMOE_OUT_BF16, (hipStream_t)stream);
   return check_launch("hsmoe_fp4_quant");
 }
@@ -716,6 +727,7 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   q.x = (const char*)x, q.codes = mem + plan.codes, q.scale = (uint8_t*)mem + plan.xs;
   q.m = m, q.k = k, q.ldx = ldx, q.units = (k + kUnit - 1) / kUnit;
   q.ld_scale = up(k / 32, 16), q.row_blocks = plan.few ? 0 : (m + 31) / 32;
+  q.across = waves_across(q.units, !plan.few);
   DealParams dx{}, dw{};
   dw.scale = (const uint8_t*)w_scale, dw.words = (uint32_t*)(mem + plan.ws);
   dw.rows = n, dw.blocks = k / 32, dw.row_blocks = (n + 31) / 32, dw.groups = q.units;
@@ -740,7 +752,7 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
   }
   p.words = mem + plan.xs, p.x_words = 0, p.w_words = (uint32_t)(plan.ws - plan.xs);
   p.words_bytes = (uint32_t)(plan.bytes - plan.xs);
-  const int64_t first = packed ? deal_blocks(dx) : quant_groups(m, q.units) * q.units;
+  const int64_t first = packed ? deal_blocks(dx) : quant_groups(m, q.units, true);
   const int64_t all = first + deal_blocks(dw);
   if (!grid_fits(all, kQuantThreads)) return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
   auto ready = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kQuantThreads), 0, st, q, dx, dw, (uint32_t)first); };
