@@ -124,7 +124,7 @@ template <int kVec, bool kF32, bool kOutF32>
 __global__ void __launch_bounds__(kThreads) embed_kernel(EmbedParams p) {
   constexpr int kAhead = ahead(kOutF32);
   const int lanes = 1 << p.shift;
-  const uint32_t slabs = kVec == 1 ? 1 : p.slabs, group = blockIdx.x / slabs, slab = blockIdx.x - group * slabs;
+  const uint32_t slabs = kVec == 1 ? 1 : p.slabs, group = slabs == 1 ? blockIdx.x : blockIdx.x / slabs, slab = blockIdx.x - group * slabs;
   const int64_t row = (int64_t)group * (kThreads >> p.shift) + (threadIdx.x >> p.shift);
   if (row >= p.m) return;
   const int id = id_of(p.ids, p.wide, row, p.vocab);

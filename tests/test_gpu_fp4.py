@@ -54,7 +54,8 @@ def values(packed, scale):
 
 
 @pytest.mark.parametrize("dtype", (BF16, F32))
-@pytest.mark.parametrize("m,k", ((1, 32), (3, 64), (5, 96), (2, 1120), (7, 4096), (130, 544), (1025, 512), (1, 65536)))
+@pytest.mark.parametrize("m,k", ((1, 32), (3, 64), (5, 96), (2, 1120), (7, 4096), (130, 544), (1025, 512), (1, 65536), (8200, 96), (4099, 1024), (4101, 544),
+                                 (2731, 1536), (2050, 2048), (1367, 2592)))
 def test_codes_and_scales(dev, m, k, dtype):
     x = normal(dev, m + k, (m, k), dtype)
     x[0, :32] = 0
