@@ -13,8 +13,9 @@
 // Sums in fp32.  All of it is bound by HBM; few rows by the latency of two sums
 // over a row, one after the other.  Measured: 8191 x 4096, rows and stream bf16, a gate
 // per channel 47 us (5.7 TB/s), fp32 stream and a full gate 90 us (5.2 TB/s; a copy by
-// workgroups of 4 KB runs at 6.2, torch's at 5.1); the gradient 84 us and 5 for the join (4.5 TB/s), with an fp32 stream
-// 4.8 TB/s; three rows 3.9 us.
+// workgroups of 4 KB runs at 6.2, torch's at 5.1); the gradient 84 us and 5 for the join
+// (4.5 TB/s), with an fp32 stream
+// 4.8 TB/s; three rows 3.2 us.
 #include <algorithm>
 
 #include "hsmoe_common.h"
@@ -297,7 +298,7 @@ __global__ void __launch_bounds__(kMax, kMax >= 512 ? 4 : 2) block_norm_grad_ker
   // 441).  The next row is loaded ahead where several share a workgroup only: otherwise
   // it costs the registers with which two workgroups share a CU, which hides more (fp32
   // rows of 4096: 129 us with, 85 without).
-  constexpr bool kLean = kC > 1, kAhead = kLanes != 0;
+  constexpr bool kLean = kC > 1 && kLanes == 0, kAhead = kLanes != 0 && kC == 1;
   Row next;
   if (kAhead) next = load(first);
   // (a_y: the rows' sums of dt y times what of the gate is a row's own; the norm's weight
@@ -473,21 +474,26 @@ __global__ void __launch_bounds__(kJoinWaves * 64) block_norm_join_kernel(JoinPa
 struct Shape {
   int lanes, threads, rows, chunks;
 };
-Shape shape_of(int64_t d) {
+Shape shape_of(int64_t d, bool grad) {
   const int chunks = (int)(d / 8);
   if (chunks <= 8) return {8, 256, 32, 1};
   if (chunks <= 16) return {16, 256, 16, 1};
   if (chunks <= 32) return {32, 256, 8, 1};
   if (chunks <= 64) return {64, 256, 4, 1};
+  // (a row of 512 to 1024 by a wave, which waits for no other: 32768 x 768 bf16 67 us, by two waves 158)
+  if (grad && chunks <= 128) return {64, 256, 4, 2};
   // (half the threads with two chunks each take longer: forward 8191 x 4096 51.5 us for 47,
   // 8191 x 6144 89 for 72)
   const int per = chunks > 1024 ? 2 : 1;
   return {0, ((chunks + per - 1) / per + 63) / 64 * 64, 1, per};
 }
-// Workgroups of the gradient: with weights' gradients to sum, what the CUs hold
-// (each leaves a row of sums); else one per row group.
-int64_t grad_groups(int64_t m, const Shape& s, bool sums) {
-  const int64_t all = (m + s.rows - 1) / s.rows, some = (s.threads > 512 ? 1 : 2) * (int64_t)device_cus();
+// Workgroups of the gradient: with weights' gradients to sum, what the CUs hold (each
+// leaves a row of sums); else one per row group.  Short rows of a workgroup each want
+// more of them to wait with (bf16 21000 x 1536 90 us with four per CU, 111 with two), if
+// they are not of fp32 (136 with two, 149 with four).
+int64_t grad_groups(int64_t m, const Shape& s, bool sums, bool f32) {
+  const int per_cu = s.threads > 512 ? 1 : s.lanes || f32 ? 2 : std::max(2, 768 / s.threads);
+  const int64_t all = (m + s.rows - 1) / s.rows, some = per_cu * (int64_t)device_cus();
   return sums && all > some ? some : std::min<int64_t>(all, 1 << 22);  // (workgroups go on to further rows)
 }
 
@@ -499,7 +505,8 @@ void launch(const Shape& s, int64_t grid, const BlockNormParams& p, hipStream_t 
     if (s.lanes == 8) return go(block_norm_grad_kernel<8, 1, 256, kF32, kS32, kW32>);
     if (s.lanes == 16) return go(block_norm_grad_kernel<16, 1, 256, kF32, kS32, kW32>);
     if (s.lanes == 32) return go(block_norm_grad_kernel<32, 1, 256, kF32, kS32, kW32>);
-    if (s.lanes == 64) return go(block_norm_grad_kernel<64, 1, 256, kF32, kS32, kW32>);
+    if (s.lanes == 64 && s.chunks == 1) return go(block_norm_grad_kernel<64, 1, 256, kF32, kS32, kW32>);
+    if (s.lanes == 64) return go(block_norm_grad_kernel<64, 2, 256, kF32, kS32, kW32>);
     if (s.threads <= 512) return go(block_norm_grad_kernel<0, 1, 512, kF32, kS32, kW32>);
     if (s.chunks == 1) return go(block_norm_grad_kernel<0, 1, 1024, kF32, kS32, kW32>);
     return go(block_norm_grad_kernel<0, 2, 1024, kF32, kS32, kW32>);
@@ -568,7 +575,7 @@ extern "C" int hsmoe_block_norm(const void* f, const void* h, int64_t m, int64_t
     return fail(HSMOE_ERR_SHAPE, "%s: rows must be 16-byte aligned", who);
   BlockNormParams p = params_of(m, d, scale, eps, spec);
   p.f = f, p.h = h, p.h_out = h_out, p.n_out = n_out;
-  const Shape s = shape_of(d);
+  const Shape s = shape_of(d, false);
   if (!grid_fits((m + s.rows - 1) / s.rows, s.threads)) return fail(HSMOE_ERR_SHAPE, "%s: too many rows of this width for one launch", who);
   launch_kinds<false>(s, (m + s.rows - 1) / s.rows, spec->row_kind == HSMOE_OUT_F32, spec->stream_kind == HSMOE_OUT_F32, p,
                       (hipStream_t)stream);
@@ -577,7 +584,7 @@ extern "C" int hsmoe_block_norm(const void* f, const void* h, int64_t m, int64_t
 
 extern "C" size_t hsmoe_block_norm_grad_workspace_size(int64_t m, int64_t d) {
   if (m < 1 || d < 8 || d > kMaxD) return 0;
-  return (size_t)grad_groups(m, shape_of(d), true) * 3 * d * sizeof(float);
+  return (size_t)grad_groups(m, shape_of(d, true), true, false) * 3 * d * sizeof(float);
 }
 
 extern "C" int hsmoe_block_norm_grad(const void* d_h, const void* d_n, const void* f, const void* h_out, int64_t m,
@@ -597,8 +604,8 @@ extern "C" int hsmoe_block_norm_grad(const void* d_h, const void* d_n, const voi
     if (!aligned(q, 16)) return fail(HSMOE_ERR_SHAPE, "%s: rows must be 16-byte aligned", who);
   if (!aligned(d_gate, spec->gate_form == kGateFull ? 16 : 4) || !aligned(d_post, 4) || !aligned(d_pre, 4))
     return fail(HSMOE_ERR_SHAPE, "%s: misaligned gradients", who);
-  const Shape s = shape_of(d);
-  const int64_t groups = m > 0 ? grad_groups(m, s, sums) : 0;
+  const Shape s = shape_of(d, true);
+  const int64_t groups = m > 0 ? grad_groups(m, s, sums, spec->row_kind == HSMOE_OUT_F32 || spec->stream_kind == HSMOE_OUT_F32) : 0;
   const size_t need = sums ? (size_t)groups * 3 * d * sizeof(float) : 0;
   if (need && (!workspace || workspace_bytes < need)) return fail(HSMOE_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", who, need);
   if (need && !aligned(workspace, 16)) return fail(HSMOE_ERR_SHAPE, "%s: misaligned workspace", who);

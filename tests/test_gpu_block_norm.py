@@ -106,7 +106,8 @@ def check_grad(a, d_h, d_n, scale, eps, g):
 
 
 SIZES = [(1, 8), (3, 64), (33, 72), (5, 128), (17, 136), (9, 256), (7, 264), (6, 512), (5, 520), (4, 1024), (3, 4096),
-         (2, 4104), (2, 8192), (1, 8200), (2, 16384), (1030, 64), (2100, 512), (1500, 1536), (700, 4096), (300, 8192), (300, 6152), (3, 12296), (300, 16384)]
+         (2, 4104), (2, 8192), (1, 8200), (2, 16384), (1030, 64), (2100, 512), (1500, 1536), (700, 4096), (300, 8192), (300, 6152), (3, 12296), (300, 16384),
+         (900, 776), (2300, 1024)]
 KINDS = [(BF16, BF16, BF16), (BF16, F32, F32), (F32, F32, F32), (F32, BF16, BF16)]
 
 
