@@ -6,6 +6,7 @@
 // Their sums of e2m1 products are exact while the exponents of one instruction
 // (two or four blocks of 32) lie within 2^10 of each other, and off by 2^-20 of
 // the largest product at most when they lie 2^20 apart (measured against 64 bits).
+#include <algorithm>
 #include <type_traits>
 
 #include "hsmoe_common.h"
@@ -568,9 +569,23 @@ __global__ void __launch_bounds__(256) fp4_few_kernel(Fp4Params p, const char* x
 }
 
 // ---------------------------------------------------------------- host
-// Rows up to which fp4_few_kernel is taken: 33 of them by 4096 x 4096 take 8.9 us with
-// it and 11.1 with tiles, 48 9.4 and 11.0, 64 10.8 and 11.1.
+int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+// Rows that fp4_few_kernel can take, and those that it does: its workgroups read x again
+// for each 16 columns, so that many columns are for the tiles.  By estimated time: us
+// from what a workgroup per CU takes (256 CUs), c of them one after the other (measured
+// with k = 4096, kernel and tiles; 1, 16 and 64 rows by 4096 columns 4.3 and 10.7, 6.7
+// and 11, 10.8 and 11.1; by 16384 8.7 and 12.3, 14.1 and 12.6, 29 and 13; by 129280 57 and
+// 63, 93 and 61, 206 and 68; k = 1024, 4096 columns 3.0 and 6.3, 5.7 and 6.5, 7.2 and 6.7,
+// 16384 columns 3.9 and 6.6, 7.9 and 6.7, 11.2 and 7.2; codes that are there 2 less with few).
 constexpr int64_t kFewRows = 64;
+bool takes_few(int64_t m, int64_t n, int64_t k, bool packed) {
+  if (m > kFewRows) return false;
+  if (up(n, 32) * up(k, kUnit) / 32 >= (1ll << 30)) return true;  // (more scales than the tiles' 32-bit offsets reach)
+  const double c = (double)n / 4096, kk = (double)k / 4096, rows = 1.45 + 0.07 * m;
+  const double few = packed ? 3.0 + c * kk * rows : 4.0 + c * kk * (m == 1 ? 1.5 : std::max(2.15, rows));
+  return few <= std::max(5.1 + 5.9 * kk, 4.0 + 1.85 * c * kk);
+}
 
 // Rows per wave, waves side by side in a row and workgroups of a quantisation.
 bool four_rows(int64_t m, int64_t units) { return m * units >= 8192; }
@@ -593,8 +608,6 @@ void launch_quant(const QuantParams& q, bool bf16, hipStream_t st) {
     hipLaunchKernelGGL((fp4_quant_kernel<kRowsF32, 1>), grid, block, 0, st, q);
 }
 
-int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
-
 // What a product does and where its workspace keeps what.
 struct Fp4Plan {
   bool few, fused;
@@ -603,8 +616,8 @@ struct Fp4Plan {
 };
 Fp4Plan plan_fp4(int64_t m, int64_t n, int64_t k, bool packed) {
   Fp4Plan p{};
-  p.few = m <= kFewRows;
-  p.fused = m <= 16 && !packed && m * up(k, kUnit) / 2 <= kFewLds;
+  p.few = takes_few(m, n, k, packed);
+  p.fused = p.few && m <= 16 && !packed && m * up(k, kUnit) / 2 <= kFewLds;
   if (p.fused) return p;
   const int64_t stages = up(k, kUnit) / kStep;
   p.codes = 0;
