@@ -275,12 +275,17 @@ struct Fp4Source {
   }
 };
 
-template <int kBR, int kBC, int kWR, int kWC, int kStages_>
-__global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) fp4_tile_kernel(Fp4Params p) {
+// kSplit 2: twice the waves, of which the second half takes every other stage into
+// memory of its own; the sums are joined at the end.
+template <int kBR, int kBC, int kWR, int kWC, int kStages_, int kSplit>
+__global__ void __launch_bounds__(kWR* kWC * 64 * kSplit) __attribute__((amdgpu_waves_per_eu(2, 2))) fp4_tile_kernel(Fp4Params p) {
   using T = Fp4Tile<kBR, kBC, kWR, kWC, kStages_>;
   constexpr int kStages = T::kStages;
-  __shared__ __align__(1024) char lds[T::kLds];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  static_assert(kSplit == 1 || (kSplit == 2 && !T::kTurns && T::kWaves * T::kFR * T::kFC * 4096 <= T::kLds), "two halves, whose sums fit");
+  __shared__ __align__(1024) char memory[kSplit * T::kLds];
+  const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = kSplit == 1 ? 0 : any / T::kWaves, wave = any - part * T::kWaves;
+  char* lds = memory + part * T::kLds;
   int rt, ct;
   if (!place_tile(blockIdx.x, (int)((p.m + kBR - 1) / kBR), (int)((p.n + kBC - 1) / kBC), rt, ct)) return;
   const int64_t m0 = (int64_t)rt * kBR, n0 = (int64_t)ct * kBC, row_bytes = p.k / 2;
@@ -379,15 +384,16 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
     }
     if (!second) turn(false);
   } else {
-    for (int s = 0; s < kStages - 1; ++s) load(s, s);
+    const int own = (steps + kSplit - 1) / kSplit;
+    for (int s = 0; s < kStages - 1; ++s) load(s * kSplit + part, s);
     int at = 0, next = kStages - 1;
-    for (int s = 0; s < steps; ++s) {
+    for (int s = 0; s < own; ++s) {
       // stage s is whole when every wave's loads of it are, and nobody reads the one
       // before any more; stages beyond the last are loaded from nowhere, for the count
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * T::kLoads) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      load(s + kStages - 1, next);
+      load((s + kStages - 1) * kSplit + part, next);
       const char* stage = lds + at * T::kStage;
       i32x4 r[T::kFR], c[T::kFC];
       read_scales(stage);
@@ -401,6 +407,28 @@ __global__ void __launch_bounds__(kWR* kWC * 64) __attribute__((amdgpu_waves_per
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no load may reach LDS once it is used for the results
   __syncthreads();
+  if constexpr (kSplit == 2) {
+    f32x4* sums = reinterpret_cast<f32x4*>(memory + T::kLds) + wave * T::kFR * T::kFC * 256 + lane;
+#pragma unroll
+    for (int i = 0; i < T::kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < T::kFC; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (part) sums[((i * T::kFC + j) * 4 + q) * 64] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 0; i < T::kFR; ++i)
+#pragma unroll
+      for (int j = 0; j < T::kFC; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = sums[((i * T::kFC + j) * 4 + q) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += v[e];
+        }
+  }
   // A lane has row lane % 32 and columns 8 q + 4 h ..+3 of a block: 32 rows at a
   // time go through the wave's own part of LDS, to leave in whole lines.
   float* mem = reinterpret_cast<float*>(lds) + wave * 32 * T::kOutPitch;
@@ -571,11 +599,16 @@ __global__ void __launch_bounds__(256) fp4_few_kernel(Fp4Params p, const char* x
 // ---------------------------------------------------------------- host
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
+// Reductions that 64 x 64 tiles of which a CU has one at most share out to two halves of
+// a workgroup: 128 rows by 4096 columns, k = 2048 8.3 us for 8.3, 4096 10.5 for 11.6, 16384
+// 24.7 for 31.
+bool halves(int64_t k) { return k > 8 * kStep; }
+
 // Rows that fp4_few_kernel can take, and those that it does: its workgroups read x again
 // for each 16 columns, so that many columns are for the tiles.  By estimated time: us
 // from what a workgroup per CU takes (256 CUs), c of them one after the other (measured
-// with k = 4096, kernel and tiles; 1, 16 and 64 rows by 4096 columns 4.3 and 10.7, 6.7
-// and 11, 10.8 and 11.1; by 16384 8.7 and 12.3, 14.1 and 12.6, 29 and 13; by 129280 57 and
+// with k = 4096, kernel and tiles; 1, 16 and 64 rows by 4096 columns 4.3 and 9.6, 6.7
+// and 9.7, 10.8 and 10.1; by 16384 8.7 and 11.3, 14.1 and 11.8, 29 and 12.5; by 129280 57 and
 // 63, 93 and 61, 206 and 68; k = 1024, 4096 columns 3.0 and 6.3, 5.7 and 6.5, 7.2 and 6.7,
 // 16384 columns 3.9 and 6.6, 7.9 and 6.7, 11.2 and 7.2; codes that are there 2 less with few).
 constexpr int64_t kFewRows = 64;
@@ -584,7 +617,7 @@ bool takes_few(int64_t m, int64_t n, int64_t k, bool packed) {
   if (up(n, 32) * up(k, kUnit) / 32 >= (1ll << 30)) return true;  // (more scales than the tiles' 32-bit offsets reach)
   const double c = (double)n / 4096, kk = (double)k / 4096, rows = 1.45 + 0.07 * m;
   const double few = packed ? 3.0 + c * kk * rows : 4.0 + c * kk * (m == 1 ? 1.5 : std::max(2.15, rows));
-  return few <= std::max(5.1 + 5.9 * kk, 4.0 + 1.85 * c * kk);
+  return few <= std::max(5.1 + (halves(k) ? 4.8 : 5.9) * kk, 4.0 + 1.85 * c * kk);
 }
 
 // Rows per wave, waves side by side in a row and workgroups of a quantisation.
@@ -610,7 +643,7 @@ void launch_quant(const QuantParams& q, bool bf16, hipStream_t st) {
 
 // What a product does and where its workspace keeps what.
 struct Fp4Plan {
-  bool few, fused;
+  bool few, fused, split;
   int tile;                    // 0: 256 x 256, 1: 128 x 128, 2: 64 x 64
   int64_t codes, xs, ws, bytes;  // offsets: x's codes, its scales, the weights' dealt words; size
 };
@@ -640,6 +673,7 @@ Fp4Plan plan_fp4(int64_t m, int64_t n, int64_t k, bool packed) {
   const int64_t r64 = rounds(64), r128 = rounds(128), r256 = rounds(256);
   const double t64 = r64 <= 2 ? 6.5 + 2.6 * r64 : 3.0 + 5.0 * r64, t128 = 7.0 + 9.8 * r128, t256 = 3.0 + 36.0 * r256;
   p.tile = t256 <= t128 && t256 <= t64 ? 0 : t128 <= t64 ? 1 : 2;
+  p.split = p.tile == 2 && r64 == 1 && halves(k);
   return p;
 }
 
@@ -655,12 +689,12 @@ int check_quant(const char* who, int64_t m, int64_t k, const void* x, int64_t st
   return HSMOE_OK;
 }
 
-template <int kBR, int kBC, int kWR, int kWC, int kStages>
+template <int kBR, int kBC, int kWR, int kWC, int kStages, int kSplit = 1>
 void launch_tile(const Fp4Params& p, hipStream_t st) {
   const int64_t tiles = ((p.m + kBR - 1) / kBR) * ((p.n + kBC - 1) / kBC);
   const int64_t size = tiles >= 8 * kChunk ? kChunk : (tiles + 7) / 8;  // place_tile's chunks, all eight XCDs'
   const int64_t grid = (tiles + 8 * size - 1) / (8 * size) * 8 * size;
-  hipLaunchKernelGGL((fp4_tile_kernel<kBR, kBC, kWR, kWC, kStages>), dim3((unsigned)grid), dim3(kWR * kWC * 64), 0, st, p);
+  hipLaunchKernelGGL((fp4_tile_kernel<kBR, kBC, kWR, kWC, kStages, kSplit>), dim3((unsigned)grid), dim3(kWR * kWC * 64 * kSplit), 0, st, p);
 }
 
 template <int kRB, int kKind>
@@ -777,6 +811,8 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
     launch_tile<256, 256, 2, 4, 0>(p, st);
   else if (plan.tile == 1)
     launch_tile<128, 128, 2, 2, 2>(p, st);
+  else if (plan.split)
+    launch_tile<64, 64, 2, 2, 4, 2>(p, st);
   else
     launch_tile<64, 64, 2, 2, 4>(p, st);
   return check_launch(who);

@@ -153,7 +153,7 @@ SIZES = [
     (1, 64, 4096), (1, 8, 32), (2, 24, 96), (3, 136, 512), (4, 64, 4096), (5, 48, 4096), (16, 40, 1024), (17, 64, 2048),
     (33, 72, 544), (48, 64, 480), (49, 128, 1056), (64, 520, 4096), (64, 8, 64), (65, 64, 64), (65, 8, 32), (66, 200, 96),
     (100, 136, 4096), (127, 72, 2016), (300, 264, 768), (513, 1000, 288), (16, 4096, 64), (1, 64, 32768), (130, 64, 16384),
-    (2, 32776, 2080), (16, 24008, 512), (33, 16392, 1024), (64, 8200, 2080), (1, 40000, 512), (2, 12000, 544),
+    (100, 1032, 1056), (250, 4096, 1024), (200, 520, 2336), (70, 72, 2048), (66, 264, 2592), (2, 32776, 2080), (16, 24008, 512), (33, 16392, 1024), (64, 8200, 2080), (1, 40000, 512), (2, 12000, 544),
 ]
 
 
