@@ -21,6 +21,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kJoinThreads = 512;
 constexpr int kChunk = 32;           // sorted tokens per chunk
+constexpr int kUnit = 8;             // .. and per group of threads, where d_out has up to
+constexpr int64_t kFew = 1 << 22;    // .. that many values
 constexpr int kSortThreads = 1024;
 constexpr int64_t kSortByRank = 65536;  // tokens up to which places are found by bisection
 constexpr uint32_t kNoId = 1u << 30;    // an id outside the table, above all others
@@ -192,7 +194,9 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(SortParams p) 
   const int id = t < p.m ? id_of(p.ids, p.wide, t, p.vocab) : -1;
   // bitonic, on (id, place): no two are the same, so the result is the stable sort's
   unsigned long long key = (unsigned long long)(id < 0 ? kNoId : (uint32_t)id) << 10 | (unsigned)i;
-  for (int size = 2; size <= kSortThreads; size *= 2)
+  // (no further than the tokens reach: what is behind them is sorted as it is)
+  const int64_t there = p.m - (int64_t)blockIdx.x * kSortThreads;
+  for (int size = 2; size <= kSortThreads && size / 2 < there; size *= 2)
     for (int step = size / 2; step > 0; step /= 2) {
       unsigned long long other;
       if (step >= 64) {
@@ -316,33 +320,41 @@ __device__ __forceinline__ void leave(float* to, const Vals<kVec>& s) {
 }
 
 // Sums of the runs of a chunk, for kVec columns per thread.  The chunk's ids and
-// tokens are read once; then eight rows are on their way at a time.
-template <int kVec, bool kF32, bool kOutF32>
+// tokens are read once; then eight rows are on their way at a time.  Few tokens: kOwn of
+// a chunk's rows are for a group of threads by itself, that takes the runs which begin
+// there, to their ends (all of it captured: 100 tokens of 4096 22 us by whole chunks, 12.6
+// so with a sort no longer than they need; 1000 24 and 20; 4096 30 and 34).
+template <int kVec, bool kF32, bool kOutF32, int kOwn>
 __global__ void __launch_bounds__(kThreads) embed_sum_kernel(SumParams p) {
   __shared__ int2 mem[kThreads / 8][kChunk + 1];  // (id, token) of the workgroup's chunks, and the id behind each
   __shared__ int before[kThreads / 8];
+  constexpr int kParts = kChunk / kOwn;
   const int lanes = 1 << p.shift, per = kThreads >> p.shift, mine = threadIdx.x >> p.shift;
-  const int64_t c0 = (int64_t)(blockIdx.x / p.slabs) * per;
-  const int64_t chunk = c0 + mine;
+  const int64_t u0 = (int64_t)(blockIdx.x / p.slabs) * per;
+  const int64_t chunk = (u0 + mine) / kParts;
   for (int i = threadIdx.x; i < per * (kChunk + 1); i += kThreads) {
-    const int64_t r = (c0 + i / (kChunk + 1)) * kChunk + i % (kChunk + 1);
+    const int64_t r = (u0 + i / (kChunk + 1)) / kParts * kChunk + i % (kChunk + 1);
     mem[i / (kChunk + 1)][i % (kChunk + 1)] = r < p.m ? make_int2(p.sorted_id[r], p.token[r]) : make_int2(-1, 0);
   }
   for (int i = threadIdx.x; i < per; i += kThreads) {
-    const int64_t r = (c0 + i) * kChunk - 1;
+    const int64_t r = (u0 + i) / kParts * kChunk - 1;
     before[i] = r >= 0 && r < p.m ? p.sorted_id[r] : -1;
   }
   __syncthreads();
   const int64_t col = ((int64_t)(blockIdx.x % p.slabs) * lanes + (threadIdx.x & (lanes - 1))) * kVec;
   if (chunk >= p.chunks || col >= p.d) return;
-  int id = mem[mine][0].x;
+  const int begin = (int)((u0 + mine) % kParts) * kOwn;
+  int id = mem[mine][begin].x;
   if (id < 0) return;
-  bool open = before[mine] == id;  // the run began before the chunk
+  bool open = begin == 0 && before[mine] == id;                            // the run began before the chunk
+  bool others = kParts > 1 && begin > 0 && mem[mine][begin - 1].x == id;  // it began in another group's rows
+  bool done = false;
   float* part = p.part + chunk * 2 * p.d + col;
   Vals<kVec> s = {};
   constexpr int kAhead = 8;
-  for (int r = 0; r < kChunk; r += kAhead) {
-    if (mem[mine][r].x < 0) break;
+  for (int r = begin; r < kChunk; r += kAhead) {
+    const int now = mem[mine][r].x;
+    if (now < 0 || (kParts > 1 && r >= begin + kOwn && (done || others || now != id))) break;
     Raw<kVec, kF32> v[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -352,16 +364,23 @@ __global__ void __launch_bounds__(kThreads) embed_sum_kernel(SumParams p) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int next = mem[mine][r + i].x;
-      if (next < 0) continue;
+      if (next < 0 || (kParts > 1 && done)) continue;
       if (next != id) {  // the run before is done
-        if (open) leave<kVec>(part, s);
-        else finish<kVec, kOutF32>(p, id, col, s);
-        open = false, id = next, s = Vals<kVec>{};
+        if (!(kParts > 1 && others)) {
+          if (open) leave<kVec>(part, s);
+          else finish<kVec, kOutF32>(p, id, col, s);
+        }
+        if (kParts > 1 && r + i >= begin + kOwn) {  // the next one is another group's
+          done = true;
+          continue;
+        }
+        open = others = false, id = next, s = Vals<kVec>{};
       }
 #pragma unroll
       for (int j = 0; j < kVec; ++j) s.v[j] += v[i].at(j);
     }
   }
+  if (kParts > 1 && (done || others)) return;
   // the last run: goes on in the next chunk, or ends here
   if (mem[mine][kChunk].x == id) leave<kVec>(part + (open ? 0 : p.d), s);
   else if (open) leave<kVec>(part, s);
@@ -469,12 +488,12 @@ bool rows16(const void* p, int64_t ld, int kind) { return aligned(p, 16) && ld *
 
 template <bool kSum, int kVec, bool kF32, bool kOutF32>
 void launch_grad(const SumParams& p, hipStream_t st) {
-  const int64_t per = kSum ? kThreads >> p.shift : 1;
-  const dim3 grid((unsigned)((p.chunks + per - 1) / per * p.slabs));
-  if constexpr (kSum)
-    hipLaunchKernelGGL((embed_sum_kernel<kVec, kF32, kOutF32>), grid, dim3(kThreads), 0, st, p);
-  else
-    hipLaunchKernelGGL((embed_join_kernel<kVec, kOutF32>), grid, dim3(kJoinThreads), 0, st, p);
+  const bool few = kSum && p.m * p.d <= kFew;
+  const int64_t per = kSum ? kThreads >> p.shift : 1, units = few ? p.chunks * (kChunk / kUnit) : p.chunks;
+  const dim3 grid((unsigned)((units + per - 1) / per * p.slabs)), block(kSum ? kThreads : kJoinThreads);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p); };
+  if constexpr (kSum) few ? go(embed_sum_kernel<kVec, kF32, kOutF32, kUnit>) : go(embed_sum_kernel<kVec, kF32, kOutF32, kChunk>);
+  else go(embed_join_kernel<kVec, kOutF32>);
 }
 template <bool kSum, int kVec>
 void launch_grad(const SumParams& p, bool f32, bool out_f32, hipStream_t st) {

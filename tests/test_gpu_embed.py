@@ -198,3 +198,20 @@ def test_refusals(dev):
                      (lambda: ops.embed_grad(d_out, ids, 4, out=table[:1].expand(4, 16)), ValueError)):
         with pytest.raises(exc):
             bad()
+
+
+@pytest.mark.parametrize("d", (8, 15, 520, 4104))
+def test_runs_of_every_length(dev, d):
+    """Runs that begin and end anywhere in the chunks and in their parts: sums of small integers, which are exact."""
+    for seed in range(8):
+        g = torch.Generator().manual_seed(seed)
+        lengths = torch.randint(1, (2, 5, 9, 17, 40, 70, 100, 12)[seed], (120,), generator=g)
+        ids = torch.repeat_interleave(torch.randperm(500, generator=g)[:120], lengths)
+        ids = ids[torch.randperm(len(ids), generator=g)].to(dev)
+        if seed % 2:
+            ids[::7] = -1
+        d_out = torch.randint(-8, 9, (len(ids), d), generator=g).to(dev, BF16)
+        want = torch.zeros(501, d, device=dev).index_add_(0, torch.where(ids < 0, 500, ids), d_out.float())[:500]
+        assert torch.equal(ops.embed_grad(d_out, ids, 500, 2.0, F32), 2 * want)
+        base = torch.full((500, d), 3.0, device=dev)
+        assert torch.equal(ops.embed_grad(d_out, ids, 500, 1.0, out=base), want + 3)
