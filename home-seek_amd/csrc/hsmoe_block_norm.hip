@@ -490,10 +490,11 @@ Shape shape_of(int64_t d, bool grad) {
 // Workgroups of the gradient: with weights' gradients to sum, what the CUs hold (each
 // leaves a row of sums); else one per row group.  Short rows of a workgroup each want
 // more of them to wait with (bf16 21000 x 1536 90 us with four per CU, 111 with two), if
-// they are not of fp32 (136 with two, 149 with four).
+// they are not of fp32 (136 with two, 149 with four).  Few rows: four for a workgroup,
+// since each of them leaves a row of sums to be joined (512 x 4096 captured 22 us by 512, 18 by 128).
 int64_t grad_groups(int64_t m, const Shape& s, bool sums, bool f32) {
   const int per_cu = s.threads > 512 ? 1 : s.lanes || f32 ? 2 : std::max(2, 768 / s.threads);
-  const int64_t all = (m + s.rows - 1) / s.rows, some = per_cu * (int64_t)device_cus();
+  const int64_t all = (m + s.rows - 1) / s.rows, some = std::min(per_cu * (int64_t)device_cus(), std::max<int64_t>(128, all / 4));
   return sums && all > some ? some : std::min<int64_t>(all, 1 << 22);  // (workgroups go on to further rows)
 }
 

@@ -28,6 +28,7 @@ constexpr int64_t kMuch = 1 << 24;   // values from which piece_kernel is worth 
 constexpr int kPer = 112;            // tensors per launch: their addresses are kernel arguments, so that a captured graph holds them
 constexpr int64_t kSmall = 32768;    // values up to which one workgroup does it all
 constexpr int kSmallThreads = 1024;
+constexpr int kSmallChunk = 1024;    // values that one of its waves takes at a time
 
 enum { kInF32 = 1, kOutF32 = 2, kInVec = 4, kOutVec = 8, kSame = 16 };
 
@@ -155,9 +156,9 @@ template <bool kMax, bool kF32, int kN>
 __device__ __forceinline__ void take_part(const void* in, int64_t a, int64_t b, bool vec, Part<kMax>& s) {
   int64_t done = a;
   if (vec) {
-    constexpr int kAhead = (kF32 ? 2 : 4) * (kN == kThreads ? 2 : 1);
+    constexpr int kAhead = (kF32 ? 2 : 4) * (kN == kThreads ? 2 : 1) / (kN == 64 ? 2 : 1);
     const int64_t whole = a + (b - a) / 8 * 8;
-    for (int64_t i = a + (int64_t)threadIdx.x * 8; i < whole; i += (int64_t)kAhead * kN * 8) {
+    for (int64_t i = a + (int64_t)(threadIdx.x % kN) * 8; i < whole; i += (int64_t)kAhead * kN * 8) {
       Raw<kF32> v[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) v[j] = i + (int64_t)j * kN * 8 < whole ? read8<kF32>(in, i + (int64_t)j * kN * 8) : Raw<kF32>{};
@@ -168,15 +169,15 @@ __device__ __forceinline__ void take_part(const void* in, int64_t a, int64_t b, 
     }
     done = whole;
   }
-  for (int64_t i = done + threadIdx.x; i < b; i += kN) s.take(read1<kF32>(in, i));
+  for (int64_t i = done + threadIdx.x % kN; i < b; i += kN) s.take(read1<kF32>(in, i));
 }
 template <bool kF32, bool kO32, int kN>
 __device__ __forceinline__ void scale_part(const void* in, void* out, int64_t a, int64_t b, bool vec, Factor c) {
   int64_t done = a;
   if (vec) {
-    constexpr int kAhead = (kF32 ? 2 : 4) * (kN == kThreads ? 2 : 1);
+    constexpr int kAhead = (kF32 ? 2 : 4) * (kN == kThreads ? 2 : 1) / (kN == 64 ? 2 : 1);
     const int64_t whole = a + (b - a) / 8 * 8;
-    for (int64_t i = a + (int64_t)threadIdx.x * 8; i < whole; i += (int64_t)kAhead * kN * 8) {
+    for (int64_t i = a + (int64_t)(threadIdx.x % kN) * 8; i < whole; i += (int64_t)kAhead * kN * 8) {
       Raw<kF32> v[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) v[j] = i + (int64_t)j * kN * 8 < whole ? read8<kF32>(in, i + (int64_t)j * kN * 8) : Raw<kF32>{};
@@ -190,7 +191,7 @@ __device__ __forceinline__ void scale_part(const void* in, void* out, int64_t a,
     }
     done = whole;
   }
-  for (int64_t i = done + threadIdx.x; i < b; i += kN) write1<kO32>(out, i, read1<kF32>(in, i) * c.a * c.b);
+  for (int64_t i = done + threadIdx.x % kN; i < b; i += kN) write1<kO32>(out, i, read1<kF32>(in, i) * c.a * c.b);
 }
 template <bool kMax, int kN>
 __device__ __forceinline__ void take_any(const Batch& t, int j, int64_t a, int64_t b, Part<kMax>& s) {
@@ -306,16 +307,25 @@ __global__ void __launch_bounds__(kThreads) piece_kernel(Batch t, const Factor* 
   }
 }
 
-// Few values: one workgroup, one launch.
+// Few values: one workgroup, one launch, whose waves take chunks of kSmallChunk (60 tensors
+// of 10000 values in all 12 us; tensor after tensor by all waves 61).
 template <bool kMax, bool kClip>
 __global__ void __launch_bounds__(kSmallThreads) small_kernel(Batch t, float max_norm, float* norm_out) {
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), chunks = t.first[t.n];
+  auto each = [&](auto f) {
+    for (uint32_t c = wave; c < chunks; c += kSmallThreads / 64) {
+      const int j = tensor_of(t, c);
+      const int64_t a = (int64_t)(c - t.first[j]) * kSmallChunk;
+      f(j, a, a + kSmallChunk < t.count[j] ? a + kSmallChunk : t.count[j]);
+    }
+  };
   Part<kMax> s;
-  for (int j = 0; j < t.n; ++j) take_any<kMax, kSmallThreads>(t, j, 0, t.count[j], s);
+  each([&](int j, int64_t a, int64_t b) { take_any<kMax, 64>(t, j, a, b, s); });
   const double norm = join_block<kMax, kSmallThreads>(s).norm();
   if (threadIdx.x == 0) *norm_out = (float)norm;
   if (!kClip) return;
   const Factor f = factor(norm, max_norm);
-  for (int j = 0; j < t.n; ++j) scale_any<kSmallThreads>(t, j, 0, t.count[j], f);
+  each([&](int j, int64_t a, int64_t b) { scale_any<64>(t, j, a, b, f); });
 }
 
 // ---------------------------------------------------------------- host
@@ -365,7 +375,7 @@ int check_tensors(const char* who, const Tensors& t, double norm_type, float max
 }
 
 // Tensors from `at` on that go into one launch; at: the first that does not.
-Batch batch_of(const Tensors& t, int64_t& at) {
+Batch batch_of(const Tensors& t, int64_t& at, int chunk = kChunk) {
   Batch b{};
   uint64_t chunks = 0;
   for (; at < t.n && b.n < kPer; ++at) {
@@ -377,7 +387,7 @@ Batch batch_of(const Tensors& t, int64_t& at) {
     b.flags[j] = (uint8_t)((f ? kInF32 : 0) | (o ? kOutF32 : 0) | (aligned(b.in[j], 16) ? kInVec : 0) | (aligned(b.out[j], 16) ? kOutVec : 0) |
                            (b.in[j] == b.out[j] && f == o ? kSame : 0));
     b.first[j] = (uint32_t)chunks;
-    chunks += (uint64_t)((c + kChunk - 1) / kChunk);  // (kPer tensors of less than 2^38 values: below 2^31)
+    chunks += (uint64_t)((c + chunk - 1) / chunk);  // (kPer tensors of less than 2^38 values: below 2^31)
     b.first[b.n] = (uint32_t)chunks;
   }
   return b;
@@ -394,7 +404,7 @@ int run_clip(const char* who, const Tensors& t, float max_norm, float* norm_out,
   }
   if (total <= kSmall && live <= kPer) {
     int64_t at = 0;
-    const Batch b = batch_of(t, at);
+    const Batch b = batch_of(t, at, kSmallChunk);
     if (t.out) hipLaunchKernelGGL((small_kernel<kMax, true>), dim3(1), dim3(kSmallThreads), 0, st, b, max_norm, norm_out);
     else hipLaunchKernelGGL((small_kernel<kMax, false>), dim3(1), dim3(kSmallThreads), 0, st, b, max_norm, norm_out);
     return check_launch(who);
