@@ -180,3 +180,22 @@ def test_refusals(dev):
         with pytest.raises(exc):
             bad()
     assert float(ops.grad_norm([a, a])) > 0  # read twice is no harm
+
+
+def test_large_replayed(dev):
+    """Much data into other tensors, captured: the norm, the factor and the copy follow the values of each replay."""
+    grads = [normal(dev, 1, (4099, 4097)), normal(dev, 2, (70001,), F32)]
+    outs = [torch.empty_like(g) for g in grads]
+    ops.clip_grads(grads, 1.0, out=outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ops.clip_grads(grads, 1.0, out=outs)
+    for i in range(4):
+        for j, g in enumerate(grads):
+            g.copy_(normal(dev, 10 * i + j, g.shape, g.dtype, (0.5, 2.0, 1e-6, 1.0)[i]))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(grads, 1.0, 2.0, norm, outs)
+        got = [o.clone() for o in outs]
+        assert torch.equal(ops.clip_grads(grads, 1.0, out=outs), norm)
+        assert all(torch.equal(a, b) for a, b in zip(got, outs))
