@@ -494,7 +494,8 @@ Shape shape_of(int64_t d, bool grad) {
 int64_t grad_groups(int64_t m, const Shape& s, bool sums, bool f32) {
   const int per_cu = s.threads > 512 ? 1 : s.lanes || f32 ? 2 : std::max(2, 768 / s.threads);
   const int64_t all = (m + s.rows - 1) / s.rows, some = std::min(per_cu * (int64_t)device_cus(), std::max<int64_t>(128, all / 4));
-  return sums && all > some ? some : std::min<int64_t>(all, 1 << 22);  // (workgroups go on to further rows)
+  // (by 1024 threads 2^22 would be one thread more than a launch counts; workgroups go on to further rows)
+  return sums && all > some ? some : std::min<int64_t>(all, (1 << 22) - 1);
 }
 
 template <bool kGrad, bool kF32, bool kS32, bool kW32>
