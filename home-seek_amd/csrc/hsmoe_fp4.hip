@@ -689,11 +689,20 @@ int check_quant(const char* who, int64_t m, int64_t k, const void* x, int64_t st
   return HSMOE_OK;
 }
 
+// Workgroups for rows by columns of tiles of kBR x kBC: place_tile's chunks, all eight XCDs'.
+int64_t tile_groups(int64_t m, int64_t n, int64_t rows, int64_t cols) {
+  const int64_t tiles = ((m + rows - 1) / rows) * ((n + cols - 1) / cols);
+  const int64_t size = tiles >= 8 * kChunk ? kChunk : (tiles + 7) / 8;
+  return (tiles + 8 * size - 1) / (8 * size) * 8 * size;
+}
+// .. and whether a launch holds those of a plan.
+bool tiles_fit(const Fp4Plan& p, int64_t m, int64_t n) {
+  const int64_t side = p.tile == 0 ? 256 : p.tile == 1 ? 128 : 64;
+  return grid_fits(tile_groups(m, n, side, side), p.tile == 0 || p.split ? 512 : 256);
+}
 template <int kBR, int kBC, int kWR, int kWC, int kStages, int kSplit = 1>
 void launch_tile(const Fp4Params& p, hipStream_t st) {
-  const int64_t tiles = ((p.m + kBR - 1) / kBR) * ((p.n + kBC - 1) / kBC);
-  const int64_t size = tiles >= 8 * kChunk ? kChunk : (tiles + 7) / 8;  // place_tile's chunks, all eight XCDs'
-  const int64_t grid = (tiles + 8 * size - 1) / (8 * size) * 8 * size;
+  const int64_t grid = tile_groups(p.m, p.n, kBR, kBC);
   hipLaunchKernelGGL((fp4_tile_kernel<kBR, kBC, kWR, kWC, kStages, kSplit>), dim3((unsigned)grid), dim3(kWR * kWC * 64 * kSplit), 0, st, p);
 }
 
@@ -751,7 +760,7 @@ extern "C" int hsmoe_fp4_linear(const void* x, int x_kind, int64_t x_row_stride,
     return fail(HSMOE_ERR_SHAPE, "%s: operands must be 16-byte aligned", who);
   const Fp4Plan plan = plan_fp4(m, n, k, packed);
   if (plan.few && !grid_fits((n + 15) / 16, 256)) return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
-  if (!plan.few && (plan.bytes - plan.xs >= (1ll << 31) - 1024 || ((m + 63) / 64) * ((n + 63) / 64) >= (1ll << 30)))
+  if (!plan.few && (plan.bytes - plan.xs >= (1ll << 31) - 1024 || !tiles_fit(plan, m, n)))
     return fail(HSMOE_ERR_SHAPE, "%s: operands too large", who);
   if (plan.bytes && (!workspace || workspace_bytes < (size_t)plan.bytes))
     return fail(HSMOE_ERR_WORKSPACE, "%s: workspace of %lld bytes needed", who, (long long)plan.bytes);

@@ -109,7 +109,7 @@ def launch_lib(tmp_path_factory):
 
 # (name, whether there are sizes that it refuses)
 @pytest.mark.parametrize("name,refuses", (("hsmoe_block_norm", True), ("hsmoe_block_norm_grad", False), ("hsmoe_embed", True),
-                                          ("hsmoe_embed_grad", True), ("hsmoe_fp4_quant", True)))
+                                          ("hsmoe_embed_grad", True), ("hsmoe_fp4_quant", True), ("hsmoe_fp4_linear", True)))
 def test_no_launch_has_more_threads_than_32_bits_count(launch_lib, name, refuses):
     res = subprocess.run([sys.executable, __file__, str(launch_lib), name], capture_output=True, text=True, timeout=120)
     assert res.returncode == 0, res.stderr[-2000:]
