@@ -92,14 +92,15 @@ __device__ __forceinline__ Part<kMax> join_block(Part<kMax> p) {
   return all;
 }
 
-// min(1, max_norm / (norm + 1e-6)) = a b; NaN stays NaN.  Where fp32 does not hold the
+// min(1, max_norm / (norm + 1e-6)) = a b; NaN stays NaN, and nothing is beyond an infinite
+// limit, an infinite norm neither (inf / inf would make NaN of every value).  Where fp32 does not hold the
 // factor with all its bits (a norm of 2^100 limits), two factors of half its exponent do.
 struct Factor {
   float a, b;
 };
 __device__ __forceinline__ Factor factor(double norm, float max_norm) {
   const double c = (double)max_norm / (norm + 1e-6);
-  if (c >= 1.0) return {1.0f, 1.0f};
+  if (c >= 1.0 || (isinf(max_norm) && !isnan(norm))) return {1.0f, 1.0f};
   if (!(c < 0x1p-100) || c == 0.0) return {1.0f, (float)c};
   const int e = ilogb(c) / 2;
   return {(float)ldexp(1.0, e), (float)ldexp(c, -e)};

@@ -708,8 +708,9 @@ def grad_norm(grads, norm_type: float = 2.0) -> torch.Tensor:
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Multiplies a list of gradients by min(1, max_norm / (norm + 1e-6)), in place or into
     the tensors of out (bf16 or fp32, of their shapes), and returns their norm before that, as
-    grad_norm (hsmoe_clip_grads).  Nothing waits for the device.  A NaN anywhere makes all of them NaN.  Tensors may
-    not overlap: one that is given twice is refused."""
+    grad_norm (hsmoe_clip_grads).  Nothing waits for the device.  A NaN anywhere makes all of them NaN; an infinity makes
+    them 0, and itself NaN, unless max_norm is infinite, which cuts nothing down.  Tensors may not overlap: one that is
+    given twice is refused."""
     return _clip(grads, float(max_norm), float(norm_type), out)
 
 

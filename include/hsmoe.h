@@ -434,7 +434,8 @@ int hsmoe_linear_plan(int product, int64_t m, int64_t n, int64_t k, int64_t n_gr
  * kind), and else overlaps none of the others.  The arrays lie in host memory and are
  * read before the call returns.  norm_out fp32 [1] on the device.  Squares and sums in
  * 64 bits; a NaN anywhere makes the norm and every output NaN, an infinity makes the
- * outputs 0 (NaN where it is).  Deterministic, nothing waits for the device.  n = 0
+ * outputs 0 (NaN where it is), unless max_norm is INFINITY: then nothing is cut down,
+ * whatever the norm, and only a NaN changes the outputs.  Deterministic, nothing waits for the device.  n = 0
  * and empty tensors are allowed.  The workspace (any contents) holds
  * hsmoe_grad_norm_workspace_size bytes for both. */
 size_t hsmoe_grad_norm_workspace_size(int64_t n);
