@@ -389,11 +389,12 @@ __global__ void __launch_bounds__(kMax, kMax >= 512 ? 4 : 2) block_norm_grad_ker
     }
     if (p.gate_kind == kGateToken && p.d_gate && live && t == 0) ((float*)p.d_gate)[first + mine] = q[1];
     if (p.d_f) {
-      const float m1 = p.post_w ? q[0] * p.per * r1 * r1 : 0.0f;
+      const float m1 = q[0] * p.per * r1 * r1;  // r1^2 mean(post_w du f)
 #pragma unroll
       for (int c = 0; c < kC; ++c) {
+        if (p.post_w)  // (without it f is no factor: an infinity or NaN there may not reach d_f as a product with 0)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) df[c].v[i] = r1 * __fmaf_rn(-r.f[c].at(i), m1, df[c].v[i]);
+          for (int i = 0; i < 8; ++i) df[c].v[i] = r1 * __fmaf_rn(-r.f[c].at(i), m1, df[c].v[i]);
         write8<kF32>(rows_buf<kF32>(p.d_f, first, left, p.d), at[c], df[c]);
       }
     }
