@@ -142,7 +142,8 @@ class _BlockNorm(Function):
     def forward(ctx, f, h, post_w, gate, pre_w, scale, eps):
         ctx.set_materialize_grads(False)  # a result that is not used has no gradient to be read
         out, n = ops.block_norm(f, h, post_w, gate, scale, pre_w, eps)
-        ctx.save_for_backward(f, out, post_w, gate, pre_w)
+        # (only the norm before the next block reads the stream again: without it, it may be written)
+        ctx.save_for_backward(f, None if pre_w is None else out, post_w, gate, pre_w)
         ctx.scale, ctx.eps = scale, eps
         return out, n
 
@@ -152,6 +153,8 @@ class _BlockNorm(Function):
         f, out, post_w, gate, pre_w = ctx.saved_tensors
         if d_h is None and d_n is None:
             return (None,) * 7
+        if out is None:
+            out = d_h = d_h.contiguous()  # (the stream's type; not read as it)
         g = ops.block_norm_grad(d_h, d_n, f, out, post_w, gate, ctx.scale, pre_w, ctx.eps, need=ctx.needs_input_grad[:5])
         like = lambda d, t: None if d is None else d.to(t.dtype)
         return g.f, g.h, like(g.post_w, post_w), like(g.gate, gate), like(g.pre_w, pre_w), None, None
