@@ -124,8 +124,9 @@ class HbmExpertStore:
         return t
 
     def _table_row(self, layer: int, eid: int) -> list[int]:
-        if (layer, eid) in self._absent:
-            return [0] * 6
+        return [0] * 6 if (layer, eid) in self._absent else self._addresses(layer, eid)
+
+    def _addresses(self, layer: int, eid: int) -> list[int]:
         b = self.buf.data_ptr() + self._expert_base(layer, eid)
         return [b + self._off[n] for n in ("w1", "s1", "w3", "s3", "w2", "s2")]
 
@@ -174,10 +175,10 @@ class HbmExpertStore:
         for w, codes, scale in zip((w1, w3, w2), views[0::2], views[1::2]):
             ops.fp4_quant(w.detach(), out=(codes, scale))
         if (layer, eid) in self._absent:
-            self._absent.discard((layer, eid))
             t = self._tables.get(layer)
-            if t is not None:
-                t[eid].copy_(torch.tensor(self._table_row(layer, eid), dtype=torch.int64))
+            if t is not None:  # (the expert is there once its row is)
+                t[eid].copy_(torch.tensor(self._addresses(layer, eid), dtype=torch.int64))
+            self._absent.discard((layer, eid))
 
     def fill_synthetic(self, seed: int, layers=None) -> None:
         """Fills experts (and shared experts) with the seeded synthetic weights."""
