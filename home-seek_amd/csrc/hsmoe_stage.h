@@ -22,8 +22,9 @@ __device__ __forceinline__ int64_t uniform64(int64_t v) {
 }
 
 // 16 bytes per lane from global memory to LDS, lane l's to dst + 16 l.  Written
-// out because the compiler waits for every such load it knows of before each
-// ds_read_b64_tr_b16, whatever it reads; the waits are reduce_*'s.  No register
+// out because the compiler waits for every such load it knows of before reads of
+// LDS, whatever they read (each ds_read_b64_tr_b16 of the bf16 tiles); the waits are
+// the kernels' own.  No register
 // is written: the load takes its address when it is issued.  (s_nop 4: a vector
 // instruction may have written the resource's scalar registers, v_readfirstlane
 // for one; a memory instruction may read them five wait states later.)

@@ -449,9 +449,10 @@ int hsmoe_clip_grads(int64_t n, const void* const* tensors_dev, const int64_t* c
 /* ---------------------------------------------------------------------------
  * Microscaled 4-bit floating point in the experts' own format (e2m1 codes, low
  * nibble first, with one E8M0 power of two per 32 values of a row): quantisation,
- * what the reference's offline quantiser does (_fp4.py:113-255,
- * quantize_weights.py:1-199), and the product of two quantised operands, which it
- * does not have.
+ * which is the reference's offline quantiser's (_fp4.py:113-255,
+ * quantize_weights.py:1-199) as far as the format goes (the scale is rounded up to a
+ * power of two, whatever that one rounds to), and the product of two quantised
+ * operands, which it does not have.
  *
  * hsmoe_fp4_quant: x [m, k] rows (HSMOE_OUT_BF16 or HSMOE_OUT_F32, x_row_stride
  * values apart) -> codes uint8 [m, k / 2] and scales uint8 [m, k / 32].  A block's
