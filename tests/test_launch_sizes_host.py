@@ -57,6 +57,15 @@ def calls(rng):
                                    rng.randint(0, 1), A, cols, kinds[1], B, many, None)
         k = 32 * sizes(rng, 2 ** 17 - 1)
         yield "hsmoe_fp4_quant", (A, k, kinds[0], m, k, A, A, None)
+        n, apart = rng.randint(1, 200), 1 << 44
+        tensors = [(i + 1) * apart for i in range(n)]
+        outs = [t if rng.random() < 0.5 else t + apart // 2 for t in tensors]
+        counts = [sizes(rng, 2 ** 38 - 1) if rng.random() < 0.1 else sizes(rng, 2 ** 20) for _ in range(n)]
+        array = lambda c, v: (c * n)(*v)
+        words, kind = array(ctypes.c_int64, counts), array(ctypes.c_int32, [kinds[0]] * n)
+        yield "hsmoe_grad_norm", (n, array(ctypes.c_uint64, tensors), words, kind, ctypes.c_double(2.0), A, B, many, None)
+        yield "hsmoe_clip_grads", (n, array(ctypes.c_uint64, tensors), words, kind, array(ctypes.c_uint64, outs), kind,
+                                   ctypes.c_double(math.inf), 1.0, A, B, many, None)
         x = rng.randint(0, 2)
         yield "hsmoe_fp4_linear", (A, x, k, A if x == 2 else None, m, k, A, A, 8 * sizes(rng, 2 ** 28 - 1), kinds[1], A, B, many, None)
 
@@ -109,7 +118,8 @@ def launch_lib(tmp_path_factory):
 
 # (name, whether there are sizes that it refuses)
 @pytest.mark.parametrize("name,refuses", (("hsmoe_block_norm", True), ("hsmoe_block_norm_grad", False), ("hsmoe_embed", True),
-                                          ("hsmoe_embed_grad", True), ("hsmoe_fp4_quant", True), ("hsmoe_fp4_linear", True)))
+                                          ("hsmoe_embed_grad", True), ("hsmoe_fp4_quant", True), ("hsmoe_fp4_linear", True),
+                                          ("hsmoe_grad_norm", False), ("hsmoe_clip_grads", False)))
 def test_no_launch_has_more_threads_than_32_bits_count(launch_lib, name, refuses):
     res = subprocess.run([sys.executable, __file__, str(launch_lib), name], capture_output=True, text=True, timeout=120)
     assert res.returncode == 0, res.stderr[-2000:]
